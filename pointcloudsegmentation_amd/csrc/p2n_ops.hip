@@ -35,8 +35,8 @@ typedef unsigned long long u64;
 // winner exchange.  What an iteration costs is instruction issue on one CU plus the exchange, so:
 //  * few, fat waves: 256 threads x up to 48 points (one wave per SIMD) -- the reductions are paid
 //    per wave, the distance updates per point;
-//  * distances for two points at a time (v_pk_add/mul_f32: same IEEE roundings as the scalar
-//    form), and the running argmax tracks only (distance, slot number); the winner's coordinates
+//  * distances for two points at a time (same IEEE roundings as one by one),
+//    and the running argmax tracks only (distance, slot number); the winner's coordinates
 //    are read back from a copy of the chunk in LDS instead of being selected per point;
 //  * workgroup argmax: DPP maximum over each 16-lane row, then one 64-bit LDS atomic max per row
 //    into a key that rotates over three words (the word two iterations ahead is cleared behind
@@ -1201,7 +1201,7 @@ extern "C" int p2n_fps(const float *xyz, int B, int N, int M, int start_idx, int
 
 // =========================================================================== ball query
 // One WAVE serves two queries (the kNN kernel's shape): the cloud streams through LDS as SoA tiles,
-// the 64 lanes test 64 consecutive points against both queries with packed fp32 arithmetic, a ballot
+// the 64 lanes test 64 consecutive points against both queries, a ballot
 // gives the hits in index order and a lane's rank among them (popcount of the lower lanes) is its
 // output slot.  A query is finished as soon as it has nsample hits (wave-uniform, no divergence), a
 // workgroup as soon as all its queries are.  The first version ran one THREAD per query: 2 waves per
@@ -1301,8 +1301,8 @@ __device__ __forceinline__ float dpp_wave_shr1(float v, float fill) {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// One wave serves TWO queries: every lane measures its candidate against both with packed fp32
-// arithmetic (v_pk_add/mul_f32: same IEEE roundings as the scalar form, half the instructions), so the
+// One wave serves TWO queries: every lane measures its candidate against both side by side
+// (the same IEEE roundings as one at a time), so the
 // LDS reads and the loop overhead are shared as well.  Each query keeps its own sorted list.
 __global__ __launch_bounds__(KNN_WAVES * 64) void p2n_knn_kernel(const float *__restrict__ query,
                                                                 const float *__restrict__ ref, int M, int N, int k,
