@@ -388,10 +388,34 @@ int p2n_forward_eval_raw(const double *points, const double *colors, int N, int 
                          const double *prep_cs, float *emb, float *global_f,
                          void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- 8-bit integer products (no counterpart in the reference) ---------------
+ * 8-bit rule for a set of values v: scale s = float32(max|v| / 127), code q = clamp(round_half_even(v / s), -127, 127)
+ * with the quotient taken exactly; s = 0 gives q = 0; a NaN or an infinity among the v gives s = NaN (and q = 0).
+ * A product of tokens x (K values each) with weights W (N, K): one scale per token and one per row of W,
+ *     y[t][n] = fl(fl(fl(sum_k qx qw) * sw[n]) * sx[t]) + bias[n]      (the sum exact in int32), then ReLU if asked.
+ * `bf16` non-zero: x and y are bfloat16, the arithmetic is the same and y is rounded once at the end. */
+long p2n_int8_weight_bytes(int K, int N);        /* -1: K or N outside 1..65536 */
+/* W (N,K) float32 and bias (N) (NULL: zeros) -> the image that the products read: codes in matrix-core fragment order, scales, bias */
+int p2n_int8_pack_weight(const float *W, const float *bias, int K, int N, void *image, void *stream);
+/* rows x[t*ld .. t*ld + K-1], t < T, ld >= K -> codes (T,K), scale (T) */
+int p2n_quantize_tokens(const void *x, int bf16, long T, int K, long ld, signed char *codes, float *scale, void *stream);
+size_t p2n_int8_linear_workspace_bytes(long T, int K, int N);
+int p2n_int8_linear(const void *x, int bf16, long T, int K, long ld, const void *image, int N, int relu, void *y,
+                    void *workspace, size_t workspace_bytes, void *stream);
+/* The layers of a shared MLP over the columns of x (B, dims[0], L): token = column, ReLU behind every layer but the last
+ * (behind that one if last_relu), hidden values put into 8 bits again by the rule.  out (B, dims[nl], L), or with
+ * group = 16 or 32 (dividing L) the maximum over groups of consecutive columns, (B, dims[nl], L/group); a NaN in a group
+ * is its maximum.  images_host: HOST array of nl device pointers.  1..8 layers, dims[0] <= 1024, others <= 256, L <= 2^24. */
+int p2n_int8_mlp(const float *x, int B, long L, int nl, const int *dims, const void *const *images_host, int last_relu,
+                 int group, float *out, void *stream);
+/* out[r] = max of in[r*ns .. r*ns + ns-1], a NaN is the maximum */
+int p2n_max_of_columns(const float *in, long rows, int ns, float *out, void *stream);
+
 /* ---- measurement aid (no counterpart in the reference) ---------------------
  * While enabled, every kernel launch is bracketed by HIP events on its stream.
  * p2n_profile_collect synchronises and fills, per kernel id (0 encoder, 1 mid,
- * 2 head, 3 fps, 5 knn, 10 cluster prep, 11 cluster count pass, 12 cluster link pass), the summed milliseconds and the number of launches since
+ * 2 head, 3 fps, 5 knn, 10 cluster prep, 11 cluster count pass, 12 cluster link pass,
+ * 20 int8 weight image, 21 token codes, 22 int8 product, 23 int8 shared MLP), the summed milliseconds and the number of launches since
  * the last collect.  HOST pointers.  Not thread-safe; off by default. */
 int p2n_profile_enable(int on);
 /* kernel_id >= 0: only that kernel's launches are bracketed (two event records per step instead of

@@ -1,0 +1,171 @@
+"""8-bit operators on the GPU (libp2n_hip.so): products in 8-bit integers with a scale for every token and channel, and
+activation checkpoints in 8 bits for the backward pass.
+
+The reference computes and keeps everything in float32 (reference src/models/point2net.py:9-34, train.py:124-131); these are
+additions with a definition of their own.  The 8-bit rule they share: a set of values v has the scale
+s = float32(max|v| / 127) and the codes q = clamp(round_half_even(v / s), -127, 127), the quotient taken exactly; s = 0 gives
+q = 0; a NaN or an infinity among the v makes s NaN, and with it every result that the scale enters.
+
+  quantize_tokens   codes and scales of the rows of a tensor
+  Int8Weight        a weight matrix (and bias) put into 8 bits once, laid out for the matrix cores
+  int8_linear       y = x W^T + b over rows of float32 or bfloat16, from one token to many
+  int8_mlp          the layers of a shared MLP over (B, C, L), activations on chip; `SharedMLP.precision = "int8"` runs it
+
+All functions take GPU tensors only and queue their work on the current stream of the tensors' device; nothing synchronises.
+"""
+import ctypes
+from typing import Optional, Sequence
+
+import torch
+
+from . import _lib
+from . import runtime as _rt
+
+
+def _gpu(t: torch.Tensor, name: str, dtypes) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a GPU tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}, got {t.dtype}")
+    return t
+
+
+def _no_grad_wanted(what: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass (rounding to 8 bits has no gradient): call it under torch.no_grad()")
+
+
+_TOKEN_TYPES = (torch.float32, torch.bfloat16)
+
+
+def _rows(x: torch.Tensor):
+    """(..., K) -> T, K, row stride and a tensor whose memory holds those rows"""
+    if x.dim() < 1:
+        raise ValueError("x must have at least one dimension")
+    K = x.size(-1)
+    if K < 1:
+        raise ValueError(f"x must have at least one value in a token, got {tuple(x.shape)}")
+    T = x.numel() // K
+    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= K:
+        return T, K, x.stride(0), x
+    return T, K, K, x.contiguous()
+
+
+def quantize_tokens(x: torch.Tensor):
+    """x (..., K) float32 or bfloat16 -> codes (..., K) int8, scale (...) float32: one scale for each row of K values."""
+    _gpu(x, "x", _TOKEN_TYPES)
+    _no_grad_wanted("quantize_tokens", x)
+    T, K, ld, rows = _rows(x)
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.lib().p2n_quantize_tokens(rows.data_ptr(), int(x.dtype == torch.bfloat16), T, K, ld, codes.data_ptr(),
+                                                  scale.data_ptr(), _rt.stream_handle(x.device)), "p2n_quantize_tokens")
+    return codes, scale
+
+
+class Int8Weight:
+    """A weight (N, K) -- or the (N, K, 1) of a Conv1d(kernel_size=1) -- and an optional bias (N), put into 8 bits with one scale
+    per output channel and laid out for the kernels.  Made once from the float32 values of that moment; make a new one after
+    the weights changed."""
+
+    def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None):
+        weight = _gpu(weight, "weight", (torch.float32,)).detach()
+        if weight.dim() == 3 and weight.size(2) == 1:
+            weight = weight.squeeze(2)
+        if weight.dim() != 2:
+            raise ValueError(f"weight must be (N,K) or (N,K,1), got {tuple(weight.shape)}")
+        self.out_features, self.in_features = weight.shape
+        self.device = weight.device
+        if bias is not None:
+            bias = _gpu(bias, "bias", (torch.float32,)).detach()
+            if bias.shape != (self.out_features,) or bias.device != weight.device:
+                raise ValueError(f"bias must be ({self.out_features},) on {weight.device}, got {tuple(bias.shape)} on {bias.device}")
+            bias = bias.contiguous()
+        L = _lib.lib()
+        n = L.p2n_int8_weight_bytes(self.in_features, self.out_features)
+        if n < 0:
+            raise ValueError(f"weight (N,K) = {tuple(weight.shape)}: both must be in 1..65536")
+        weight = weight.contiguous()
+        self.image = torch.empty(n, dtype=torch.uint8, device=weight.device)
+        with torch.cuda.device(weight.device):
+            _lib.check(L.p2n_int8_pack_weight(weight.data_ptr(), _rt.ptr(bias), self.in_features, self.out_features,
+                                              self.image.data_ptr(), _rt.stream_handle(weight.device)), "p2n_int8_pack_weight")
+
+    @property
+    def scale(self) -> torch.Tensor:
+        """(N,) float32, one for each output channel"""
+        n = (self.out_features + 31) // 32 * 32
+        return self.image[-8 * n:].view(torch.float32)[:self.out_features]
+
+    @property
+    def codes(self) -> torch.Tensor:
+        """(N, K) int8, put back in order (a copy)"""
+        ct, kt = (self.out_features + 31) // 32, (self.in_features + 63) // 64 * 2
+        f = self.image[:ct * kt * 1024].view(torch.int8).view(ct, kt, 2, 32, 4, 4)     # tile, tile, half, row, group, j
+        return f.permute(0, 3, 1, 4, 2, 5).reshape(ct * 32, kt * 32)[:self.out_features, :self.in_features].contiguous()
+
+
+def int8_linear(x: torch.Tensor, weight: Int8Weight, relu: bool = False) -> torch.Tensor:
+    """x (..., K) float32 or bfloat16 -> (..., N) of the same type: every token's values and the weight in 8 bits, their
+    product exact in 32-bit integers, scaled, plus the weight's bias, then ReLU if asked."""
+    _gpu(x, "x", _TOKEN_TYPES)
+    _no_grad_wanted("int8_linear", x)
+    T, K, ld, rows = _rows(x)
+    if K != weight.in_features:
+        raise ValueError(f"x has {K} values in a token, the weight takes {weight.in_features}")
+    if x.device != weight.device:
+        raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
+    L = _lib.lib()
+    N = weight.out_features
+    y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    if T == 0:
+        return y
+    # from torch's allocator and not from the stream's shared buffer: a captured graph keeps the memory it was captured with
+    ws = torch.empty(L.p2n_int8_linear_workspace_bytes(T, K, N), dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        _lib.check(L.p2n_int8_linear(rows.data_ptr(), int(x.dtype == torch.bfloat16), T, K, ld, weight.image.data_ptr(), N,
+                                     int(relu), y.data_ptr(), ws.data_ptr(), ws.numel(), _rt.stream_handle(x.device)),
+                   "p2n_int8_linear")
+    return y
+
+
+def int8_mlp(x: torch.Tensor, weights: Sequence[Int8Weight], last_relu: bool = True, group: int = 0) -> torch.Tensor:
+    """x (B, C, L) float32 -> (B, N, L): the products of `weights` one after another over the columns of x, ReLU between them
+    (and behind the last if last_relu); what passes from a layer to the next is put into 8 bits again, one scale a column.
+    group > 0: followed by the maximum over groups of `group` consecutive columns -> (B, N, L // group).
+    1..8 layers, C <= 1024, every layer's N <= 256."""
+    x = _gpu(x, "x", (torch.float32,))
+    _no_grad_wanted("int8_mlp", x)
+    if x.dim() != 3:
+        raise ValueError(f"x must be (B,C,L), got {tuple(x.shape)}")
+    weights = list(weights)
+    if not weights:
+        raise ValueError("int8_mlp needs at least one layer")
+    B, C, L = x.shape
+    dims = [C]
+    for i, w in enumerate(weights):
+        if w.in_features != dims[-1]:
+            raise ValueError(f"layer {i} takes {w.in_features} channels, gets {dims[-1]}")
+        if w.device != x.device:
+            raise ValueError(f"x is on {x.device}, the weight of layer {i} on {w.device}")
+        dims.append(w.out_features)
+    if group < 0 or (group and L % group):
+        raise ValueError(f"columns per cloud ({L}) are not a multiple of the group size ({group})")
+    x = x.contiguous()
+    lib = _lib.lib()
+    # in the kernel: groups of 16 or 32; larger multiples of 32 finish on the maxima of 32, other sizes on the columns
+    inner = 0 if group <= 1 else group if group == 16 else 32 if group % 32 == 0 else 0
+    out = torch.empty((B, dims[-1], L // inner if inner else L), dtype=torch.float32, device=x.device)
+    arr = (ctypes.c_int * len(dims))(*dims)
+    images = (ctypes.c_void_p * len(weights))(*[w.image.data_ptr() for w in weights])
+    with torch.cuda.device(x.device):
+        _lib.check(lib.p2n_int8_mlp(x.data_ptr(), B, L, len(weights), arr, images, int(last_relu), inner, out.data_ptr(),
+                                    _rt.stream_handle(x.device)), "p2n_int8_mlp")
+        rest = group // inner if inner else group
+        if rest > 1:
+            res = torch.empty((B, dims[-1], L // group), dtype=torch.float32, device=x.device)
+            _lib.check(lib.p2n_max_of_columns(out.data_ptr(), res.numel(), rest, res.data_ptr(), _rt.stream_handle(x.device)),
+                       "p2n_max_of_columns")
+            out = res
+    return out

@@ -1,0 +1,336 @@
+"""GPU: products in 8-bit integers (quant.quantize_tokens, int8_linear, int8_mlp) against their definition evaluated in
+64 bits.  Codes are whole numbers and have to be equal; the results differ from the definition's by the roundings that it
+names: three of float32 on the product (conversion of the sum, two scales), one for the bias, so 4 * 2^-24 relative to the
+largest of |product|, |bias| and |result|, and for bfloat16 one more of 2^-8 of the result."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+E32 = 2.0 ** -24
+
+
+def rule64(v, dim):
+    """codes and scales in 64 bits along dim, the scale a float32 number"""
+    v = v.detach().double().cpu()
+    amax = v.abs().amax(dim, keepdim=True)
+    s = (amax / 127).float().double()
+    q = (v / torch.where(s > 0, s, torch.ones_like(s))).round().clamp(-127, 127)
+    bad = ~torch.isfinite(amax)
+    q = torch.where((s > 0) & ~bad, q, torch.zeros_like(q))
+    return q, torch.where(bad, torch.full_like(s, float("nan")), s)
+
+
+def linear64(x, W, b, relu):
+    qx, sx = rule64(x, -1)
+    qw, sw = rule64(W, 1)
+    p = (qx @ qw.t()) * sx * sw.t()
+    y = p if b is None else p + b.double().cpu()
+    size = torch.maximum(p.abs(), y.abs())
+    if b is not None:
+        size = torch.maximum(size, b.double().cpu().abs().expand_as(size))
+    return (y.clamp_min(0) if relu else y), size
+
+
+def check(got, want, size, dtype):
+    got = got.detach().double().cpu()
+    tol = 4 * E32 * size * 1.01
+    if dtype == torch.bfloat16:
+        tol = tol + 2.0 ** -8 * (want.abs() + tol)
+    err = (got - want).abs()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert bool((err[~torch.isnan(want)] <= tol[~torch.isnan(want)]).all()), float((err - tol).nan_to_num().max())
+
+
+def make(T, K, N, dtype=torch.float32, seed=0, bias=True):
+    g = torch.Generator().manual_seed(seed + 1000 * T + 10 * K + N)
+    x = (torch.randn(T, K, generator=g) * (0.2 + torch.rand(T, 1, generator=g))).to(dtype).cuda()
+    W = (torch.randn(N, K, generator=g) / K ** 0.5).cuda()
+    b = (torch.randn(N, generator=g) * 0.3).cuda() if bias else None
+    return x, W, b
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,K", [(1, 1), (1, 64), (3, 6), (33, 131), (128, 512), (5, 1111), (64, 4096)])
+def test_token_codes_are_the_definition(T, K, dtype):
+    from pointcloudsegmentation_amd import quant
+    x, _, _ = make(T, K, 1, dtype)
+    codes, scale = quant.quantize_tokens(x)
+    q, s = rule64(x, 1)
+    assert codes.dtype == torch.int8 and scale.shape == (T,)
+    assert torch.equal(codes.double().cpu(), q)
+    assert torch.equal(scale.double().cpu(), s[:, 0])
+
+
+def test_token_codes_on_and_next_to_ties():
+    """values that sit on a tie, and one float32 step to either side of it, at scales of every size"""
+    from pointcloudsegmentation_amd import quant
+    rows = []
+    g = torch.Generator().manual_seed(5)
+    for e in (-149, -140, -127, -126, -120, -101, -100, -99, -60, -10, -3, 0, 1, 20, 100, 119):
+        for _ in range(8):
+            amax = (1.0 + torch.rand(1, generator=g).item()) * 2.0 ** (e + 7)
+            amax = torch.tensor(amax, dtype=torch.float32)
+            s = (amax.double() / 127).float()
+            ties = (torch.arange(-126, 126).double() + 0.5) * s.double()
+            t = ties.float()
+            row = torch.cat([t, torch.nextafter(t, torch.tensor(float("inf"))), torch.nextafter(t, torch.tensor(-float("inf")))])
+            row = row.clamp(-amax, amax)
+            rows.append(torch.cat([row, amax.reshape(1)]))
+    x = torch.stack(rows)
+    q, s = rule64(x, 1)
+    codes, scale = quant.quantize_tokens(x.cuda())
+    assert torch.equal(scale.double().cpu(), s[:, 0])
+    assert torch.equal(codes.double().cpu(), q)
+    # the same decisions inside the product: weights that single out one value each
+    eye = torch.eye(x.shape[1]).cuda()
+    y = quant.int8_linear(x.cuda(), quant.Int8Weight(eye))
+    want, size = linear64(x, eye, None, False)
+    check(y, want, size + 2.0 ** -126, torch.float32)
+
+
+@pytest.mark.parametrize("N,K", [(1, 1), (7, 6), (32, 32), (33, 64), (256, 131), (100, 1000)])
+def test_weight_codes(N, K):
+    from pointcloudsegmentation_amd import quant
+    _, W, b = make(1, K, N)
+    if N > 2:
+        W[1] = 0
+    w = quant.Int8Weight(W, b)
+    q, s = rule64(W, 1)
+    assert torch.equal(w.codes.double().cpu(), q)
+    assert torch.equal(w.scale.double().cpu(), s[:, 0])
+    c = quant.Int8Weight(W.unsqueeze(2), b)       # Conv1d(kernel_size=1)
+    assert torch.equal(c.image, w.image)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,K,N", [
+    (1, 1, 1), (1, 512, 256), (1, 4096, 100), (2, 6, 64), (16, 64, 16), (17, 4096, 40), (31, 33, 31), (32, 32, 32), (33, 100, 129),
+    (127, 131, 128), (129, 64, 257), (300, 777, 200), (1000, 96, 1000), (2048, 256, 256), (5, 20000, 3), (260, 2048, 520), (4099, 40, 8)])
+def test_linear(T, K, N, dtype):
+    from pointcloudsegmentation_amd import quant
+    relu, bias = (T + N) % 2 == 0, K % 2 == 0
+    x, W, b = make(T, K, N, dtype, bias=bias)
+    y = quant.int8_linear(x, quant.Int8Weight(W, b), relu=relu)
+    assert y.dtype == dtype and y.shape == (T, N)
+    check(y, *linear64(x, W, b, relu), dtype)
+
+
+def test_linear_shapes_and_strides():
+    from pointcloudsegmentation_amd import quant
+    x, W, b = make(60, 40, 24)
+    w = quant.Int8Weight(W, b)
+    want = quant.int8_linear(x, w)
+    assert torch.equal(quant.int8_linear(x.view(3, 4, 5, 40), w), want.view(3, 4, 5, 24))
+    assert torch.equal(quant.int8_linear(x[7], w), want[7])
+    wide = torch.full((60, 77), float("nan"), device="cuda")
+    wide[:, 3:43] = x
+    assert torch.equal(quant.int8_linear(wide[:, 3:43], w), want)                 # rows apart, not 16-byte aligned
+    assert torch.equal(quant.int8_linear(x.t().contiguous().t(), w), want)        # columns first
+    assert torch.equal(quant.int8_linear(x[:1].expand(9, 40), w), want[:1].expand(9, 24))
+    assert torch.equal(quant.int8_linear(x[::2], w), want[::2])
+    assert quant.int8_linear(x[:0], w).shape == (0, 24)
+    assert quant.int8_linear(x.new_empty(2, 0, 40), w).shape == (2, 0, 24)
+    xb = x.bfloat16()
+    wideb = torch.full((60, 77), float("nan"), device="cuda", dtype=torch.bfloat16)
+    wideb[:, 3:43] = xb
+    assert torch.equal(quant.int8_linear(wideb[:, 3:43], w), quant.int8_linear(xb, w))
+
+
+def test_linear_zero_and_nonfinite_tokens():
+    """a token of zeros gives the bias; a NaN or an infinity spoils its own row and no other; so with the weight's rows"""
+    from pointcloudsegmentation_amd import quant
+    for T in (6, 200):
+        x, W, b = make(T, 70, 40)
+        w = quant.Int8Weight(W, b)
+        clean = quant.int8_linear(x, w)
+        x[0] = 0
+        x[1, 5] = float("nan")
+        x[2, 69] = float("inf")
+        x[3, 0] = -float("inf")
+        y = quant.int8_linear(x, w)
+        assert torch.equal(y[0], b)
+        assert bool(torch.isnan(y[1:4]).all())
+        assert torch.equal(y[4:], clean[4:])
+        codes, scale = quant.quantize_tokens(x)
+        assert bool((codes[:4] == 0).all()) and bool(torch.isnan(scale[1:4]).all()) and scale[0] == 0
+        yr = quant.int8_linear(x, w, relu=True)
+        assert bool(torch.isnan(yr[1:4]).all())
+        W2 = W.clone()
+        W2[7, 3] = float("nan")
+        y2 = quant.int8_linear(x, quant.Int8Weight(W2, b))
+        assert bool(torch.isnan(y2[:, 7]).all())
+        keep = torch.arange(40, device="cuda") != 7
+        assert torch.equal(y2[4:][:, keep], clean[4:][:, keep])
+
+
+def test_linear_captured_graphs_keep_their_own_memory():
+    from pointcloudsegmentation_amd import quant
+    sizes = [(64, 128, 96), (3, 1000, 40)]
+    graphs, data = [], []
+    for T, K, N in sizes:
+        x, W, b = make(T, K, N)
+        w = quant.Int8Weight(W, b)
+        quant.int8_linear(x, w)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = quant.int8_linear(x, w)
+        graphs.append(g)
+        data.append((x, w, y))
+    for rep in range(4):
+        for (x, w, y), g in zip(data, graphs):
+            x.normal_()
+            g.replay()
+        quant.int8_linear(torch.randn(700, 300, device="cuda"), quant.Int8Weight(torch.randn(64, 300, device="cuda")))
+        torch.cuda.synchronize()
+        for x, w, y in data:
+            assert torch.equal(y, quant.int8_linear(x, w))
+
+
+def test_linear_on_another_stream():
+    from pointcloudsegmentation_amd import quant
+    x, W, b = make(500, 300, 200)
+    w = quant.Int8Weight(W, b)
+    want = quant.int8_linear(x, w)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = quant.int8_linear(x, w)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
+
+
+# ---------------------------------------------------------------- shared MLP
+def mlp_by_layers(x, layers, last_relu, group):
+    """the chain with its float32 steps one by one (sums exact in float64), which its definition fixes bit by bit"""
+    h = x.detach().float().cpu()
+    for i, (W, b) in enumerate(layers):
+        q, s = rule64(h, 1)
+        qw, sw = rule64(W, 1)
+        acc = torch.matmul(qw, q).float()
+        h = acc * sw.float() * s.float()
+        if b is not None:
+            h = h + b.cpu()[:, None]
+        if i + 1 < len(layers) or last_relu:
+            h = torch.where(h <= 0, torch.zeros_like(h), h)
+    if group:
+        h = h.view(h.shape[0], h.shape[1], -1, group).amax(3)
+    return h
+
+
+def make_mlp(B, L, dims, seed=0):
+    g = torch.Generator().manual_seed(seed + sum(dims) + L)
+    x = (torch.randn(B, dims[0], L, generator=g) * (0.3 + torch.rand(B, 1, L, generator=g))).cuda()
+    layers = [((torch.randn(n, k, generator=g) * (2.0 / k) ** 0.5).cuda(), (torch.randn(n, generator=g) * 0.1).cuda())
+              for k, n in zip(dims, dims[1:])]
+    return x, layers
+
+
+@pytest.mark.parametrize("B,L,dims,last_relu,group", [
+    (1, 1, [1, 1], True, 0), (2, 5, [6, 7], False, 0), (1, 32, [32, 32, 32], True, 0), (3, 33, [6, 32, 32, 64], True, 0),
+    (2, 300, [131, 128, 128, 256], True, 0), (1, 515, [384, 256, 256], True, 0), (2, 100, [67, 64, 64, 128], False, 0),
+    (1, 70, [1024, 256, 40], False, 0), (1, 64, [600, 100, 256], True, 0), (2, 64, [500, 33], False, 0), (1, 130, [128, 128, 64], False, 0),
+    (2, 40, [3, 16, 16, 16, 16, 16, 16, 16, 9], True, 0), (4, 31, [200, 20, 250, 30], False, 0), (2, 96, [250, 60, 33], False, 0),
+    (2, 96, [6, 32, 64], True, 32), (3, 48, [6, 32, 64], True, 16), (1, 16, [9, 5], False, 16), (2, 128, [67, 64, 128], True, 64),
+    (2, 72, [6, 32, 40], False, 24), (1, 64, [131, 128, 256], False, 32), (2, 40, [6, 32, 64], True, 8), (1, 7, [6, 9], True, 1)])
+def test_mlp_equals_its_steps(B, L, dims, last_relu, group):
+    """every step of the chain is fixed, so the result is equal bit by bit"""
+    from pointcloudsegmentation_amd import quant
+    x, layers = make_mlp(B, L, dims)
+    y = quant.int8_mlp(x, [quant.Int8Weight(W, b) for W, b in layers], last_relu=last_relu, group=group)
+    want = mlp_by_layers(x, layers, last_relu, group)
+    assert y.shape == want.shape
+    assert torch.equal(y.cpu(), want), float((y.cpu() - want).abs().max())
+
+
+def test_mlp_single_layer_is_the_linear_product():
+    from pointcloudsegmentation_amd import quant
+    x, layers = make_mlp(2, 77, [100, 60])
+    w = quant.Int8Weight(*layers[0])
+    a = quant.int8_mlp(x, [w], last_relu=True)
+    b = quant.int8_linear(x.transpose(1, 2), w, relu=True).transpose(1, 2)
+    assert torch.equal(a, b)
+
+
+def test_mlp_nonfinite_columns_stay_apart():
+    from pointcloudsegmentation_amd import quant
+    x, layers = make_mlp(2, 64, [40, 64, 64])
+    ws = [quant.Int8Weight(W, b) for W, b in layers]
+    clean = quant.int8_mlp(x, ws)
+    cleang = quant.int8_mlp(x, ws, group=32)
+    x[0, 3, 10] = float("nan")
+    x[1, 0, 40] = float("inf")
+    x[1, :, 7] = 0
+    y = quant.int8_mlp(x, ws)
+    assert bool(torch.isnan(y[0, :, 10]).all()) and bool(torch.isnan(y[1, :, 40]).all())
+    keep = torch.ones(2, 64, dtype=torch.bool)
+    keep[0, 10] = keep[1, 40] = keep[1, 7] = False
+    assert torch.equal(y.transpose(1, 2)[keep], clean.transpose(1, 2)[keep])
+    assert torch.equal(y[:, :, 7][1].cpu(), mlp_by_layers(x[1:, :, 7:8], layers, True, 0)[0, :, 0])
+    for group in (32, 16, 64, 8):
+        yg = quant.int8_mlp(x, ws, group=group)
+        assert torch.equal(torch.isnan(yg).cpu(), torch.isnan(y.view(2, 64, -1, group)).any(3).cpu())
+    yg = quant.int8_mlp(x, ws, group=32)
+    assert torch.equal(yg[0, :, 1], cleang[0, :, 1])
+    # negative results: the maximum of a group below zero
+    W = -torch.ones(8, 40, device="cuda")
+    xp = torch.rand(1, 40, 64, device="cuda") + 0.1
+    yn = quant.int8_mlp(xp, [quant.Int8Weight(W)], last_relu=False)
+    assert bool((yn < 0).all())
+    assert torch.equal(quant.int8_mlp(xp, [quant.Int8Weight(W)], last_relu=False, group=16), yn.view(1, 8, 4, 16).amax(3))
+
+
+def test_mlp_leaves_memory_behind_its_result():
+    """channels and columns that fill no tile: nothing is written past the result's end"""
+    from pointcloudsegmentation_amd import _lib, quant, runtime as rt
+    import ctypes
+    x, layers = make_mlp(2, 45, [37, 40, 33])
+    ws = [quant.Int8Weight(W, b) for W, b in layers]
+    want = quant.int8_mlp(x, ws)
+    guard = torch.full((2 * 33 * 45 + 4096,), 7.0, device="cuda")
+    images = (ctypes.c_void_p * 2)(*[w.image.data_ptr() for w in ws])
+    _lib.check(_lib.lib().p2n_int8_mlp(x.data_ptr(), 2, 45, 2, (ctypes.c_int * 3)(37, 40, 33), images, 1, 0, guard.data_ptr(),
+                                       rt.stream_handle(x.device)), "p2n_int8_mlp")
+    assert torch.equal(guard[:2 * 33 * 45].view(2, 33, 45), want)
+    assert bool((guard[2 * 33 * 45:] == 7.0).all())
+
+
+# ---------------------------------------------------------------- refusals
+def test_refusals():
+    from pointcloudsegmentation_amd import quant
+    x, W, b = make(4, 16, 8)
+    w = quant.Int8Weight(W, b)
+    with pytest.raises(TypeError):
+        quant.int8_linear(x.half(), w)
+    with pytest.raises(ValueError):
+        quant.int8_linear(x.cpu(), w)
+    with pytest.raises(ValueError):
+        quant.int8_linear(x[:, :15], w)
+    with pytest.raises(ValueError):
+        quant.int8_linear(x.new_empty(4, 0), w)
+    with pytest.raises(RuntimeError):
+        quant.int8_linear(x.clone().requires_grad_(), w)
+    with pytest.raises(ValueError):
+        quant.Int8Weight(W.cpu())
+    with pytest.raises(TypeError):
+        quant.Int8Weight(W.bfloat16())
+    with pytest.raises(ValueError):
+        quant.Int8Weight(W, b[:3])
+    with pytest.raises(ValueError):
+        quant.Int8Weight(W[0])
+    m = torch.randn(2, 16, 30, device="cuda")
+    with pytest.raises(ValueError):
+        quant.int8_mlp(m, [])
+    with pytest.raises(ValueError):
+        quant.int8_mlp(m[0], [w])
+    with pytest.raises(ValueError):
+        quant.int8_mlp(m, [w, w])
+    with pytest.raises(ValueError):
+        quant.int8_mlp(m, [w], group=16)
+    with pytest.raises(TypeError):
+        quant.int8_mlp(m.bfloat16(), [w])
+    with pytest.raises(ValueError):
+        quant.int8_mlp(m, [quant.Int8Weight(torch.randn(300, 16, device="cuda"))])
+    with pytest.raises(ValueError):
+        quant.int8_mlp(torch.randn(1, 1025, 4, device="cuda"), [quant.Int8Weight(torch.randn(3, 1025, device="cuda"))])
