@@ -411,11 +411,39 @@ int p2n_int8_mlp(const float *x, int B, long L, int nl, const int *dims, const v
 /* out[r] = max of in[r*ns .. r*ns + ns-1], a NaN is the maximum */
 int p2n_max_of_columns(const float *in, long rows, int ns, float *out, void *stream);
 
+/* ---- training layers that keep their input in 8 bits (no counterpart in the reference) --
+ * h = W . a + bias over x (B,K,L), W (N,K), h (B,N,L); a = relu(norm(x)) with gamma and beta (BatchNorm over the B*L points of
+ * a channel: biased variance, u = (x - mu) * r, y = gamma*u + beta), a = x with gamma = beta = NULL.  `kept` receives what the
+ * backward pass needs instead of x: the codes of u (of x) by the 8-bit rule above, one scale for 128 consecutive points of a
+ * row, the bits [y > 0], mu and r -- 1.16 bytes a value.  running_mean / running_var (both or NULL) are updated in place with
+ * `momentum` (unbiased variance); momentum < 0: the running statistics are used and left as they are (`frozen` in the
+ * backward pass).  Backward, with uh and ah the values that the codes stand for:
+ *   dW = g . ah^T, db = sum g, dy = [y > 0] * (W^T . g), dbeta = sum dy, dgamma = sum dy*uh,
+ *   dx = gamma*r*(dy - dbeta/P - uh*dgamma/P), P = B*L   (frozen: gamma*r*dy; without a norm: W^T . g)
+ * dW and db may be NULL (not computed), and dx without a norm; with a norm dgamma and dbeta need dx.  Limits: 1..1024
+ * channels, L <= 2^24.  kept and workspace 256-byte aligned; the workspace holds nothing between calls. */
+size_t p2n_act8_kept_bytes(int B, int C, long L, int norm);
+size_t p2n_act8_workspace_bytes(int B, int K, long L, int N);      /* N = 0: the norm + ReLU calls */
+int p2n_act8_forward(const float *x, int B, int K, long L, const float *W, const float *bias, int N,
+                     const float *gamma, const float *beta, float *running_mean, float *running_var, float momentum, float eps,
+                     float *h, void *kept, size_t kept_bytes, void *workspace, size_t workspace_bytes, void *stream);
+int p2n_act8_backward(const float *g, int B, int K, long L, const float *W, int N, const float *gamma, const float *beta,
+                      int frozen, const void *kept, size_t kept_bytes, float *dx, float *dW, float *db, float *dgamma,
+                      float *dbeta, void *workspace, size_t workspace_bytes, void *stream);
+/* the norm and ReLU alone: out = relu(norm(x)), the end of a chain */
+int p2n_act8_norm_relu_forward(const float *x, int B, int C, long L, const float *gamma, const float *beta,
+                               float *running_mean, float *running_var, float momentum, float eps, float *out,
+                               void *kept, size_t kept_bytes, void *workspace, size_t workspace_bytes, void *stream);
+int p2n_act8_norm_relu_backward(const float *g, int B, int C, long L, const float *gamma, int frozen, const void *kept,
+                                size_t kept_bytes, float *dx, float *dgamma, float *dbeta, void *workspace,
+                                size_t workspace_bytes, void *stream);
+
 /* ---- measurement aid (no counterpart in the reference) ---------------------
  * While enabled, every kernel launch is bracketed by HIP events on its stream.
  * p2n_profile_collect synchronises and fills, per kernel id (0 encoder, 1 mid,
  * 2 head, 3 fps, 5 knn, 10 cluster prep, 11 cluster count pass, 12 cluster link pass,
- * 20 int8 weight image, 21 token codes, 22 int8 product, 23 int8 shared MLP), the summed milliseconds and the number of launches since
+ * 20 int8 weight image, 21 token codes, 22 int8 product, 23 int8 shared MLP, 24 / 25 forward / backward
+ * of the 8-bit-checkpoint layers), the summed milliseconds and the number of launches since
  * the last collect.  HOST pointers.  Not thread-safe; off by default. */
 int p2n_profile_enable(int on);
 /* kernel_id >= 0: only that kernel's launches are bracketed (two event records per step instead of

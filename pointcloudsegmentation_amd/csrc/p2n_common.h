@@ -139,6 +139,8 @@ __device__ __forceinline__ float p2n_tile_half_max(const f32x16 v, int lane) {
 #define P2N_K_INT8_TOKENS 21
 #define P2N_K_INT8_GEMM 22
 #define P2N_K_INT8_MLP 23
+#define P2N_K_ACT8_FWD 24
+#define P2N_K_ACT8_BWD 25
 #define P2N_K_COUNT 32
 int p2n_prof_begin(int kernel_id, hipStream_t s);
 void p2n_prof_end(int slot, hipStream_t s);

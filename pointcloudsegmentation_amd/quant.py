@@ -10,6 +10,9 @@ q = 0; a NaN or an infinity among the v makes s NaN, and with it every result th
   Int8Weight        a weight matrix (and bias) put into 8 bits once, laid out for the matrix cores
   int8_linear       y = x W^T + b over rows of float32 or bfloat16, from one token to many
   int8_mlp          the layers of a shared MLP over (B, C, L), activations on chip; `SharedMLP.precision = "int8"` runs it
+  act8_linear       W relu(norm(x)) + b (or W x + b) over (B, C, L), differentiable, its input kept in 8 bits
+  act8_norm_relu    relu(norm(x)), differentiable, its input kept in 8 bits
+                    `SharedMLP.checkpoint = "int8"` trains on these two
 
 All functions take GPU tensors only and queue their work on the current stream of the tensors' device; nothing synchronises.
 """
@@ -17,6 +20,7 @@ import ctypes
 from typing import Optional, Sequence
 
 import torch
+import torch.nn as nn
 
 from . import _lib
 from . import runtime as _rt
@@ -169,3 +173,162 @@ def int8_mlp(x: torch.Tensor, weights: Sequence[Int8Weight], last_relu: bool = T
                        "p2n_max_of_columns")
             out = res
     return out
+
+
+# ------------------------------------------------------------------ activation checkpoints in 8 bits
+def _norm_args(norm: Optional[nn.BatchNorm1d], x: torch.Tensor):
+    """gamma, beta, running mean, running variance, momentum (< 0: running statistics used as they are), eps of a BatchNorm1d"""
+    if norm is None:
+        return None, None, None, None, 0.0, 0.0
+    if not isinstance(norm, nn.BatchNorm1d):
+        raise TypeError(f"norm must be a BatchNorm1d or None, got {type(norm).__name__}")
+    if not norm.affine:
+        raise NotImplementedError("the 8-bit checkpoint layers need BatchNorm1d(affine=True)")
+    if norm.num_features != x.size(1):
+        raise ValueError(f"norm has {norm.num_features} channels, x has {x.size(1)}")
+    for t, name in ((norm.weight, "norm.weight"), (norm.bias, "norm.bias"), (norm.running_mean, "norm.running_mean"),
+                    (norm.running_var, "norm.running_var")):
+        if t is not None and not (t.device == x.device and t.dtype == torch.float32 and t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous float32 tensor on the input's GPU")
+    frozen = not norm.training and norm.running_mean is not None
+    if not frozen and x.size(0) * x.size(2) < 2:
+        raise ValueError(f"Expected more than 1 value per channel when training, got input size {tuple(x.shape)}")
+    if frozen:
+        momentum = -1.0
+    elif norm.training and norm.running_mean is not None:
+        if norm.momentum is None:
+            raise NotImplementedError("BatchNorm1d(momentum=None) (cumulative average) is not implemented on the GPU path")
+        momentum = norm.momentum
+    else:
+        momentum = 0.0
+    tracked = frozen or (norm.training and norm.running_mean is not None)
+    return norm.weight, norm.bias, norm.running_mean if tracked else None, norm.running_var if tracked else None, momentum, norm.eps
+
+
+def _count_batch(norm: Optional[nn.BatchNorm1d]) -> None:
+    if norm is not None and norm.training and norm.num_batches_tracked is not None:
+        with torch.no_grad():
+            norm.num_batches_tracked += 1
+
+
+def _bytes(n: int, device) -> torch.Tensor:
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+class _Act8Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, gamma, beta, running_mean, running_var, momentum, eps):
+        L_ = _lib.lib()
+        B, K, L = x.shape
+        N = weight.size(0)
+        dev = x.device
+        normed = gamma is not None
+        nkept, nws = L_.p2n_act8_kept_bytes(B, K, L, int(normed)), L_.p2n_act8_workspace_bytes(B, K, L, N)
+        if nkept == 0 or nws == 0:
+            raise ValueError("act8_linear: " + L_.p2n_last_error().decode(errors="replace"))
+        kept, ws = _bytes(nkept, dev), _bytes(nws, dev)
+        h = torch.empty((B, N, L), dtype=torch.float32, device=dev)
+        with torch.cuda.device(dev):
+            _lib.check(L_.p2n_act8_forward(x.data_ptr(), B, K, L, weight.data_ptr(), _rt.ptr(bias), N, _rt.ptr(gamma), _rt.ptr(beta),
+                                           _rt.ptr(running_mean), _rt.ptr(running_var), momentum, eps, h.data_ptr(), kept.data_ptr(),
+                                           nkept, ws.data_ptr(), nws, _rt.stream_handle(dev)), "p2n_act8_forward")
+        ctx.save_for_backward(kept, weight, gamma, beta)
+        ctx.meta = (B, K, L, N, normed and momentum < 0, bias is not None)
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        kept, weight, gamma, beta = ctx.saved_tensors
+        B, K, L, N, frozen, has_bias = ctx.meta
+        L_ = _lib.lib()
+        g = g.contiguous()
+        dev = g.device
+        need = ctx.needs_input_grad
+
+        def out(wanted, *shape):
+            return torch.empty(shape, dtype=torch.float32, device=dev) if wanted else None
+
+        normed = gamma is not None
+        dgamma, dbeta = out(normed and need[3], K), out(normed and need[4], K)
+        dx = out(need[0] or dgamma is not None or dbeta is not None, B, K, L)     # the norm's gradients are formed on its way
+        dW, db = out(need[1], N, K), out(has_bias and need[2], N)
+        ws = _bytes(L_.p2n_act8_workspace_bytes(B, K, L, N), dev)
+        with torch.cuda.device(dev):
+            _lib.check(L_.p2n_act8_backward(g.data_ptr(), B, K, L, weight.data_ptr(), N, _rt.ptr(gamma), _rt.ptr(beta), int(frozen),
+                                            kept.data_ptr(), kept.numel(), _rt.ptr(dx), _rt.ptr(dW), _rt.ptr(db), _rt.ptr(dgamma),
+                                            _rt.ptr(dbeta), ws.data_ptr(), ws.numel(), _rt.stream_handle(dev)), "p2n_act8_backward")
+        return dx if need[0] else None, dW, db, dgamma, dbeta, None, None, None, None
+
+
+def act8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                norm: Optional[nn.BatchNorm1d] = None) -> torch.Tensor:
+    """x (B, K, L) float32 -> W relu(norm(x)) + b, or W x + b without a norm: (B, N, L), differentiable in x, weight (N, K) or
+    (N, K, 1), bias and the norm's parameters.  The output is computed from the float32 values; for the backward pass the
+    normalised input (the input itself without a norm) is kept in 8 bits, one scale for 128 consecutive points of a channel,
+    with one bit for each of the ReLU's decisions: 1.16 bytes a value instead of 4.  norm.training decides between the
+    batch's statistics (running statistics updated, as BatchNorm1d does) and the running ones.  1..1024 channels."""
+    x = _gpu(x, "x", (torch.float32,))
+    if x.dim() != 3 or 0 in x.shape:
+        raise ValueError(f"x must be (B,K,L) with at least one value, got {tuple(x.shape)}")
+    w = weight.squeeze(2) if weight.dim() == 3 and weight.size(2) == 1 else weight
+    if w.dim() != 2 or w.size(1) != x.size(1):
+        raise ValueError(f"weight must be (N,{x.size(1)}) or (N,{x.size(1)},1), got {tuple(weight.shape)}")
+    if bias is not None and bias.shape != (w.size(0),):
+        raise ValueError(f"bias must be ({w.size(0)},), got {tuple(bias.shape)}")
+    for t, name in ((w, "weight"), (bias, "bias")):
+        if t is not None and not (t.device == x.device and t.dtype == torch.float32):
+            raise ValueError(f"{name} must be a float32 tensor on the input's GPU")
+    h = _Act8Linear.apply(x.contiguous(), w.contiguous(), None if bias is None else bias.contiguous(), *_norm_args(norm, x))
+    _count_batch(norm)
+    return h
+
+
+class _Act8NormRelu(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gamma, beta, running_mean, running_var, momentum, eps):
+        L_ = _lib.lib()
+        B, C, L = x.shape
+        dev = x.device
+        nkept, nws = L_.p2n_act8_kept_bytes(B, C, L, 1), L_.p2n_act8_workspace_bytes(B, C, L, 0)
+        if nkept == 0 or nws == 0:
+            raise ValueError("act8_norm_relu: " + L_.p2n_last_error().decode(errors="replace"))
+        kept, ws = _bytes(nkept, dev), _bytes(nws, dev)
+        y = torch.empty((B, C, L), dtype=torch.float32, device=dev)
+        with torch.cuda.device(dev):
+            _lib.check(L_.p2n_act8_norm_relu_forward(x.data_ptr(), B, C, L, gamma.data_ptr(), beta.data_ptr(), _rt.ptr(running_mean),
+                                                     _rt.ptr(running_var), momentum, eps, y.data_ptr(), kept.data_ptr(), nkept,
+                                                     ws.data_ptr(), nws, _rt.stream_handle(dev)), "p2n_act8_norm_relu_forward")
+        ctx.save_for_backward(kept, gamma)
+        ctx.meta = (B, C, L, momentum < 0)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        kept, gamma = ctx.saved_tensors
+        B, C, L, frozen = ctx.meta
+        L_ = _lib.lib()
+        g = g.contiguous()
+        dev = g.device
+        dx = torch.empty((B, C, L), dtype=torch.float32, device=dev)
+        dgamma, dbeta = (torch.empty(C, dtype=torch.float32, device=dev) if ctx.needs_input_grad[i] else None for i in (1, 2))
+        ws = _bytes(L_.p2n_act8_workspace_bytes(B, C, L, 0), dev)
+        with torch.cuda.device(dev):
+            _lib.check(L_.p2n_act8_norm_relu_backward(g.data_ptr(), B, C, L, gamma.data_ptr(), int(frozen), kept.data_ptr(), kept.numel(),
+                                                      dx.data_ptr(), _rt.ptr(dgamma), _rt.ptr(dbeta), ws.data_ptr(), ws.numel(),
+                                                      _rt.stream_handle(dev)), "p2n_act8_norm_relu_backward")
+        return dx, dgamma, dbeta, None, None, None, None
+
+
+def act8_norm_relu(x: torch.Tensor, norm: nn.BatchNorm1d) -> torch.Tensor:
+    """x (B, C, L) float32 -> relu(norm(x)), differentiable in x and the norm's parameters; what the backward pass needs of x is
+    kept in 8 bits and the ReLU's decisions as bits, as in act8_linear."""
+    x = _gpu(x, "x", (torch.float32,))
+    if x.dim() != 3 or 0 in x.shape:
+        raise ValueError(f"x must be (B,C,L) with at least one value, got {tuple(x.shape)}")
+    if norm is None:
+        raise TypeError("norm must be a BatchNorm1d, got None")
+    y = _Act8NormRelu.apply(x.contiguous(), *_norm_args(norm, x))
+    _count_batch(norm)
+    return y
