@@ -82,6 +82,7 @@ class PointNet2Encoder(nn.Module):
         self.mlp3 = _mlp(128, 256, 256)
         self.in_channels = in_channels
         self.precision = DEFAULT_PRECISION   # "fp32" | "fp32x3" | "bf16" (GPU tensors only)
+        self.checkpoint = None               # "int8": training keeps its activations in 8 bits (GPU tensors only)
         self._cache = _PackedCache()
 
     def forward(self, x):
@@ -120,6 +121,18 @@ class Point2Net(nn.Module):
         # "bf16" (bf16 operands, 2e-2 parity).  Plain attribute: not part of the state_dict.
         self.precision = DEFAULT_PRECISION
         self._cache = _PackedCache()
+
+    # Not in the reference: what training on GPU tensors keeps of the activations -- None (float32, as the reference) or
+    # "int8" (quant.act8_linear: 1.16 bytes a value, gradients from the kept values; the products stay float32-accurate)
+    @property
+    def checkpoint(self):
+        return self.encoder.checkpoint
+
+    @checkpoint.setter
+    def checkpoint(self, value):
+        if value not in (None, "int8"):
+            raise ValueError(f"checkpoint must be None or 'int8', got {value!r}")
+        self.encoder.checkpoint = value
 
     # ---- GPU paths -----------------------------------------------------
     def _needs_grad(self, x):

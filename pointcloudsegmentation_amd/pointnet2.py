@@ -24,6 +24,7 @@ import torch.nn as nn
 
 from . import _lib
 from . import ops
+from . import quant
 from . import runtime as _rt
 
 
@@ -269,12 +270,78 @@ class _SharedMLPTrainFn(torch.autograd.Function):
         return (dx, None, None, None, None, None, *grads)
 
 
-def shared_mlp_train(net: nn.Sequential, x: torch.Tensor, group: int = 0, eval_stats: bool = False) -> torch.Tensor:
+class _GroupMax(torch.autograd.Function):
+    """(B,C,G*ns) -> (B,C,G): the maximum of each group of ns consecutive columns; keeps one byte a group (its position)"""
+
+    @staticmethod
+    def forward(ctx, y, ns):
+        L_ = _lib.lib()
+        B, C, L = y.shape
+        out = torch.empty((B, C, L // ns), dtype=torch.float32, device=y.device)
+        arg = torch.empty((B, C, L // ns), dtype=torch.uint8, device=y.device)
+        with torch.cuda.device(y.device):
+            for r0, n in _row_blocks(B * C):
+                _lib.check(L_.p2n_group_max_cm(y.data_ptr() + 4 * r0 * L, n, L, L // ns, ns, out.data_ptr() + 4 * r0 * (L // ns),
+                                               arg.data_ptr() + r0 * (L // ns), _rt.stream_handle(y.device)), "p2n_group_max_cm")
+        ctx.save_for_backward(arg)
+        ctx.ns = ns
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        arg, = ctx.saved_tensors
+        g = g.contiguous()
+        B, C, G = g.shape
+        L = G * ctx.ns
+        dy = torch.empty((B, C, L), dtype=torch.float32, device=g.device)
+        with torch.cuda.device(g.device):
+            for r0, n in _row_blocks(B * C):
+                _lib.check(_lib.lib().p2n_group_max_cm_bwd(g.data_ptr() + 4 * r0 * G, arg.data_ptr() + r0 * G, n, G, ctx.ns, L,
+                                                           dy.data_ptr() + 4 * r0 * L, _rt.stream_handle(g.device)), "p2n_group_max_cm_bwd")
+        return dy, None
+
+
+def _row_blocks(rows: int):
+    """the kernels take up to 65,535 rows a launch"""
+    return [(r0, min(65535, rows - r0)) for r0 in range(0, rows, 65535)]
+
+
+CHECKPOINTS = (None, "int8")
+
+
+def _shared_mlp_act8(mods: List[nn.Module], x: torch.Tensor, group: int) -> torch.Tensor:
+    """the layers of a shared MLP with their inputs kept in 8 bits: conv, (norm, ReLU, conv)*, and norm, ReLU at the end of a
+    chain whose last layer is not plain.  Every BatchNorm1d goes by its own training flag."""
+    y = quant.act8_linear(x, mods[0].weight, mods[0].bias)
+    i = 1
+    while i < len(mods):                                    # mods[i], mods[i+1]: norm, ReLU
+        if i + 2 < len(mods):
+            y = quant.act8_linear(y, mods[i + 2].weight, mods[i + 2].bias, norm=mods[i])
+        else:
+            y = quant.act8_norm_relu(y, mods[i])
+        i += 3
+    if not group:
+        return y
+    B, C, L = y.shape
+    if L % group:
+        raise ValueError(f"columns per cloud ({L}) are not a multiple of the group size ({group})")
+    if L % 4 == 0 and group <= 255:
+        return _GroupMax.apply(y, group)
+    return y.view(B, C, L // group, group).max(dim=3).values
+
+
+def shared_mlp_train(net: nn.Sequential, x: torch.Tensor, group: int = 0, eval_stats: bool = False,
+                     checkpoint: Optional[str] = None) -> torch.Tensor:
     """Train-mode forward, with autograd, of nn.Sequential(Conv1d(k=1), BatchNorm1d, ReLU, ... [, Conv1d(k=1)]) on a
     GPU tensor (B,C,L) through p2n_mlp_train_forward / p2n_mlp_train_backward; BatchNorm buffers are updated as
     nn.BatchNorm1d does in train() mode.  group > 0: followed by the maximum over groups of `group` consecutive
     columns -> (B, Cout, L // group), i.e. net(x).view(B, Cout, L // group, group).max(dim=3).values.
-    eval_stats: eval-mode BatchNorm under autograd -- running statistics used, nothing updated."""
+    eval_stats: eval-mode BatchNorm under autograd -- running statistics used, nothing updated.
+    checkpoint = "int8": what the backward pass needs of the activations is kept in 8 bits (quant.act8_linear): 1.16 bytes a
+    value instead of 4, the output as before, the gradients those of the kept values."""
+    if checkpoint not in CHECKPOINTS:
+        raise ValueError(f"checkpoint must be one of {CHECKPOINTS}, got {checkpoint!r}")
     mods, i = list(net), 0
     if not mods or not isinstance(mods[0], nn.Conv1d):
         raise NotImplementedError("a shared MLP starts with a Conv1d")
@@ -303,6 +370,8 @@ def shared_mlp_train(net: nn.Sequential, x: torch.Tensor, group: int = 0, eval_s
             last_plain = True
             buffers += [None, None]
             i += 1
+    if checkpoint == "int8":
+        return _shared_mlp_act8(mods, _rt.require_cuda_f32(x, "x"), int(group))
     if eval_stats:
         return _SharedMLPTrainFn.apply(x, tuple(dims), last_plain, -1.0, tuple(buffers), int(group), *params)
     if len({bn.momentum for bn in bns}) > 1:
@@ -328,6 +397,11 @@ class SharedMLP(nn.Module):
             if not plain:
                 layers += [nn.BatchNorm1d(channels[i + 1]), nn.ReLU()]
         self.net = nn.Sequential(*layers)
+        # GPU tensors only, plain attributes (not part of the state_dict).  precision "int8": eval products in 8-bit integers
+        # (quant.int8_mlp).  checkpoint "int8": training keeps its activations in 8 bits (quant.act8_linear).
+        self.precision = "fp32"
+        self.checkpoint = None
+        self._int8 = (None, None)
 
     def _folded(self):
         out, mods, i = [], list(self.net), 0
@@ -348,7 +422,21 @@ class SharedMLP(nn.Module):
 
     def _forward_train(self, x, group: int = 0):
         """with autograd: batch statistics in train() mode, the running statistics (left untouched) in eval() mode"""
-        return shared_mlp_train(self.net, x, group, eval_stats=not self.training)
+        return shared_mlp_train(self.net, x, group, eval_stats=not self.training, checkpoint=self.checkpoint)
+
+    def int8_weights(self):
+        """[(Int8Weight of the layer, BatchNorm folded in)], last layer has a ReLU; rebuilt only when a parameter or buffer changed"""
+        tensors = [t for m in self.net for t in list(m.parameters()) + list(m.buffers())]
+        key = tuple((t.data_ptr(), t._version) for t in tensors)      # num_batches_tracked stands in for the running statistics
+        if key != self._int8[0]:
+            folded = self._folded()
+            self._int8 = (key, ([quant.Int8Weight(w * s[:, None], t) for w, s, t, _ in folded], bool(folded[-1][3])))
+        return self._int8[1]
+
+    def forward_int8(self, x, group: int = 0):
+        """eval forward in 8-bit integers: (B,C,L) -> (B,Cout,L), or with group the maximum over groups of columns"""
+        weights, last_relu = self.int8_weights()
+        return quant.int8_mlp(x, weights, last_relu=last_relu, group=group)
 
     def needs_autograd(self, x) -> bool:
         return torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters()))
@@ -358,6 +446,10 @@ class SharedMLP(nn.Module):
             return self.net(x)
         if self.training or self.needs_autograd(x):
             return self._forward_train(x)
+        if self.precision not in ("fp32", "int8"):
+            raise ValueError(f"precision must be 'fp32' or 'int8', got {self.precision!r}")
+        if self.precision == "int8":
+            return self.forward_int8(x)
         L = _lib.lib()
         x = _rt.require_cuda_f32(x, "x")
         B, _, n = x.shape
@@ -437,6 +529,8 @@ class SetAbstraction(nn.Module):
             with torch.cuda.device(xyz.device):
                 _lib.check(L.p2n_sa_group(xyz.data_ptr(), new_xyz.data_ptr(), _rt.ptr(feat), gidx.data_ptr(), B, C, N, M,
                                           ns, grouped.data_ptr(), _rt.stream_handle(xyz.device)), "p2n_sa_group")
+            if self.mlp.precision == "int8" and not self.training:
+                return new_xyz, self.mlp.forward_int8(grouped.view(B, C + 3, M * ns), group=ns)   # MLP + max over the group
             y = self.mlp(grouped.view(B, C + 3, M * ns))
             out = torch.empty((B, y.size(1), M), dtype=torch.float32, device=xyz.device)
             with torch.cuda.device(xyz.device):
@@ -521,6 +615,38 @@ class Point2NetSA(nn.Module):
         self.fp1 = FeaturePropagation(128 + c, [128, 128])
         self.head = SharedMLP([128, 128, embedding_dim], last_plain=True)
 
+    def _mlps(self):
+        return [m.mlp for m in (self.sa1, self.sa2, self.sa3, self.fp3, self.fp2, self.fp1)] + [self.head]
+
+    def _uniform(self, name):
+        values = {getattr(m, name) for m in self._mlps()}
+        return values.pop() if len(values) == 1 else "mixed"
+
+    @property
+    def precision(self):
+        """eval precision of the shared MLPs: "fp32" (the fused levels) or "int8" (products in 8-bit integers, level by
+        level; groups and channels as quant.int8_mlp takes them)"""
+        return self._uniform("precision")
+
+    @precision.setter
+    def precision(self, value):
+        if value not in ("fp32", "int8"):
+            raise ValueError(f"precision must be 'fp32' or 'int8', got {value!r}")
+        for m in self._mlps():
+            m.precision = value
+
+    @property
+    def checkpoint(self):
+        """what training keeps of the activations: None (float32) or "int8" (quant.act8_linear)"""
+        return self._uniform("checkpoint")
+
+    @checkpoint.setter
+    def checkpoint(self, value):
+        if value not in CHECKPOINTS:
+            raise ValueError(f"checkpoint must be one of {CHECKPOINTS}, got {value!r}")
+        for m in self._mlps():
+            m.checkpoint = value
+
     def forward(self, x):                                   # (B,N,feature_dim) -> (B,N,E)
         if x.dim() != 3 or x.size(2) != self.feature_dim:
             raise ValueError(f"expected x of shape (B, N, {self.feature_dim}), got {tuple(x.shape)}")
@@ -542,6 +668,8 @@ class Point2NetSA(nn.Module):
     def _fused_ok(self) -> bool:
         if self.training or (torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters())):
             return False      # training / autograd: the per-operator path (train-mode shared MLPs, differentiable operators)
+        if any(m.precision != "fp32" for m in self._mlps()):
+            return False      # 8-bit products: per-operator path
         c = self.feature_dim - 3
         return (self.sa1.fused_supported() and self.sa2.fused_supported() and self.sa3.fused_supported()
                 and self.fp3.fused_supported(self.sa2.mlp.net[-3].out_channels)

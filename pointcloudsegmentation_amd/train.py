@@ -101,7 +101,7 @@ class _Point2NetTrainFn(torch.autograd.Function):
 def forward_train(model, x):
     """Train-mode forward of a Point2Net on a GPU tensor (B,N,F) -> (B,N,E) with autograd."""
     eval_stats = not model.training   # eval-mode BatchNorm under autograd: running statistics, left untouched
-    if x.requires_grad:
+    if x.requires_grad or model.checkpoint is not None:
         return forward_train_with_input_grad(model, x)
     x = _rt.require_cuda_f32(x, "x")
     if not eval_stats and x.size(0) * x.size(1) < 2:
@@ -137,9 +137,10 @@ def encode_train(encoder, x):
     if not ev and x.size(0) * x.size(1) < 2:
         raise ValueError("Expected more than 1 value per channel when training")
     xt = x.transpose(1, 2)
-    f1 = shared_mlp_train(encoder.mlp1, xt, eval_stats=ev)
-    f2 = shared_mlp_train(encoder.mlp2, f1, eval_stats=ev)
-    f3 = shared_mlp_train(encoder.mlp3, f2, eval_stats=ev)
+    ck = encoder.checkpoint
+    f1 = shared_mlp_train(encoder.mlp1, xt, eval_stats=ev, checkpoint=ck)
+    f2 = shared_mlp_train(encoder.mlp2, f1, eval_stats=ev, checkpoint=ck)
+    f3 = shared_mlp_train(encoder.mlp3, f2, eval_stats=ev, checkpoint=ck)
     if not ev:
         encoder._cache.key = None       # running statistics changed behind the packed eval image's back
     return f1, f2, f3, torch.max(f3, dim=2)[0]
@@ -147,11 +148,12 @@ def encode_train(encoder, x):
 
 def forward_train_with_input_grad(model, x):
     """Point2Net (train() or eval() mode) when the input points need a gradient: the reference's op sequence
-    (point2net.py:75-87) on train-mode shared MLPs, which produce d/dx; the fused p2n_train_forward path does not."""
+    (point2net.py:75-87) on train-mode shared MLPs, which produce d/dx; the fused p2n_train_forward path does not.  Also the
+    path of model.checkpoint = "int8", whose layers keep their inputs in 8 bits (quant.act8_linear)."""
     from .pointnet2 import shared_mlp_train   # noqa: WPS433
     f1, f2, f3, g = encode_train(model.encoder, x)
     combined = torch.cat([f3, g.unsqueeze(2).expand(-1, -1, f3.size(2))], dim=1)
-    emb = shared_mlp_train(model.embedding_net, combined, eval_stats=not model.training).transpose(1, 2)
+    emb = shared_mlp_train(model.embedding_net, combined, eval_stats=not model.training, checkpoint=model.checkpoint).transpose(1, 2)
     if model.training:
         model._cache.key = None
     return emb
