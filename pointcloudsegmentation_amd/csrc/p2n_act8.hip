@@ -27,8 +27,11 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
     } while (0)
 
 // ---------------------------------------------------------------- what is kept
-// codes (B, C, 128 NB) | scales (B, C, NB) | bits (B, C, 4 NB) 32-bit words | mu[C], r[C];  NB = ceil(L / 128); codes and
-// bits behind the last point are zero
+// For each (cloud, block of 128 points) in turn, C4 = channels rounded up to 4, NB = ceil(L / 128):
+//   codes  [C][128]      a byte a value; zero behind the last point
+//   scales [C4]          float32
+//   bits   [4][C4]       (norm) word w: points 32w .. 32w+31, point p at bit (p >> 1) + 16 (p & 1); zero behind the last point
+// each part for all blocks before the next, and mu[C], r[C] at the end.
 struct Act8Kept {
     long NB;
     size_t scale, bits, stat, total;
@@ -37,13 +40,18 @@ struct Act8Kept {
 static Act8Kept act8_kept(int B, int C, long L, int norm) {
     Act8Kept k;
     k.NB = (L + ACT8_GROUP - 1) / ACT8_GROUP;
-    const size_t groups = (size_t)B * C * k.NB;
-    k.scale = groups * ACT8_GROUP;
-    k.bits = k.scale + ((groups * 4 + 255) & ~(size_t)255);
-    k.stat = k.bits + (norm ? (groups * 16 + 255) & ~(size_t)255 : 0);
+    const size_t blocks = (size_t)B * k.NB, C4 = (C + 3) / 4 * 4;
+    k.scale = (blocks * C * ACT8_GROUP + 255) & ~(size_t)255;
+    k.bits = k.scale + ((blocks * C4 * 4 + 255) & ~(size_t)255);
+    k.stat = k.bits + (norm ? (blocks * C4 * 16 + 255) & ~(size_t)255 : 0);
     k.total = k.stat + (norm ? ((size_t)C * 8 + 255) & ~(size_t)255 : 0);
     return k;
 }
+
+// loads of 2 or 4 values from any 4-byte address
+typedef float f32x2u __attribute__((ext_vector_type(2), aligned(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ float act8_relu(float y) { return y <= 0.f ? 0.f : y; }   // a NaN stays
 
@@ -52,21 +60,26 @@ __device__ __forceinline__ float act8_relu(float y) { return y <= 0.f ? 0.f : y;
 __global__ __launch_bounds__(256) void p2n_act8_stats_kernel(const float *__restrict__ x, int B, int C, long L, long blocks, long per, double *__restrict__ part) {
     __shared__ double sh[8];
     const int c = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long NB = (L + 1023) / 1024;                      // a block: 1024 columns of a cloud
+    const long NB = (L + 2047) / 2048;                      // a block: 2048 columns of a cloud
     const float pivot = x[(long)c * L];
     double u = 0.0, v = 0.0;
+    auto add = [&](float e) __attribute__((always_inline)) {
+        const double d = (double)e - (double)pivot;
+        u += d;
+        v += d * d;
+    };
     const long b0 = (long)blockIdx.y * per, b1 = b0 + per < blocks ? b0 + per : blocks;
     for (long i = b0; i < b1; ++i) {
-        const long b = i / NB, l0 = (i % NB) * 1024;
+        const long b = i / NB, l0 = (i % NB) * 2048;
         const float *row = x + (b * C + c) * L;
+        if (l0 + 2048 <= L) {
+            f32x4u e[2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const long l = l0 + 256 * j + threadIdx.x;
-            if (l < L) {
-                const double d = (double)row[l] - (double)pivot;
-                u += d;
-                v += d * d;
-            }
+            for (int j = 0; j < 2; ++j) e[j] = *reinterpret_cast<const f32x4u *>(row + l0 + 1024 * j + 4 * threadIdx.x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) add(e[j >> 2][j & 3]);
+        } else {
+            for (long l = l0 + threadIdx.x; l < L; l += 256) add(row[l]);
         }
     }
 #pragma unroll
@@ -83,14 +96,13 @@ __global__ __launch_bounds__(256) void p2n_act8_stats_kernel(const float *__rest
 }
 
 // mu, r kept as float32; tab = {mu, gamma*r, beta} for the forward loader, zero behind the last channel.  frozen: from the
-// running statistics.  One thread a channel.
+// running statistics.  One wave a channel.
 __global__ void p2n_act8_norm_kernel(const double *__restrict__ part, int S, const float *__restrict__ x, int C, int Cpad, long L, double P,
                                      const float *__restrict__ gamma, const float *__restrict__ beta, float *__restrict__ rmean,
                                      float *__restrict__ rvar, double momentum, double eps, int frozen, float *__restrict__ stat, float *__restrict__ tab) {
-    const int c = blockIdx.x * blockDim.x + threadIdx.x;
-    if (c >= Cpad) return;
+    const int c = blockIdx.x, lane = threadIdx.x;
     if (c >= C) {
-        tab[c] = tab[Cpad + c] = tab[2 * Cpad + c] = 0.f;
+        if (lane < 3) tab[lane * Cpad + c] = 0.f;
         return;
     }
     double mean, var;
@@ -99,16 +111,22 @@ __global__ void p2n_act8_norm_kernel(const double *__restrict__ part, int S, con
         var = rvar[c];
     } else {
         double u = 0.0, v = 0.0;
-        for (int s = 0; s < S; ++s) { u += part[((long)c * S + s) * 2]; v += part[((long)c * S + s) * 2 + 1]; }
+        for (int s = lane; s < S; s += 64) { u += part[((long)c * S + s) * 2]; v += part[((long)c * S + s) * 2 + 1]; }
+#pragma unroll
+        for (int m = 32; m > 0; m >>= 1) {
+            u += __shfl_xor(u, m);
+            v += __shfl_xor(v, m);
+        }
         const double d = u / P;
         mean = (double)x[(long)c * L] + d;
         var = v / P - d * d;
         if (var < 0.0) var = 0.0;
-        if (rmean) {
+        if (rmean && lane == 0) {
             rmean[c] = (float)((1.0 - momentum) * rmean[c] + momentum * mean);
             rvar[c] = (float)((1.0 - momentum) * rvar[c] + momentum * var * (P / (P - 1.0)));
         }
     }
+    if (lane) return;
     const float mu = (float)mean, r = (float)(1.0 / sqrt(var + eps));
     stat[c] = mu;
     stat[C + c] = r;
@@ -118,39 +136,78 @@ __global__ void p2n_act8_norm_kernel(const double *__restrict__ part, int S, con
 }
 
 // ---------------------------------------------------------------- codes
-// one wave per group of 128 points: u, its scale, codes, the ReLU's bits
+// A workgroup takes 32 channels of a block of 128 points, a wave 8 of them, a lane two neighbouring points: u, the scales, codes,
+// the ReLU's bits.  The channels' maxima are formed by a halving exchange (8 registers shrink to one while lanes pair up), so
+// lane i holds the maximum of channel i & 7 and one division serves eight channels.
 template <bool NORM>
-__global__ __launch_bounds__(256) void p2n_act8_pack_kernel(const float *__restrict__ x, long groups, int C, long L, long NB, const float *__restrict__ stat,
+__global__ __launch_bounds__(256) void p2n_act8_pack_kernel(const float *__restrict__ x, int C, int C4, long L, long NB, const float *__restrict__ stat,
                                                             const float *__restrict__ gamma, const float *__restrict__ beta, signed char *__restrict__ codes,
                                                             float *__restrict__ scale, unsigned *__restrict__ bits) {
     const int lane = threadIdx.x & 63;
-    const long grp = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    if (grp >= groups) return;
-    const long row = grp / NB, l0 = (grp % NB) * ACT8_GROUP;      // row = cloud * C + channel
-    const int c = (int)(row % C);
-    const float *p = x + row * L + l0;
-    const bool ok0 = l0 + lane < L, ok1 = l0 + 64 + lane < L;
-    float v0 = ok0 ? p[lane] : 0.f, v1 = ok1 ? p[64 + lane] : 0.f;
-    if (NORM) {
-        const float mu = stat[c], r = stat[C + c], ga = gamma[c], be = beta[c];
-        v0 = ok0 ? (v0 - mu) * r : 0.f;
-        v1 = ok1 ? (v1 - mu) * r : 0.f;
-        const unsigned long long m0 = __ballot(ok0 && !(fmaf(ga, v0, be) <= 0.f)), m1 = __ballot(ok1 && !(fmaf(ga, v1, be) <= 0.f));
-        if (lane < 4) bits[grp * 4 + lane] = (unsigned)((lane < 2 ? m0 : m1) >> (32 * (lane & 1)));
-    }
-    unsigned am = p2n_absbits(v0), o = p2n_absbits(v1);
-    am = o > am ? o : am;
+    const int c0 = blockIdx.y * 32 + 8 * __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    if (c0 >= C4) return;
+    const long blk = blockIdx.x, b = blk / NB, l = (blk % NB) * ACT8_GROUP + 2 * lane;
+    const bool ok0 = l < L, ok1 = l + 1 < L;
+    float v[8][2];
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        o = (unsigned)__shfl_xor((int)am, m);
-        am = o > am ? o : am;
+    for (int i = 0; i < 8; ++i) {
+        const float *row = x + (b * C + (c0 + i < C ? c0 + i : C - 1)) * L;
+        v[i][0] = v[i][1] = 0.f;
+        if (ok1) {
+            const f32x2u e = *reinterpret_cast<const f32x2u *>(row + l);
+            v[i][0] = e[0]; v[i][1] = e[1];
+        } else if (ok0) {
+            v[i][0] = row[l];
+        }
     }
-    const float s = p2n_q8_scale(am);
+    unsigned word = 0;
+    const int q = (lane >> 3) & 3;
+    unsigned am[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int c = c0 + i < C ? c0 + i : C - 1;
+        if (NORM) {
+            const float mu = stat[c], r = stat[C + c], ga = gamma[c], be = beta[c];
+            v[i][0] = ok0 ? (v[i][0] - mu) * r : 0.f;
+            v[i][1] = ok1 ? (v[i][1] - mu) * r : 0.f;
+            const unsigned long long e = __ballot(ok0 && !(fmaf(ga, v[i][0], be) <= 0.f)), o = __ballot(ok1 && !(fmaf(ga, v[i][1], be) <= 0.f));
+            const unsigned w = ((unsigned)(e >> (16 * q)) & 0xFFFFu) | (unsigned)(o >> (16 * q)) << 16;
+            word = (lane & 7) == i ? w : word;
+        }
+        const unsigned a = p2n_absbits(v[i][0]), a1 = p2n_absbits(v[i][1]);
+        am[i] = a > a1 ? a : a1;
+    }
+#pragma unroll
+    for (int n = 4, m = 1; n >= 1; n >>= 1, m <<= 1)
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const bool up = lane & m;
+            const unsigned keep = up ? am[2 * i + 1] : am[2 * i], give = up ? am[2 * i] : am[2 * i + 1];
+            const unsigned o = (unsigned)__shfl_xor((int)give, m);
+            am[i] = keep > o ? keep : o;
+        }
+#pragma unroll
+    for (int m = 8; m < 64; m <<= 1) {
+        const unsigned o = (unsigned)__shfl_xor((int)am[0], m);
+        am[0] = o > am[0] ? o : am[0];
+    }
+    float s = p2n_q8_scale(am[0]);                  // of channel c0 + (lane & 7)
     const P2nQ8 Q = p2n_q8_make(s);
-    const bool bad = !(s == s);
-    if (lane == 0) scale[grp] = s;
-    codes[grp * ACT8_GROUP + lane] = bad ? 0 : (signed char)p2n_q8_decide(v0, Q);
-    codes[grp * ACT8_GROUP + 64 + lane] = bad ? 0 : (signed char)p2n_q8_decide(v1, Q);
+    if (lane < 8 && c0 + lane < C4) scale[blk * C4 + c0 + lane] = c0 + lane < C ? s : 0.f;
+    if (NORM && lane < 32 && c0 + (lane & 7) < C4) bits[(blk * 4 + q) * C4 + c0 + (lane & 7)] = c0 + (lane & 7) < C ? word : 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (c0 + i >= C) break;
+        P2nQ8 R;
+        R.s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(Q.s), i));
+        R.up = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(Q.up), i));
+        R.inv = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(Q.inv), i));
+        float e[4] = {v[i][0], v[i][1], 0.f, 0.f};
+        int code[1];
+        p2n_q8_pack(e, R, code);
+        if (!(R.s == R.s)) code[0] = 0;
+        *reinterpret_cast<unsigned short *>(codes + (blk * C + c0 + i) * ACT8_GROUP + 2 * lane) = (unsigned short)code[0];
+    }
 }
 
 // ---------------------------------------------------------------- weight image of a product
@@ -191,7 +248,7 @@ struct Act8Gemm {
     const unsigned *bits;
     float *part;           // ACT8_DY: {sum dy, sum dy*uh}[rows][2][gridDim.x]
     long L, NB;
-    int K, Kpad, KS, CTP, rows;
+    int K, Kpad, KS, CTP, rows, rows4;
 };
 enum { ACT8_PLAIN = 0, ACT8_NORM = 1 };     // operand
 enum { ACT8_OUT = 0, ACT8_DY = 1 };         // epilogue
@@ -210,6 +267,11 @@ __device__ __forceinline__ f32x16 act8_mma6(f32x16 acc, bf16x8 ah, bf16x8 am, bf
     acc = MFMAB(ah, bm, acc);
     return MFMAB(ah, bh, acc);
 }
+
+// The matrix cores cut the low bits of a sum towards minus infinity (measured: the mean of h is off by -1.5e-8 of its deviation at
+// 256 channels whatever its sign, the float32 instruction's by 3e-11), and a sum over 10^5 points adds that up.  Half of the points go
+// through with their sign turned round, so the cuts cancel.
+__device__ __forceinline__ float act8_flip(float v, unsigned flip) { return __uint_as_float(__float_as_uint(v) ^ flip); }
 
 __device__ __forceinline__ void act8_split(const float (&v)[8], bf16x8 &h, bf16x8 &m, bf16x8 &l) {
 #pragma unroll
@@ -250,6 +312,7 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : 2) void p2n_act8_gemm_kernel(Act
     const long b = blockIdx.x / A.NB, nb = blockIdx.x % A.NB, l = nb * ACT8_GROUP + 32 * wave + p;
     const bool valid = l < A.L;
     const int ct0 = blockIdx.y * CT;                 // first channel tile of this workgroup
+    const unsigned flip = (unsigned)(p & 1) << 31;   // see act8_flip
     const int nchunk = A.KS / CKS;
     const float *xb = A.x + b * A.K * A.L;
     const unsigned off = (unsigned)((8 * h * A.L + (valid ? l : A.L - 1)) * 4);
@@ -295,6 +358,8 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : 2) void p2n_act8_gemm_kernel(Act
 #pragma unroll
                 for (int i = 0; i < 8; ++i) raw[s][i] = act8_relu(fmaf(raw[s][i] - tab[k + i], tab[A.Kpad + k + i], tab[2 * A.Kpad + k + i]));
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) raw[s][i] = act8_flip(raw[s][i], flip);
             act8_split(raw[s], xh[s], xm[s], xl[s]);
         }
         if (c + 1 < nchunk) {
@@ -313,20 +378,29 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : 2) void p2n_act8_gemm_kernel(Act
     for (int ct = 0; ct < CT; ++ct) {
         const int r0 = 32 * (ct0 + ct);
         if (r0 >= A.rows) continue;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[ct][e] = act8_flip(acc[ct][e], flip);
         const __amdgpu_buffer_rsrc_t ro = act8_rsrc(A.out + (b * A.rows + r0) * A.L, (long)(A.rows - r0) * A.L * 4);
         const unsigned oo = (unsigned)((4 * h * A.L + l) * 4);
         if (EPI == ACT8_DY) {
             float s1[16], s2[16];
+            const long blk = blockIdx.x;
+            const int bit = (p >> 1) + 16 * (p & 1);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int row = r0 + 8 * (e >> 2) + 4 * h + (e & 3);
-                const long grp = (b * A.rows + (row < A.rows ? row : A.rows - 1)) * A.NB + nb;
-                const bool on = row < A.rows && (A.bits[grp * 4 + wave] >> p & 1);
-                const float uh = (float)A.codes[grp * ACT8_GROUP + 32 * wave + p] * A.scale[grp];
-                const float dy = on ? acc[ct][e] : 0.f;
-                acc[ct][e] = dy;
-                s1[e] = dy;
-                s2[e] = on ? dy * uh : 0.f;
+            for (int q = 0; q < 4; ++q) {
+                const int row = r0 + 8 * q + 4 * h, c4 = row < A.rows4 ? row : A.rows4 - 4;
+                const i32x4 w = *reinterpret_cast<const i32x4 *>(A.bits + (blk * 4 + wave) * A.rows4 + c4);
+                const f32x4 sc = *reinterpret_cast<const f32x4 *>(A.scale + blk * A.rows4 + c4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int e = 4 * q + j, c = row + j < A.rows ? row + j : A.rows - 1;
+                    const bool on = w[j] >> bit & 1;               // rows past the last one are not stored
+                    const float uh = (float)A.codes[(blk * A.rows + c) * ACT8_GROUP + 32 * wave + p] * sc[j];
+                    const float dy = on ? acc[ct][e] : 0.f;
+                    acc[ct][e] = dy;
+                    s1[e] = dy;
+                    s2[e] = on ? dy * uh : 0.f;
+                }
             }
             const float t1 = act8_half_sum(s1, lane), t2 = act8_half_sum(s2, lane);
             const int i = lane & 15, c = 32 * ct + 8 * (i >> 2) + 4 * h + (i & 3);
@@ -390,165 +464,216 @@ __global__ __launch_bounds__(256) void p2n_act8_sums_kernel(const float *__restr
     }
 }
 
-// dx = gamma*r*(dy - m1 - uh*m2), in place; one wave per group
-__global__ __launch_bounds__(256) void p2n_act8_dx_kernel(float *__restrict__ dy, long groups, int C, long L, long NB, const float *__restrict__ tab,
+// dx = gamma*r*(dy - m1 - uh*m2), in place: a workgroup takes 32 channels of a block of 128 points, a thread four points of four channels
+__global__ __launch_bounds__(256) void p2n_act8_dx_kernel(float *__restrict__ dy, int C, int C4, long L, long NB, const float *__restrict__ tab,
                                                           const signed char *__restrict__ codes, const float *__restrict__ scale) {
-    const int lane = threadIdx.x & 63;
-    const long grp = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    if (grp >= groups) return;
-    const long row = grp / NB, l0 = (grp % NB) * ACT8_GROUP;
-    const int c = (int)(row % C);
-    const float a = tab[c], m1 = tab[C + c], m2 = tab[2 * C + c], s = scale[grp];
-    float *d = dy + row * L + l0;
+    const long blk = blockIdx.x, b = blk / NB, l0 = (blk % NB) * ACT8_GROUP;
+    const int p = 4 * (threadIdx.x & 31);
+    const bool whole = l0 + p + 4 <= L;
+    float *d[4];
+    f32x4 v[4];
+    int q[4], c[4];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int i = 64 * j + lane;
-        if (l0 + i < L) d[i] = a * (d[i] - m1 - (float)codes[grp * ACT8_GROUP + i] * s * m2);
+    for (int i = 0; i < 4; ++i) {
+        c[i] = blockIdx.y * 32 + 8 * i + (threadIdx.x >> 5);
+        const int cc = c[i] < C ? c[i] : C - 1;
+        d[i] = dy + (b * C + cc) * L + l0 + p;
+        q[i] = *reinterpret_cast<const int *>(codes + (blk * C + cc) * ACT8_GROUP + p);
+        if (whole) v[i] = *reinterpret_cast<const f32x4u *>(d[i]);
+        else
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i][j] = l0 + p + j < L ? d[i][j] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (c[i] >= C) continue;
+        const float a = tab[c[i]], m1 = tab[C + c[i]], m2 = tab[2 * C + c[i]], s = scale[blk * C4 + c[i]];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i][j] = a * (v[i][j] - m1 - (float)(signed char)(q[i] >> (8 * j)) * s * m2);
+        if (whole) *reinterpret_cast<f32x4u *>(d[i]) = v[i];
+        else
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (l0 + p + j < L) d[i][j] = v[i][j];
     }
 }
 
 // ---------------------------------------------------------------- weight gradient
-// dW[n][k] = sum over points g[n] * ah[k]: both operands are rows of consecutive points.  A workgroup makes 128 x 128 of dW over a
-// slice of the points, 32 at a time, split into three bf16 parts on the way to LDS; slices are added by a second kernel, in order.
+// dW[n][k] = sum over points g[n] * ah[k]: lane = row of either operand, and both are rows of consecutive points, so a lane's 8 points
+// of a k-step are one 32-byte load (g) and one 8-byte load (codes): no LDS, no barrier.  The order of the points inside
+// a product is free as long as both operands agree; a lane takes 32 neighbouring points of a block of 64, a whole
+// cache line of g, in four k-steps.  A wave makes 32 RT x 32 CT of dW over its share of the points; the four waves of a workgroup
+// take consecutive shares and are added in LDS, the workgroups by a second kernel, both in order.
 struct Act8Wgrad {
     const float *g;        // (B, N, L)
-    const signed char *codes;   // (B, K, 128 NB)
+    const signed char *codes;
     const float *scale;
     const unsigned *bits;  // NULL: a = uh
     const float *gamma, *beta;
-    float *part;           // [slices][N][K]
-    float *dbpart;         // [slices][N]
-    long L, NB, steps, per;   // steps of 32 points in all, per slice
-    int N, K;
+    float *part;           // [slices][N * K + N]: dW, db
+    long L, NB, blocks, per;   // blocks of 64 points in all, per wave
+    int N, K, K4, ntc, slices;
 };
-#define AW_LD 40                            // bf16 elements per parked row of 32 points (80 bytes)
-#define AW_TILE (128 * AW_LD)
 
-__global__ __launch_bounds__(256, 2) void p2n_act8_wgrad_kernel(Act8Wgrad A) {
-    __shared__ __attribute__((aligned(16))) __bf16 sa[3 * AW_TILE], sb[3 * AW_TILE];
-    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int r = lane & 31, h = lane >> 5, wr = wave >> 1, wc = wave & 1;
-    const int ntc = (A.K + 127) / 128;
-    const int n0 = (blockIdx.x / ntc) * 128, k0 = (blockIdx.x % ntc) * 128;
-    const long s0 = (long)blockIdx.y * A.per, s1 = s0 + A.per < A.steps ? s0 + A.per : A.steps;
-    const long spc = 4 * A.NB;              // steps of a cloud
-    // staging: a thread takes 8 consecutive points of rows t/4 and t/4 + 64 of either operand
-    const int seg = (t & 3) * 8, srow = t >> 2;
-    float ga[2], be[2];
+template <int RT, int CT>
+__global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : RT * CT >= 4 ? 2 : 3) void p2n_act8_wgrad_kernel(Act8Wgrad A) {
+    __shared__ float join[RT * CT * 1024 + 32 * RT];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int r = lane & 31, h = lane >> 5;
+    // neighbouring workgroups go to the eight dies in turn: the tiles of one slice stay on one die, whose L2 then holds its rows
+    const int nt = gridDim.x / A.slices, w8 = blockIdx.x >> 3, full = A.slices / 8 * 8;
+    int tile, slice;
+    if ((int)blockIdx.x < full * nt) { tile = w8 % nt; slice = w8 / nt * 8 + (blockIdx.x & 7); }
+    else { const int i = blockIdx.x - full * nt; tile = i % nt; slice = full + i / nt; }
+    const int n0 = tile / A.ntc * 32 * RT, k0 = tile % A.ntc * 32 * CT;
+    const long i0 = ((long)slice * 4 + wave) * A.per, i1 = i0 + A.per < A.blocks ? i0 + A.per : A.blocks;
+    const unsigned flip = (unsigned)((slice * 4 + wave) & 1) << 31;       // every other share with its sign turned round (act8_flip)
+    const bool want_db = k0 == 0;
+    int nrow[RT], krow[CT];
+    float ga[CT], be[CT], poison[CT], db[RT];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int k = k0 + srow + 64 * i;
-        ga[i] = A.bits && k < A.K ? A.gamma[k] : 1.f;
-        be[i] = A.bits && k < A.K ? A.beta[k] : 0.f;
+    for (int i = 0; i < RT; ++i) {
+        const int n = n0 + 32 * i + r;
+        nrow[i] = n < A.N ? n : A.N - 1;
+        db[i] = 0.f;
     }
-    float va[2][8], sc[2], db[2] = {0.f, 0.f};
-    unsigned long long qb[2];
-    unsigned mb[2];
-    auto fetch = [&](long s) __attribute__((always_inline)) {
-        const long b = s / spc, l0 = (s % spc) * 32, l = l0 + seg;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int n = n0 + srow + 64 * i, k = k0 + srow + 64 * i;
-            const float *q = A.g + (b * A.N + (n < A.N ? n : A.N - 1)) * A.L;
+    for (int i = 0; i < CT; ++i) {
+        const int k = k0 + 32 * i + r;
+        krow[i] = k < A.K ? k : A.K - 1;
+        ga[i] = A.bits ? A.gamma[krow[i]] : 1.f;
+        be[i] = A.bits ? A.beta[krow[i]] : 0.f;
+        poison[i] = 0.f;
+    }
+    f32x16 acc[RT][CT];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) va[i][j] = n < A.N && l + j < A.L ? q[l + j] : 0.f;
-            const long grp = (b * A.K + (k < A.K ? k : A.K - 1)) * A.NB + (l0 >> 7);
-            qb[i] = *reinterpret_cast<const unsigned long long *>(A.codes + grp * ACT8_GROUP + (l0 & 127) + seg);
-            sc[i] = k < A.K ? A.scale[grp] : 0.f;
-            mb[i] = k < A.K ? (A.bits ? A.bits[grp * 4 + ((l0 >> 5) & 3)] >> seg : 0xFFu) : 0u;
-        }
-    };
-    auto park = [&]() __attribute__((always_inline)) {
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            bf16x8 xh, xm, xl;
-            act8_split(va[i], xh, xm, xl);
-            __bf16 *d = sa + (srow + 64 * i) * AW_LD + seg;
-            *reinterpret_cast<bf16x8 *>(d) = xh;
-            *reinterpret_cast<bf16x8 *>(d + AW_TILE) = xm;
-            *reinterpret_cast<bf16x8 *>(d + 2 * AW_TILE) = xl;
-            db[i] += ((va[i][0] + va[i][1]) + (va[i][2] + va[i][3])) + ((va[i][4] + va[i][5]) + (va[i][6] + va[i][7]));
-            float w[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float uh = (float)(signed char)(qb[i] >> (8 * j)) * sc[i];
-                const float a = A.bits ? act8_relu(fmaf(ga[i], uh, be[i])) : uh;
-                w[j] = mb[i] >> j & 1 ? a : 0.f;
-            }
-            act8_split(w, xh, xm, xl);
-            d = sb + (srow + 64 * i) * AW_LD + seg;
-            *reinterpret_cast<bf16x8 *>(d) = xh;
-            *reinterpret_cast<bf16x8 *>(d + AW_TILE) = xm;
-            *reinterpret_cast<bf16x8 *>(d + 2 * AW_TILE) = xl;
-        }
-    };
-    f32x16 acc[2][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < CT; ++k)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][k][e] = 0.f;
-    if (s0 < s1) {
-        fetch(s0);
-        park();
-    }
-    for (long s = s0; s < s1; ++s) {
-        __syncthreads();
-        const bool more = s + 1 < s1;
-        if (more) fetch(s + 1);
+    const long bpc = 2 * A.NB;              // blocks of 64 points of a cloud
+    float va[RT][8];
+    unsigned long long qb[CT];
+    auto fetch = [&](long i, int j) __attribute__((always_inline)) {      // k-step j of block i
+        const long b = i / bpc, l = (i % bpc) * 64 + 32 * h + 8 * j;
+        const bool tail = (i % bpc) * 64 + 64 > A.L;                     // wave-uniform
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            bf16x8 a[2][3], bq[2][3];
+        for (int t = 0; t < RT; ++t) {
+            const float *q = A.g + (b * A.N + nrow[t]) * A.L + l;
+            if (!tail) {
+                const f32x4u e0 = *reinterpret_cast<const f32x4u *>(q), e1 = *reinterpret_cast<const f32x4u *>(q + 4);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+                for (int x = 0; x < 4; ++x) { va[t][x] = e0[x]; va[t][4 + x] = e1[x]; }
+            } else {
 #pragma unroll
-                for (int q = 0; q < 3; ++q) {
-                    a[i][q] = *reinterpret_cast<const bf16x8 *>(sa + q * AW_TILE + (64 * wr + 32 * i + r) * AW_LD + 8 * h + 16 * ks);
-                    bq[i][q] = *reinterpret_cast<const bf16x8 *>(sb + q * AW_TILE + (64 * wc + 32 * i + r) * AW_LD + 8 * h + 16 * ks);
-                }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) acc[i][k] = act8_mma6(acc[i][k], a[i][0], a[i][1], a[i][2], bq[k][0], bq[k][1], bq[k][2]);
-        }
-        if (more) {
-            __syncthreads();
-            park();
-        }
-    }
-    float *part = A.part + (long)blockIdx.y * A.N * A.K;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int col = k0 + 64 * wc + 32 * k + r;
-            if (col >= A.K) continue;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int row = n0 + 64 * wr + 32 * i + 8 * (e >> 2) + 4 * h + (e & 3);
-                if (row < A.N) part[(long)row * A.K + col] = acc[i][k][e];
+                for (int x = 0; x < 8; ++x) va[t][x] = l + x < A.L ? q[x] : 0.f;
             }
         }
-    if (k0 == 0) {
+        const long blk = i >> 1;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float v = db[i];
-            v += __shfl_xor(v, 1);
-            v += __shfl_xor(v, 2);
-            const int n = n0 + srow + 64 * i;
-            if ((t & 3) == 0 && n < A.N) A.dbpart[(long)blockIdx.y * A.N + n] = v;
+        for (int t = 0; t < CT; ++t)
+            qb[t] = *reinterpret_cast<const unsigned long long *>(A.codes + (blk * A.K + krow[t]) * ACT8_GROUP + 64 * (i & 1) + 32 * h + 8 * j);
+    };
+    float cs[CT];
+    unsigned mb[CT];
+    if (i0 < i1) fetch(i0, 0);
+#pragma unroll 1
+    for (long i = i0; i < i1; ++i) {
+        const long blk = i >> 1;
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            cs[t] = ga[t] * A.scale[blk * A.K4 + krow[t]];
+            poison[t] += cs[t] * 0.f;                       // NaN with a NaN scale
+            mb[t] = A.bits ? A.bits[(blk * 4 + 2 * (i & 1) + h) * A.K4 + krow[t]] : 0u;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            bf16x8 a[RT][3], w[CT][3];
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                if (want_db) db[t] += ((va[t][0] + va[t][1]) + (va[t][2] + va[t][3])) + ((va[t][4] + va[t][5]) + (va[t][6] + va[t][7]));
+#pragma unroll
+                for (int x = 0; x < 8; ++x) va[t][x] = act8_flip(va[t][x], flip);
+                act8_split(va[t], a[t][0], a[t][1], a[t][2]);
+            }
+#pragma unroll
+            for (int t = 0; t < CT; ++t) {
+                float v[8];
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    const float q = (float)(signed char)(qb[t] >> (8 * x));
+                    if (A.bits) {
+                        const float y = fmaxf(fmaf(cs[t], q, be[t]), 0.f);
+                        const int p = 8 * j + x;
+                        const int on = (int)(mb[t] << (31 - ((p >> 1) + 16 * (p & 1)))) >> 31;
+                        v[x] = __int_as_float(__float_as_int(y) & on);
+                    } else {
+                        v[x] = q * cs[t];
+                    }
+                }
+                act8_split(v, w[t][0], w[t][1], w[t][2]);
+            }
+            if (j < 3) fetch(i, j + 1);
+            else if (i + 1 < i1) fetch(i + 1, 0);
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int k = 0; k < CT; ++k) acc[t][k] = act8_mma6(acc[t][k], a[t][0], a[t][1], a[t][2], w[k][0], w[k][1], w[k][2]);
         }
     }
+    // the four waves' shares, added in order
+#pragma unroll
+    for (int t = 0; t < RT; ++t) db[t] += __shfl_xor(db[t], 32);
+#pragma unroll 1
+    for (int w = 0; w < 4; ++w) {
+        if (wave == w) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+#pragma unroll
+                for (int k = 0; k < CT; ++k)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        float *d = join + (t * CT + k) * 1024 + e * 64 + lane;
+                        const float v = act8_flip(acc[t][k][e], flip) + poison[k];
+                        *d = w ? *d + v : v;
+                    }
+                if (h == 0) {
+                    float *d = join + RT * CT * 1024 + 32 * t + r;
+                    *d = w ? *d + db[t] : db[t];
+                }
+            }
+        }
+        __syncthreads();
+    }
+    float *part = A.part + (long)slice * (A.N * A.K + A.N);
+    for (int i = threadIdx.x; i < RT * CT * 1024; i += 256) {
+        const int t = i / (CT * 1024), k = i / 1024 % CT, e = i / 64 % 16, ln = i & 63;
+        const int row = n0 + 32 * t + 8 * (e >> 2) + 4 * (ln >> 5) + (e & 3), col = k0 + 32 * k + (ln & 31);
+        if (row < A.N && col < A.K) part[(long)row * A.K + col] = join[i];
+    }
+    if (want_db && threadIdx.x < 32 * RT && n0 + (int)threadIdx.x < A.N) part[(long)A.N * A.K + n0 + threadIdx.x] = join[RT * CT * 1024 + threadIdx.x];
 }
 
-// out[i] = sum over slices, in order
-__global__ __launch_bounds__(256) void p2n_act8_join_kernel(const float *__restrict__ part, long n, int slices, float *__restrict__ out) {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
+// out[i] = sum over slices, in a fixed order: 32 results a workgroup, the slices dealt to 32 rows of threads.  The first n0 results are
+// dW, the others db (either may be NULL).
+__global__ __launch_bounds__(1024) void p2n_act8_join_kernel(const float *__restrict__ part, long n, long n0, int slices, float *__restrict__ dW, float *__restrict__ db) {
+    __shared__ float sh[32][33];
+    const int o = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const long i = (long)blockIdx.x * 32 + o;
     float s = 0.f;
-    for (int k = 0; k < slices; ++k) s += part[k * n + i];
-    out[i] = s;
+    if (i < n)
+        for (int k = y; k < slices; k += 32) s += part[k * n + i];
+    sh[y][o] = s;
+    __syncthreads();
+    if (y == 0 && i < n) {
+        for (int k = 1; k < 32; ++k) s += sh[k][o];
+        if (i < n0) {
+            if (dW) dW[i] = s;
+        } else if (db) {
+            db[i - n0] = s;
+        }
+    }
 }
 
 // ---------------------------------------------------------------- norm + ReLU alone (the end of a chain)
@@ -566,27 +691,31 @@ __global__ __launch_bounds__(256) void p2n_act8_apply_kernel(const float *__rest
     }
 }
 
-// dy = [y > 0] * g and its sums; one workgroup per (channel, slice of the (cloud, group) list)
-__global__ __launch_bounds__(256) void p2n_act8_dy_kernel(const float *__restrict__ g, int B, int C, long L, long NB, long per, const signed char *__restrict__ codes,
-                                                          const float *__restrict__ scale, const unsigned *__restrict__ bits, float *__restrict__ dy,
-                                                          float *__restrict__ part) {
+// dy = [y > 0] * g and its sums; one workgroup per (channel, slice of the (cloud, block) list), a wave takes a block, a lane two points
+__global__ __launch_bounds__(256) void p2n_act8_dy_kernel(const float *__restrict__ g, int B, int C, int C4, long L, long NB, long per,
+                                                          const signed char *__restrict__ codes, const float *__restrict__ scale, const unsigned *__restrict__ bits,
+                                                          float *__restrict__ dy, float *__restrict__ part) {
     __shared__ float sh[8];
     const int c = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long n = (long)B * NB, i0 = (long)blockIdx.y * per, i1 = i0 + per < n ? i0 + per : n;
     float u = 0.f, v = 0.f;
     for (long i = i0 + wave; i < i1; i += 4) {
-        const long b = i / NB, nb = i % NB, row = b * C + c, grp = row * NB + nb;
-        const float s = scale[grp];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const long l = nb * ACT8_GROUP + 64 * j + lane;
-            if (l >= L) continue;
-            const unsigned w = bits[grp * 4 + 2 * j + (lane >> 5)];
-            const float d = w >> (lane & 31) & 1 ? g[row * L + l] : 0.f;
-            dy[row * L + l] = d;
-            u += d;
-            if (d != 0.f) v += d * ((float)codes[grp * ACT8_GROUP + 64 * j + lane] * s);
-        }
+        const long b = i / NB, l = (i % NB) * ACT8_GROUP + 2 * lane, row = b * C + c;
+        const float s = scale[i * C4 + c];
+        const unsigned w = bits[(i * 4 + (lane >> 4)) * C4 + c];
+        const int q = *reinterpret_cast<const unsigned short *>(codes + (i * C + c) * ACT8_GROUP + 2 * lane);
+        if (l >= L) continue;
+        const bool two = l + 1 < L, on0 = w >> (lane & 15) & 1, on1 = w >> (16 + (lane & 15)) & 1;
+        f32x2 e = {0.f, 0.f};
+        if (two) e = *reinterpret_cast<const f32x2u *>(g + row * L + l);
+        else e[0] = g[row * L + l];
+        e[0] = on0 ? e[0] : 0.f;
+        e[1] = on1 ? e[1] : 0.f;
+        if (two) *reinterpret_cast<f32x2u *>(dy + row * L + l) = e;
+        else dy[row * L + l] = e[0];
+        u += e[0] + e[1];
+        if (on0) v += e[0] * ((float)(signed char)q * s);
+        if (on1) v += e[1] * ((float)(signed char)(q >> 8) * s);
     }
 #pragma unroll
     for (int m = 32; m > 0; m >>= 1) {
@@ -609,8 +738,8 @@ struct Act8 {
     int Kpad, KSf, CTf, KSb, CTb;     // forward product (rows N, inner K), data gradient (rows K, inner N): k-steps, padded channel tiles
     int S;                   // slices of the statistics
     long per;
-    int slices;              // of the weight gradient
-    long steps, wper;
+    int RT, CT, ntc, nt, slices;     // weight gradient: 32-row tiles of a wave, tiles, slices of the points
+    long wblocks, wper;
 };
 
 int act8_tiles(int rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8; }   // channel tiles of a workgroup
@@ -629,19 +758,23 @@ int act8_init(Act8 &a, const char *fn, int B, int K, long L, int N) {
     const int cf = act8_tiles(N ? N : 1), cb = act8_tiles(K);
     a.KSf = act8_ksteps(K, cf); a.CTf = act8_padded(N ? N : 1, cf);
     a.KSb = act8_ksteps(N ? N : 1, cb); a.CTb = act8_padded(K, cb);
-    const long blocks = (long)B * ((L + 1023) / 1024);
+    const long blocks = (long)B * ((L + 2047) / 2048);
     long s = 2048 / K > 1 ? 2048 / K : 1;
     if (s > blocks) s = blocks;
     if (s > 1024) s = 1024;
     a.per = (blocks + s - 1) / s;
     a.S = (int)((blocks + a.per - 1) / a.per);
-    a.steps = (long)B * a.NB * 4;
-    const long tiles = (long)((N + 127) / 128) * ((K + 127) / 128);
-    long sl = tiles ? 512 / tiles : 1;
-    if (sl < 1) sl = 1;
-    if (sl > (a.steps + 15) / 16) sl = (a.steps + 15) / 16;
-    a.wper = (a.steps + sl - 1) / sl;
-    a.slices = (int)((a.steps + a.wper - 1) / a.wper);
+    // a wave makes up to 128 x 128; the points go to about as many waves as are resident at that tile's register count
+    auto tiles = [](int n) { return n <= 32 ? 1 : n <= 64 ? 2 : 4; };
+    a.RT = tiles(N ? N : 1); a.CT = tiles(K);
+    a.ntc = (K + 32 * a.CT - 1) / (32 * a.CT);
+    a.nt = ((N ? N : 1) + 32 * a.RT - 1) / (32 * a.RT) * a.ntc;
+    a.wblocks = (long)B * a.NB * 2;
+    const long wgs = a.RT * a.CT >= 8 ? 256 : a.RT * a.CT >= 4 ? 512 : 768;
+    long sl = wgs / a.nt > 1 ? wgs / a.nt : 1;
+    if (sl > (a.wblocks + 3) / 4) sl = (a.wblocks + 3) / 4;
+    a.wper = (a.wblocks + 4 * sl - 1) / (4 * sl);
+    a.slices = (int)((a.wblocks + 4 * a.wper - 1) / (4 * a.wper));
     return P2N_OK;
 }
 
@@ -673,7 +806,7 @@ FwdSpace fwd_space(const Act8 &a, char *base) {
 }
 
 struct BwdSpace {
-    float *part, *tab, *wpart, *dbpart;
+    float *part, *tab, *wpart;
     __bf16 *img;
     long nparts;
     size_t total;
@@ -685,8 +818,7 @@ BwdSpace bwd_space(const Act8 &a, char *base) {
     f.part = c.take<float>((size_t)2 * a.K * f.nparts);
     f.tab = c.take<float>((size_t)3 * a.K);
     f.img = c.take<__bf16>((size_t)a.CTb * a.KSb * 1536);
-    f.wpart = c.take<float>((size_t)a.slices * a.N * a.K);
-    f.dbpart = c.take<float>((size_t)a.slices * a.N);
+    f.wpart = c.take<float>((size_t)a.slices * (a.N * (size_t)a.K + a.N));
     f.total = c.off;
     return f;
 }
@@ -712,6 +844,21 @@ int act8_launch_gemm(const Act8Gemm &g, long groups, hipStream_t s) {
     return P2N_OK;
 }
 
+template <int RT>
+int act8_launch_wgrad_rt(const Act8 &a, const Act8Wgrad &w, hipStream_t s) {
+    const dim3 grid((unsigned)(a.nt * a.slices)), blk(256);
+    switch (a.CT) {
+        case 1: hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 1>), grid, blk, 0, s, w); break;
+        case 2: hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 2>), grid, blk, 0, s, w); break;
+        default: hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 4>), grid, blk, 0, s, w);
+    }
+    P2N_CHECK_HIP(hipGetLastError());
+    return P2N_OK;
+}
+int act8_launch_wgrad(const Act8 &a, const Act8Wgrad &w, hipStream_t s) {
+    return a.RT == 1 ? act8_launch_wgrad_rt<1>(a, w, s) : a.RT == 2 ? act8_launch_wgrad_rt<2>(a, w, s) : act8_launch_wgrad_rt<4>(a, w, s);
+}
+
 int act8_space_check(const char *fn, const void *p, size_t have, size_t need, const char *what) {
     if (!p || have < need) {
         p2n_set_error("%s: %s %zu bytes < required %zu", fn, what, have, need);
@@ -726,23 +873,23 @@ int act8_keep(const Act8 &a, const char *fn, const float *x, const float *gamma,
               float eps, char *kept, const FwdSpace &f, hipStream_t s) {
     const Act8Kept k = act8_kept(a.B, a.K, a.L, gamma != nullptr);
     float *stat = (float *)(kept + k.stat);
-    const long groups = (long)a.B * a.K * a.NB;
-    const dim3 pgrid((unsigned)((groups + 3) / 4)), blk(256);
+    const int K4 = (a.K + 3) / 4 * 4;
+    const dim3 pgrid((unsigned)((long)a.B * a.NB), (unsigned)((a.K + 31) / 32)), blk(256);
     if (gamma) {
         const bool frozen = momentum < 0.f;
         const double P = (double)a.B * a.L;
         if (!frozen) {
-            const long blocks = (long)a.B * ((a.L + 1023) / 1024);
+            const long blocks = (long)a.B * ((a.L + 2047) / 2048);
             hipLaunchKernelGGL(p2n_act8_stats_kernel, dim3(a.K, a.S), blk, 0, s, x, a.B, a.K, a.L, blocks, a.per, f.part);
             P2N_CHECK_HIP(hipGetLastError());
         }
-        hipLaunchKernelGGL(p2n_act8_norm_kernel, dim3(a.Kpad / 64), dim3(64), 0, s, f.part, a.S, x, a.K, a.Kpad, a.L, P, gamma, beta, rmean, rvar,
+        hipLaunchKernelGGL(p2n_act8_norm_kernel, dim3(a.Kpad), dim3(64), 0, s, f.part, a.S, x, a.K, a.Kpad, a.L, P, gamma, beta, rmean, rvar,
                            (double)momentum, (double)eps, frozen ? 1 : 0, stat, f.tab);
         P2N_CHECK_HIP(hipGetLastError());
-        hipLaunchKernelGGL(p2n_act8_pack_kernel<true>, pgrid, blk, 0, s, x, groups, a.K, a.L, a.NB, stat, gamma, beta, (signed char *)kept,
+        hipLaunchKernelGGL(p2n_act8_pack_kernel<true>, pgrid, blk, 0, s, x, a.K, K4, a.L, a.NB, stat, gamma, beta, (signed char *)kept,
                            (float *)(kept + k.scale), (unsigned *)(kept + k.bits));
     } else {
-        hipLaunchKernelGGL(p2n_act8_pack_kernel<false>, pgrid, blk, 0, s, x, groups, a.K, a.L, a.NB, nullptr, nullptr, nullptr, (signed char *)kept,
+        hipLaunchKernelGGL(p2n_act8_pack_kernel<false>, pgrid, blk, 0, s, x, a.K, K4, a.L, a.NB, nullptr, nullptr, nullptr, (signed char *)kept,
                            (float *)(kept + k.scale), nullptr);
     }
     P2N_CHECK_HIP(hipGetLastError());
@@ -818,27 +965,26 @@ extern "C" int p2n_act8_backward(const float *g, int B, int K, long L, const flo
     hipStream_t s = (hipStream_t)stream_;
     const int ps = p2n_prof_begin(P2N_K_ACT8_BWD, s);
     const long groups = (long)B * a.NB;
+    const int K4 = (K + 3) / 4 * 4;
     if (dW || db) {
         Act8Wgrad w = {};
-        w.g = g; w.codes = codes; w.scale = scale; w.bits = bits; w.gamma = gamma; w.beta = beta; w.part = f.wpart; w.dbpart = f.dbpart;
-        w.L = L; w.NB = a.NB; w.steps = a.steps; w.per = a.wper; w.N = N; w.K = K;
-        hipLaunchKernelGGL(p2n_act8_wgrad_kernel, dim3(((N + 127) / 128) * ((K + 127) / 128), a.slices), dim3(256), 0, s, w);
-        P2N_CHECK_HIP(hipGetLastError());
-        const long n = (long)N * K;
-        if (dW) hipLaunchKernelGGL(p2n_act8_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, f.wpart, n, a.slices, dW);
-        if (db) hipLaunchKernelGGL(p2n_act8_join_kernel, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, s, f.dbpart, (long)N, a.slices, db);
+        w.g = g; w.codes = codes; w.scale = scale; w.bits = bits; w.gamma = gamma; w.beta = beta; w.part = f.wpart;
+        w.L = L; w.NB = a.NB; w.blocks = a.wblocks; w.per = a.wper; w.N = N; w.K = K; w.K4 = K4; w.ntc = a.ntc; w.slices = a.slices;
+        TRY(act8_launch_wgrad(a, w, s));
+        const long n = (long)N * K + N;
+        hipLaunchKernelGGL(p2n_act8_join_kernel, dim3((unsigned)((n + 31) / 32)), dim3(1024), 0, s, f.wpart, n, (long)N * K, a.slices, dW, db);
         P2N_CHECK_HIP(hipGetLastError());
     }
     if (dx) {
         TRY(act8_split_weights(W, K, N, 1, a.CTb, a.KSb, f.img, s));
         Act8Gemm q = {};
         q.x = g; q.img = f.img; q.out = dx; q.codes = codes; q.scale = scale; q.bits = bits; q.part = f.part; q.L = L; q.NB = a.NB;
-        q.K = N; q.Kpad = (N + 63) / 64 * 64; q.KS = a.KSb; q.CTP = a.CTb; q.rows = K;
+        q.K = N; q.Kpad = (N + 63) / 64 * 64; q.KS = a.KSb; q.CTP = a.CTb; q.rows = K; q.rows4 = K4;
         if (gamma) {
             TRY((act8_launch_gemm<ACT8_PLAIN, ACT8_DY>(q, groups, s)));
             hipLaunchKernelGGL(p2n_act8_sums_kernel, dim3(K), dim3(256), 0, s, f.part, f.nparts, K, (double)B * L, gamma, stat, frozen ? 1 : 0, dgamma, dbeta, f.tab);
             P2N_CHECK_HIP(hipGetLastError());
-            hipLaunchKernelGGL(p2n_act8_dx_kernel, dim3((unsigned)((groups * K + 3) / 4)), dim3(256), 0, s, dx, groups * K, K, L, a.NB, f.tab, codes, scale);
+            hipLaunchKernelGGL(p2n_act8_dx_kernel, dim3((unsigned)groups, (unsigned)((K + 31) / 32)), dim3(256), 0, s, dx, K, K4, L, a.NB, f.tab, codes, scale);
             P2N_CHECK_HIP(hipGetLastError());
         } else {
             TRY((act8_launch_gemm<ACT8_PLAIN, ACT8_OUT>(q, groups, s)));
@@ -884,12 +1030,13 @@ extern "C" int p2n_act8_norm_relu_backward(const float *g, int B, int C, long L,
     const float *scale = (const float *)(kept + k.scale), *stat = (const float *)(kept + k.stat);
     hipStream_t s = (hipStream_t)stream_;
     const int ps = p2n_prof_begin(P2N_K_ACT8_BWD, s);
-    const long n = (long)B * a.NB, per = (n + a.S - 1) / a.S, groups = n * C;
-    hipLaunchKernelGGL(p2n_act8_dy_kernel, dim3(C, a.S), dim3(256), 0, s, g, B, C, L, a.NB, per, codes, scale, (const unsigned *)(kept + k.bits), dx, f.part);
+    const long n = (long)B * a.NB, per = (n + a.S - 1) / a.S;
+    const int C4 = (C + 3) / 4 * 4;
+    hipLaunchKernelGGL(p2n_act8_dy_kernel, dim3(C, a.S), dim3(256), 0, s, g, B, C, C4, L, a.NB, per, codes, scale, (const unsigned *)(kept + k.bits), dx, f.part);
     P2N_CHECK_HIP(hipGetLastError());
     hipLaunchKernelGGL(p2n_act8_sums_kernel, dim3(C), dim3(256), 0, s, f.part, f.nparts, C, (double)B * L, gamma, stat, frozen ? 1 : 0, dgamma, dbeta, f.tab);
     P2N_CHECK_HIP(hipGetLastError());
-    hipLaunchKernelGGL(p2n_act8_dx_kernel, dim3((unsigned)((groups + 3) / 4)), dim3(256), 0, s, dx, groups, C, L, a.NB, f.tab, codes, scale);
+    hipLaunchKernelGGL(p2n_act8_dx_kernel, dim3((unsigned)n, (unsigned)((C + 31) / 32)), dim3(256), 0, s, dx, C, C4, L, a.NB, f.tab, codes, scale);
     P2N_CHECK_HIP(hipGetLastError());
     p2n_prof_end(ps, s);
     return P2N_OK;

@@ -201,23 +201,25 @@ def test_what_is_kept(B, K, L, norm):
     nk, nw = lib.p2n_act8_kept_bytes(B, K, L, int(norm)), lib.p2n_act8_workspace_bytes(B, K, L, N)
     kept = torch.full((nk + 256,), 0x5A, dtype=torch.uint8, device="cuda")
     ws, h = torch.empty(nw, dtype=torch.uint8, device="cuda"), torch.empty(B, N, L, device="cuda")
-    p = rt.ptr
-    _lib.check(lib.p2n_act8_forward(x.data_ptr(), B, K, L, W.data_ptr(), b.data_ptr(), N, p(bn.weight) if norm else None, p(bn.bias) if norm else None,
+    q = rt.ptr
+    _lib.check(lib.p2n_act8_forward(x.data_ptr(), B, K, L, W.data_ptr(), b.data_ptr(), N, q(bn.weight) if norm else None, q(bn.bias) if norm else None,
                                     None, None, 0.0, 1e-5, h.data_ptr(), kept.data_ptr(), nk, ws.data_ptr(), nw, rt.stream_handle(x.device)), "fwd")
     assert bool((kept[nk:] == 0x5A).all())
-    NB = (L + 127) // 128
-    groups = B * K * NB
-    codes = kept[:groups * 128].view(torch.int8).view(B, K, NB, 128)
+    NB, K4 = (L + 127) // 128, (K + 3) // 4 * 4
+    up = lambda n: (n + 255) // 256 * 256                                             # noqa: E731
+    codes = kept[:B * NB * K * 128].view(torch.int8).view(B, NB, K, 128).transpose(1, 2)
     assert torch.equal(codes.cpu().double(), ref.q)
-    scale = kept[groups * 128:groups * 132].view(torch.float32).view(B, K, NB, 1)
-    assert torch.equal(scale.cpu().double(), ref.s)
+    off = up(B * NB * K * 128)
+    scale = kept[off:off + B * NB * K4 * 4].view(torch.float32).view(B, NB, K4)
+    assert torch.equal(scale[:, :, :K].transpose(1, 2).unsqueeze(3).cpu().double(), ref.s) and float(scale[:, :, K:].abs().sum()) == 0
     if norm:
-        off = groups * 128 + (groups * 4 + 255) // 256 * 256
-        words = kept[off:off + groups * 16].view(torch.int32).view(B, K, NB * 4).cpu()
-        bits = (words.unsqueeze(3) >> torch.arange(32, dtype=torch.int32)) & 1
-        bits = bits.reshape(B, K, -1)
-        assert torch.equal(bits[:, :, :L].double(), ref.m) and int(bits[:, :, L:].sum()) == 0
-        off += (groups * 16 + 255) // 256 * 256
+        off += up(B * NB * K4 * 4)
+        words = kept[off:off + B * NB * 4 * K4 * 4].view(torch.int32).view(B, NB, 4, K4).cpu()
+        p = torch.arange(32, dtype=torch.int32)
+        bits = (words.unsqueeze(4) >> ((p >> 1) + 16 * (p & 1))) & 1                  # (B, NB, 4, K4, 32)
+        bits = bits.permute(0, 3, 1, 2, 4).reshape(B, K4, -1)
+        assert torch.equal(bits[:, :K, :L].double(), ref.m) and int(bits[:, :K, L:].sum()) == 0 and int(bits[:, K:].sum()) == 0
+        off += up(B * NB * 4 * K4 * 4)
         stat = kept[off:off + 8 * K].view(torch.float32).cpu()
         assert torch.equal(stat[:K], ref.mu[:, 0]) and torch.equal(stat[K:], ref.r[:, 0])
 

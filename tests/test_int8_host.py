@@ -45,9 +45,9 @@ def test_cpu_tensors_are_refused():
 def test_checkpoint_layers_refuse_bad_shapes():
     from pointcloudsegmentation_amd import _lib
     lib = _lib.lib()
-    # codes, scales (rounded up to 256 bytes), bits, mean and 1/deviation
-    assert lib.p2n_act8_kept_bytes(2, 64, 300, 1) == 2 * 64 * 3 * 128 + 2 * 64 * 3 * 4 + 2 * 64 * 3 * 16 + 64 * 8
-    assert lib.p2n_act8_kept_bytes(2, 64, 300, 0) == 2 * 64 * 3 * 128 + 2 * 64 * 3 * 4
+    # codes, scales, bits, mean and 1/deviation, each part rounded up to 256 bytes
+    assert lib.p2n_act8_kept_bytes(2, 64, 300, 1) == 2 * 3 * 64 * 128 + 2 * 3 * 64 * 4 + 2 * 3 * 64 * 16 + 64 * 8
+    assert lib.p2n_act8_kept_bytes(2, 6, 300, 0) == 2 * 3 * 6 * 128 + 256                # 6 scales as 8: 192 bytes
     for bad in ((0, 64, 300, 1), (2, 0, 300, 1), (2, 1025, 300, 1), (2, 64, 0, 1), (2, 64, (1 << 24) + 1, 1), (1 << 20, 1024, 300, 1)):
         assert lib.p2n_act8_kept_bytes(*bad) == 0
         assert lib.p2n_act8_workspace_bytes(*bad[:3], 8) == 0
