@@ -300,13 +300,18 @@ __device__ __forceinline__ float act8_half_sum(float (&m)[16], int lane) {
     return m[0] + __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(m[0]), 0x401F));
 }
 
-template <int IN, int EPI, int CT>
-__global__ __launch_bounds__(256, CT <= 4 ? 3 : 2) void p2n_act8_gemm_kernel(Act8Gemm A) {
-    constexpr int CKS = CT >= 4 ? 1 : 4 / CT;       // k-steps of 16 in a chunk: 12 or 24 fragments, a multiple of the four waves
-    constexpr int F = CKS * CT * 3;
-    __shared__ __attribute__((aligned(16))) char wbuf[2][F * 1024];
-    __shared__ __attribute__((aligned(16))) float tab[IN == ACT8_NORM ? 3 * ACT8_MAX_C : 4];
+// k-steps of 16 in a chunk of the weights: 6 to 24 fragments
+__host__ __device__ constexpr int act8_chunk(int CT) { return CT >= 4 ? 1 : 2; }
+
+// TABK: channels that the norm's table in LDS has room for; 512 leaves room for two workgroups on a CU at 256 output channels
+template <int IN, int EPI, int CT, int TABK>
+__global__ __launch_bounds__(256, CT <= 4 ? 3 : TABK <= 512 ? 2 : 1) void p2n_act8_gemm_kernel(Act8Gemm A) {
+    constexpr int CKS = act8_chunk(CT);
+    constexpr int F = CKS * CT * 3, FW = (F + 3) / 4;      // fragments of a chunk, of a wave
+    __shared__ __attribute__((aligned(16))) char wbuf[3][F * 1024];
+    __shared__ __attribute__((aligned(16))) float tab[IN == ACT8_NORM ? 3 * TABK : 4];
     __shared__ float red[EPI == ACT8_DY ? 4 * 2 * 32 * CT : 1];
+    __shared__ float bias[EPI == ACT8_OUT ? 32 * CT : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int p = lane & 31, h = lane >> 5;
     const long b = blockIdx.x / A.NB, nb = blockIdx.x % A.NB, l = nb * ACT8_GROUP + 32 * wave + p;
@@ -318,19 +323,21 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : 2) void p2n_act8_gemm_kernel(Act
     const unsigned off = (unsigned)((8 * h * A.L + (valid ? l : A.L - 1)) * 4);
     if (IN == ACT8_NORM)
         for (int i = threadIdx.x; i < 3 * A.Kpad; i += 256) tab[i] = A.tab[i];
+    if (EPI == ACT8_OUT && (int)threadIdx.x < 32 * CT)
+        bias[threadIdx.x] = A.bias && 32 * ct0 + (int)threadIdx.x < A.rows ? A.bias[32 * ct0 + threadIdx.x] : 0.f;
 
-    auto stage = [&](int c) __attribute__((always_inline)) {
+    auto stage = [&](int c, int slot) __attribute__((always_inline)) {
         const __amdgpu_buffer_rsrc_t rs = act8_rsrc(A.img, (long)A.CTP * A.KS * 3072);
 #pragma unroll
-        for (int i = 0; i < F / 4; ++i) {
-            const int f = wave * (F / 4) + i;        // fragment of the chunk: k-step f / (3 CT), the rest in image order
+        for (int i = 0; i < FW; ++i) {
+            const int g = wave * FW + i, f = g < F ? g : F - 1;   // fragment of the chunk: k-step f / (3 CT), the rest in image order
             const int ks = c * CKS + f / (3 * CT);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (act8_lds_t *)(wbuf[c & 1] + f * 1024), 16, lane * 16,
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (act8_lds_t *)(wbuf[slot] + f * 1024), 16, lane * 16,
                                                      ((ks * A.CTP + ct0) * 3 + f % (3 * CT)) * 1024, 0, 0);
         }
     };
-    float raw[CKS][8];
-    auto fetch = [&](int c) __attribute__((always_inline)) {
+    float raw[2][CKS][8];
+    auto fetch = [&](int c, float (&raw)[CKS][8]) __attribute__((always_inline)) {
 #pragma unroll
         for (int s = 0; s < CKS; ++s) {
             const int k0 = 16 * (c * CKS + s);
@@ -345,11 +352,17 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : 2) void p2n_act8_gemm_kernel(Act
     for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[ct][e] = 0.f;
-    stage(0);
-    fetch(0);
-#pragma unroll 1
-    for (int c = 0; c < nchunk; ++c) {
-        p2n_dma_barrier();                            // chunk c is in LDS, this wave's rows of it in registers
+    // Chunks c+1 and c+2 are on their way while chunk c is multiplied: a load from memory takes about as long as one chunk's products.
+    // Every chunk issues GROUP vector-memory operations, in order, so "at most GROUP outstanding" means chunk c has arrived.
+    // (The last two iterations fetch the last chunk again: the count stays the same, nobody reads it.)
+    constexpr int GROUP = FW + 8 * CKS;
+    static_assert(GROUP < 64, "the counter holds six bits");
+    int slot = 0;
+    auto body = [&](int c, float (&raw)[CKS][8]) __attribute__((always_inline)) {
+        __builtin_amdgcn_s_waitcnt((GROUP & 15) | (7 << 4) | (0 << 8) | ((GROUP >> 4) << 14));
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();                 // every wave's part of chunk c is in LDS, and nobody reads chunk c-1 any more
+        asm volatile("" ::: "memory");
         bf16x8 xh[CKS], xm[CKS], xl[CKS];
 #pragma unroll
         for (int s = 0; s < CKS; ++s) {
@@ -362,18 +375,62 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : 2) void p2n_act8_gemm_kernel(Act
             for (int i = 0; i < 8; ++i) raw[s][i] = act8_flip(raw[s][i], flip);
             act8_split(raw[s], xh[s], xm[s], xl[s]);
         }
-        if (c + 1 < nchunk) {
-            stage(c + 1);
-            fetch(c + 1);
-        }
+        const int ahead = c + 2 < nchunk ? c + 2 : nchunk - 1;
+        stage(ahead, slot >= 1 ? slot - 1 : 2);       // (slot + 2) % 3
+        fetch(ahead, raw);
+        // two channel tiles at a time (independent sums), their fragments read one pair ahead
+        __builtin_amdgcn_sched_barrier(0);
+        const bf16x8 *w = reinterpret_cast<const bf16x8 *>(wbuf[slot]) + lane;
+        constexpr int NT = CKS * CT, PW = NT < 2 ? 1 : 2, NP = NT / PW;
+        bf16x8 f[2][PW][3];
 #pragma unroll
-        for (int s = 0; s < CKS; ++s)
+        for (int u = 0; u < PW; ++u)
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
-                const bf16x8 *w = reinterpret_cast<const bf16x8 *>(wbuf[c & 1] + (s * CT + ct) * 3072) + lane;
-                acc[ct] = act8_mma6(acc[ct], w[0], w[64], w[128], xh[s], xm[s], xl[s]);
+            for (int q = 0; q < 3; ++q) f[0][u][q] = w[(u * 3 + q) * 64];
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            if (i + 1 < NP) {
+#pragma unroll
+                for (int u = 0; u < PW; ++u)
+#pragma unroll
+                    for (int q = 0; q < 3; ++q) f[(i + 1) & 1][u][q] = w[(((i + 1) * PW + u) * 3 + q) * 64];
             }
+#pragma unroll
+            for (int q = 0; q < 6; ++q)
+#pragma unroll
+                for (int u = 0; u < PW; ++u) {
+                    const int t = i * PW + u, ks = t / CT, ct = t % CT;
+                    const bf16x8 wq = f[i & 1][u][q == 0 ? 2 : q == 1 || q >= 4 ? 0 : 1];
+                    const bf16x8 xq = q == 1 ? xl[ks] : q == 2 || q == 4 ? xm[ks] : xh[ks];     // l.h, h.l, m.m, m.h, h.m, h.h
+                    acc[ct] = MFMAB(wq, xq, acc[ct]);
+                }
+        }
+        __builtin_amdgcn_sched_group_barrier(0x100, 3 * PW * (NP > 1 ? 2 : 1), 0);      // LDS reads
+#pragma unroll
+        for (int i = 0; i + 2 < NP; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 6 * PW, 0);                       // matrix products
+            __builtin_amdgcn_sched_group_barrier(0x100, 3 * PW, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 6 * PW * (NP > 1 ? 2 : 1), 0);
+        __builtin_amdgcn_sched_barrier(0);
+        slot = slot == 2 ? 0 : slot + 1;
+    };
+    __syncthreads();                                  // the table; from here on waits are counted by hand
+    stage(0, 0);
+    fetch(0, raw[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    stage(nchunk > 1 ? 1 : 0, 1);
+    fetch(nchunk > 1 ? 1 : 0, raw[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    int c = 0;
+#pragma unroll 1
+    for (; c + 1 < nchunk; c += 2) {
+        body(c, raw[0]);
+        body(c + 1, raw[1]);
     }
+    if (c < nchunk) body(c, raw[0]);
+    __builtin_amdgcn_s_waitcnt(7 << 4);               // nothing may be on its way into LDS when the workgroup ends
+    asm volatile("" ::: "memory");
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         const int r0 = 32 * (ct0 + ct);
@@ -413,10 +470,7 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : 2) void p2n_act8_gemm_kernel(Act
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 float v = acc[ct][e];
-                if (EPI == ACT8_OUT && A.bias) {
-                    const int row = r0 + 8 * (e >> 2) + 4 * h + (e & 3);
-                    v += A.bias[row < A.rows ? row : A.rows - 1];
-                }
+                if (EPI == ACT8_OUT) v += bias[32 * ct + 8 * (e >> 2) + 4 * h + (e & 3)];
                 __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(v), ro, oo + (unsigned)((8 * (e >> 2) + (e & 3)) * A.L * 4), 0, 0);
             }
         }
@@ -744,7 +798,7 @@ struct Act8 {
 
 int act8_tiles(int rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8; }   // channel tiles of a workgroup
 int act8_ksteps(int k, int ct) {
-    const int cks = ct >= 4 ? 1 : 4 / ct, ks = (k + 15) / 16;
+    const int cks = act8_chunk(ct), ks = (k + 15) / 16;
     return (ks + cks - 1) / cks * cks;
 }
 int act8_padded(int rows, int ct) { return ((rows + 31) / 32 + ct - 1) / ct * ct; }
@@ -830,18 +884,24 @@ int act8_split_weights(const float *W, int rows, int cols, int trans, int CTP, i
     return P2N_OK;
 }
 
-template <int IN, int EPI>
-int act8_launch_gemm(const Act8Gemm &g, long groups, hipStream_t s) {
+template <int IN, int EPI, int TABK>
+int act8_launch_gemm_tab(const Act8Gemm &g, long groups, hipStream_t s) {
     const int ct = act8_tiles(g.rows);
     const dim3 grid((unsigned)groups, (unsigned)(g.CTP / ct)), blk(256);
     switch (ct) {
-        case 1: hipLaunchKernelGGL((p2n_act8_gemm_kernel<IN, EPI, 1>), grid, blk, 0, s, g); break;
-        case 2: hipLaunchKernelGGL((p2n_act8_gemm_kernel<IN, EPI, 2>), grid, blk, 0, s, g); break;
-        case 4: hipLaunchKernelGGL((p2n_act8_gemm_kernel<IN, EPI, 4>), grid, blk, 0, s, g); break;
-        default: hipLaunchKernelGGL((p2n_act8_gemm_kernel<IN, EPI, 8>), grid, blk, 0, s, g);
+        case 1: hipLaunchKernelGGL((p2n_act8_gemm_kernel<IN, EPI, 1, TABK>), grid, blk, 0, s, g); break;
+        case 2: hipLaunchKernelGGL((p2n_act8_gemm_kernel<IN, EPI, 2, TABK>), grid, blk, 0, s, g); break;
+        case 4: hipLaunchKernelGGL((p2n_act8_gemm_kernel<IN, EPI, 4, TABK>), grid, blk, 0, s, g); break;
+        default: hipLaunchKernelGGL((p2n_act8_gemm_kernel<IN, EPI, 8, TABK>), grid, blk, 0, s, g);
     }
     P2N_CHECK_HIP(hipGetLastError());
     return P2N_OK;
+}
+template <int IN, int EPI>
+int act8_launch_gemm(const Act8Gemm &g, long groups, hipStream_t s) {
+    if constexpr (IN == ACT8_NORM)
+        if (g.Kpad > 512) return act8_launch_gemm_tab<IN, EPI, ACT8_MAX_C>(g, groups, s);
+    return act8_launch_gemm_tab<IN, EPI, 512>(g, groups, s);
 }
 
 template <int RT>
