@@ -553,11 +553,12 @@ __global__ __launch_bounds__(256) void p2n_act8_dx_kernel(float *__restrict__ dy
 }
 
 // ---------------------------------------------------------------- weight gradient
-// dW[n][k] = sum over points g[n] * ah[k]: lane = row of either operand, and both are rows of consecutive points, so a lane's 8 points
-// of a k-step are one 32-byte load (g) and one 8-byte load (codes): no LDS, no barrier.  The order of the points inside
-// a product is free as long as both operands agree; a lane takes 32 neighbouring points of a block of 64, a whole
-// cache line of g, in four k-steps.  A wave makes 32 RT x 32 CT of dW over its share of the points; the four waves of a workgroup
-// take consecutive shares and are added in LDS, the workgroups by a second kernel, both in order.
+// dW[n][k] = sum over points g[n] * ah[k]: lane = row of either operand, both are rows of consecutive points, and the order of the
+// points inside a product is free as long as both operands agree.  A wave makes 32 RT x 32 CT of dW over its share of the
+// points, 32 at a time, a lane 16 of them: its codes are one 16-byte load; g passes through a piece of LDS that belongs to the
+// wave alone (LDS-DMA in whole cache lines, two buffers, no barrier; read straight from memory a lane touches its line
+// four times, by which time it has left the L1).  The four waves of a workgroup take consecutive shares and are
+// added in LDS, the workgroups by a second kernel, both in order.
 struct Act8Wgrad {
     const float *g;        // (B, N, L)
     const signed char *codes;
@@ -565,13 +566,16 @@ struct Act8Wgrad {
     const unsigned *bits;  // NULL: a = uh
     const float *gamma, *beta;
     float *part;           // [slices][N * K + N]: dW, db
-    long L, NB, blocks, per;   // blocks of 64 points in all, per wave
+    long L, NB, steps, per;   // steps of 32 points in all, per wave
     int N, K, K4, ntc, slices;
 };
 
-template <int RT, int CT>
-__global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : RT * CT >= 4 ? 2 : 3) void p2n_act8_wgrad_kernel(Act8Wgrad A) {
-    __shared__ float join[RT * CT * 1024 + 32 * RT];
+// DMA: rows of g start 16-byte aligned (L a multiple of 4); without, its values are loaded from memory as they are needed
+template <int RT, int CT, bool DMA>
+__global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : 2) void p2n_act8_wgrad_kernel(Act8Wgrad A) {
+    constexpr int BUF = RT * 4096;                   // 32 RT rows of 128 bytes
+    constexpr int JOIN = (RT * CT * 1024 + 4 * 32 * RT) * 4;
+    __shared__ __attribute__((aligned(16))) char lds[DMA && 8 * BUF > JOIN ? 8 * BUF : JOIN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int r = lane & 31, h = lane >> 5;
     // neighbouring workgroups go to the eight dies in turn: the tiles of one slice stay on one die, whose L2 then holds its rows
@@ -580,17 +584,13 @@ __global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : RT * CT >= 4 ? 2 : 3) void 
     if ((int)blockIdx.x < full * nt) { tile = w8 % nt; slice = w8 / nt * 8 + (blockIdx.x & 7); }
     else { const int i = blockIdx.x - full * nt; tile = i % nt; slice = full + i / nt; }
     const int n0 = tile / A.ntc * 32 * RT, k0 = tile % A.ntc * 32 * CT;
-    const long i0 = ((long)slice * 4 + wave) * A.per, i1 = i0 + A.per < A.blocks ? i0 + A.per : A.blocks;
+    const long i0 = ((long)slice * 4 + wave) * A.per, i1 = i0 + A.per < A.steps ? i0 + A.per : A.steps;
     const unsigned flip = (unsigned)((slice * 4 + wave) & 1) << 31;       // every other share with its sign turned round (act8_flip)
     const bool want_db = k0 == 0;
-    int nrow[RT], krow[CT];
+    int krow[CT];
     float ga[CT], be[CT], poison[CT], db[RT];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        const int n = n0 + 32 * i + r;
-        nrow[i] = n < A.N ? n : A.N - 1;
-        db[i] = 0.f;
-    }
+    for (int i = 0; i < RT; ++i) db[i] = 0.f;
 #pragma unroll
     for (int i = 0; i < CT; ++i) {
         const int k = k0 + 32 * i + r;
@@ -606,107 +606,152 @@ __global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : RT * CT >= 4 ? 2 : 3) void 
         for (int k = 0; k < CT; ++k)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][k][e] = 0.f;
-    const long bpc = 2 * A.NB;              // blocks of 64 points of a cloud
-    float va[RT][8];
-    unsigned long long qb[CT];
-    auto fetch = [&](long i, int j) __attribute__((always_inline)) {      // k-step j of block i
-        const long b = i / bpc, l = (i % bpc) * 64 + 32 * h + 8 * j;
-        const bool tail = (i % bpc) * 64 + 64 > A.L;                     // wave-uniform
+    const long spc = 4 * A.NB;              // steps of a cloud
+    // LDS image of a step: row R's 16-byte piece q (points 4q .. 4q+3) lies in slot q ^ (R >> 1 & 7) of the row, so that the 16 rows of a
+    // read fall into different banks.  DMA instruction i fills rows 8i .. 8i+7: lane -> row lane >> 3, slot lane & 7.
+    char *const mine = lds + wave * 2 * BUF;
+    const int drow = lane >> 3, piece = (lane & 7) ^ (lane >> 4);
+    const int left = A.N - n0;              // rows past the last one read the last one
+    const unsigned off_full = (unsigned)(drow * A.L * 4), off_part = (unsigned)((drow < (left & 7) ? drow : (left & 7) - 1) * A.L * 4);
+    auto dma = [&](long s, int buf) __attribute__((always_inline)) {
+        const long b = s / spc, l0 = (s % spc) * 32;
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const float *q = A.g + (b * A.N + nrow[t]) * A.L + l;
-            if (!tail) {
-                const f32x4u e0 = *reinterpret_cast<const f32x4u *>(q), e1 = *reinterpret_cast<const f32x4u *>(q + 4);
-#pragma unroll
-                for (int x = 0; x < 4; ++x) { va[t][x] = e0[x]; va[t][4 + x] = e1[x]; }
-            } else {
-#pragma unroll
-                for (int x = 0; x < 8; ++x) va[t][x] = l + x < A.L ? q[x] : 0.f;
-            }
+        for (int i = 0; i < RT * 4; ++i) {
+            const bool part = 8 * i < left && left < 8 * i + 8, none = 8 * i >= left;        // wave-uniform
+            const long row = b * A.N + (none ? A.N - 1 : n0 + 8 * i);
+            const __amdgpu_buffer_rsrc_t rs = act8_rsrc(A.g + row * A.L + l0, ((b + 1) * A.N - row) * A.L * 4 - l0 * 4);
+            const unsigned off = (none ? 0u : part ? off_part : off_full) + 16u * (unsigned)(piece ^ (4 * (i & 1)));
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (act8_lds_t *)(mine + buf * BUF + i * 1024), 16, off, 0, 0, 0);
         }
-        const long blk = i >> 1;
-#pragma unroll
-        for (int t = 0; t < CT; ++t)
-            qb[t] = *reinterpret_cast<const unsigned long long *>(A.codes + (blk * A.K + krow[t]) * ACT8_GROUP + 64 * (i & 1) + 32 * h + 8 * j);
     };
-    float cs[CT];
-    unsigned mb[CT];
-    if (i0 < i1) fetch(i0, 0);
-#pragma unroll 1
-    for (long i = i0; i < i1; ++i) {
-        const long blk = i >> 1;
+    int qn[CT][4];
+    float sn[CT];
+    unsigned mn[CT];
+    auto meta = [&](long s) __attribute__((always_inline)) {
+        const long blk = s >> 2;
+        const int w = (int)(s & 3);
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
-            cs[t] = ga[t] * A.scale[blk * A.K4 + krow[t]];
-            poison[t] += cs[t] * 0.f;                       // NaN with a NaN scale
-            mb[t] = A.bits ? A.bits[(blk * 4 + 2 * (i & 1) + h) * A.K4 + krow[t]] : 0u;
-        }
+            const i32x4 q = *reinterpret_cast<const i32x4 *>(A.codes + (blk * A.K + krow[t]) * ACT8_GROUP + 32 * w + 16 * h);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+            for (int x = 0; x < 4; ++x) qn[t][x] = q[x];
+            sn[t] = A.scale[blk * A.K4 + krow[t]];
+            mn[t] = A.bits ? A.bits[(blk * 4 + w) * A.K4 + krow[t]] : 0u;
+        }
+    };
+    if (i0 < i1) {
+        if (DMA) dma(i0, 0);
+        meta(i0);
+    }
+#pragma unroll 1
+    for (long s = i0; s < i1; ++s) {
+        const int buf = (int)(s - i0) & 1;
+        __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));         // vmcnt(0): this step's rows and codes have arrived
+        asm volatile("" ::: "memory");
+        int q[CT][4];
+        float cs[CT];
+        unsigned mb[CT];
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) q[t][x] = qn[t][x];
+            cs[t] = ga[t] * sn[t];
+            poison[t] += cs[t] * 0.f;                       // NaN with a NaN scale
+            mb[t] = mn[t] >> (8 * h);                       // points 16h .. 16h+15: bits 8h .. of either half-word
+        }
+        if (s + 1 < i1) {
+            if (DMA) dma(s + 1, buf ^ 1);
+            meta(s + 1);
+        }
+        const long b = s / spc, l0 = (s % spc) * 32;
+        const bool tail = l0 + 32 > A.L;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
             bf16x8 a[RT][3], w[CT][3];
+            const long l = l0 + 16 * h + 8 * j;
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-                if (want_db) db[t] += ((va[t][0] + va[t][1]) + (va[t][2] + va[t][3])) + ((va[t][4] + va[t][5]) + (va[t][6] + va[t][7]));
+                float va[8];
+                if (DMA) {
+                    const char *row = mine + buf * BUF + (32 * t + r) * 128;
+                    const int key = r >> 1 & 7;
+                    const f32x4 e0 = *reinterpret_cast<const f32x4 *>(row + ((4 * h + 2 * j) ^ key) * 16);
+                    const f32x4 e1 = *reinterpret_cast<const f32x4 *>(row + ((4 * h + 2 * j + 1) ^ key) * 16);
 #pragma unroll
-                for (int x = 0; x < 8; ++x) va[t][x] = act8_flip(va[t][x], flip);
-                act8_split(va[t], a[t][0], a[t][1], a[t][2]);
+                    for (int x = 0; x < 4; ++x) { va[x] = e0[x]; va[4 + x] = e1[x]; }
+                    if (tail) {
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) va[x] = l + x < A.L ? va[x] : 0.f;
+                    }
+                } else {
+                    const int n = n0 + 32 * t + r;
+                    const float *p = A.g + (b * A.N + (n < A.N ? n : A.N - 1)) * A.L + l;
+                    if (!tail) {
+                        const f32x4u e0 = *reinterpret_cast<const f32x4u *>(p), e1 = *reinterpret_cast<const f32x4u *>(p + 4);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) { va[x] = e0[x]; va[4 + x] = e1[x]; }
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) va[x] = l + x < A.L ? p[x] : 0.f;
+                    }
+                }
+                if (want_db) db[t] += ((va[0] + va[1]) + (va[2] + va[3])) + ((va[4] + va[5]) + (va[6] + va[7]));
+#pragma unroll
+                for (int x = 0; x < 8; ++x) va[x] = act8_flip(va[x], flip);
+                act8_split(va, a[t][0], a[t][1], a[t][2]);
             }
 #pragma unroll
             for (int t = 0; t < CT; ++t) {
                 float v[8];
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
-                    const float q = (float)(signed char)(qb[t] >> (8 * x));
+                    const float c = (float)(signed char)(q[t][2 * j + (x >> 2)] >> (8 * (x & 3)));
                     if (A.bits) {
-                        const float y = fmaxf(fmaf(cs[t], q, be[t]), 0.f);
-                        const int p = 8 * j + x;
-                        const int on = (int)(mb[t] << (31 - ((p >> 1) + 16 * (p & 1)))) >> 31;
+                        const float y = fmaxf(fmaf(cs[t], c, be[t]), 0.f);
+                        const int on = (int)(mb[t] << (31 - ((4 * j + (x >> 1)) + 16 * (x & 1)))) >> 31;
                         v[x] = __int_as_float(__float_as_int(y) & on);
                     } else {
-                        v[x] = q * cs[t];
+                        v[x] = c * cs[t];
                     }
                 }
                 act8_split(v, w[t][0], w[t][1], w[t][2]);
             }
-            if (j < 3) fetch(i, j + 1);
-            else if (i + 1 < i1) fetch(i + 1, 0);
 #pragma unroll
             for (int t = 0; t < RT; ++t)
 #pragma unroll
                 for (int k = 0; k < CT; ++k) acc[t][k] = act8_mma6(acc[t][k], a[t][0], a[t][1], a[t][2], w[k][0], w[k][1], w[k][2]);
         }
     }
-    // the four waves' shares, added in order
+    // the four waves' shares, added in order: a quarter of the tile's registers at a time, all waves at once
 #pragma unroll
     for (int t = 0; t < RT; ++t) db[t] += __shfl_xor(db[t], 32);
-#pragma unroll 1
-    for (int w = 0; w < 4; ++w) {
-        if (wave == w) {
-#pragma unroll
-            for (int t = 0; t < RT; ++t) {
-#pragma unroll
-                for (int k = 0; k < CT; ++k)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        float *d = join + (t * CT + k) * 1024 + e * 64 + lane;
-                        const float v = act8_flip(acc[t][k][e], flip) + poison[k];
-                        *d = w ? *d + v : v;
-                    }
-                if (h == 0) {
-                    float *d = join + RT * CT * 1024 + 32 * t + r;
-                    *d = w ? *d + db[t] : db[t];
-                }
-            }
-        }
-        __syncthreads();
-    }
+    float *const join = reinterpret_cast<float *>(lds);
     float *part = A.part + (long)slice * (A.N * A.K + A.N);
-    for (int i = threadIdx.x; i < RT * CT * 1024; i += 256) {
-        const int t = i / (CT * 1024), k = i / 1024 % CT, e = i / 64 % 16, ln = i & 63;
-        const int row = n0 + 32 * t + 8 * (e >> 2) + 4 * (ln >> 5) + (e & 3), col = k0 + 32 * k + (ln & 31);
-        if (row < A.N && col < A.K) part[(long)row * A.K + col] = join[i];
+    constexpr int Q = RT * CT * 4;          // registers of a quarter
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        __syncthreads();                    // the last rows (c = 0), the last quarter have been read
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+            const int v = c * Q + i, tk = v / 16, e = v % 16;
+            join[(wave * Q + i) * 64 + lane] = act8_flip(acc[tk / CT][tk % CT][e], flip) + poison[tk % CT];
+        }
+        if (c == 0 && h == 0)
+#pragma unroll
+            for (int t = 0; t < RT; ++t) join[RT * CT * 1024 + (wave * RT + t) * 32 + r] = db[t];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < Q / 4; ++i) {
+            const int o = i * 256 + threadIdx.x, v = c * Q + o / 64, tk = v / 16, e = v % 16, ln = o & 63;
+            const int row = n0 + 32 * (tk / CT) + 8 * (e >> 2) + 4 * (ln >> 5) + (e & 3), col = k0 + 32 * (tk % CT) + (ln & 31);
+            const float sum = ((join[o] + join[o + Q * 64]) + join[o + 2 * Q * 64]) + join[o + 3 * Q * 64];
+            if (row < A.N && col < A.K) part[(long)row * A.K + col] = sum;
+        }
+        if (c == 0 && want_db && threadIdx.x < 32 * RT && n0 + (int)threadIdx.x < A.N) {
+            const float *d = join + RT * CT * 1024 + threadIdx.x;
+            part[(long)A.N * A.K + n0 + threadIdx.x] = ((d[0] + d[32 * RT]) + d[64 * RT]) + d[96 * RT];
+        }
     }
-    if (want_db && threadIdx.x < 32 * RT && n0 + (int)threadIdx.x < A.N) part[(long)A.N * A.K + n0 + threadIdx.x] = join[RT * CT * 1024 + threadIdx.x];
 }
 
 // out[i] = sum over slices, in a fixed order: 32 results a workgroup, the slices dealt to 32 rows of threads.  The first n0 results are
@@ -793,7 +838,7 @@ struct Act8 {
     int S;                   // slices of the statistics
     long per;
     int RT, CT, ntc, nt, slices;     // weight gradient: 32-row tiles of a wave, tiles, slices of the points
-    long wblocks, wper;
+    long wsteps, wper;
 };
 
 int act8_tiles(int rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8; }   // channel tiles of a workgroup
@@ -818,17 +863,20 @@ int act8_init(Act8 &a, const char *fn, int B, int K, long L, int N) {
     if (s > 1024) s = 1024;
     a.per = (blocks + s - 1) / s;
     a.S = (int)((blocks + a.per - 1) / a.per);
-    // a wave makes up to 128 x 128; the points go to about as many waves as are resident at that tile's register count
-    auto tiles = [](int n) { return n <= 32 ? 1 : n <= 64 ? 2 : 4; };
+    // a wave makes up to 128 x 128 where there are points enough to fill the card with such waves (256 clouds' blocks of 128:
+    // measured at 8,192 points, 256 x 384: 56 us against 27 with 64 x 64), up to 64 x 64 otherwise; the points go to about as
+    // many waves as are resident at that tile's register count
+    a.wsteps = (long)B * a.NB * 4;
+    const int cap = a.wsteps < 2048 ? 2 : 4;
+    auto tiles = [cap](int n) { return n <= 32 ? 1 : n <= 64 ? 2 : cap; };
     a.RT = tiles(N ? N : 1); a.CT = tiles(K);
     a.ntc = (K + 32 * a.CT - 1) / (32 * a.CT);
     a.nt = ((N ? N : 1) + 32 * a.RT - 1) / (32 * a.RT) * a.ntc;
-    a.wblocks = (long)B * a.NB * 2;
-    const long wgs = a.RT * a.CT >= 8 ? 256 : a.RT * a.CT >= 4 ? 512 : 768;
+    const long wgs = a.RT * a.CT >= 8 ? 256 : 512;
     long sl = wgs / a.nt > 1 ? wgs / a.nt : 1;
-    if (sl > (a.wblocks + 3) / 4) sl = (a.wblocks + 3) / 4;
-    a.wper = (a.wblocks + 4 * sl - 1) / (4 * sl);
-    a.slices = (int)((a.wblocks + 4 * a.wper - 1) / (4 * a.wper));
+    if (sl > (a.wsteps + 7) / 8) sl = (a.wsteps + 7) / 8;
+    a.wper = (a.wsteps + 4 * sl - 1) / (4 * sl);
+    a.slices = (int)((a.wsteps + 4 * a.wper - 1) / (4 * a.wper));
     return P2N_OK;
 }
 
@@ -904,19 +952,23 @@ int act8_launch_gemm(const Act8Gemm &g, long groups, hipStream_t s) {
     return act8_launch_gemm_tab<IN, EPI, 512>(g, groups, s);
 }
 
-template <int RT>
+template <int RT, bool DMA>
 int act8_launch_wgrad_rt(const Act8 &a, const Act8Wgrad &w, hipStream_t s) {
     const dim3 grid((unsigned)(a.nt * a.slices)), blk(256);
     switch (a.CT) {
-        case 1: hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 1>), grid, blk, 0, s, w); break;
-        case 2: hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 2>), grid, blk, 0, s, w); break;
-        default: hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 4>), grid, blk, 0, s, w);
+        case 1: hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 1, DMA>), grid, blk, 0, s, w); break;
+        case 2: hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 2, DMA>), grid, blk, 0, s, w); break;
+        default: hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 4, DMA>), grid, blk, 0, s, w);
     }
     P2N_CHECK_HIP(hipGetLastError());
     return P2N_OK;
 }
+template <bool DMA>
+int act8_launch_wgrad_any(const Act8 &a, const Act8Wgrad &w, hipStream_t s) {
+    return a.RT == 1 ? act8_launch_wgrad_rt<1, DMA>(a, w, s) : a.RT == 2 ? act8_launch_wgrad_rt<2, DMA>(a, w, s) : act8_launch_wgrad_rt<4, DMA>(a, w, s);
+}
 int act8_launch_wgrad(const Act8 &a, const Act8Wgrad &w, hipStream_t s) {
-    return a.RT == 1 ? act8_launch_wgrad_rt<1>(a, w, s) : a.RT == 2 ? act8_launch_wgrad_rt<2>(a, w, s) : act8_launch_wgrad_rt<4>(a, w, s);
+    return a.L % 4 == 0 && ((uintptr_t)w.g & 15) == 0 ? act8_launch_wgrad_any<true>(a, w, s) : act8_launch_wgrad_any<false>(a, w, s);
 }
 
 int act8_space_check(const char *fn, const void *p, size_t have, size_t need, const char *what) {
@@ -1029,7 +1081,7 @@ extern "C" int p2n_act8_backward(const float *g, int B, int K, long L, const flo
     if (dW || db) {
         Act8Wgrad w = {};
         w.g = g; w.codes = codes; w.scale = scale; w.bits = bits; w.gamma = gamma; w.beta = beta; w.part = f.wpart;
-        w.L = L; w.NB = a.NB; w.blocks = a.wblocks; w.per = a.wper; w.N = N; w.K = K; w.K4 = K4; w.ntc = a.ntc; w.slices = a.slices;
+        w.L = L; w.NB = a.NB; w.steps = a.wsteps; w.per = a.wper; w.N = N; w.K = K; w.K4 = K4; w.ntc = a.ntc; w.slices = a.slices;
         TRY(act8_launch_wgrad(a, w, s));
         const long n = (long)N * K + N;
         hipLaunchKernelGGL(p2n_act8_join_kernel, dim3((unsigned)((n + 31) / 32)), dim3(1024), 0, s, f.wpart, n, (long)N * K, a.slices, dW, db);
