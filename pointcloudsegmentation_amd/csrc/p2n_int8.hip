@@ -123,52 +123,122 @@ __global__ __launch_bounds__(256) void p2n_quantize_tokens_kernel(const TX *__re
     for (int k = lane; k < K; k += 64) codes[t * K + k] = bad ? 0 : (signed char)p2n_q8_decide(int8_load(row + k), Q);
 }
 
-// The same into fragments: tile tt of 32 tokens, fragment tt * KT + kt laid out as in the weight image; scales (32 TT).
-// A workgroup takes one tile of tokens; lane = (token, half), a wave every fourth k-tile.  Tokens behind the last one
-// have code and scale 0.
-template <typename TX>
-__global__ __launch_bounds__(256) void p2n_int8_tile_kernel(const TX *__restrict__ x, long T, int K, long ld, int KT, char *__restrict__ img,
-                                                            float *__restrict__ scale) {
-    __shared__ unsigned sh[4][32];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int r = lane & 31, h = lane >> 5;
-    const long tt = blockIdx.x, t = tt * 32 + r;
-    const TX *row = x + (t < T ? t : T - 1) * ld;
-    unsigned am = 0;
-    for (int kt = wave; kt < KT; kt += 4)
+// The 16 values of a token that one lane of a fragment holds: k = 32kt + 8g + 4h + j, g and j from 0 to 3.  f32: four 16-byte loads
+// from any 4-byte address, bf16: four 8-byte loads (VEC: rows start on 4 bytes) or value by value.
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef __bf16 bf16x4u __attribute__((ext_vector_type(4), aligned(4)));
+template <bool VEC>
+__device__ __forceinline__ void int8_chunk(const float *row, int K, int k, float (&v)[4]) {
+    if (k + 4 <= K) {
+        const f32x4u e = *reinterpret_cast<const f32x4u *>(row + k);
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
+        for (int j = 0; j < 4; ++j) v[j] = e[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = k + j < K ? row[k + j] : 0.f;
+    }
+}
+template <bool VEC>
+__device__ __forceinline__ void int8_chunk(const __bf16 *row, int K, int k, float (&v)[4]) {
+    if (VEC && k + 4 <= K) {
+        const bf16x4u e = *reinterpret_cast<const bf16x4u *>(row + k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = (float)e[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = k + j < K ? (float)row[k + j] : 0.f;
+    }
+}
+
+// One token into fragments by 1 << shift lanes (2 * KT of them at least, or 64): lane i of them takes half i & 1 of k-tiles i >> 1,
+// (i >> 1) + 32, ...; put(kt, h, codes) stores 16 bytes.  Up to HOLD rounds of 1024 values stay in registers between the maximum and
+// the codes, longer rows are read twice.  Returns the token's scale.
+#define INT8_HOLD 4
+template <bool VEC, typename TX, typename PUT>
+__device__ __forceinline__ float int8_token(const TX *row, int K, int KT, int i, int shift, PUT put) {
+    const int h = i & 1, kstep = 1 << (shift - 1), rounds = (KT + kstep - 1) >> (shift - 1);
+    float v[INT8_HOLD][16];
+    unsigned am = 0;
+#pragma unroll
+    for (int n = 0; n < INT8_HOLD; ++n) {
+        const int kt = n * kstep + (i >> 1);
+        if (n < rounds) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                float e[4];
+                int8_chunk<VEC>(row, K, 32 * kt + 8 * g + 4 * h, e);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[n][4 * g + j] = e[j];
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < INT8_HOLD; ++n)
+        if (n < rounds) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const unsigned u = p2n_absbits(v[n][e]);
+                am = u > am ? u : am;
+            }
+        }
+    for (int n = INT8_HOLD; n < rounds; ++n) {
+        const int kt = n * kstep + (i >> 1);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float e[4];
+            int8_chunk<VEC>(row, K, 32 * kt + 8 * g + 4 * h, e);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int k = 32 * kt + 8 * g + 4 * h + j;
-                const unsigned b = p2n_absbits(int8_load(row + (k < K ? k : K - 1)));   // a value read twice moves no maximum
-                am = b > am ? b : am;
+                const unsigned u = p2n_absbits(e[j]);
+                am = u > am ? u : am;
             }
-    {
-        const unsigned o = (unsigned)__shfl_xor((int)am, 32);
+        }
+    }
+    for (int m = 1; m < 1 << shift; m <<= 1) {
+        const unsigned o = (unsigned)__shfl_xor((int)am, m);
         am = o > am ? o : am;
     }
-    if (h == 0) sh[wave][r] = am;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 4; ++w) am = sh[w][r] > am ? sh[w][r] : am;
-    const float s = t < T ? p2n_q8_scale(am) : 0.f;
+    const float s = p2n_q8_scale(am);
     const P2nQ8 Q = p2n_q8_make(s);
-    if (wave == 0 && h == 0) scale[t] = s;
-    for (int kt = wave; kt < KT; kt += 4) {
-        float v[16];
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int k = 32 * kt + 8 * g + 4 * h + j;
-                const float e = int8_load(row + (k < K ? k : K - 1));
-                v[4 * g + j] = k < K ? e : 0.f;
-            }
-        int c[4];
-        p2n_q8_pack(v, Q, c);
-        *reinterpret_cast<i32x4 *>(img + ((tt * KT + kt) * 64 + lane) * 16) = i32x4{c[0], c[1], c[2], c[3]};
+    for (int n = 0; n < INT8_HOLD; ++n) {
+        const int kt = n * kstep + (i >> 1);
+        if (n < rounds) {
+            int c[4];
+            p2n_q8_pack(v[n], Q, c);
+            if (kt < KT) put(kt, h, i32x4{c[0], c[1], c[2], c[3]});
+        }
     }
+    for (int n = INT8_HOLD; n < rounds; ++n) {
+        const int kt = n * kstep + (i >> 1);
+        float e[16];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float q[4];
+            int8_chunk<VEC>(row, K, 32 * kt + 8 * g + 4 * h, q);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) e[4 * g + j] = q[j];
+        }
+        int c[4];
+        p2n_q8_pack(e, Q, c);
+        if (kt < KT) put(kt, h, i32x4{c[0], c[1], c[2], c[3]});
+    }
+    return s;
+}
+
+// Tokens into fragments: tile tt of 32 tokens, fragment tt * KT + kt laid out as in the weight image; scales (32 TT).  The rows behind
+// the last token of a tile are left as they are: what they give is not stored.
+template <typename TX, bool VEC>
+__global__ __launch_bounds__(256) void p2n_int8_tile_kernel(const TX *__restrict__ x, long T, int K, long ld, int KT, int shift, char *__restrict__ img,
+                                                            float *__restrict__ scale) {
+    const long t = ((long)blockIdx.x * 256 + threadIdx.x) >> shift;
+    const int i = threadIdx.x & ((1 << shift) - 1);
+    const bool real = t < T;                                   // every lane stays: the maximum is taken over whole waves
+    char *dst = img + ((t >> 5) * KT * 64 + (t & 31)) * 16;
+    const float s = int8_token<VEC>(x + (real ? t : T - 1) * ld, K, KT, i, shift, [&](int kt, int h, i32x4 c) {
+        if (real) *reinterpret_cast<i32x4 *>(dst + ((long)kt * 64 + 32 * h) * 16) = c;
+    });
+    if (real && i == 0) scale[t] = s;
 }
 
 __device__ __forceinline__ void int8_store(float *p, float v) { *p = v; }
@@ -180,44 +250,187 @@ __device__ __forceinline__ float int8_value(int acc, float sx, float sw, float b
 }
 
 // ---------------------------------------------------------------- product of fragments
-// D = X . W^T, registers = tokens, lane = channel: a workgroup of four waves makes 128 tokens x 128 channels, a wave 64 x 64.
-template <typename TY>
-__global__ __launch_bounds__(256) void p2n_int8_gemm_kernel(const char *__restrict__ xi, const float *__restrict__ sx, const char *__restrict__ wi,
-                                                            const float *__restrict__ sw, const float *__restrict__ bias, long T, int N, int TT, int CT,
-                                                            int KT, int relu, TY *__restrict__ y) {
+// D = X . W^T, registers = tokens, lane = channel.  Four waves make 64 TM tokens x 64 TM channels, a wave 32 TM x 32 TM.  Both operands
+// pass through LDS by DMA, 64 values of k at a time, in a ring of four; a read of the next fragments is always on its
+// way while the matrix cores work on the present ones.
+typedef __attribute__((address_space(3))) void int8_lds_t;
+
+template <typename TY, int TM>
+__global__ __launch_bounds__(256, TM >= 4 ? 1 : TM == 2 ? 2 : 4) void p2n_int8_gemm_kernel(const char *__restrict__ xi, const float *__restrict__ sx,
+                                                                                          const char *__restrict__ wi, const float *__restrict__ sw,
+                                                                                          const float *__restrict__ bias, long T, int N, long TT, int CT, int KT,
+                                                                                          int relu, int gx, long tiles, TY *__restrict__ y) {
+    constexpr int STAGE = 8 * TM * 1024;              // 2 TM tiles of tokens and of channels, two k-tiles each
+    constexpr int GROUP = 2 * TM;                     // DMA instructions of a wave and stage
+    __shared__ __attribute__((aligned(16))) char ring[4 * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int r = lane & 31, h = lane >> 5;
-    const int t0 = blockIdx.y * 4 + (wave >> 1) * 2, c0 = blockIdx.x * 4 + (wave & 1) * 2;
-    if (t0 >= TT || c0 >= CT) return;
-    const i32x4 *xa = reinterpret_cast<const i32x4 *>(xi) + lane, *wb = reinterpret_cast<const i32x4 *>(wi) + lane;
-    const int t1 = t0 + 1 < TT ? t0 + 1 : t0, c1 = c0 + 1 < CT ? c0 + 1 : c0;
-    i32x16 acc[2][2];
+    // neighbouring workgroups go to the eight dies in turn: each die takes a band of the tiles, in squares of 4 rows, so
+    // that what its L2 holds is used by several workgroups
+    const long per = (tiles + 7) / 8, id = (long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (id >= tiles) return;
+    const long gy = tiles / gx, band = id / (4L * gx), rows = gy - 4 * band < 4 ? gy - 4 * band : 4, in = id - band * 4 * gx;
+    const long t0 = (4 * band + in % rows) * 2 * TM;
+    const int c0 = (int)(in / rows) * 2 * TM;
+    const int ns = KT / 2;                            // stages (KT is even)
+    // waves 0, 1 fetch the tokens' tiles, waves 2, 3 the channels'; tiles past the last one fetch that
+    const char *src[TM];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < TM; ++i) {
+        const int tile = (wave & 1) * TM + i;
+        const long at = wave < 2 ? (t0 + tile < TT ? t0 + tile : TT - 1) : (c0 + tile < CT ? c0 + tile : CT - 1);
+        src[i] = (wave < 2 ? xi : wi) + at * KT * 1024;
+    }
+    auto stage = [&](int s) __attribute__((always_inline)) {
+        const int k = s < ns ? s : ns - 1;            // past the end the last stage again: the count of outstanding loads stays the same
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int i = 0; i < TM; ++i) {
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(src[i]), 0, KT * 1024, 0x00020000);
+            char *dst = ring + (s & 3) * STAGE + (wave * TM + i) * 2048;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (int8_lds_t *)dst, 16, lane * 16, k * 2048, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (int8_lds_t *)(dst + 1024), 16, lane * 16, k * 2048 + 1024, 0, 0);
+        }
+    };
+    const int wr = wave >> 1, wc = wave & 1;
+    i32x4 fa[2][TM], fb[2][TM];
+    auto read = [&](int s, int kt, i32x4 (&a)[TM], i32x4 (&b)[TM]) __attribute__((always_inline)) {
+        const char *base = ring + (s & 3) * STAGE + kt * 1024 + lane * 16;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            a[i] = *reinterpret_cast<const i32x4 *>(base + (wr * TM + i) * 2048);
+            b[i] = *reinterpret_cast<const i32x4 *>(base + (2 * TM + wc * TM + i) * 2048);
+        }
+    };
+    i32x16 acc[TM][TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int c = 0; c < TM; ++c)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][c][e] = 0;
-    for (int kt = 0; kt < KT; ++kt) {
-        const i32x4 a0 = xa[((long)t0 * KT + kt) * 64], a1 = xa[((long)t1 * KT + kt) * 64];
-        const i32x4 b0 = wb[((long)c0 * KT + kt) * 64], b1 = wb[((long)c1 * KT + kt) * 64];
-        acc[0][0] = MFMA_I8(a0, b0, acc[0][0]);
-        acc[0][1] = MFMA_I8(a0, b1, acc[0][1]);
-        acc[1][0] = MFMA_I8(a1, b0, acc[1][0]);
-        acc[1][1] = MFMA_I8(a1, b1, acc[1][1]);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        stage(s);
+        __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_waitcnt(((3 * GROUP) & 15) | (7 << 4) | (((3 * GROUP) >> 4) << 14));       // stage 0 has arrived
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(0, 0, fa[0], fb[0]);
+#pragma unroll 1
+    for (int s = 0; s < ns; ++s) {
+        __builtin_amdgcn_sched_barrier(0);
+        read(s, 1, fa[1], fb[1]);
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        const int n = 32 * (c0 + c) + r;
-        if (n >= N) continue;
-        const float w = sw[n], b = bias[n];
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+            for (int c = 0; c < TM; ++c) acc[i][c] = MFMA_I8(fa[0][i], fb[0][c], acc[i][c]);
+        __builtin_amdgcn_sched_barrier(0);
+        // stage s+1 has arrived everywhere, and every wave has read the last of stage s, whose place stage s+4 takes
+        __builtin_amdgcn_s_waitcnt(((2 * GROUP) & 15) | (7 << 4) | (0 << 8) | (((2 * GROUP) >> 4) << 14));
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        stage(s + 4);
+        read(s + 1, 0, fa[0], fb[0]);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const long t = 32L * (t0 + i) + 8 * (e >> 2) + 4 * h + (e & 3);
-                if (t < T) int8_store(y + t * N + n, int8_value(acc[i][c][e], sx[t], w, b, relu));
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int c = 0; c < TM; ++c) acc[i][c] = MFMA_I8(fa[1][i], fb[1][c], acc[i][c]);
+    }
+    __builtin_amdgcn_s_waitcnt(7 << 4);               // nothing may be on its way into LDS when the workgroup ends
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < TM; ++c) {
+        const int n = 32 * (c0 + wc * TM + c) + r;
+        const bool col = n < N;
+        const float w = col ? sw[n] : 0.f, b = col ? bias[n] : 0.f;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const long t = 32L * (t0 + wr * TM + i) + 8 * g + 4 * h;
+                if (t >= T) continue;
+                const f32x4 s4 = *reinterpret_cast<const f32x4 *>(sx + t);      // the scales of a tile are 32, written or not
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (col && t + j < T) int8_store(y + (t + j) * N + n, int8_value(acc[i][c][4 * g + j], s4[j], w, b, relu));
             }
+    }
+}
+
+// ---------------------------------------------------------------- few tokens
+// Up to 16 TT tokens: the weights' way from memory is the time, so a workgroup takes 16 channels and its eight waves share the length
+// K, each streaming its part of the weights straight from memory into 16 x 16 x 64 products; the eight sums meet in LDS
+// (whole numbers: any order).  OWN: up to 8 tokens of up to 4096 values are put into 8 bits here, a wave a token, into
+// LDS; otherwise the tokens' fragments come from p2n_int8_tile_kernel.
+#define MFMA_I8_16(a, b, c) __builtin_amdgcn_mfma_i32_16x16x64_i8((a), (b), (c), 0, 0, 0)
+#define INT8_OWN_K 4096
+template <typename TX, int TT, bool OWN, bool VEC>
+__global__ __launch_bounds__(512) void p2n_int8_few_kernel(const TX *__restrict__ x, int T, int K, long ld, const char *__restrict__ xi, const float *__restrict__ sx,
+                                                           const char *__restrict__ wi, const float *__restrict__ sw, const float *__restrict__ bias, int N,
+                                                           int KT, int relu, TX *__restrict__ y) {
+    __shared__ __attribute__((aligned(16))) char own[OWN ? 8 * INT8_OWN_K : 16];      // [k-tile][half][8 tokens][16 codes]
+    __shared__ float ssx[16 * TT];
+    __shared__ int red[8][TT][256];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int r = lane & 15, q = lane >> 4;           // operand lane: row r, 16 codes of k-tile 2kb + (q >> 1), half q & 1
+    const int c0 = blockIdx.x * 16;
+    const char *wb = wi + ((long)(c0 >> 5) * KT * 64 + (q >> 1) * 64 + (q & 1) * 32 + (c0 & 16) + r) * 16;
+    const int nb = KT / 2;
+    constexpr int AHEAD = 8;                          // k-blocks of a wave whose weights are on their way at once
+    i32x4 w[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+        const int kb = wave + 8 * i;
+        w[i] = *reinterpret_cast<const i32x4 *>(wb + (long)(kb < nb ? kb : 0) * 2048);
+    }
+    if (OWN) {
+        if (wave < T) {
+            const float s = int8_token<VEC>(x + (long)wave * ld, K, KT, lane, 6, [&](int kt, int h, i32x4 c) {
+                *reinterpret_cast<i32x4 *>(own + ((kt * 2 + h) * 8 + wave) * 16) = c;
+            });
+            if (lane == 0) ssx[wave] = s;
+        }
+    } else if ((int)threadIdx.x < 16 * TT) {
+        ssx[threadIdx.x] = (int)threadIdx.x < T ? sx[threadIdx.x] : 0.f;
+    }
+    if (OWN) __syncthreads();
+    i32x4 acc[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[t] = i32x4{0, 0, 0, 0};
+    for (int k0 = wave; k0 < nb; k0 += 8 * AHEAD) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int kb = k0 + 8 * i;
+            if (kb < nb) {
+#pragma unroll
+                for (int t = 0; t < TT; ++t) {
+                    i32x4 a;
+                    if (OWN) a = *reinterpret_cast<const i32x4 *>(own + (((2 * kb + (q >> 1)) * 2 + (q & 1)) * 8 + (r & 7)) * 16);
+                    else a = *reinterpret_cast<const i32x4 *>(xi + (((long)(t >> 1) * KT + 2 * kb + (q >> 1)) * 64 + (q & 1) * 32 + 16 * (t & 1) + r) * 16);
+                    acc[t] = MFMA_I8_16(a, w[i], acc[t]);
+                }
+            }
+            const int kn = kb + 8 * AHEAD;
+            if (kn < nb) w[i] = *reinterpret_cast<const i32x4 *>(wb + (long)kn * 2048);
+        }
+    }
+    // D: column = lane & 15 (channel), row = 4 (lane >> 4) + register (token)
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) red[wave][t][(4 * q + e) * 16 + r] = acc[t][e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < TT * 256; i += 512) {
+        const int t = i >> 4, n = c0 + (i & 15);
+        if (t >= T || n >= N) continue;
+        int sum = 0;
+#pragma unroll
+        for (int v = 0; v < 8; ++v) sum += red[v][i >> 8][i & 255];
+        int8_store(y + (long)t * N + n, int8_value(sum, ssx[t], sw[n], bias[n], relu));
     }
 }
 
@@ -240,26 +453,58 @@ extern "C" int p2n_quantize_tokens(const void *x, int bf16, long T, int K, long 
     return P2N_OK;
 }
 
+// Which kernel: up to 64 tokens the one that streams the weights once (16 tokens x 4096 x 4096: 7 us against 49 with 128 x 128
+// tiles), and of these up to 8 tokens of up to 4096 values put into 8 bits on the way (one launch instead of two).
+static bool int8_is_few(long T) { return T <= 64; }
+static bool int8_is_own(long T, int K) { return T <= 8 && K <= INT8_OWN_K; }
+
 extern "C" size_t p2n_int8_linear_workspace_bytes(long T, int K, int N) {
     if (T < 1 || T >= (1L << 31) || K < 1 || K > INT8_MAX_K || N < 1 || N > INT8_MAX_N) return 0;
-    return int8_tiles_bytes(T, K);
+    return int8_is_own(T, K) ? 0 : int8_tiles_bytes(T, K);
 }
 
-template <typename TX>
+template <typename TX, bool VEC>
+static void int8_launch_few(const TX *x, int T, int K, long ld, const char *ws, const float *sx, const char *img, int N, int relu, TX *y, hipStream_t s) {
+    const Int8Image I = int8_image(K, N);
+    const float *sw = (const float *)(img + I.scale), *b = (const float *)(img + I.bias);
+    const dim3 grid((unsigned)((N + 15) / 16)), blk(512);
+    if (int8_is_own(T, K)) hipLaunchKernelGGL((p2n_int8_few_kernel<TX, 1, true, VEC>), grid, blk, 0, s, x, T, K, ld, nullptr, nullptr, img, sw, b, N, I.KT, relu, y);
+    else if (T <= 16) hipLaunchKernelGGL((p2n_int8_few_kernel<TX, 1, false, VEC>), grid, blk, 0, s, x, T, K, ld, ws, sx, img, sw, b, N, I.KT, relu, y);
+    else if (T <= 32) hipLaunchKernelGGL((p2n_int8_few_kernel<TX, 2, false, VEC>), grid, blk, 0, s, x, T, K, ld, ws, sx, img, sw, b, N, I.KT, relu, y);
+    else hipLaunchKernelGGL((p2n_int8_few_kernel<TX, 4, false, VEC>), grid, blk, 0, s, x, T, K, ld, ws, sx, img, sw, b, N, I.KT, relu, y);
+}
+
+template <typename TX, int TM>
+static void int8_launch_gemm(const char *ws, const float *sx, const char *img, const Int8Image &I, long T, int N, int relu, TX *y, hipStream_t s) {
+    const long TT = (T + 31) / 32, gy = (TT + 2 * TM - 1) / (2 * TM);
+    const int gx = (I.CT + 2 * TM - 1) / (2 * TM);
+    const long tiles = gx * gy;
+    hipLaunchKernelGGL((p2n_int8_gemm_kernel<TX, TM>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(256), 0, s, ws, sx, img, (const float *)(img + I.scale),
+                       (const float *)(img + I.bias), T, N, TT, I.CT, I.KT, relu, gx, tiles, y);
+}
+
+template <typename TX, bool VEC>
 static int int8_linear_run(const TX *x, long T, int K, long ld, const char *img, int N, int relu, TX *y, char *ws, hipStream_t s) {
     const Int8Image I = int8_image(K, N);
     const long TT = (T + 31) / 32;
     float *sx = (float *)(ws + (size_t)TT * I.KT * 1024);
-    hipLaunchKernelGGL(p2n_int8_tile_kernel<TX>, dim3((unsigned)TT), dim3(256), 0, s, x, T, K, ld, I.KT, ws, sx);
-    P2N_CHECK_HIP(hipGetLastError());
-    for (long t0 = 0; t0 < TT; t0 += 4L * 65535) {   // grid.y holds 65,535 workgroups
-        const long n = TT - t0 < 4L * 65535 ? TT - t0 : 4L * 65535;
-        const long rows = T - 32 * t0;
-        hipLaunchKernelGGL(p2n_int8_gemm_kernel<TX>, dim3((unsigned)((I.CT + 3) / 4), (unsigned)((n + 3) / 4)), dim3(256), 0, s, ws + (size_t)t0 * I.KT * 1024,
-                           sx + 32 * t0, img, (const float *)(img + I.scale), (const float *)(img + I.bias), rows, N, (int)n, I.CT, I.KT, relu,
-                           y + 32 * t0 * N);
+    if (!int8_is_own(T, K)) {
+        int shift = 1;                                // lanes of a token: enough for its k-tiles' halves, at most a wave
+        while (shift < 6 && (1 << shift) < 2 * I.KT) ++shift;
+        hipLaunchKernelGGL((p2n_int8_tile_kernel<TX, VEC>), dim3((unsigned)(((T << shift) + 255) / 256)), dim3(256), 0, s, x, T, K, ld, I.KT, shift, ws, sx);
         P2N_CHECK_HIP(hipGetLastError());
     }
+    if (int8_is_few(T)) {
+        int8_launch_few<TX, VEC>(x, (int)T, K, ld, ws, sx, img, N, relu, y, s);
+    } else {
+        // the largest tile that still gives the 256 compute units a workgroup each: larger tiles read less, fewer of them leave
+        // compute units idle
+        auto tiles = [&](int tm) { return ((TT + 2 * tm - 1) / (2 * tm)) * ((I.CT + 2 * tm - 1) / (2 * tm)); };
+        if (tiles(4) >= 256) int8_launch_gemm<TX, 4>(ws, sx, img, I, T, N, relu, y, s);
+        else if (tiles(2) >= 256) int8_launch_gemm<TX, 2>(ws, sx, img, I, T, N, relu, y, s);
+        else int8_launch_gemm<TX, 1>(ws, sx, img, I, T, N, relu, y, s);
+    }
+    P2N_CHECK_HIP(hipGetLastError());
     return P2N_OK;
 }
 
@@ -270,15 +515,19 @@ extern "C" int p2n_int8_linear(const void *x, int bf16, long T, int K, long ld, 
     if (T == 0) return P2N_OK;
     P2N_REQUIRE(x && image && y, "p2n_int8_linear: null pointer");
     const size_t need = p2n_int8_linear_workspace_bytes(T, K, N);
-    if (!workspace || workspace_bytes < need) {
+    if (need && (!workspace || workspace_bytes < need)) {
         p2n_set_error("p2n_int8_linear: workspace %zu bytes < required %zu", workspace_bytes, need);
         return P2N_EWORKSPACE;
     }
     P2N_REQUIRE((((uintptr_t)workspace | (uintptr_t)image) & 15) == 0, "p2n_int8_linear: workspace and image must be 16-byte aligned");
     hipStream_t s = (hipStream_t)stream_;
     const int ps = p2n_prof_begin(P2N_K_INT8_GEMM, s);
-    const int rc = bf16 ? int8_linear_run<__bf16>((const __bf16 *)x, T, K, ld, (const char *)image, N, relu, (__bf16 *)y, (char *)workspace, s)
-                        : int8_linear_run<float>((const float *)x, T, K, ld, (const char *)image, N, relu, (float *)y, (char *)workspace, s);
+    const bool vec = ld % 2 == 0 && ((uintptr_t)x & 3) == 0;        // bfloat16 rows that start on 4 bytes
+    const char *img = (const char *)image;
+    char *ws = (char *)workspace;
+    const int rc = !bf16 ? int8_linear_run<float, true>((const float *)x, T, K, ld, img, N, relu, (float *)y, ws, s)
+                   : vec ? int8_linear_run<__bf16, true>((const __bf16 *)x, T, K, ld, img, N, relu, (__bf16 *)y, ws, s)
+                         : int8_linear_run<__bf16, false>((const __bf16 *)x, T, K, ld, img, N, relu, (__bf16 *)y, ws, s);
     p2n_prof_end(ps, s);
     return rc;
 }

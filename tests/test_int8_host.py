@@ -16,7 +16,8 @@ def test_library_refuses_bad_shapes():
     assert lib.p2n_quantize_tokens(None, 0, 0, 8, 8, None, None, None) == 0
     assert lib.p2n_int8_linear(None, 0, 4, 8, 8, None, 4, 0, None, None, 0, None) == 1
     assert lib.p2n_int8_linear(None, 0, 0, 8, 8, None, 4, 0, None, None, 0, None) == 0
-    assert lib.p2n_int8_linear(16, 0, 4, 8, 8, 16, 4, 0, 16, 16, 1, None) == 2       # workspace too small
+    assert lib.p2n_int8_linear_workspace_bytes(4, 8, 4) == 0 and lib.p2n_int8_linear_workspace_bytes(100, 8, 4) == 4 * 2048 + 4 * 128
+    assert lib.p2n_int8_linear(16, 0, 100, 8, 8, 16, 4, 0, 16, 16, 1, None) == 2     # workspace too small
     assert b"workspace" in lib.p2n_last_error()
     dims = (ctypes.c_int * 3)(6, 32, 300)
     images = (ctypes.c_void_p * 2)(16, 16)
