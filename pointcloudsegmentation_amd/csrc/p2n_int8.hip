@@ -150,12 +150,12 @@ __device__ __forceinline__ void int8_chunk(const __bf16 *row, int K, int k, floa
     }
 }
 
-// One token into fragments by 1 << shift lanes (2 * KT of them at least, or 64): lane i of them takes half i & 1 of k-tiles i >> 1,
-// (i >> 1) + 32, ...; put(kt, h, codes) stores 16 bytes.  Up to HOLD rounds of 1024 values stay in registers between the maximum and
-// the codes, longer rows are read twice.  Returns the token's scale.
+// One token into fragments by 1 << shift lanes: lane i of them takes half i & 1 of k-tiles i >> 1, (i >> 1) + (1 << shift - 1), ...;
+// put(kt, h, codes) stores 16 bytes.  Up to HOLD such rounds stay in registers between the maximum and the codes, longer
+// rows are read twice.  `across` takes the maximum over the waves of a token.  Returns the token's scale.
 #define INT8_HOLD 4
-template <bool VEC, typename TX, typename PUT>
-__device__ __forceinline__ float int8_token(const TX *row, int K, int KT, int i, int shift, PUT put) {
+template <bool VEC, typename TX, typename PUT, typename MAX>
+__device__ __forceinline__ float int8_token(const TX *row, int K, int KT, int i, int shift, PUT put, MAX across) {
     const int h = i & 1, kstep = 1 << (shift - 1), rounds = (KT + kstep - 1) >> (shift - 1);
     float v[INT8_HOLD][16];
     unsigned am = 0;
@@ -194,11 +194,11 @@ __device__ __forceinline__ float int8_token(const TX *row, int K, int KT, int i,
             }
         }
     }
-    for (int m = 1; m < 1 << shift; m <<= 1) {
+    for (int m = 1; m < 1 << shift && m < 64; m <<= 1) {
         const unsigned o = (unsigned)__shfl_xor((int)am, m);
         am = o > am ? o : am;
     }
-    const float s = p2n_q8_scale(am);
+    const float s = p2n_q8_scale(across(am));
     const P2nQ8 Q = p2n_q8_make(s);
 #pragma unroll
     for (int n = 0; n < INT8_HOLD; ++n) {
@@ -231,12 +231,24 @@ __device__ __forceinline__ float int8_token(const TX *row, int K, int KT, int i,
 template <typename TX, bool VEC>
 __global__ __launch_bounds__(256) void p2n_int8_tile_kernel(const TX *__restrict__ x, long T, int K, long ld, int KT, int shift, char *__restrict__ img,
                                                             float *__restrict__ scale) {
+    __shared__ unsigned sh[4];
     const long t = ((long)blockIdx.x * 256 + threadIdx.x) >> shift;
     const int i = threadIdx.x & ((1 << shift) - 1);
     const bool real = t < T;                                   // every lane stays: the maximum is taken over whole waves
     char *dst = img + ((t >> 5) * KT * 64 + (t & 31)) * 16;
     const float s = int8_token<VEC>(x + (real ? t : T - 1) * ld, K, KT, i, shift, [&](int kt, int h, i32x4 c) {
         if (real) *reinterpret_cast<i32x4 *>(dst + ((long)kt * 64 + 32 * h) * 16) = c;
+    }, [&](unsigned am) {
+        if (shift <= 6) return am;
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = am;
+        __syncthreads();
+        const int w0 = shift == 7 ? (threadIdx.x >> 7) * 2 : 0;
+        unsigned m = sh[w0] > sh[w0 + 1] ? sh[w0] : sh[w0 + 1];
+        if (shift == 8) {
+            const unsigned o = sh[2] > sh[3] ? sh[2] : sh[3];
+            m = o > m ? o : m;
+        }
+        return m;
     });
     if (real && i == 0) scale[t] = s;
 }
@@ -250,18 +262,48 @@ __device__ __forceinline__ float int8_value(int acc, float sx, float sw, float b
 }
 
 // ---------------------------------------------------------------- product of fragments
-// D = X . W^T, registers = tokens, lane = channel.  Four waves make 64 TM tokens x 64 TM channels, a wave 32 TM x 32 TM.  Both operands
+// D = X . W^T, registers = tokens, lane = channel.  WR x WC waves of 32 TM tokens x 32 TN channels each.  Both operands
 // pass through LDS by DMA, 64 values of k at a time, in a ring of four; a read of the next fragments is always on its
 // way while the matrix cores work on the present ones.
 typedef __attribute__((address_space(3))) void int8_lds_t;
 
-template <typename TY, int TM>
-__global__ __launch_bounds__(256, TM >= 4 ? 1 : TM == 2 ? 2 : 4) void p2n_int8_gemm_kernel(const char *__restrict__ xi, const float *__restrict__ sx,
+// a tile's results to memory: lane = channel n, v[j] = token t + j
+__device__ __forceinline__ void int8_store4(float *y, long t, long T, int N, int n, bool col, const float (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (col && t + j < T) y[(t + j) * N + n] = v[j];
+}
+// bfloat16: neighbouring lanes exchange, an even lane stores two channels of tokens t and t + 2, an odd one of t + 1 and t + 3, so that a
+// store is a whole dword.  Only where rows start on 4 bytes (N even) and both channels are real.
+__device__ __forceinline__ void int8_store4(__bf16 *y, long t, long T, int N, int n, bool col, const float (&v)[4]) {
+    if (N & 1) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (col && t + j < T) y[(t + j) * N + n] = (__bf16)v[j];
+        return;
+    }
+    const bool odd = n & 1;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+        const float keep = odd ? v[2 * p + 1] : v[2 * p], give = odd ? v[2 * p] : v[2 * p + 1];
+        const float got = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(give), 0xB1, 0xF, 0xF, true));   // lane ^ 1
+        __bf16 two[2];
+        two[0] = (__bf16)(odd ? got : keep);
+        two[1] = (__bf16)(odd ? keep : got);
+        const long tt = t + 2 * p + (odd ? 1 : 0);
+        if (col && tt < T) *reinterpret_cast<unsigned *>(y + tt * N + (n & ~1)) = *reinterpret_cast<const unsigned *>(two);
+    }
+}
+
+template <typename TY, int TM, int TN, int WR, int WC>
+__global__ __launch_bounds__(64 * WR * WC, TM * TN >= 4 ? 2 : 4) void p2n_int8_gemm_kernel(const char *__restrict__ xi, const float *__restrict__ sx,
                                                                                           const char *__restrict__ wi, const float *__restrict__ sw,
                                                                                           const float *__restrict__ bias, long T, int N, long TT, int CT, int KT,
                                                                                           int relu, int gx, long tiles, TY *__restrict__ y) {
-    constexpr int STAGE = 8 * TM * 1024;              // 2 TM tiles of tokens and of channels, two k-tiles each
-    constexpr int GROUP = 2 * TM;                     // DMA instructions of a wave and stage
+    constexpr int TILES = WR * TM + WC * TN, TPW = TILES / (WR * WC);       // 32-row tiles of both operands; fetched by a wave
+    static_assert(TPW * WR * WC == TILES, "every wave fetches the same number of tiles");
+    constexpr int STAGE = TILES * 2048;               // two k-tiles each
+    constexpr int GROUP = 2 * TPW;                    // DMA instructions of a wave and stage
     __shared__ __attribute__((aligned(16))) char ring[4 * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int r = lane & 31, h = lane >> 5;
@@ -270,42 +312,40 @@ __global__ __launch_bounds__(256, TM >= 4 ? 1 : TM == 2 ? 2 : 4) void p2n_int8_g
     const long per = (tiles + 7) / 8, id = (long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if (id >= tiles) return;
     const long gy = tiles / gx, band = id / (4L * gx), rows = gy - 4 * band < 4 ? gy - 4 * band : 4, in = id - band * 4 * gx;
-    const long t0 = (4 * band + in % rows) * 2 * TM;
-    const int c0 = (int)(in / rows) * 2 * TM;
+    const long t0 = (4 * band + in % rows) * WR * TM;
+    const int c0 = (int)(in / rows) * WC * TN;
     const int ns = KT / 2;                            // stages (KT is even)
-    // waves 0, 1 fetch the tokens' tiles, waves 2, 3 the channels'; tiles past the last one fetch that
-    const char *src[TM];
+    const char *src[TPW];                             // tiles past the last one fetch that
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        const int tile = (wave & 1) * TM + i;
-        const long at = wave < 2 ? (t0 + tile < TT ? t0 + tile : TT - 1) : (c0 + tile < CT ? c0 + tile : CT - 1);
-        src[i] = (wave < 2 ? xi : wi) + at * KT * 1024;
+    for (int i = 0; i < TPW; ++i) {
+        const int tile = wave * TPW + i, ch = tile - WR * TM;
+        const long at = tile < WR * TM ? (t0 + tile < TT ? t0 + tile : TT - 1) : (c0 + ch < CT ? c0 + ch : CT - 1);
+        src[i] = (tile < WR * TM ? xi : wi) + at * KT * 1024;
     }
     auto stage = [&](int s) __attribute__((always_inline)) {
         const int k = s < ns ? s : ns - 1;            // past the end the last stage again: the count of outstanding loads stays the same
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
+        for (int i = 0; i < TPW; ++i) {
             const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(src[i]), 0, KT * 1024, 0x00020000);
-            char *dst = ring + (s & 3) * STAGE + (wave * TM + i) * 2048;
+            char *dst = ring + (s & 3) * STAGE + (wave * TPW + i) * 2048;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (int8_lds_t *)dst, 16, lane * 16, k * 2048, 0, 0);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (int8_lds_t *)(dst + 1024), 16, lane * 16, k * 2048 + 1024, 0, 0);
         }
     };
-    const int wr = wave >> 1, wc = wave & 1;
-    i32x4 fa[2][TM], fb[2][TM];
-    auto read = [&](int s, int kt, i32x4 (&a)[TM], i32x4 (&b)[TM]) __attribute__((always_inline)) {
+    const int wr = wave / WC, wc = wave % WC;
+    i32x4 fa[2][TM], fb[2][TN];
+    auto read = [&](int s, int kt, i32x4 (&a)[TM], i32x4 (&b)[TN]) __attribute__((always_inline)) {
         const char *base = ring + (s & 3) * STAGE + kt * 1024 + lane * 16;
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            a[i] = *reinterpret_cast<const i32x4 *>(base + (wr * TM + i) * 2048);
-            b[i] = *reinterpret_cast<const i32x4 *>(base + (2 * TM + wc * TM + i) * 2048);
-        }
+        for (int i = 0; i < TM; ++i) a[i] = *reinterpret_cast<const i32x4 *>(base + (wr * TM + i) * 2048);
+#pragma unroll
+        for (int i = 0; i < TN; ++i) b[i] = *reinterpret_cast<const i32x4 *>(base + (WR * TM + wc * TN + i) * 2048);
     };
-    i32x16 acc[TM][TM];
+    i32x16 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int c = 0; c < TM; ++c)
+        for (int c = 0; c < TN; ++c)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][c][e] = 0;
 #pragma unroll
@@ -325,7 +365,7 @@ __global__ __launch_bounds__(256, TM >= 4 ? 1 : TM == 2 ? 2 : 4) void p2n_int8_g
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int c = 0; c < TM; ++c) acc[i][c] = MFMA_I8(fa[0][i], fb[0][c], acc[i][c]);
+            for (int c = 0; c < TN; ++c) acc[i][c] = MFMA_I8(fa[0][i], fb[0][c], acc[i][c]);
         __builtin_amdgcn_sched_barrier(0);
         // stage s+1 has arrived everywhere, and every wave has read the last of stage s, whose place stage s+4 takes
         __builtin_amdgcn_s_waitcnt(((2 * GROUP) & 15) | (7 << 4) | (0 << 8) | (((2 * GROUP) >> 4) << 14));
@@ -338,13 +378,13 @@ __global__ __launch_bounds__(256, TM >= 4 ? 1 : TM == 2 ? 2 : 4) void p2n_int8_g
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int c = 0; c < TM; ++c) acc[i][c] = MFMA_I8(fa[1][i], fb[1][c], acc[i][c]);
+            for (int c = 0; c < TN; ++c) acc[i][c] = MFMA_I8(fa[1][i], fb[1][c], acc[i][c]);
     }
     __builtin_amdgcn_s_waitcnt(7 << 4);               // nothing may be on its way into LDS when the workgroup ends
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int c = 0; c < TM; ++c) {
-        const int n = 32 * (c0 + wc * TM + c) + r;
+    for (int c = 0; c < TN; ++c) {
+        const int n = 32 * (c0 + wc * TN + c) + r;
         const bool col = n < N;
         const float w = col ? sw[n] : 0.f, b = col ? bias[n] : 0.f;
 #pragma unroll
@@ -352,11 +392,12 @@ __global__ __launch_bounds__(256, TM >= 4 ? 1 : TM == 2 ? 2 : 4) void p2n_int8_g
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const long t = 32L * (t0 + wr * TM + i) + 8 * g + 4 * h;
-                if (t >= T) continue;
-                const f32x4 s4 = *reinterpret_cast<const f32x4 *>(sx + t);      // the scales of a tile are 32, written or not
+                const bool some = t < T;                                          // (a lane stays for its neighbour's exchange)
+                const f32x4 s4 = *reinterpret_cast<const f32x4 *>(sx + (some ? t : 0));      // the scales of a tile are 32, written or not
+                float v[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (col && t + j < T) int8_store(y + (t + j) * N + n, int8_value(acc[i][c][4 * g + j], s4[j], w, b, relu));
+                for (int j = 0; j < 4; ++j) v[j] = int8_value(acc[i][c][4 * g + j], s4[j], w, b, relu);
+                int8_store4(y, t, T, N, n, col, v);
             }
     }
 }
@@ -391,7 +432,7 @@ __global__ __launch_bounds__(512) void p2n_int8_few_kernel(const TX *__restrict_
         if (wave < T) {
             const float s = int8_token<VEC>(x + (long)wave * ld, K, KT, lane, 6, [&](int kt, int h, i32x4 c) {
                 *reinterpret_cast<i32x4 *>(own + ((kt * 2 + h) * 8 + wave) * 16) = c;
-            });
+            }, [](unsigned am) { return am; });
             if (lane == 0) ssx[wave] = s;
         }
     } else if ((int)threadIdx.x < 16 * TT) {
@@ -474,13 +515,13 @@ static void int8_launch_few(const TX *x, int T, int K, long ld, const char *ws, 
     else hipLaunchKernelGGL((p2n_int8_few_kernel<TX, 4, false, VEC>), grid, blk, 0, s, x, T, K, ld, ws, sx, img, sw, b, N, I.KT, relu, y);
 }
 
-template <typename TX, int TM>
+template <typename TX, int TM, int TN, int WR, int WC>
 static void int8_launch_gemm(const char *ws, const float *sx, const char *img, const Int8Image &I, long T, int N, int relu, TX *y, hipStream_t s) {
-    const long TT = (T + 31) / 32, gy = (TT + 2 * TM - 1) / (2 * TM);
-    const int gx = (I.CT + 2 * TM - 1) / (2 * TM);
+    const long TT = (T + 31) / 32, gy = (TT + WR * TM - 1) / (WR * TM);
+    const int gx = (I.CT + WC * TN - 1) / (WC * TN);
     const long tiles = gx * gy;
-    hipLaunchKernelGGL((p2n_int8_gemm_kernel<TX, TM>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(256), 0, s, ws, sx, img, (const float *)(img + I.scale),
-                       (const float *)(img + I.bias), T, N, TT, I.CT, I.KT, relu, gx, tiles, y);
+    hipLaunchKernelGGL((p2n_int8_gemm_kernel<TX, TM, TN, WR, WC>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * WR * WC), 0, s, ws, sx, img,
+                       (const float *)(img + I.scale), (const float *)(img + I.bias), T, N, TT, I.CT, I.KT, relu, gx, tiles, y);
 }
 
 template <typename TX, bool VEC>
@@ -489,8 +530,11 @@ static int int8_linear_run(const TX *x, long T, int K, long ld, const char *img,
     const long TT = (T + 31) / 32;
     float *sx = (float *)(ws + (size_t)TT * I.KT * 1024);
     if (!int8_is_own(T, K)) {
-        int shift = 1;                                // lanes of a token: enough for its k-tiles' halves, at most a wave
-        while (shift < 6 && (1 << shift) < 2 * I.KT) ++shift;
+        // lanes of a token: 64 values each (the reductions and divisions of a token cost as much as some 20 of them), fewer where that
+        // leaves the card empty: below 2048 threads a compute unit, down to 16 values, at most four waves
+        int shift = 1;
+        while (shift < 8 && (1 << shift) * INT8_HOLD < 2 * I.KT) ++shift;
+        while (shift < 8 && (1 << shift) < 2 * I.KT && (T << shift) < 256 * 2048) ++shift;
         hipLaunchKernelGGL((p2n_int8_tile_kernel<TX, VEC>), dim3((unsigned)(((T << shift) + 255) / 256)), dim3(256), 0, s, x, T, K, ld, I.KT, shift, ws, sx);
         P2N_CHECK_HIP(hipGetLastError());
     }
@@ -500,9 +544,9 @@ static int int8_linear_run(const TX *x, long T, int K, long ld, const char *img,
         // the largest tile that still gives the 256 compute units a workgroup each: larger tiles read less, fewer of them leave
         // compute units idle
         auto tiles = [&](int tm) { return ((TT + 2 * tm - 1) / (2 * tm)) * ((I.CT + 2 * tm - 1) / (2 * tm)); };
-        if (tiles(4) >= 256) int8_launch_gemm<TX, 4>(ws, sx, img, I, T, N, relu, y, s);
-        else if (tiles(2) >= 256) int8_launch_gemm<TX, 2>(ws, sx, img, I, T, N, relu, y, s);
-        else int8_launch_gemm<TX, 1>(ws, sx, img, I, T, N, relu, y, s);
+        if (tiles(4) >= 256) int8_launch_gemm<TX, 4, 2, 2, 4>(ws, sx, img, I, T, N, relu, y, s);
+        else if (tiles(2) >= 256) int8_launch_gemm<TX, 2, 2, 2, 2>(ws, sx, img, I, T, N, relu, y, s);
+        else int8_launch_gemm<TX, 1, 1, 2, 2>(ws, sx, img, I, T, N, relu, y, s);
     }
     P2N_CHECK_HIP(hipGetLastError());
     return P2N_OK;

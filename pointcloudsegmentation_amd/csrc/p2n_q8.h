@@ -43,8 +43,8 @@ __device__ __forceinline__ float p2n_q8_decide(float v, const P2nQ8 &Q) {
 }
 
 // Codes of NV values (a multiple of 4) of one scale, packed four to a dword in order.  Round-to-even of t is the code unless t
-// lies within 1.6e-5 of a tie; the rounding is the addition of 1.5 * 2^23 (one rounding to a whole number, whose low byte
-// is the code).  Any lane near a tie sends its wave through the decision for these values: about one tile in 60.
+// lies within 1.6e-5 of a tie (two roundings of 2^-24 at up to 127.5); the rounding is the addition of 1.5 * 2^23 (one rounding to a whole number, whose low byte
+// is the code).  Any lane near a tie sends its wave through the decision for these values: one time in 25 for 16 values of 64 lanes.
 #define P2N_Q8_MAGIC 12582912.0f
 template <int NV>
 __device__ __forceinline__ void p2n_q8_pack(const float (&v)[NV], const P2nQ8 &Q, int (&code)[NV / 4]) {
@@ -56,7 +56,7 @@ __device__ __forceinline__ void p2n_q8_pack(const float (&v)[NV], const P2nQ8 &Q
         m[i] = __float_as_uint(a);
         near = fmaxf(near, fabsf(t - (a - P2N_Q8_MAGIC)));
     }
-    if (__any(near > 0.4999f)) {
+    if (__any(near > 0.49998f)) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) m[i] = __float_as_uint(p2n_q8_decide(v[i], Q) + P2N_Q8_MAGIC);
     }
