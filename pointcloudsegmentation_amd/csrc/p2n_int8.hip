@@ -56,7 +56,8 @@ __global__ __launch_bounds__(256) void p2n_int8_pack_kernel(const float *__restr
     const P2nQ8 Q = p2n_q8_make(s);
     if (lane == 0) {
         scale[n] = n < N ? s : 0.f;
-        bimg[n] = n < N && bias ? bias[n] : 0.f;
+        // a NaN without a sign: the ReLU of p2n_int8_mlp is a maximum of bit patterns
+        bimg[n] = n < N && bias ? (bias[n] == bias[n] ? bias[n] : __uint_as_float(0x7FC00000u)) : 0.f;
     }
     const int ct = n >> 5, r = n & 31;
     const bool bad = !(s == s);
@@ -601,15 +602,32 @@ __device__ __forceinline__ int int8_key(float v) {
 }
 __device__ __forceinline__ int int8_unkey(int k) { return k ^ ((k >> 31) & 0x7FFFFFFF); }
 
-// The 16 channels 32kt + 8g + 4h + j of this lane's point.  The resource starts at row 32kt and ends with the cloud's last
-// row, so channels past C read as zero; `off` is the lane's byte offset (half's rows and column).
-__device__ __forceinline__ void int8_mlp_load(const float *xb, long L, int C, int kt, int off, float (&v)[16]) {
-    const long left = (long)(C - 32 * kt) * L * 4;
+// The 16 channels 32kt + 8g + 4h + j of this lane's point; `off` is the lane's byte offset (half's rows and column).  The resource
+// starts at row 32kt and ends with the cloud's last row.  In a whole tile the rows' offsets are scalar operands; in the last one
+// of a ragged C they are part of the lane's offset, which the resource's end is checked against (it is not checked with the scalar
+// one): channels past C read as zero, and groups of eight that hold none are not read.
+__device__ __forceinline__ void int8_mlp_load(const float *xb, long L, int C, int kt, unsigned off, float (&v)[16]) {
+    const int real = C - 32 * kt;
+    const long left = (long)real * L * 4;
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(xb + 32L * kt * L), 0,
                                                                          (int)(left < 0xFFFFFFFFL ? left : 0xFFFFFFFFL), 0x00020000);
+    if (real >= 32) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-        v[e] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, off + (int)((8 * (e >> 2) + (e & 3)) * L * 4), 0, 0));
+        for (int e = 0; e < 16; ++e)
+            v[e] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, off, (int)((8 * (e >> 2) + (e & 3)) * L * 4), 0));
+    } else {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            if (8 * g < real) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    v[4 * g + j] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, off + (unsigned)((8 * g + j) * L * 4), 0, 0));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[4 * g + j] = 0.f;
+            }
+        }
+    }
 }
 
 // CTM: channel tiles of the widest layer; KTM >= CTM: k-tiles of the widest operand
@@ -621,30 +639,43 @@ __global__ __launch_bounds__(256, CTM <= 2 ? 4 : CTM <= 4 ? 3 : KTM <= 8 ? 2 : 1
         const long b = tile / A.tiles, l = (tile % A.tiles) * 32 + p;
         const bool valid = l < A.L;
         const float *xb = A.x + b * A.C * A.L;
-        const int off = (int)((4 * h * A.L + (valid ? l : A.L - 1)) * 4);   // bytes; L <= 2^24 keeps 32 rows below 2^31
+        const unsigned off = (unsigned)((4 * h * A.L + (valid ? l : A.L - 1)) * 4);   // bytes; L <= 2^24 keeps 32 rows below 2^31
         const int KT0 = A.layer[0].KT;
-        unsigned am = 0;
-#pragma unroll 1
-        for (int kt = 0; kt < KT0; ++kt) {
-            float v[16];
-            int8_mlp_load(xb, A.L, A.C, kt, off, v);
+        constexpr bool HOLD = KTM <= 2;       // the input stays in registers between its maximum and its codes; longer ones are read twice
+        unsigned am = 0, o;
+        float s, v[HOLD ? KTM : 1][16];
+        int cq[KTM][4];
+        auto top = [&](const float (&e)[16]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const unsigned u = p2n_absbits(v[e]);
+            for (int i = 0; i < 16; ++i) {
+                const unsigned u = p2n_absbits(e[i]);
                 am = u > am ? u : am;
             }
+        };
+        if constexpr (HOLD) {
+#pragma unroll
+            for (int kt = 0; kt < KTM; ++kt)
+                if (kt < KT0) int8_mlp_load(xb, A.L, A.C, kt, off, v[kt]);
+#pragma unroll
+            for (int kt = 0; kt < KTM; ++kt)
+                if (kt < KT0) top(v[kt]);
+        } else {
+#pragma unroll 2
+            for (int kt = 0; kt < KT0; ++kt) {
+                int8_mlp_load(xb, A.L, A.C, kt, off, v[0]);
+                top(v[0]);
+            }
         }
-        unsigned o = (unsigned)__shfl_xor((int)am, 32);
-        float s = p2n_q8_scale(o > am ? o : am);
-        int cq[KTM][4];
+        o = (unsigned)__shfl_xor((int)am, 32);
+        s = p2n_q8_scale(o > am ? o : am);
         {
             const P2nQ8 Q = p2n_q8_make(s);
 #pragma unroll
             for (int kt = 0; kt < KTM; ++kt)
                 if (kt < KT0) {
-                    float v[16];
-                    int8_mlp_load(xb, A.L, A.C, kt, off, v);
-                    p2n_q8_pack(v, Q, cq[kt]);
+                    float (&e)[16] = v[HOLD ? kt : 0];
+                    if constexpr (!HOLD) int8_mlp_load(xb, A.L, A.C, kt, off, e);
+                    p2n_q8_pack(e, Q, cq[kt]);
                     __builtin_amdgcn_sched_barrier(0);   // one tile at a time: interleaved tiles cost registers
                 }
         }
@@ -671,11 +702,12 @@ __global__ __launch_bounds__(256, CTM <= 2 ? 4 : CTM <= 4 ? 3 : KTM <= 8 ? 2 : 1
                         const f32x4 bi = *reinterpret_cast<const f32x4 *>(Y.bias + 32 * ct + 8 * g + 4 * h);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            float v = (float)acc[4 * g + j] * sc[j] * s + bi[j];
-                            if (relu) v = v <= 0.f ? 0.f : v;   // a NaN stays
-                            y[ct][4 * g + j] = v;
-                            const unsigned u = p2n_absbits(v);
-                            am = u > am ? u : am;
+                            const float v = (float)acc[4 * g + j] * sc[j] * s + bi[j];
+                            // the ReLU as a maximum of bit patterns: every NaN here has its sign bit clear (scales and biases are
+                            // made so, and so is what the arithmetic makes) and stays.  Past it the bits order as they are.
+                            const int bv = __float_as_int(v), u = relu ? (bv > 0 ? bv : 0) : bv;
+                            y[ct][4 * g + j] = __int_as_float(u);
+                            am = (unsigned)u > am ? (unsigned)u : am;
                         }
                     }
                     __builtin_amdgcn_sched_barrier(0);
@@ -691,7 +723,11 @@ __global__ __launch_bounds__(256, CTM <= 2 ? 4 : CTM <= 4 ? 3 : KTM <= 8 ? 2 : 1
                         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
                             ob + 32L * ct * W, 0, (int)(left < 0xFFFFFFFFL ? left : 0xFFFFFFFFL), 0x00020000);
                         if (!A.group) {
-                            if (valid) {
+                            if (valid && 32 * ct + 32 <= Y.N) {
+#pragma unroll
+                                for (int e = 0; e < 16; ++e)
+                                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(y[ct][e]), rs, off, (int)((8 * (e >> 2) + (e & 3)) * W * 4), 0);
+                            } else if (valid) {
 #pragma unroll
                                 for (int e = 0; e < 16; ++e)
                                     __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(y[ct][e]), rs, off + (int)((8 * (e >> 2) + (e & 3)) * W * 4), 0, 0);
@@ -701,7 +737,7 @@ __global__ __launch_bounds__(256, CTM <= 2 ? 4 : CTM <= 4 ? 3 : KTM <= 8 ? 2 : 1
                             // the lanes of a 16-lane row pair up; lane i of a row ends with register i's channel
                             int m[16];
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) m[e] = int8_key(y[ct][e]);
+                            for (int e = 0; e < 16; ++e) m[e] = relu ? __float_as_int(y[ct][e]) : int8_key(y[ct][e]);
                             p2n_halve_max<8, 0xB1>(m, lane & 1);
                             p2n_halve_max<4, 0x4E>(m, lane & 2);
                             p2n_halve_max<2, 0x124>(m, lane & 4);
@@ -713,7 +749,7 @@ __global__ __launch_bounds__(256, CTM <= 2 ? 4 : CTM <= 4 ? 3 : KTM <= 8 ? 2 : 1
                             const int i = lane & 15, c = 8 * (i >> 2) + 4 * h + (i & 3);
                             const int q = A.group == 32 ? (int)(l >> 5) : (int)(l >> 4);
                             if (valid && (A.group == 16 || !(lane & 16)))
-                                __builtin_amdgcn_raw_buffer_store_b32(int8_unkey(m[0]), rs, (int)((c * W + q) * 4), 0, 0);
+                                __builtin_amdgcn_raw_buffer_store_b32(relu ? m[0] : int8_unkey(m[0]), rs, (int)((c * W + q) * 4), 0, 0);
                         }
                     }
                 break;

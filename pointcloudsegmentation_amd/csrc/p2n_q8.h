@@ -13,13 +13,18 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 // running maximum of |v| as a bit pattern: unsigned order puts the infinities and the NaNs on top
 __device__ __forceinline__ unsigned p2n_absbits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
+// amax / 127, correctly rounded: a first quotient with the rounded reciprocal is off by at most one step, its residual is exact, and
+// one correction step with a correctly rounded reciprocal gives the rounded quotient (Markstein) -- as long as nothing
+// underflows, below that the division itself.
 __device__ __forceinline__ float p2n_q8_scale(unsigned amax_bits) {
-    if (amax_bits >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
-    return __uint_as_float(amax_bits) / 127.0f;   // IEEE division: correctly rounded
+    const float a = __uint_as_float(amax_bits), y = 1.0f / 127.0f, q = a * y;
+    float s = fmaf(fmaf(-127.0f, q, a), y, q);
+    if (a < 7.9e-31f) s = a / 127.0f;
+    return amax_bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : s;
 }
 
 // What the codes of one scale are formed with: s and v times `up` (2^100 where s is under 2^-100 and has no reciprocal in
-// float32, else 1; the product is exact), and 1/(s * up); 0 where there is nothing to divide by (s = 0, NaN).
+// float32, else 1; the product is exact), and 1/(s * up) to one step; 0 where there is nothing to divide by (s = 0, NaN).
 struct P2nQ8 {
     float s, up, inv;
 };
@@ -27,11 +32,11 @@ __device__ __forceinline__ P2nQ8 p2n_q8_make(float s) {
     P2nQ8 Q;
     Q.up = s < 7.9e-31f ? 1.2676506e30f : 1.f;
     Q.s = s * Q.up;
-    Q.inv = Q.s > 0.f ? 1.0f / Q.s : 0.f;
+    Q.inv = Q.s > 0.f ? __builtin_amdgcn_rcpf(Q.s) : 0.f;
     return Q;
 }
 
-// The code next to a tie.  t = v * inv is off by less than 1.6e-5 and may sit on the other side of a tie than the true
+// The code next to a tie.  v * inv is off by less than 1.6e-5 and may sit on the other side of a tie than the true
 // quotient; the residual v - q*s decides: there it is a multiple of ulp(s)/2 below 2^25 of them, so the fma gives it exactly.
 __device__ __forceinline__ float p2n_q8_decide(float v, const P2nQ8 &Q) {
     v *= Q.up;
@@ -42,9 +47,10 @@ __device__ __forceinline__ float p2n_q8_decide(float v, const P2nQ8 &Q) {
     return fminf(fmaxf(q, -127.f), 127.f);
 }
 
-// Codes of NV values (a multiple of 4) of one scale, packed four to a dword in order.  Round-to-even of t is the code unless t
-// lies within 1.6e-5 of a tie (two roundings of 2^-24 at up to 127.5); the rounding is the addition of 1.5 * 2^23 (one rounding to a whole number, whose low byte
-// is the code).  Any lane near a tie sends its wave through the decision for these values: one time in 25 for 16 values of 64 lanes.
+// Codes of NV values (a multiple of 4) of one scale, packed four to a dword in order.  v * inv is off by less than 1.6e-5 (inv by
+// 2^-23, at up to 127.5), so its rounding to even is the code unless it lies within that of a tie.  The rounding is the addition
+// of 1.5 * 2^23 in one fma (one rounding to a whole number, whose low byte is the code).  Any lane near a tie sends its wave
+// through the decision for these values: one time in 16 for 16 values of 64 lanes.
 #define P2N_Q8_MAGIC 12582912.0f
 template <int NV>
 __device__ __forceinline__ void p2n_q8_pack(const float (&v)[NV], const P2nQ8 &Q, int (&code)[NV / 4]) {
@@ -52,11 +58,11 @@ __device__ __forceinline__ void p2n_q8_pack(const float (&v)[NV], const P2nQ8 &Q
     unsigned m[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const float t = v[i] * Q.inv, a = t + P2N_Q8_MAGIC;
+        const float a = fmaf(v[i], Q.inv, P2N_Q8_MAGIC);
         m[i] = __float_as_uint(a);
-        near = fmaxf(near, fabsf(t - (a - P2N_Q8_MAGIC)));
+        near = fmaxf(near, fabsf(fmaf(v[i], Q.inv, P2N_Q8_MAGIC - a)));
     }
-    if (__any(near > 0.49998f)) {
+    if (__any(near > 0.49997f)) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) m[i] = __float_as_uint(p2n_q8_decide(v[i], Q) + P2N_Q8_MAGIC);
     }
