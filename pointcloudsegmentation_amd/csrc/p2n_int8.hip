@@ -577,11 +577,10 @@ extern "C" int p2n_int8_linear(const void *x, int bf16, long T, int K, long ld, 
     return rc;
 }
 
-// ---------------------------------------------------------------- shared MLP, register-resident
-// Lane = point, registers = channels (D = W . X): a wave carries 32 points through every layer.  The 32 x 32 product leaves
+// ---------------------------------------------------------------- shared MLP, on chip
+// Lane = point, registers = channels (D = W . X), 32 points at a time through every layer.  The 32 x 32 product leaves
 // channel 32ct + 8g + 4h + j of a lane's point in register 4g + j of its half h; four neighbours packed to a dword are the
-// operand of the next layer in the k order of the weight image.  Nothing of a hidden layer leaves the wave: its scale is a
-// maximum over the lane's registers and the other half (one shuffle).
+// operand of the next layer in the k order of the weight image: nothing moves between lanes.
 struct MlpLayer {
     const char *img;
     const float *scale, *bias;
@@ -630,147 +629,229 @@ __device__ __forceinline__ void int8_mlp_load(const float *xb, long L, int C, in
     }
 }
 
-// CTM: channel tiles of the widest layer; KTM >= CTM: k-tiles of the widest operand
-template <int CTM, int KTM>
-__global__ __launch_bounds__(256, CTM <= 2 ? 4 : CTM <= 4 ? 3 : KTM <= 8 ? 2 : 1) void p2n_int8_mlp_kernel(Int8MlpArgs A) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int p = lane & 31, h = lane >> 5;
-    for (long tile = (long)blockIdx.x * 4 + wave; tile < A.total; tile += (long)gridDim.x * 4) {
-        const long b = tile / A.tiles, l = (tile % A.tiles) * 32 + p;
-        const bool valid = l < A.L;
-        const float *xb = A.x + b * A.C * A.L;
-        const unsigned off = (unsigned)((4 * h * A.L + (valid ? l : A.L - 1)) * 4);   // bytes; L <= 2^24 keeps 32 rows below 2^31
-        const int KT0 = A.layer[0].KT;
-        constexpr bool HOLD = KTM <= 2;       // the input stays in registers between its maximum and its codes; longer ones are read twice
-        unsigned am = 0, o;
-        float s, v[HOLD ? KTM : 1][16];
-        int cq[KTM][4];
-        auto top = [&](const float (&e)[16]) __attribute__((always_inline)) {
+// A tile's values y (a ReLU behind them or not) to memory: channel tile ct of cloud b, columns of the wave's 32 points, or the maxima of its groups
+__device__ __forceinline__ void int8_mlp_out(const Int8MlpArgs &A, int N, bool relu, long b, long l, bool valid, unsigned off, int ct, int lane,
+                                             const float (&y)[16]) {
+    const int h = lane >> 5;
+    const long W = A.group ? A.L / A.group : A.L;   // columns of a result row
+    // the resource starts at row 32ct and ends with the cloud's last row: channels past N are not written
+    const long left = (long)(N - 32 * ct) * W * 4;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(A.out + (b * N + 32L * ct) * W, 0,
+                                                                         (int)(left < 0xFFFFFFFFL ? left : 0xFFFFFFFFL), 0x00020000);
+    if (!A.group) {
+        if (valid && 32 * ct + 32 <= N) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const unsigned u = p2n_absbits(e[i]);
-                am = u > am ? u : am;
-            }
-        };
-        if constexpr (HOLD) {
+            for (int e = 0; e < 16; ++e)
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(y[e]), rs, off, (int)((8 * (e >> 2) + (e & 3)) * W * 4), 0);
+        } else if (valid) {
 #pragma unroll
-            for (int kt = 0; kt < KTM; ++kt)
-                if (kt < KT0) int8_mlp_load(xb, A.L, A.C, kt, off, v[kt]);
-#pragma unroll
-            for (int kt = 0; kt < KTM; ++kt)
-                if (kt < KT0) top(v[kt]);
-        } else {
-#pragma unroll 2
-            for (int kt = 0; kt < KT0; ++kt) {
-                int8_mlp_load(xb, A.L, A.C, kt, off, v[0]);
-                top(v[0]);
-            }
+            for (int e = 0; e < 16; ++e)
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(y[e]), rs, off + (unsigned)((8 * (e >> 2) + (e & 3)) * W * 4), 0, 0);
         }
-        o = (unsigned)__shfl_xor((int)am, 32);
-        s = p2n_q8_scale(o > am ? o : am);
-        {
-            const P2nQ8 Q = p2n_q8_make(s);
+        return;
+    }
+    // maximum over 32 (or 16) neighbouring points of every channel: the registers shrink 16 -> 1 while the lanes of a
+    // 16-lane row pair up; lane i of a row ends with register i's channel
+    int m[16];
 #pragma unroll
-            for (int kt = 0; kt < KTM; ++kt)
-                if (kt < KT0) {
-                    float (&e)[16] = v[HOLD ? kt : 0];
-                    if constexpr (!HOLD) int8_mlp_load(xb, A.L, A.C, kt, off, e);
-                    p2n_q8_pack(e, Q, cq[kt]);
-                    __builtin_amdgcn_sched_barrier(0);   // one tile at a time: interleaved tiles cost registers
-                }
-        }
-#pragma unroll 1
-        for (int li = 0; li < A.nl; ++li) {
-            const MlpLayer Y = A.layer[li];
-            const bool last = li == A.nl - 1;
-            const bool relu = !last || A.last_relu;
-            const i32x4 *wf = reinterpret_cast<const i32x4 *>(Y.img) + lane;
-            float y[CTM][16];
-            am = 0;
+    for (int e = 0; e < 16; ++e) m[e] = relu ? __float_as_int(y[e]) : int8_key(y[e]);
+    p2n_halve_max<8, 0xB1>(m, lane & 1);
+    p2n_halve_max<4, 0x4E>(m, lane & 2);
+    p2n_halve_max<2, 0x124>(m, lane & 4);
+    p2n_halve_max<1, 0x128>(m, lane & 8);
+    if (A.group == 32) {
+        const int t = __builtin_amdgcn_ds_swizzle(m[0], 0x401F);   // lane ^ 16
+        m[0] = t > m[0] ? t : m[0];
+    }
+    const int i = lane & 15, c = 8 * (i >> 2) + 4 * h + (i & 3);
+    const int q = A.group == 32 ? (int)(l >> 5) : (int)(l >> 4);
+    if (valid && (A.group == 16 || !(lane & 16)))
+        __builtin_amdgcn_raw_buffer_store_b32(relu ? m[0] : int8_unkey(m[0]), rs, (int)((c * W + q) * 4), 0, 0);
+}
+
+// A tile's sums to its values: scales, bias, ReLU; into `am` the largest of them as bits.  The ReLU is a maximum of bit patterns: every NaN here has
+// its sign bit clear (scales and biases are made so, and so is what the arithmetic makes) and stays.  Past it the bits order as they are.
+__device__ __forceinline__ void int8_mlp_values(const i32x16 &acc, const MlpLayer &Y, int ct, int h, float s, bool relu, float (&y)[16], unsigned &am) {
 #pragma unroll
-            for (int ct = 0; ct < CTM; ++ct)
-                if (ct < Y.CT) {
-                    i32x16 acc;
+    for (int g = 0; g < 4; ++g) {
+        const f32x4 sc = *reinterpret_cast<const f32x4 *>(Y.scale + 32 * ct + 8 * g + 4 * h);
+        const f32x4 bi = *reinterpret_cast<const f32x4 *>(Y.bias + 32 * ct + 8 * g + 4 * h);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) acc[e] = 0;
-#pragma unroll
-                    for (int kt = 0; kt < KTM; ++kt)
-                        if (kt < Y.KT) acc = MFMA_I8(wf[(ct * Y.KTI + kt) * 64], (i32x4{cq[kt][0], cq[kt][1], cq[kt][2], cq[kt][3]}), acc);
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const f32x4 sc = *reinterpret_cast<const f32x4 *>(Y.scale + 32 * ct + 8 * g + 4 * h);
-                        const f32x4 bi = *reinterpret_cast<const f32x4 *>(Y.bias + 32 * ct + 8 * g + 4 * h);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float v = (float)acc[4 * g + j] * sc[j] * s + bi[j];
-                            // the ReLU as a maximum of bit patterns: every NaN here has its sign bit clear (scales and biases are
-                            // made so, and so is what the arithmetic makes) and stays.  Past it the bits order as they are.
-                            const int bv = __float_as_int(v), u = relu ? (bv > 0 ? bv : 0) : bv;
-                            y[ct][4 * g + j] = __int_as_float(u);
-                            am = (unsigned)u > am ? (unsigned)u : am;
-                        }
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            if (last) {
-                const long W = A.group ? A.L / A.group : A.L;   // columns of a result row
-                float *ob = A.out + b * Y.N * W;
-#pragma unroll
-                for (int ct = 0; ct < CTM; ++ct)
-                    if (ct < Y.CT) {
-                        // the resource starts at row 32ct and ends with the cloud's last row: channels past N are not written
-                        const long left = (long)(Y.N - 32 * ct) * W * 4;
-                        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-                            ob + 32L * ct * W, 0, (int)(left < 0xFFFFFFFFL ? left : 0xFFFFFFFFL), 0x00020000);
-                        if (!A.group) {
-                            if (valid && 32 * ct + 32 <= Y.N) {
-#pragma unroll
-                                for (int e = 0; e < 16; ++e)
-                                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(y[ct][e]), rs, off, (int)((8 * (e >> 2) + (e & 3)) * W * 4), 0);
-                            } else if (valid) {
-#pragma unroll
-                                for (int e = 0; e < 16; ++e)
-                                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(y[ct][e]), rs, off + (int)((8 * (e >> 2) + (e & 3)) * W * 4), 0, 0);
-                            }
-                        } else {
-                            // maximum over 32 (or 16) neighbouring points of every channel: the registers shrink 16 -> 1 while
-                            // the lanes of a 16-lane row pair up; lane i of a row ends with register i's channel
-                            int m[16];
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) m[e] = relu ? __float_as_int(y[ct][e]) : int8_key(y[ct][e]);
-                            p2n_halve_max<8, 0xB1>(m, lane & 1);
-                            p2n_halve_max<4, 0x4E>(m, lane & 2);
-                            p2n_halve_max<2, 0x124>(m, lane & 4);
-                            p2n_halve_max<1, 0x128>(m, lane & 8);
-                            if (A.group == 32) {
-                                const int t = __builtin_amdgcn_ds_swizzle(m[0], 0x401F);   // lane ^ 16
-                                m[0] = t > m[0] ? t : m[0];
-                            }
-                            const int i = lane & 15, c = 8 * (i >> 2) + 4 * h + (i & 3);
-                            const int q = A.group == 32 ? (int)(l >> 5) : (int)(l >> 4);
-                            if (valid && (A.group == 16 || !(lane & 16)))
-                                __builtin_amdgcn_raw_buffer_store_b32(relu ? m[0] : int8_unkey(m[0]), rs, (int)((c * W + q) * 4), 0, 0);
-                        }
-                    }
-                break;
-            }
-            o = (unsigned)__shfl_xor((int)am, 32);
-            s = p2n_q8_scale(o > am ? o : am);
-            const P2nQ8 Q = p2n_q8_make(s);
-#pragma unroll
-            for (int ct = 0; ct < CTM; ++ct)
-                if (ct < Y.CT) {
-                    p2n_q8_pack(y[ct], Q, cq[ct]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+        for (int j = 0; j < 4; ++j) {
+            const float v = (float)acc[4 * g + j] * sc[j] * s + bi[j];
+            const int bv = __float_as_int(v), u = relu ? (bv > 0 ? bv : 0) : bv;
+            y[4 * g + j] = __int_as_float(u);
+            am = (unsigned)u > am ? (unsigned)u : am;
         }
     }
 }
 
-template <int CTM, int KTM>
-static void launch_int8_mlp(const Int8MlpArgs &a, hipStream_t s) {
-    const long wgs = (a.total + 3) / 4;
-    hipLaunchKernelGGL((p2n_int8_mlp_kernel<CTM, KTM>), dim3((unsigned)(wgs < 65536 ? wgs : 65536)), dim3(256), 0, s, a);
+__device__ __forceinline__ void int8_mlp_top(const float (&e)[16], unsigned &am) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const unsigned u = p2n_absbits(e[i]);
+        am = u > am ? u : am;
+    }
+}
+
+// codes of an input tile; groups of eight channels past the last one are zero: nothing to form (a level's first layer has six)
+__device__ __forceinline__ void int8_mlp_codes(const float (&e)[16], int real, const P2nQ8 &Q, int (&c)[4]) {
+    float near = 0.f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        c[g] = 0;
+        if (8 * g < real) c[g] = p2n_q8_four(e + 4 * g, Q, near);
+    }
+    if (p2n_q8_tie(near, Q)) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) c[g] = p2n_q8_decide4(e + 4 * g, Q);
+    }
+}
+
+// Up to 64 channels everywhere: one wave carries its 32 points through every layer in registers.
+__global__ __launch_bounds__(256, 4) void p2n_int8_mlp_narrow_kernel(Int8MlpArgs A) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int p = lane & 31, h = lane >> 5;
+    const i32x16 zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    const long tile = (long)blockIdx.x * 4 + wave;
+    if (tile >= A.total) return;
+    const long b = tile / A.tiles, l = (tile % A.tiles) * 32 + p;
+    const bool valid = l < A.L;
+    const float *xb = A.x + b * A.C * A.L;
+    const unsigned off = (unsigned)((4 * h * A.L + (valid ? l : A.L - 1)) * 4);   // bytes; L <= 2^24 keeps 32 rows below 2^31
+    const int KT0 = A.layer[0].KT;
+    unsigned am = 0, o;
+    float v[2][16];
+    int cq[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+        if (kt < KT0) int8_mlp_load(xb, A.L, A.C, kt, off, v[kt]);
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+        if (kt < KT0) int8_mlp_top(v[kt], am);
+    o = (unsigned)__shfl_xor((int)am, 32);
+    float s = p2n_q8_scale(o > am ? o : am);
+    {
+        const P2nQ8 Q = p2n_q8_make(s);
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+            if (kt < KT0) int8_mlp_codes(v[kt], A.C - 32 * kt, Q, cq[kt]);
+    }
+#pragma unroll 1
+    for (int li = 0; li < A.nl; ++li) {
+        const MlpLayer Y = A.layer[li];
+        const bool last = li == A.nl - 1, relu = !last || A.last_relu;
+        const i32x4 *wf = reinterpret_cast<const i32x4 *>(Y.img) + lane;
+        am = 0;
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct)
+            if (ct < Y.CT) {
+                i32x16 acc = MFMA_I8(wf[ct * Y.KTI * 64], (i32x4{cq[0][0], cq[0][1], cq[0][2], cq[0][3]}), zero);
+                // the image has an even number of k-tiles: where the second holds no channels its codes are zero
+                acc = MFMA_I8(wf[(ct * Y.KTI + 1) * 64], (i32x4{cq[1][0], cq[1][1], cq[1][2], cq[1][3]}), acc);
+                int8_mlp_values(acc, Y, ct, h, s, relu, v[ct], am);
+            }
+        if (last) {
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct)
+                if (ct < Y.CT) int8_mlp_out(A, Y.N, relu, b, l, valid, off, ct, lane, v[ct]);
+            break;
+        }
+        o = (unsigned)__shfl_xor((int)am, 32);
+        s = p2n_q8_scale(o > am ? o : am);
+        const P2nQ8 Q = p2n_q8_make(s);
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct)
+            if (ct < Y.CT) p2n_q8_pack(v[ct], Q, cq[ct]);
+    }
+}
+
+// Wider layers: NW waves carry 32 points together, a wave its share of the channel tiles.  Codes go round through LDS in operand order; a point's
+// maximum is joined over the waves there too.  Two barriers a layer; a layer's first weights are on their way before the last one ends.
+template <int NW>
+__global__ __launch_bounds__(64 * NW, 4) void p2n_int8_mlp_wide_kernel(Int8MlpArgs A) {
+    constexpr int KTI = 4 * NW;      // k-tiles of the input: 1024 (512) channels in, a channel tile a wave: 256 (128) out
+    constexpr int AHEAD = 4;                                // weight fragments on their way
+    __shared__ __attribute__((aligned(16))) char codes[KTI * 1024];
+    __shared__ unsigned top[NW][32];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int p = lane & 31, h = lane >> 5;
+    const long tile = blockIdx.x, b = tile / A.tiles, l = (tile % A.tiles) * 32 + p;
+    const bool valid = l < A.L;
+    const float *xb = A.x + b * A.C * A.L;
+    const unsigned off = (unsigned)((4 * h * A.L + (valid ? l : A.L - 1)) * 4);
+    const int KT0 = A.layer[0].KT;
+    float v[4][16];
+    unsigned am = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (wave + NW * i < KT0) int8_mlp_load(xb, A.L, A.C, wave + NW * i, off, v[i]);
+    i32x4 w[AHEAD];
+    auto ahead = [&](const MlpLayer &Y, int ct) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            w[i] = reinterpret_cast<const i32x4 *>(Y.img)[((ct < Y.CT ? ct : 0) * Y.KTI + (i < Y.KTI ? i : 0)) * 64 + lane];
+    };
+    ahead(A.layer[0], wave);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (wave + NW * i < KT0) int8_mlp_top(v[i], am);
+    // the largest of every point over the waves -> its scale
+    auto join = [&]() __attribute__((always_inline)) {
+        const unsigned o = (unsigned)__shfl_xor((int)am, 32);
+        if (h == 0) top[wave][p] = o > am ? o : am;
+        __syncthreads();
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) m = top[i][p] > m ? top[i][p] : m;
+        return p2n_q8_scale(m);
+    };
+    float s = join();
+    {
+        const P2nQ8 Q = p2n_q8_make(s);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (wave + NW * i < KT0) {
+                int c[4];
+                int8_mlp_codes(v[i], A.C - 32 * (wave + NW * i), Q, c);
+                *reinterpret_cast<i32x4 *>(codes + ((wave + NW * i) * 64 + lane) * 16) = i32x4{c[0], c[1], c[2], c[3]};
+            }
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int li = 0; li < A.nl; ++li) {
+        const MlpLayer Y = A.layer[li];
+        const bool last = li == A.nl - 1, relu = !last || A.last_relu;
+        am = 0;
+        const bool mine = wave < Y.CT;
+        if (mine) {
+            const i32x4 *wf = reinterpret_cast<const i32x4 *>(Y.img) + (long)wave * Y.KTI * 64 + lane;
+            i32x16 acc;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[e] = 0;
+            for (int k0 = 0; k0 < Y.KT; k0 += AHEAD) {
+#pragma unroll
+                for (int q = 0; q < AHEAD; ++q) {
+                    if (k0 + q < Y.KT) acc = MFMA_I8(w[q], *reinterpret_cast<const i32x4 *>(codes + ((k0 + q) * 64 + lane) * 16), acc);
+                    if (k0 + q + AHEAD < Y.KT) w[q] = wf[(k0 + q + AHEAD) * 64];
+                }
+            }
+            int8_mlp_values(acc, Y, wave, h, s, relu, v[0], am);
+        }
+        if (last) {
+            if (mine) int8_mlp_out(A, Y.N, relu, b, l, valid, off, wave, lane, v[0]);
+            break;
+        }
+        ahead(A.layer[li + 1], wave);
+        s = join();                            // behind its barrier every wave has read this layer's codes
+        if (mine) {
+            const P2nQ8 Q = p2n_q8_make(s);
+            int c[4];
+            p2n_q8_pack(v[0], Q, c);
+            *reinterpret_cast<i32x4 *>(codes + (wave * 64 + lane) * 16) = i32x4{c[0], c[1], c[2], c[3]};
+        }
+        __syncthreads();
+    }
 }
 
 // x (B, dims[0], L) -> out (B, dims[nl], L), or (B, dims[nl], L/group) with the maximum over groups of 16 or 32 consecutive
@@ -800,21 +881,13 @@ extern "C" int p2n_int8_mlp(const float *x, int B, long L, int nl, const int *di
         y.KT = (dims[l] + 31) / 32; y.KTI = I.KT; y.CT = I.CT; y.N = dims[l + 1];
         if (I.CT > ctm) ctm = I.CT;
     }
-    if (ctm > ktm) ktm = ctm;
+    P2N_REQUIRE(a.total < (1L << 31), "p2n_int8_mlp: too many columns");
     hipStream_t s = (hipStream_t)stream_;
     const int ps = p2n_prof_begin(P2N_K_INT8_MLP, s);
-    if (ktm > 8) {
-        if (ktm > 16) launch_int8_mlp<8, 32>(a, s);
-        else launch_int8_mlp<8, 16>(a, s);
-    } else if (ctm > 4) {
-        launch_int8_mlp<8, 8>(a, s);
-    } else if (ctm > 2) {
-        if (ktm > 4) launch_int8_mlp<4, 8>(a, s);
-        else launch_int8_mlp<4, 4>(a, s);
-    } else {
-        if (ktm > 2) launch_int8_mlp<2, 8>(a, s);
-        else launch_int8_mlp<2, 2>(a, s);
-    }
+    // one wave to 32 points up to 64 channels (fewer registers than four waves would share out), four up to 128, eight up to 256
+    if (ctm <= 2 && ktm <= 2) hipLaunchKernelGGL(p2n_int8_mlp_narrow_kernel, dim3((unsigned)((a.total + 3) / 4)), dim3(256), 0, s, a);
+    else if (ctm <= 4 && ktm <= 16) hipLaunchKernelGGL(p2n_int8_mlp_wide_kernel<4>, dim3((unsigned)a.total), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(p2n_int8_mlp_wide_kernel<8>, dim3((unsigned)a.total), dim3(512), 0, s, a);
     p2n_prof_end(ps, s);
     P2N_CHECK_HIP(hipGetLastError());
     return P2N_OK;

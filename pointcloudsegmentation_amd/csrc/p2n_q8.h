@@ -19,7 +19,7 @@ __device__ __forceinline__ unsigned p2n_absbits(float v) { return __float_as_uin
 __device__ __forceinline__ float p2n_q8_scale(unsigned amax_bits) {
     const float a = __uint_as_float(amax_bits), y = 1.0f / 127.0f, q = a * y;
     float s = fmaf(fmaf(-127.0f, q, a), y, q);
-    if (a < 7.9e-31f) s = a / 127.0f;
+    if (__any(a > 0.f && a < 7.9e-31f)) s = a < 7.9e-31f ? a / 127.0f : s;
     return amax_bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : s;
 }
 
@@ -42,8 +42,8 @@ __device__ __forceinline__ float p2n_q8_decide(float v, const P2nQ8 &Q) {
     v *= Q.up;
     float q = rintf(v * Q.inv);
     const float r = fmaf(-q, Q.s, v), d = 2.f * fabsf(r) - Q.s;
-    const bool odd = ((int)q & 1) != 0;
-    if (d > 0.f || (d == 0.f && odd)) q += r < 0.f ? -1.f : 1.f;
+    const bool past = (d > 0.f) | ((d == 0.f) & (((int)q & 1) != 0));
+    q += past ? (r < 0.f ? -1.f : 1.f) : 0.f;
     return fminf(fmaxf(q, -127.f), 127.f);
 }
 
@@ -52,25 +52,34 @@ __device__ __forceinline__ float p2n_q8_decide(float v, const P2nQ8 &Q) {
 // of 1.5 * 2^23 in one fma (one rounding to a whole number, whose low byte is the code).  Any lane near a tie sends its wave
 // through the decision for these values: one time in 16 for 16 values of 64 lanes.
 #define P2N_Q8_MAGIC 12582912.0f
-template <int NV>
-__device__ __forceinline__ void p2n_q8_pack(const float (&v)[NV], const P2nQ8 &Q, int (&code)[NV / 4]) {
-    float near = Q.up > 1.f ? 1.f : 0.f;
-    unsigned m[NV];
+// four values: their dword, and into `near` how far the farthest lies from its code
+__device__ __forceinline__ int p2n_q8_four(const float *v, const P2nQ8 &Q, float &near) {
+    unsigned m[4];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
+    for (int i = 0; i < 4; ++i) {
         const float a = fmaf(v[i], Q.inv, P2N_Q8_MAGIC);
         m[i] = __float_as_uint(a);
         near = fmaxf(near, fabsf(fmaf(v[i], Q.inv, P2N_Q8_MAGIC - a)));
     }
-    if (__any(near > 0.49997f)) {
+    const unsigned lo = __builtin_amdgcn_perm(m[1], m[0], 0x0C0C0400u);        // bytes 0,1 = low bytes of v0, v1
+    const unsigned hi = __builtin_amdgcn_perm(m[3], m[2], 0x04000C0Cu);        // bytes 2,3 = low bytes of v2, v3
+    return (int)(lo | hi);
+}
+__device__ __forceinline__ bool p2n_q8_tie(float near, const P2nQ8 &Q) { return __any((near > 0.49997f) | (Q.up > 1.f)); }
+__device__ __forceinline__ int p2n_q8_decide4(const float *v, const P2nQ8 &Q) {
+    unsigned c = 0;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) m[i] = __float_as_uint(p2n_q8_decide(v[i], Q) + P2N_Q8_MAGIC);
-    }
+    for (int i = 0; i < 4; ++i) c |= ((unsigned)(int)p2n_q8_decide(v[i], Q) & 0xFFu) << (8 * i);
+    return (int)c;
+}
+template <int NV>
+__device__ __forceinline__ void p2n_q8_pack(const float (&v)[NV], const P2nQ8 &Q, int (&code)[NV / 4]) {
+    float near = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV / 4; ++i) {
-        const unsigned lo = __builtin_amdgcn_perm(m[4 * i + 1], m[4 * i], 0x0C0C0400u);        // bytes 0,1 = low bytes of v0, v1
-        const unsigned hi = __builtin_amdgcn_perm(m[4 * i + 3], m[4 * i + 2], 0x04000C0Cu);    // bytes 2,3 = low bytes of v2, v3
-        code[i] = (int)(lo | hi);
+    for (int i = 0; i < NV / 4; ++i) code[i] = p2n_q8_four(v + 4 * i, Q, near);
+    if (p2n_q8_tie(near, Q)) {
+#pragma unroll
+        for (int i = 0; i < NV / 4; ++i) code[i] = p2n_q8_decide4(v + 4 * i, Q);
     }
 }
 #endif
