@@ -17,6 +17,7 @@ q = 0; a NaN or an infinity among the v makes s NaN, and with it every result th
 All functions take GPU tensors only and queue their work on the current stream of the tensors' device; nothing synchronises.
 """
 import ctypes
+from functools import lru_cache
 from typing import Optional, Sequence
 
 import torch
@@ -34,9 +35,20 @@ def _gpu(t: torch.Tensor, name: str, dtypes) -> torch.Tensor:
     return t
 
 
-def _no_grad_wanted(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _no_grad_wanted(what: str, t: torch.Tensor) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{what} has no backward pass (rounding to 8 bits has no gradient): call it under torch.no_grad()")
+
+
+def _call(fn, what: str, dev: torch.device, *args) -> None:
+    """fn(*args, current stream of dev) with dev as the current device, its return code turned into an error"""
+    if torch._C._cuda_getDevice() == dev.index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc:
+        _lib.check(rc, what)
 
 
 _TOKEN_TYPES = (torch.float32, torch.bfloat16)
@@ -62,9 +74,8 @@ def quantize_tokens(x: torch.Tensor):
     T, K, ld, rows = _rows(x)
     codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.lib().p2n_quantize_tokens(rows.data_ptr(), int(x.dtype == torch.bfloat16), T, K, ld, codes.data_ptr(),
-                                                  scale.data_ptr(), _rt.stream_handle(x.device)), "p2n_quantize_tokens")
+    _call(_lib.lib().p2n_quantize_tokens, "p2n_quantize_tokens", x.device, rows.data_ptr(), int(x.dtype == torch.bfloat16), T, K, ld,
+          codes.data_ptr(), scale.data_ptr())
     return codes, scale
 
 
@@ -92,9 +103,8 @@ class Int8Weight:
             raise ValueError(f"weight (N,K) = {tuple(weight.shape)}: both must be in 1..65536")
         weight = weight.contiguous()
         self.image = torch.empty(n, dtype=torch.uint8, device=weight.device)
-        with torch.cuda.device(weight.device):
-            _lib.check(L.p2n_int8_pack_weight(weight.data_ptr(), _rt.ptr(bias), self.in_features, self.out_features,
-                                              self.image.data_ptr(), _rt.stream_handle(weight.device)), "p2n_int8_pack_weight")
+        _call(L.p2n_int8_pack_weight, "p2n_int8_pack_weight", weight.device, weight.data_ptr(), _rt.ptr(bias), self.in_features,
+              self.out_features, self.image.data_ptr())
 
     @property
     def scale(self) -> torch.Tensor:
@@ -126,11 +136,10 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, relu: bool = False) -> torc
     if T == 0:
         return y
     # from torch's allocator and not from the stream's shared buffer: a captured graph keeps the memory it was captured with
-    ws = torch.empty(L.p2n_int8_linear_workspace_bytes(T, K, N), dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        _lib.check(L.p2n_int8_linear(rows.data_ptr(), int(x.dtype == torch.bfloat16), T, K, ld, weight.image.data_ptr(), N,
-                                     int(relu), y.data_ptr(), ws.data_ptr(), ws.numel(), _rt.stream_handle(x.device)),
-                   "p2n_int8_linear")
+    nws = L.p2n_int8_linear_workspace_bytes(T, K, N)
+    ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
+    _call(L.p2n_int8_linear, "p2n_int8_linear", x.device, rows.data_ptr(), int(x.dtype == torch.bfloat16), T, K, ld,
+          weight.image.data_ptr(), N, int(relu), y.data_ptr(), _rt.ptr(ws), nws)
     return y
 
 
@@ -163,15 +172,12 @@ def int8_mlp(x: torch.Tensor, weights: Sequence[Int8Weight], last_relu: bool = T
     out = torch.empty((B, dims[-1], L // inner if inner else L), dtype=torch.float32, device=x.device)
     arr = (ctypes.c_int * len(dims))(*dims)
     images = (ctypes.c_void_p * len(weights))(*[w.image.data_ptr() for w in weights])
-    with torch.cuda.device(x.device):
-        _lib.check(lib.p2n_int8_mlp(x.data_ptr(), B, L, len(weights), arr, images, int(last_relu), inner, out.data_ptr(),
-                                    _rt.stream_handle(x.device)), "p2n_int8_mlp")
-        rest = group // inner if inner else group
-        if rest > 1:
-            res = torch.empty((B, dims[-1], L // group), dtype=torch.float32, device=x.device)
-            _lib.check(lib.p2n_max_of_columns(out.data_ptr(), res.numel(), rest, res.data_ptr(), _rt.stream_handle(x.device)),
-                       "p2n_max_of_columns")
-            out = res
+    _call(lib.p2n_int8_mlp, "p2n_int8_mlp", x.device, x.data_ptr(), B, L, len(weights), arr, images, int(last_relu), inner, out.data_ptr())
+    rest = group // inner if inner else group
+    if rest > 1:
+        res = torch.empty((B, dims[-1], L // group), dtype=torch.float32, device=x.device)
+        _call(lib.p2n_max_of_columns, "p2n_max_of_columns", x.device, out.data_ptr(), res.numel(), rest, res.data_ptr())
+        out = res
     return out
 
 
@@ -215,6 +221,16 @@ def _bytes(n: int, device) -> torch.Tensor:
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
+@lru_cache(maxsize=256)
+def _act8_bytes(what: str, B: int, C: int, L: int, norm: bool, N: int):
+    """sizes of the kept buffer and of the workspace (numbers of the shape alone)"""
+    L_ = _lib.lib()
+    nkept, nws = L_.p2n_act8_kept_bytes(B, C, L, int(norm)), L_.p2n_act8_workspace_bytes(B, C, L, N)
+    if nkept == 0 or nws == 0:
+        raise ValueError(f"{what}: " + L_.p2n_last_error().decode(errors="replace"))
+    return nkept, nws
+
+
 class _Act8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, gamma, beta, running_mean, running_var, momentum, eps):
@@ -223,15 +239,12 @@ class _Act8Linear(torch.autograd.Function):
         N = weight.size(0)
         dev = x.device
         normed = gamma is not None
-        nkept, nws = L_.p2n_act8_kept_bytes(B, K, L, int(normed)), L_.p2n_act8_workspace_bytes(B, K, L, N)
-        if nkept == 0 or nws == 0:
-            raise ValueError("act8_linear: " + L_.p2n_last_error().decode(errors="replace"))
+        nkept, nws = _act8_bytes("act8_linear", B, K, L, normed, N)
         kept, ws = _bytes(nkept, dev), _bytes(nws, dev)
         h = torch.empty((B, N, L), dtype=torch.float32, device=dev)
-        with torch.cuda.device(dev):
-            _lib.check(L_.p2n_act8_forward(x.data_ptr(), B, K, L, weight.data_ptr(), _rt.ptr(bias), N, _rt.ptr(gamma), _rt.ptr(beta),
-                                           _rt.ptr(running_mean), _rt.ptr(running_var), momentum, eps, h.data_ptr(), kept.data_ptr(),
-                                           nkept, ws.data_ptr(), nws, _rt.stream_handle(dev)), "p2n_act8_forward")
+        _call(L_.p2n_act8_forward, "p2n_act8_forward", dev, x.data_ptr(), B, K, L, weight.data_ptr(), _rt.ptr(bias), N, _rt.ptr(gamma),
+              _rt.ptr(beta), _rt.ptr(running_mean), _rt.ptr(running_var), momentum, eps, h.data_ptr(), kept.data_ptr(), nkept,
+              ws.data_ptr(), nws)
         ctx.save_for_backward(kept, weight, gamma, beta)
         ctx.meta = (B, K, L, N, normed and momentum < 0, bias is not None)
         return h
@@ -245,19 +258,19 @@ class _Act8Linear(torch.autograd.Function):
         g = g.contiguous()
         dev = g.device
         need = ctx.needs_input_grad
-
-        def out(wanted, *shape):
-            return torch.empty(shape, dtype=torch.float32, device=dev) if wanted else None
-
         normed = gamma is not None
-        dgamma, dbeta = out(normed and need[3], K), out(normed and need[4], K)
-        dx = out(need[0] or dgamma is not None or dbeta is not None, B, K, L)     # the norm's gradients are formed on its way
-        dW, db = out(need[1], N, K), out(has_bias and need[2], N)
-        ws = _bytes(L_.p2n_act8_workspace_bytes(B, K, L, N), dev)
-        with torch.cuda.device(dev):
-            _lib.check(L_.p2n_act8_backward(g.data_ptr(), B, K, L, weight.data_ptr(), N, _rt.ptr(gamma), _rt.ptr(beta), int(frozen),
-                                            kept.data_ptr(), kept.numel(), _rt.ptr(dx), _rt.ptr(dW), _rt.ptr(db), _rt.ptr(dgamma),
-                                            _rt.ptr(dbeta), ws.data_ptr(), ws.numel(), _rt.stream_handle(dev)), "p2n_act8_backward")
+
+        def out(*shape):
+            return torch.empty(shape, dtype=torch.float32, device=dev)
+
+        dgamma, dbeta = out(K) if normed and need[3] else None, out(K) if normed and need[4] else None
+        dx = out(B, K, L) if need[0] or dgamma is not None or dbeta is not None else None     # the norm's gradients are formed on its way
+        dW, db = out(N, K) if need[1] else None, out(N) if has_bias and need[2] else None
+        nkept, nws = _act8_bytes("act8_linear", B, K, L, normed, N)
+        ws = _bytes(nws, dev)
+        _call(L_.p2n_act8_backward, "p2n_act8_backward", dev, g.data_ptr(), B, K, L, weight.data_ptr(), N, _rt.ptr(gamma), _rt.ptr(beta),
+              int(frozen), kept.data_ptr(), nkept, _rt.ptr(dx), _rt.ptr(dW), _rt.ptr(db), _rt.ptr(dgamma), _rt.ptr(dbeta),
+              ws.data_ptr(), nws)
         return dx if need[0] else None, dW, db, dgamma, dbeta, None, None, None, None
 
 
@@ -290,15 +303,11 @@ class _Act8NormRelu(torch.autograd.Function):
         L_ = _lib.lib()
         B, C, L = x.shape
         dev = x.device
-        nkept, nws = L_.p2n_act8_kept_bytes(B, C, L, 1), L_.p2n_act8_workspace_bytes(B, C, L, 0)
-        if nkept == 0 or nws == 0:
-            raise ValueError("act8_norm_relu: " + L_.p2n_last_error().decode(errors="replace"))
+        nkept, nws = _act8_bytes("act8_norm_relu", B, C, L, True, 0)
         kept, ws = _bytes(nkept, dev), _bytes(nws, dev)
         y = torch.empty((B, C, L), dtype=torch.float32, device=dev)
-        with torch.cuda.device(dev):
-            _lib.check(L_.p2n_act8_norm_relu_forward(x.data_ptr(), B, C, L, gamma.data_ptr(), beta.data_ptr(), _rt.ptr(running_mean),
-                                                     _rt.ptr(running_var), momentum, eps, y.data_ptr(), kept.data_ptr(), nkept,
-                                                     ws.data_ptr(), nws, _rt.stream_handle(dev)), "p2n_act8_norm_relu_forward")
+        _call(L_.p2n_act8_norm_relu_forward, "p2n_act8_norm_relu_forward", dev, x.data_ptr(), B, C, L, gamma.data_ptr(), beta.data_ptr(),
+              _rt.ptr(running_mean), _rt.ptr(running_var), momentum, eps, y.data_ptr(), kept.data_ptr(), nkept, ws.data_ptr(), nws)
         ctx.save_for_backward(kept, gamma)
         ctx.meta = (B, C, L, momentum < 0)
         return y
@@ -313,11 +322,10 @@ class _Act8NormRelu(torch.autograd.Function):
         dev = g.device
         dx = torch.empty((B, C, L), dtype=torch.float32, device=dev)
         dgamma, dbeta = (torch.empty(C, dtype=torch.float32, device=dev) if ctx.needs_input_grad[i] else None for i in (1, 2))
-        ws = _bytes(L_.p2n_act8_workspace_bytes(B, C, L, 0), dev)
-        with torch.cuda.device(dev):
-            _lib.check(L_.p2n_act8_norm_relu_backward(g.data_ptr(), B, C, L, gamma.data_ptr(), int(frozen), kept.data_ptr(), kept.numel(),
-                                                      dx.data_ptr(), _rt.ptr(dgamma), _rt.ptr(dbeta), ws.data_ptr(), ws.numel(),
-                                                      _rt.stream_handle(dev)), "p2n_act8_norm_relu_backward")
+        nkept, nws = _act8_bytes("act8_norm_relu", B, C, L, True, 0)
+        ws = _bytes(nws, dev)
+        _call(L_.p2n_act8_norm_relu_backward, "p2n_act8_norm_relu_backward", dev, g.data_ptr(), B, C, L, gamma.data_ptr(), int(frozen),
+              kept.data_ptr(), nkept, dx.data_ptr(), _rt.ptr(dgamma), _rt.ptr(dbeta), ws.data_ptr(), nws)
         return dx, dgamma, dbeta, None, None, None, None
 
 
