@@ -431,6 +431,27 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : TABK <= 512 ? 2 : 1) void p2n_ac
     if (c < nchunk) body(c, raw[0]);
     __builtin_amdgcn_s_waitcnt(7 << 4);               // nothing may be on its way into LDS when the workgroup ends
     asm volatile("" ::: "memory");
+    // what was kept of a channel tile: codes, bits, scales; one tile ahead of its use
+    struct Meta {
+        int q[16];
+        i32x4 w[4];
+        f32x4 s[4];
+    } meta[2];
+    auto fetch_meta = [&](Meta &M, int ct) __attribute__((always_inline)) {
+        const long blk = blockIdx.x;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int row = 32 * (ct0 + ct) + 8 * q + 4 * h, c4 = row < A.rows4 ? row : A.rows4 - 4;
+            M.w[q] = *reinterpret_cast<const i32x4 *>(A.bits + (blk * 4 + wave) * A.rows4 + c4);
+            M.s[q] = *reinterpret_cast<const f32x4 *>(A.scale + blk * A.rows4 + c4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = row + j < A.rows ? row + j : A.rows - 1;
+                M.q[4 * q + j] = A.codes[(blk * A.rows + c) * ACT8_GROUP + 32 * wave + p];
+            }
+        }
+    };
+    if (EPI == ACT8_DY) fetch_meta(meta[0], 0);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         const int r0 = 32 * (ct0 + ct);
@@ -441,23 +462,17 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : TABK <= 512 ? 2 : 1) void p2n_ac
         const unsigned oo = (unsigned)((4 * h * A.L + l) * 4);
         if (EPI == ACT8_DY) {
             float s1[16], s2[16];
-            const long blk = blockIdx.x;
             const int bit = (p >> 1) + 16 * (p & 1);
+            const Meta &M = meta[ct & 1];
+            if (ct + 1 < CT) fetch_meta(meta[(ct + 1) & 1], ct + 1);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int row = r0 + 8 * q + 4 * h, c4 = row < A.rows4 ? row : A.rows4 - 4;
-                const i32x4 w = *reinterpret_cast<const i32x4 *>(A.bits + (blk * 4 + wave) * A.rows4 + c4);
-                const f32x4 sc = *reinterpret_cast<const f32x4 *>(A.scale + blk * A.rows4 + c4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int e = 4 * q + j, c = row + j < A.rows ? row + j : A.rows - 1;
-                    const bool on = w[j] >> bit & 1;               // rows past the last one are not stored
-                    const float uh = (float)A.codes[(blk * A.rows + c) * ACT8_GROUP + 32 * wave + p] * sc[j];
-                    const float dy = on ? acc[ct][e] : 0.f;
-                    acc[ct][e] = dy;
-                    s1[e] = dy;
-                    s2[e] = on ? dy * uh : 0.f;
-                }
+            for (int e = 0; e < 16; ++e) {
+                const bool on = M.w[e >> 2][e & 3] >> bit & 1;               // rows past the last one are not stored
+                const float uh = (float)M.q[e] * M.s[e >> 2][e & 3];
+                const float dy = on ? acc[ct][e] : 0.f;
+                acc[ct][e] = dy;
+                s1[e] = dy;
+                s2[e] = on ? dy * uh : 0.f;
             }
             const float t1 = act8_half_sum(s1, lane), t2 = act8_half_sum(s2, lane);
             const int i = lane & 15, c = 32 * ct + 8 * (i >> 2) + 4 * h + (i & 3);
@@ -841,7 +856,13 @@ struct Act8 {
     long wsteps, wper;
 };
 
-int act8_tiles(int rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8; }   // channel tiles of a workgroup
+// Channel tiles of a workgroup: all of them (the points are then read once), fewer where there are so few blocks of points that compute
+// units would stay without one (384 -> 256 at 8,192 points, 64 blocks: 36 us with 8 tiles, 17 with 2).
+int act8_tiles(int rows, long blocks) {
+    int ct = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
+    while (ct > 1 && blocks * ((rows + 32 * ct - 1) / (32 * ct)) < 256) ct >>= 1;
+    return ct;
+}
 int act8_ksteps(int k, int ct) {
     const int cks = act8_chunk(ct), ks = (k + 15) / 16;
     return (ks + cks - 1) / cks * cks;
@@ -854,7 +875,7 @@ int act8_init(Act8 &a, const char *fn, int B, int K, long L, int N) {
     a.B = B; a.K = K; a.N = N; a.L = L; a.NB = (L + ACT8_GROUP - 1) / ACT8_GROUP;
     P2N_REQUIRE((long)B * a.NB * K < (1L << 31) && (long)B * ((L + 1023) / 1024) * K < (1L << 31), "%s: too many points", fn);
     a.Kpad = (K + 63) / 64 * 64;
-    const int cf = act8_tiles(N ? N : 1), cb = act8_tiles(K);
+    const int cf = act8_tiles(N ? N : 1, (long)B * a.NB), cb = act8_tiles(K, (long)B * a.NB);
     a.KSf = act8_ksteps(K, cf); a.CTf = act8_padded(N ? N : 1, cf);
     a.KSb = act8_ksteps(N ? N : 1, cb); a.CTb = act8_padded(K, cb);
     const long blocks = (long)B * ((L + 2047) / 2048);
@@ -934,7 +955,7 @@ int act8_split_weights(const float *W, int rows, int cols, int trans, int CTP, i
 
 template <int IN, int EPI, int TABK>
 int act8_launch_gemm_tab(const Act8Gemm &g, long groups, hipStream_t s) {
-    const int ct = act8_tiles(g.rows);
+    const int ct = act8_tiles(g.rows, groups);
     const dim3 grid((unsigned)groups, (unsigned)(g.CTP / ct)), blk(256);
     switch (ct) {
         case 1: hipLaunchKernelGGL((p2n_act8_gemm_kernel<IN, EPI, 1, TABK>), grid, blk, 0, s, g); break;
