@@ -273,14 +273,23 @@ __device__ __forceinline__ f32x16 act8_mma6(f32x16 acc, bf16x8 ah, bf16x8 am, bf
 // through with their sign turned round, so the cuts cancel.
 __device__ __forceinline__ float act8_flip(float v, unsigned flip) { return __uint_as_float(__float_as_uint(v) ^ flip); }
 
+// Three parts of 8 values, cut instead of rounded: a part is the upper half of a float32, what it leaves is exact, and the third holds
+// the rest: bit operations and exact subtractions.  The dropped products stay under 2^-21 of the product, 2^-23 on average.
 __device__ __forceinline__ void act8_split(const float (&v)[8], bf16x8 &h, bf16x8 &m, bf16x8 &l) {
+    i32x4 ph, pm, pl;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        h[i] = (__bf16)v[i];
-        const float r = v[i] - (float)h[i];
-        m[i] = (__bf16)r;
-        l[i] = (__bf16)(r - (float)m[i]);
+    for (int i = 0; i < 4; ++i) {
+        const unsigned a0 = __float_as_uint(v[2 * i]), a1 = __float_as_uint(v[2 * i + 1]);
+        const float r0 = v[2 * i] - __uint_as_float(a0 & 0xFFFF0000u), r1 = v[2 * i + 1] - __uint_as_float(a1 & 0xFFFF0000u);
+        const unsigned b0 = __float_as_uint(r0), b1 = __float_as_uint(r1);
+        const float s0 = r0 - __uint_as_float(b0 & 0xFFFF0000u), s1 = r1 - __uint_as_float(b1 & 0xFFFF0000u);
+        ph[i] = (int)__builtin_amdgcn_perm(a1, a0, 0x07060302u);
+        pm[i] = (int)__builtin_amdgcn_perm(b1, b0, 0x07060302u);
+        pl[i] = (int)__builtin_amdgcn_perm(__float_as_uint(s1), __float_as_uint(s0), 0x07060302u);
     }
+    h = __builtin_bit_cast(bf16x8, ph);
+    m = __builtin_bit_cast(bf16x8, pm);
+    l = __builtin_bit_cast(bf16x8, pl);
 }
 
 // sums of 16 registers over the 32 lanes of a half, as p2n_tile_half_max: lane i of a 16-lane row ends with register i's sum
@@ -570,10 +579,11 @@ __global__ __launch_bounds__(256) void p2n_act8_dx_kernel(float *__restrict__ dy
 // ---------------------------------------------------------------- weight gradient
 // dW[n][k] = sum over points g[n] * ah[k]: lane = row of either operand, both are rows of consecutive points, and the order of the
 // points inside a product is free as long as both operands agree.  A wave makes 32 RT x 32 CT of dW over its share of the
-// points, 32 at a time, a lane 16 of them: its codes are one 16-byte load; g passes through a piece of LDS that belongs to the
-// wave alone (LDS-DMA in whole cache lines, two buffers, no barrier; read straight from memory a lane touches its line
-// four times, by which time it has left the L1).  The four waves of a workgroup take consecutive shares and are
-// added in LDS, the workgroups by a second kernel, both in order.
+// points, 32 at a time, a lane 16 of them: its codes are one 16-byte load, its g passes through a piece of
+// LDS that belongs to the wave alone (no barrier): it is read in whole cache lines, eight lanes a row (a lane reading its own row's
+// bytes keeps the address unit busy for 113 cycles an instruction), and handed over as rows.  The next step's g waits in
+// registers meanwhile, for a 128 x 128 tile, which has none left, in a second piece that LDS-DMA fills.  The four waves of a
+// workgroup are added in LDS, the workgroups by a second kernel, both in order.
 struct Act8Wgrad {
     const float *g;        // (B, N, L)
     const signed char *codes;
@@ -581,16 +591,18 @@ struct Act8Wgrad {
     const unsigned *bits;  // NULL: a = uh
     const float *gamma, *beta;
     float *part;           // [slices][N * K + N]: dW, db
-    long L, NB, steps, per;   // steps of 32 points in all, per wave
-    int N, K, K4, ntc, slices;
+    long L, NB;
+    int N, K, K4, ntc, slices, steps;        // steps of 32 points in all
 };
 
-// DMA: rows of g start 16-byte aligned (L a multiple of 4); without, its values are loaded from memory as they are needed
-template <int RT, int CT, bool DMA>
+// DMA (128 x 128 only): rows of g start 16-byte aligned (L a multiple of 4); without, its values are loaded as they are needed
+template <int RT, int CT, bool DMA, bool NORM>
 __global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : 2) void p2n_act8_wgrad_kernel(Act8Wgrad A) {
+    constexpr bool REG = RT * CT < 16;
     constexpr int BUF = RT * 4096;                   // 32 RT rows of 128 bytes
     constexpr int JOIN = (RT * CT * 1024 + 4 * 32 * RT) * 4;
-    __shared__ __attribute__((aligned(16))) char lds[DMA && 8 * BUF > JOIN ? 8 * BUF : JOIN];
+    constexpr int OWN = DMA ? 8 * BUF : REG ? 4 * BUF : 0;
+    __shared__ __attribute__((aligned(16))) char lds[OWN > JOIN ? OWN : JOIN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int r = lane & 31, h = lane >> 5;
     // neighbouring workgroups go to the eight dies in turn: the tiles of one slice stay on one die, whose L2 then holds its rows
@@ -599,7 +611,19 @@ __global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : 2) void p2n_act8_wgrad_kern
     if ((int)blockIdx.x < full * nt) { tile = w8 % nt; slice = w8 / nt * 8 + (blockIdx.x & 7); }
     else { const int i = blockIdx.x - full * nt; tile = i % nt; slice = full + i / nt; }
     const int n0 = tile / A.ntc * 32 * RT, k0 = tile % A.ntc * 32 * CT;
-    const long i0 = ((long)slice * 4 + wave) * A.per, i1 = i0 + A.per < A.steps ? i0 + A.per : A.steps;
+    // waves take turns: those that run at the same time read neighbouring lines of the same rows (shares of consecutive steps
+    // instead scatter the card's reads over as many pages of memory as there are rows in flight)
+    struct Step {
+        int b, q;                           // cloud, 32 points in it
+    };
+    const int turn = A.slices * 4, first = slice * 4 + wave, spc = (int)(4 * A.NB);
+    const int turn_b = turn / spc, turn_q = turn % spc;
+    auto after = [&](Step s) __attribute__((always_inline)) {
+        s.b += turn_b;
+        s.q += turn_q;
+        if (s.q >= spc) { s.q -= spc; s.b += 1; }
+        return s;
+    };
     const unsigned flip = (unsigned)((slice * 4 + wave) & 1) << 31;       // every other share with its sign turned round (act8_flip)
     const bool want_db = k0 == 0;
     int krow[CT];
@@ -610,8 +634,8 @@ __global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : 2) void p2n_act8_wgrad_kern
     for (int i = 0; i < CT; ++i) {
         const int k = k0 + 32 * i + r;
         krow[i] = k < A.K ? k : A.K - 1;
-        ga[i] = A.bits ? A.gamma[krow[i]] : 1.f;
-        be[i] = A.bits ? A.beta[krow[i]] : 0.f;
+        ga[i] = NORM ? A.gamma[krow[i]] : 1.f;
+        be[i] = NORM ? A.beta[krow[i]] : 0.f;
         poison[i] = 0.f;
     }
     f32x16 acc[RT][CT];
@@ -621,15 +645,14 @@ __global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : 2) void p2n_act8_wgrad_kern
         for (int k = 0; k < CT; ++k)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][k][e] = 0.f;
-    const long spc = 4 * A.NB;              // steps of a cloud
     // LDS image of a step: row R's 16-byte piece q (points 4q .. 4q+3) lies in slot q ^ (R >> 1 & 7) of the row, so that the 16 rows of a
     // read fall into different banks.  DMA instruction i fills rows 8i .. 8i+7: lane -> row lane >> 3, slot lane & 7.
-    char *const mine = lds + wave * 2 * BUF;
+    char *const mine = lds + wave * (DMA ? 2 * BUF : BUF);
     const int drow = lane >> 3, piece = (lane & 7) ^ (lane >> 4);
     const int left = A.N - n0;              // rows past the last one read the last one
     const unsigned off_full = (unsigned)(drow * A.L * 4), off_part = (unsigned)((drow < (left & 7) ? drow : (left & 7) - 1) * A.L * 4);
-    auto dma = [&](long s, int buf) __attribute__((always_inline)) {
-        const long b = s / spc, l0 = (s % spc) * 32;
+    auto dma = [&](Step s, int buf) __attribute__((always_inline)) {
+        const long b = s.b, l0 = (long)s.q * 32;
 #pragma unroll
         for (int i = 0; i < RT * 4; ++i) {
             const bool part = 8 * i < left && left < 8 * i + 8, none = 8 * i >= left;        // wave-uniform
@@ -642,27 +665,49 @@ __global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : 2) void p2n_act8_wgrad_kern
     int qn[CT][4];
     float sn[CT];
     unsigned mn[CT];
-    auto meta = [&](long s) __attribute__((always_inline)) {
-        const long blk = s >> 2;
-        const int w = (int)(s & 3);
+    auto meta = [&](Step s) __attribute__((always_inline)) {
+        const long blk = s.b * A.NB + (s.q >> 2);
+        const int w = s.q & 3;
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
             const i32x4 q = *reinterpret_cast<const i32x4 *>(A.codes + (blk * A.K + krow[t]) * ACT8_GROUP + 32 * w + 16 * h);
 #pragma unroll
             for (int x = 0; x < 4; ++x) qn[t][x] = q[x];
             sn[t] = A.scale[blk * A.K4 + krow[t]];
-            mn[t] = A.bits ? A.bits[(blk * 4 + w) * A.K4 + krow[t]] : 0u;
+            mn[t] = NORM ? A.bits[(blk * 4 + w) * A.K4 + krow[t]] : 0u;
         }
     };
-    if (i0 < i1) {
-        if (DMA) dma(i0, 0);
-        meta(i0);
+    f32x4 vn[REG ? RT * 4 : 1];
+    auto rows = [&](Step s) __attribute__((always_inline)) {
+        const long b = s.b, l0 = (long)s.q * 32, l = l0 + 4 * (lane & 7);
+        const bool tail = l0 + 32 > A.L;
+#pragma unroll
+        for (int i = 0; i < (REG ? RT * 4 : 0); ++i) {
+            const int n = n0 + 8 * i + drow;
+            const float *p = A.g + (b * A.N + (n < A.N ? n : A.N - 1)) * A.L + l;
+            if (!tail) vn[i] = *reinterpret_cast<const f32x4u *>(p);
+            else
+#pragma unroll
+                for (int x = 0; x < 4; ++x) vn[i][x] = l + x < A.L ? p[x] : 0.f;
+        }
+    };
+    Step step = {first / spc, first % spc};
+    if (first < A.steps) {
+        if (DMA) dma(step, 0);
+        if (REG) rows(step);
+        meta(step);
     }
+    int buf = 0;
 #pragma unroll 1
-    for (long s = i0; s < i1; ++s) {
-        const int buf = (int)(s - i0) & 1;
-        __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));         // vmcnt(0): this step's rows and codes have arrived
-        asm volatile("" ::: "memory");
+    for (int s = first; s < A.steps; s += turn, buf ^= 1) {
+        if (DMA) {
+            __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));     // vmcnt(0): this step's rows and codes have arrived
+            asm volatile("" ::: "memory");
+        }
+        if (REG) {
+#pragma unroll
+            for (int i = 0; i < (REG ? RT * 4 : 0); ++i) *reinterpret_cast<f32x4 *>(mine + i * 1024 + drow * 128 + (piece ^ (4 * (i & 1))) * 16) = vn[i];
+        }
         int q[CT][4];
         float cs[CT];
         unsigned mb[CT];
@@ -674,11 +719,14 @@ __global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : 2) void p2n_act8_wgrad_kern
             poison[t] += cs[t] * 0.f;                       // NaN with a NaN scale
             mb[t] = mn[t] >> (8 * h);                       // points 16h .. 16h+15: bits 8h .. of either half-word
         }
-        if (s + 1 < i1) {
-            if (DMA) dma(s + 1, buf ^ 1);
-            meta(s + 1);
+        const Step next = after(step);
+        if (s + turn < A.steps) {
+            if (DMA) dma(next, buf ^ 1);
+            if (REG) rows(next);
+            meta(next);
         }
-        const long b = s / spc, l0 = (s % spc) * 32;
+        const long b = step.b, l0 = (long)step.q * 32;
+        step = next;
         const bool tail = l0 + 32 > A.L;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -687,14 +735,14 @@ __global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : 2) void p2n_act8_wgrad_kern
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
                 float va[8];
-                if (DMA) {
-                    const char *row = mine + buf * BUF + (32 * t + r) * 128;
+                if (REG || DMA) {
+                    const char *row = mine + (DMA ? buf * BUF : 0) + (32 * t + r) * 128;
                     const int key = r >> 1 & 7;
                     const f32x4 e0 = *reinterpret_cast<const f32x4 *>(row + ((4 * h + 2 * j) ^ key) * 16);
                     const f32x4 e1 = *reinterpret_cast<const f32x4 *>(row + ((4 * h + 2 * j + 1) ^ key) * 16);
 #pragma unroll
                     for (int x = 0; x < 4; ++x) { va[x] = e0[x]; va[4 + x] = e1[x]; }
-                    if (tail) {
+                    if (DMA && tail) {
 #pragma unroll
                         for (int x = 0; x < 8; ++x) va[x] = l + x < A.L ? va[x] : 0.f;
                     }
@@ -721,7 +769,7 @@ __global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : 2) void p2n_act8_wgrad_kern
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
                     const float c = (float)(signed char)(q[t][2 * j + (x >> 2)] >> (8 * (x & 3)));
-                    if (A.bits) {
+                    if (NORM) {
                         const float y = fmaxf(fmaf(cs[t], c, be[t]), 0.f);
                         const int on = (int)(mb[t] << (31 - ((4 * j + (x >> 1)) + 16 * (x & 1)))) >> 31;
                         v[x] = __int_as_float(__float_as_int(y) & on);
@@ -853,7 +901,7 @@ struct Act8 {
     int S;                   // slices of the statistics
     long per;
     int RT, CT, ntc, nt, slices;     // weight gradient: 32-row tiles of a wave, tiles, slices of the points
-    long wsteps, wper;
+    long wsteps;
 };
 
 // Channel tiles of a workgroup: all of them (the points are then read once), fewer where there are so few blocks of points that compute
@@ -873,7 +921,7 @@ int act8_init(Act8 &a, const char *fn, int B, int K, long L, int N) {
     P2N_REQUIRE(B >= 1 && L >= 1 && L <= (1L << 24), "%s: bad shape B=%d L=%ld (1 to 2^24 columns a cloud)", fn, B, L);
     P2N_REQUIRE(K >= 1 && K <= ACT8_MAX_C && N >= 0 && N <= ACT8_MAX_C, "%s: %d or %d channels, not in [1,%d]", fn, K, N, ACT8_MAX_C);
     a.B = B; a.K = K; a.N = N; a.L = L; a.NB = (L + ACT8_GROUP - 1) / ACT8_GROUP;
-    P2N_REQUIRE((long)B * a.NB * K < (1L << 31) && (long)B * ((L + 1023) / 1024) * K < (1L << 31), "%s: too many points", fn);
+    P2N_REQUIRE((long)B * a.NB * 4 < (1L << 30) && (long)B * a.NB * K < (1L << 31) && (long)B * ((L + 1023) / 1024) * K < (1L << 31), "%s: too many points", fn);
     a.Kpad = (K + 63) / 64 * 64;
     const int cf = act8_tiles(N ? N : 1, (long)B * a.NB), cb = act8_tiles(K, (long)B * a.NB);
     a.KSf = act8_ksteps(K, cf); a.CTf = act8_padded(N ? N : 1, cf);
@@ -893,11 +941,10 @@ int act8_init(Act8 &a, const char *fn, int B, int K, long L, int N) {
     a.RT = tiles(N ? N : 1); a.CT = tiles(K);
     a.ntc = (K + 32 * a.CT - 1) / (32 * a.CT);
     a.nt = ((N ? N : 1) + 32 * a.RT - 1) / (32 * a.RT) * a.ntc;
-    const long wgs = a.RT * a.CT >= 8 ? 256 : 512;
+    const long wgs = a.RT * a.CT >= 8 ? 256 : a.RT * a.CT >= 4 ? 512 : a.RT * a.CT == 2 ? 768 : 1024;
     long sl = wgs / a.nt > 1 ? wgs / a.nt : 1;
     if (sl > (a.wsteps + 7) / 8) sl = (a.wsteps + 7) / 8;
-    a.wper = (a.wsteps + 4 * sl - 1) / (4 * sl);
-    a.slices = (int)((a.wsteps + 4 * a.wper - 1) / (4 * a.wper));
+    a.slices = (int)sl;
     return P2N_OK;
 }
 
@@ -973,23 +1020,19 @@ int act8_launch_gemm(const Act8Gemm &g, long groups, hipStream_t s) {
     return act8_launch_gemm_tab<IN, EPI, 512>(g, groups, s);
 }
 
-template <int RT, bool DMA>
+template <int RT, bool NORM>
 int act8_launch_wgrad_rt(const Act8 &a, const Act8Wgrad &w, hipStream_t s) {
     const dim3 grid((unsigned)(a.nt * a.slices)), blk(256);
-    switch (a.CT) {
-        case 1: hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 1, DMA>), grid, blk, 0, s, w); break;
-        case 2: hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 2, DMA>), grid, blk, 0, s, w); break;
-        default: hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 4, DMA>), grid, blk, 0, s, w);
-    }
+    if (a.CT == 1) hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 1, false, NORM>), grid, blk, 0, s, w);
+    else if (a.CT == 2) hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 2, false, NORM>), grid, blk, 0, s, w);
+    else if (RT == 4 && a.L % 4 == 0 && ((uintptr_t)w.g & 15) == 0) hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 4, RT == 4, NORM>), grid, blk, 0, s, w);
+    else hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 4, false, NORM>), grid, blk, 0, s, w);
     P2N_CHECK_HIP(hipGetLastError());
     return P2N_OK;
 }
-template <bool DMA>
-int act8_launch_wgrad_any(const Act8 &a, const Act8Wgrad &w, hipStream_t s) {
-    return a.RT == 1 ? act8_launch_wgrad_rt<1, DMA>(a, w, s) : a.RT == 2 ? act8_launch_wgrad_rt<2, DMA>(a, w, s) : act8_launch_wgrad_rt<4, DMA>(a, w, s);
-}
+template <bool NORM>
 int act8_launch_wgrad(const Act8 &a, const Act8Wgrad &w, hipStream_t s) {
-    return a.L % 4 == 0 && ((uintptr_t)w.g & 15) == 0 ? act8_launch_wgrad_any<true>(a, w, s) : act8_launch_wgrad_any<false>(a, w, s);
+    return a.RT == 1 ? act8_launch_wgrad_rt<1, NORM>(a, w, s) : a.RT == 2 ? act8_launch_wgrad_rt<2, NORM>(a, w, s) : act8_launch_wgrad_rt<4, NORM>(a, w, s);
 }
 
 int act8_space_check(const char *fn, const void *p, size_t have, size_t need, const char *what) {
@@ -1102,8 +1145,8 @@ extern "C" int p2n_act8_backward(const float *g, int B, int K, long L, const flo
     if (dW || db) {
         Act8Wgrad w = {};
         w.g = g; w.codes = codes; w.scale = scale; w.bits = bits; w.gamma = gamma; w.beta = beta; w.part = f.wpart;
-        w.L = L; w.NB = a.NB; w.steps = a.wsteps; w.per = a.wper; w.N = N; w.K = K; w.K4 = K4; w.ntc = a.ntc; w.slices = a.slices;
-        TRY(act8_launch_wgrad(a, w, s));
+        w.L = L; w.NB = a.NB; w.steps = (int)a.wsteps; w.N = N; w.K = K; w.K4 = K4; w.ntc = a.ntc; w.slices = a.slices;
+        TRY(gamma ? act8_launch_wgrad<true>(a, w, s) : act8_launch_wgrad<false>(a, w, s));
         const long n = (long)N * K + N;
         hipLaunchKernelGGL(p2n_act8_join_kernel, dim3((unsigned)((n + 31) / 32)), dim3(1024), 0, s, f.wpart, n, (long)N * K, a.slices, dW, db);
         P2N_CHECK_HIP(hipGetLastError());
