@@ -136,22 +136,32 @@ __global__ void p2n_act8_norm_kernel(const double *__restrict__ part, int S, con
 }
 
 // ---------------------------------------------------------------- codes
-// A workgroup takes 32 channels of a block of 128 points, a wave 8 of them, a lane two neighbouring points: u, the scales, codes,
-// the ReLU's bits.  The channels' maxima are formed by a halving exchange (8 registers shrink to one while lanes pair up), so
-// lane i holds the maximum of channel i & 7 and one division serves eight channels.
-template <bool NORM>
-__global__ __launch_bounds__(256) void p2n_act8_pack_kernel(const float *__restrict__ x, int C, int C4, long L, long NB, const float *__restrict__ stat,
-                                                            const float *__restrict__ gamma, const float *__restrict__ beta, signed char *__restrict__ codes,
-                                                            float *__restrict__ scale, unsigned *__restrict__ bits) {
+// What is kept of a block of 128 points, 32 channels a workgroup and 8 a wave, a lane two neighbouring points: u, the scales, codes, the ReLU's
+// bits.  The channels' maxima are formed by a halving exchange (8 registers shrink to one while lanes pair up), so lane i holds
+// the maximum of channel i & 7 and one division serves eight channels.  OUT (the end of a chain): relu(y)
+// to `out` as well.
+struct Act8Keep {
+    const float *x;
+    const float *stat, *gamma, *beta;    // NORM
+    signed char *codes;
+    float *scale;
+    unsigned *bits;
+    float *out;                          // OUT
+    long L, NB;
+    int C, C4;
+};
+template <bool NORM, bool OUT>
+__global__ __launch_bounds__(256) void p2n_act8_keep_kernel(Act8Keep A) {
     const int lane = threadIdx.x & 63;
     const int c0 = blockIdx.y * 32 + 8 * __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    if (c0 >= C4) return;
-    const long blk = blockIdx.x, b = blk / NB, l = (blk % NB) * ACT8_GROUP + 2 * lane;
-    const bool ok0 = l < L, ok1 = l + 1 < L;
+    const long blk = blockIdx.x;
+    if (c0 >= A.C4) return;
+    const long b = blk / A.NB, l = (blk % A.NB) * ACT8_GROUP + 2 * lane;
+    const bool ok0 = l < A.L, ok1 = l + 1 < A.L;
     float v[8][2];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float *row = x + (b * C + (c0 + i < C ? c0 + i : C - 1)) * L;
+        const float *row = A.x + (b * A.C + (c0 + i < A.C ? c0 + i : A.C - 1)) * A.L;
         v[i][0] = v[i][1] = 0.f;
         if (ok1) {
             const f32x2u e = *reinterpret_cast<const f32x2u *>(row + l);
@@ -165,14 +175,20 @@ __global__ __launch_bounds__(256) void p2n_act8_pack_kernel(const float *__restr
     unsigned am[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const int c = c0 + i < C ? c0 + i : C - 1;
+        const int c = c0 + i < A.C ? c0 + i : A.C - 1;
         if (NORM) {
-            const float mu = stat[c], r = stat[C + c], ga = gamma[c], be = beta[c];
+            const float mu = A.stat[c], r = A.stat[A.C + c], ga = A.gamma[c], be = A.beta[c];
             v[i][0] = ok0 ? (v[i][0] - mu) * r : 0.f;
             v[i][1] = ok1 ? (v[i][1] - mu) * r : 0.f;
-            const unsigned long long e = __ballot(ok0 && !(fmaf(ga, v[i][0], be) <= 0.f)), o = __ballot(ok1 && !(fmaf(ga, v[i][1], be) <= 0.f));
+            const float y0 = fmaf(ga, v[i][0], be), y1 = fmaf(ga, v[i][1], be);
+            const unsigned long long e = __ballot(ok0 && !(y0 <= 0.f)), o = __ballot(ok1 && !(y1 <= 0.f));
             const unsigned w = ((unsigned)(e >> (16 * q)) & 0xFFFFu) | (unsigned)(o >> (16 * q)) << 16;
             word = (lane & 7) == i ? w : word;
+            if (OUT && c0 + i < A.C) {
+                float *row = A.out + (b * A.C + c0 + i) * A.L;
+                if (ok1) *reinterpret_cast<f32x2u *>(row + l) = f32x2u{act8_relu(y0), act8_relu(y1)};
+                else if (ok0) row[l] = act8_relu(y0);
+            }
         }
         const unsigned a = p2n_absbits(v[i][0]), a1 = p2n_absbits(v[i][1]);
         am[i] = a > a1 ? a : a1;
@@ -191,13 +207,13 @@ __global__ __launch_bounds__(256) void p2n_act8_pack_kernel(const float *__restr
         const unsigned o = (unsigned)__shfl_xor((int)am[0], m);
         am[0] = o > am[0] ? o : am[0];
     }
-    float s = p2n_q8_scale(am[0]);                  // of channel c0 + (lane & 7)
+    const float s = p2n_q8_scale(am[0]);                  // of channel c0 + (lane & 7)
     const P2nQ8 Q = p2n_q8_make(s);
-    if (lane < 8 && c0 + lane < C4) scale[blk * C4 + c0 + lane] = c0 + lane < C ? s : 0.f;
-    if (NORM && lane < 32 && c0 + (lane & 7) < C4) bits[(blk * 4 + q) * C4 + c0 + (lane & 7)] = c0 + (lane & 7) < C ? word : 0u;
+    if (lane < 8 && c0 + lane < A.C4) A.scale[blk * A.C4 + c0 + lane] = c0 + lane < A.C ? s : 0.f;
+    if (NORM && lane < 32 && c0 + (lane & 7) < A.C4) A.bits[(blk * 4 + q) * A.C4 + c0 + (lane & 7)] = c0 + (lane & 7) < A.C ? word : 0u;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        if (c0 + i >= C) break;
+        if (c0 + i >= A.C) break;
         P2nQ8 R;
         R.s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(Q.s), i));
         R.up = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(Q.up), i));
@@ -206,7 +222,7 @@ __global__ __launch_bounds__(256) void p2n_act8_pack_kernel(const float *__restr
         int code[1];
         p2n_q8_pack(e, R, code);
         if (!(R.s == R.s)) code[0] = 0;
-        *reinterpret_cast<unsigned short *>(codes + (blk * C + c0 + i) * ACT8_GROUP + 2 * lane) = (unsigned short)code[0];
+        *reinterpret_cast<unsigned short *>(A.codes + (blk * A.C + c0 + i) * ACT8_GROUP + 2 * lane) = (unsigned short)code[0];
     }
 }
 
@@ -259,14 +275,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t act8_rsrc(const void *base, lo
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)(bytes < 0xFFFFFFFFL ? bytes : 0xFFFFFFFFL), 0x00020000);
 }
 
-__device__ __forceinline__ f32x16 act8_mma6(f32x16 acc, bf16x8 ah, bf16x8 am, bf16x8 al, bf16x8 bh, bf16x8 bm, bf16x8 bl) {
-    acc = MFMAB(al, bh, acc);      // the small ones first
-    acc = MFMAB(ah, bl, acc);
-    acc = MFMAB(am, bm, acc);
-    acc = MFMAB(am, bh, acc);
-    acc = MFMAB(ah, bm, acc);
-    return MFMAB(ah, bh, acc);
-}
+// the six products of the three parts, the small ones first: l.h, h.l, m.m, m.h, h.m, h.h
+__device__ constexpr int act8_first(int c) { return c == 0 ? 2 : c == 1 || c >= 4 ? 0 : 1; }
+__device__ constexpr int act8_second(int c) { return c == 1 ? 2 : c == 2 || c == 4 ? 1 : 0; }
 
 // The matrix cores cut the low bits of a sum towards minus infinity (measured: the mean of h is off by -1.5e-8 of its deviation at
 // 256 channels whatever its sign, the float32 instruction's by 3e-11), and a sum over 10^5 points adds that up.  Half of the points go
@@ -409,9 +420,8 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : TABK <= 512 ? 2 : 1) void p2n_ac
 #pragma unroll
                 for (int u = 0; u < PW; ++u) {
                     const int t = i * PW + u, ks = t / CT, ct = t % CT;
-                    const bf16x8 wq = f[i & 1][u][q == 0 ? 2 : q == 1 || q >= 4 ? 0 : 1];
-                    const bf16x8 xq = q == 1 ? xl[ks] : q == 2 || q == 4 ? xm[ks] : xh[ks];     // l.h, h.l, m.m, m.h, h.m, h.h
-                    acc[ct] = MFMAB(wq, xq, acc[ct]);
+                    const bf16x8 xq = act8_second(q) == 2 ? xl[ks] : act8_second(q) == 1 ? xm[ks] : xh[ks];
+                    acc[ct] = MFMAB(f[i & 1][u][act8_first(q)], xq, acc[ct]);
                 }
         }
         __builtin_amdgcn_sched_group_barrier(0x100, 3 * PW * (NP > 1 ? 2 : 1), 0);      // LDS reads
@@ -782,7 +792,9 @@ __global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : 2) void p2n_act8_wgrad_kern
 #pragma unroll
             for (int t = 0; t < RT; ++t)
 #pragma unroll
-                for (int k = 0; k < CT; ++k) acc[t][k] = act8_mma6(acc[t][k], a[t][0], a[t][1], a[t][2], w[k][0], w[k][1], w[k][2]);
+                for (int k = 0; k < CT; ++k)
+#pragma unroll
+                    for (int c = 0; c < 6; ++c) acc[t][k] = MFMAB(a[t][act8_first(c)], w[k][act8_second(c)], acc[t][k]);
         }
     }
     // the four waves' shares, added in order: a quarter of the tile's registers at a time, all waves at once
@@ -838,21 +850,7 @@ __global__ __launch_bounds__(1024) void p2n_act8_join_kernel(const float *__rest
     }
 }
 
-// ---------------------------------------------------------------- norm + ReLU alone (the end of a chain)
-__global__ __launch_bounds__(256) void p2n_act8_apply_kernel(const float *__restrict__ x, long rows, int C, int Cpad, long L, const float *__restrict__ tab, float *__restrict__ out) {
-    const long LB = (L + 1023) / 1024;
-    const long row = blockIdx.x / LB, l0 = (blockIdx.x % LB) * 1024;
-    const int c = (int)(row % C);
-    const float mu = tab[c], s = tab[Cpad + c], t = tab[2 * Cpad + c];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const long l = l0 + 256 * j + threadIdx.x;
-        if (l < L) {
-            out[row * L + l] = act8_relu(fmaf(x[row * L + l] - mu, s, t));
-        }
-    }
-}
-
+// ---------------------------------------------------------------- norm + ReLU alone (the end of a chain), backward
 // dy = [y > 0] * g and its sums; one workgroup per (channel, slice of the (cloud, block) list), a wave takes a block, a lane two points
 __global__ __launch_bounds__(256) void p2n_act8_dy_kernel(const float *__restrict__ g, int B, int C, int C4, long L, long NB, long per,
                                                           const signed char *__restrict__ codes, const float *__restrict__ scale, const unsigned *__restrict__ bits,
@@ -932,13 +930,12 @@ int act8_init(Act8 &a, const char *fn, int B, int K, long L, int N) {
     if (s > 1024) s = 1024;
     a.per = (blocks + s - 1) / s;
     a.S = (int)((blocks + a.per - 1) / a.per);
-    // a wave makes up to 128 x 128 where there are points enough to fill the card with such waves (256 clouds' blocks of 128:
-    // measured at 8,192 points, 256 x 384: 56 us against 27 with 64 x 64), up to 64 x 64 otherwise; the points go to about as
-    // many waves as are resident at that tile's register count
+    // a wave makes up to 64 x 64, two of them on a SIMD; 128 x 128 (which fills the registers alone, and splits each operand half as
+    // often) where both sides are that long and there are points enough for such waves: 256 x 256 at 131,072 points 140 us against
+    // 155, 64 x 128 at 262,144 points 70 against 55 with 128 rows, 256 x 384 at 8,192 points 56 against 19
     a.wsteps = (long)B * a.NB * 4;
-    const int cap = a.wsteps < 2048 ? 2 : 4;
-    auto tiles = [cap](int n) { return n <= 32 ? 1 : n <= 64 ? 2 : cap; };
-    a.RT = tiles(N ? N : 1); a.CT = tiles(K);
+    const bool big = N >= 128 && K >= 128 && a.wsteps >= 2048;
+    a.RT = big ? 4 : N <= 32 ? 1 : 2; a.CT = big ? 4 : K <= 32 ? 1 : 2;
     a.ntc = (K + 32 * a.CT - 1) / (32 * a.CT);
     a.nt = ((N ? N : 1) + 32 * a.RT - 1) / (32 * a.RT) * a.ntc;
     const long wgs = a.RT * a.CT >= 8 ? 256 : a.RT * a.CT >= 4 ? 512 : a.RT * a.CT == 2 ? 768 : 1024;
@@ -1020,19 +1017,20 @@ int act8_launch_gemm(const Act8Gemm &g, long groups, hipStream_t s) {
     return act8_launch_gemm_tab<IN, EPI, 512>(g, groups, s);
 }
 
-template <int RT, bool NORM>
-int act8_launch_wgrad_rt(const Act8 &a, const Act8Wgrad &w, hipStream_t s) {
-    const dim3 grid((unsigned)(a.nt * a.slices)), blk(256);
-    if (a.CT == 1) hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 1, false, NORM>), grid, blk, 0, s, w);
-    else if (a.CT == 2) hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 2, false, NORM>), grid, blk, 0, s, w);
-    else if (RT == 4 && a.L % 4 == 0 && ((uintptr_t)w.g & 15) == 0) hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 4, RT == 4, NORM>), grid, blk, 0, s, w);
-    else hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, 4, false, NORM>), grid, blk, 0, s, w);
-    P2N_CHECK_HIP(hipGetLastError());
-    return P2N_OK;
+template <int RT, int CT, bool DMA, bool NORM>
+void act8_launch_wgrad_as(const Act8 &a, const Act8Wgrad &w, hipStream_t s) {
+    hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, CT, DMA, NORM>), dim3((unsigned)(a.nt * a.slices)), dim3(256), 0, s, w);
 }
 template <bool NORM>
 int act8_launch_wgrad(const Act8 &a, const Act8Wgrad &w, hipStream_t s) {
-    return a.RT == 1 ? act8_launch_wgrad_rt<1, NORM>(a, w, s) : a.RT == 2 ? act8_launch_wgrad_rt<2, NORM>(a, w, s) : act8_launch_wgrad_rt<4, NORM>(a, w, s);
+    if (a.RT == 4 && a.L % 4 == 0 && ((uintptr_t)w.g & 15) == 0) act8_launch_wgrad_as<4, 4, true, NORM>(a, w, s);
+    else if (a.RT == 4) act8_launch_wgrad_as<4, 4, false, NORM>(a, w, s);
+    else if (a.RT == 2 && a.CT == 2) act8_launch_wgrad_as<2, 2, false, NORM>(a, w, s);
+    else if (a.RT == 2) act8_launch_wgrad_as<2, 1, false, NORM>(a, w, s);
+    else if (a.CT == 2) act8_launch_wgrad_as<1, 2, false, NORM>(a, w, s);
+    else act8_launch_wgrad_as<1, 1, false, NORM>(a, w, s);
+    P2N_CHECK_HIP(hipGetLastError());
+    return P2N_OK;
 }
 
 int act8_space_check(const char *fn, const void *p, size_t have, size_t need, const char *what) {
@@ -1044,30 +1042,28 @@ int act8_space_check(const char *fn, const void *p, size_t have, size_t need, co
     return P2N_OK;
 }
 
-// statistics, tables and codes of x; returns with f.tab set (norm)
-int act8_keep(const Act8 &a, const char *fn, const float *x, const float *gamma, const float *beta, float *rmean, float *rvar, float momentum,
-              float eps, char *kept, const FwdSpace &f, hipStream_t s) {
+// statistics and tables of x (norm), and what is kept of it; relu(y) to `out` where given
+int act8_keep(const Act8 &a, const float *x, const float *gamma, const float *beta, float *rmean, float *rvar, float momentum, float eps,
+                    char *kept, const FwdSpace &f, float *out, hipStream_t s) {
     const Act8Kept k = act8_kept(a.B, a.K, a.L, gamma != nullptr);
     float *stat = (float *)(kept + k.stat);
-    const int K4 = (a.K + 3) / 4 * 4;
-    const dim3 pgrid((unsigned)((long)a.B * a.NB), (unsigned)((a.K + 31) / 32)), blk(256);
     if (gamma) {
         const bool frozen = momentum < 0.f;
         const double P = (double)a.B * a.L;
         if (!frozen) {
             const long blocks = (long)a.B * ((a.L + 2047) / 2048);
-            hipLaunchKernelGGL(p2n_act8_stats_kernel, dim3(a.K, a.S), blk, 0, s, x, a.B, a.K, a.L, blocks, a.per, f.part);
+            hipLaunchKernelGGL(p2n_act8_stats_kernel, dim3(a.K, a.S), dim3(256), 0, s, x, a.B, a.K, a.L, blocks, a.per, f.part);
             P2N_CHECK_HIP(hipGetLastError());
         }
         hipLaunchKernelGGL(p2n_act8_norm_kernel, dim3(a.Kpad), dim3(64), 0, s, f.part, a.S, x, a.K, a.Kpad, a.L, P, gamma, beta, rmean, rvar,
                            (double)momentum, (double)eps, frozen ? 1 : 0, stat, f.tab);
         P2N_CHECK_HIP(hipGetLastError());
-        hipLaunchKernelGGL(p2n_act8_pack_kernel<true>, pgrid, blk, 0, s, x, a.K, K4, a.L, a.NB, stat, gamma, beta, (signed char *)kept,
-                           (float *)(kept + k.scale), (unsigned *)(kept + k.bits));
-    } else {
-        hipLaunchKernelGGL(p2n_act8_pack_kernel<false>, pgrid, blk, 0, s, x, a.K, K4, a.L, a.NB, nullptr, nullptr, nullptr, (signed char *)kept,
-                           (float *)(kept + k.scale), nullptr);
     }
+    const Act8Keep keep{x, stat, gamma, beta, (signed char *)kept, (float *)(kept + k.scale), (unsigned *)(kept + k.bits), out, a.L, a.NB, a.K, (a.K + 3) / 4 * 4};
+    const dim3 grid((unsigned)((long)a.B * a.NB), (unsigned)((a.K + 31) / 32));
+    if (out) hipLaunchKernelGGL((p2n_act8_keep_kernel<true, true>), grid, dim3(256), 0, s, keep);
+    else if (gamma) hipLaunchKernelGGL((p2n_act8_keep_kernel<true, false>), grid, dim3(256), 0, s, keep);
+    else hipLaunchKernelGGL((p2n_act8_keep_kernel<false, false>), grid, dim3(256), 0, s, keep);
     P2N_CHECK_HIP(hipGetLastError());
     return P2N_OK;
 }
@@ -1109,9 +1105,9 @@ extern "C" int p2n_act8_forward(const float *x, int B, int K, long L, const floa
     const FwdSpace f = fwd_space(a, (char *)workspace);
     hipStream_t s = (hipStream_t)stream_;
     const int ps = p2n_prof_begin(P2N_K_ACT8_FWD, s);
-    TRY(act8_keep(a, fn, x, gamma, beta, running_mean, running_var, momentum, eps, (char *)kept, f, s));
-    TRY(act8_split_weights(W, N, K, 0, a.CTf, a.KSf, f.img, s));
     Act8Gemm g = {};
+    TRY(act8_keep(a, x, gamma, beta, running_mean, running_var, momentum, eps, (char *)kept, f, nullptr, s));
+    TRY(act8_split_weights(W, N, K, 0, a.CTf, a.KSf, f.img, s));
     g.x = x; g.img = f.img; g.tab = f.tab; g.bias = bias; g.out = h; g.L = L; g.NB = a.NB;
     g.K = K; g.Kpad = a.Kpad; g.KS = a.KSf; g.CTP = a.CTf; g.rows = N;
     const long groups = (long)B * a.NB;
@@ -1183,10 +1179,7 @@ extern "C" int p2n_act8_norm_relu_forward(const float *x, int B, int C, long L, 
     const FwdSpace f = fwd_space(a, (char *)workspace);
     hipStream_t s = (hipStream_t)stream_;
     const int ps = p2n_prof_begin(P2N_K_ACT8_FWD, s);
-    TRY(act8_keep(a, fn, x, gamma, beta, running_mean, running_var, momentum, eps, (char *)kept, f, s));
-    const long rows = (long)B * C;
-    hipLaunchKernelGGL(p2n_act8_apply_kernel, dim3((unsigned)(rows * ((L + 1023) / 1024))), dim3(256), 0, s, x, rows, C, a.Kpad, L, f.tab, out);
-    P2N_CHECK_HIP(hipGetLastError());
+    TRY(act8_keep(a, x, gamma, beta, running_mean, running_var, momentum, eps, (char *)kept, f, out, s));
     p2n_prof_end(ps, s);
     return P2N_OK;
 }
