@@ -135,6 +135,35 @@ __global__ void p2n_act8_norm_kernel(const double *__restrict__ part, int S, con
     tab[2 * Cpad + c] = beta[c];
 }
 
+// ---------------------------------------------------------------- weight image of a product
+// three-way split w = h + m + l: fragment (ks * CTP + ct) * 3 + part, 1 KiB: lane holds part(M[32ct + (lane&31)][16ks + 8(lane>>5) + i]),
+// i < 8; M = W (rows N) or W^T (rows K); zero outside.  CTP = channel tiles rounded up to what a workgroup makes.  It is made by
+// the first workgroups of a launch that the product follows anyway (a launch of its own: 4 us; by the last workgroups: 6).
+struct Act8Split {
+    const float *W;
+    __bf16 *img;
+    int rows, cols, trans, CTP, KS;
+};
+__device__ __forceinline__ void act8_split_weights(const Act8Split &A, long i) {      // i: (fragment without part, lane)
+    const int lane = (int)(i & 63);
+    const long f = i >> 6;
+    if (f >= (long)A.CTP * A.KS) return;
+    const int ct = (int)(f % A.CTP), ks = (int)(f / A.CTP);
+    const int row = 32 * ct + (lane & 31), k0 = 16 * ks + 8 * (lane >> 5);
+    bf16x8 h, m, l;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int k = k0 + j;
+        const float v = row < A.rows && k < A.cols ? (A.trans ? A.W[(long)k * A.rows + row] : A.W[(long)row * A.cols + k]) : 0.f;
+        h[j] = (__bf16)v;
+        const float r = v - (float)h[j];
+        m[j] = (__bf16)r;
+        l[j] = (__bf16)(r - (float)m[j]);
+    }
+    bf16x8 *d = reinterpret_cast<bf16x8 *>(A.img) + f * 3 * 64 + lane;
+    d[0] = h; d[64] = m; d[128] = l;
+}
+
 // ---------------------------------------------------------------- codes
 // What is kept of a block of 128 points, 32 channels a workgroup and 8 a wave, a lane two neighbouring points: u, the scales, codes, the ReLU's
 // bits.  The channels' maxima are formed by a halving exchange (8 registers shrink to one while lanes pair up), so lane i holds
@@ -147,14 +176,19 @@ struct Act8Keep {
     float *scale;
     unsigned *bits;
     float *out;                          // OUT
-    long L, NB;
+    long L, NB, split_wgs;               // the first workgroups make the image
     int C, C4;
+    Act8Split split;
 };
 template <bool NORM, bool OUT>
 __global__ __launch_bounds__(256) void p2n_act8_keep_kernel(Act8Keep A) {
     const int lane = threadIdx.x & 63;
     const int c0 = blockIdx.y * 32 + 8 * __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const long blk = blockIdx.x;
+    const long blk = blockIdx.x - A.split_wgs;
+    if (blk < 0) {
+        if (blockIdx.y == 0) act8_split_weights(A.split, (long)blockIdx.x * 256 + threadIdx.x);
+        return;
+    }
     if (c0 >= A.C4) return;
     const long b = blk / A.NB, l = (blk % A.NB) * ACT8_GROUP + 2 * lane;
     const bool ok0 = l < A.L, ok1 = l + 1 < A.L;
@@ -224,30 +258,6 @@ __global__ __launch_bounds__(256) void p2n_act8_keep_kernel(Act8Keep A) {
         if (!(R.s == R.s)) code[0] = 0;
         *reinterpret_cast<unsigned short *>(A.codes + (blk * A.C + c0 + i) * ACT8_GROUP + 2 * lane) = (unsigned short)code[0];
     }
-}
-
-// ---------------------------------------------------------------- weight image of a product
-// three-way split w = h + m + l: fragment (ks * CTP + ct) * 3 + part, 1 KiB: lane holds part(M[32ct + (lane&31)][16ks + 8(lane>>5) + i]),
-// i < 8; M = W (rows N) or W^T (rows K); zero outside.  CTP = channel tiles rounded up to what a workgroup makes.
-__global__ __launch_bounds__(256) void p2n_act8_split_kernel(const float *__restrict__ W, int rows, int cols, int trans, int CTP, int KS, __bf16 *__restrict__ img) {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;          // (fragment without part, lane)
-    const int lane = (int)(i & 63);
-    const long f = i >> 6;
-    if (f >= (long)CTP * KS) return;
-    const int ct = (int)(f % CTP), ks = (int)(f / CTP);
-    const int row = 32 * ct + (lane & 31), k0 = 16 * ks + 8 * (lane >> 5);
-    bf16x8 h, m, l;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int k = k0 + j;
-        const float v = row < rows && k < cols ? (trans ? W[(long)k * rows + row] : W[(long)row * cols + k]) : 0.f;
-        h[j] = (__bf16)v;
-        const float r = v - (float)h[j];
-        m[j] = (__bf16)r;
-        l[j] = (__bf16)(r - (float)m[j]);
-    }
-    bf16x8 *d = reinterpret_cast<bf16x8 *>(img) + f * 3 * 64 + lane;
-    d[0] = h; d[64] = m; d[128] = l;
 }
 
 // ---------------------------------------------------------------- products over points
@@ -830,11 +840,17 @@ __global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : 2) void p2n_act8_wgrad_kern
 }
 
 // out[i] = sum over slices, in a fixed order: 32 results a workgroup, the slices dealt to 32 rows of threads.  The first n0 results are
-// dW, the others db (either may be NULL).
-__global__ __launch_bounds__(1024) void p2n_act8_join_kernel(const float *__restrict__ part, long n, long n0, int slices, float *__restrict__ dW, float *__restrict__ db) {
+// dW, the others db (either may be NULL).  The first split_wgs workgroups make the image of W^T.
+__global__ __launch_bounds__(1024) void p2n_act8_join_kernel(const float *__restrict__ part, long n, long n0, int slices, float *__restrict__ dW, float *__restrict__ db,
+                                                             Act8Split split, int split_wgs) {
     __shared__ float sh[32][33];
+    const int blk = (int)blockIdx.x - split_wgs;
+    if (blk < 0) {
+        act8_split_weights(split, (long)blockIdx.x * 1024 + threadIdx.x);
+        return;
+    }
     const int o = threadIdx.x & 31, y = threadIdx.x >> 5;
-    const long i = (long)blockIdx.x * 32 + o;
+    const long i = (long)blk * 32 + o;
     float s = 0.f;
     if (i < n)
         for (int k = y; k < slices; k += 32) s += part[k * n + i];
@@ -990,13 +1006,6 @@ BwdSpace bwd_space(const Act8 &a, char *base) {
     return f;
 }
 
-int act8_split_weights(const float *W, int rows, int cols, int trans, int CTP, int KS, __bf16 *img, hipStream_t s) {
-    const long n = (long)CTP * KS * 64;
-    hipLaunchKernelGGL(p2n_act8_split_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, W, rows, cols, trans, CTP, KS, img);
-    P2N_CHECK_HIP(hipGetLastError());
-    return P2N_OK;
-}
-
 template <int IN, int EPI, int TABK>
 int act8_launch_gemm_tab(const Act8Gemm &g, long groups, hipStream_t s) {
     const int ct = act8_tiles(g.rows, groups);
@@ -1042,9 +1051,9 @@ int act8_space_check(const char *fn, const void *p, size_t have, size_t need, co
     return P2N_OK;
 }
 
-// statistics and tables of x (norm), and what is kept of it; relu(y) to `out` where given
+// statistics and tables of x (norm), and what is kept of it; relu(y) to `out`, or the image of `split`
 int act8_keep(const Act8 &a, const float *x, const float *gamma, const float *beta, float *rmean, float *rvar, float momentum, float eps,
-                    char *kept, const FwdSpace &f, float *out, hipStream_t s) {
+              char *kept, const FwdSpace &f, float *out, const Act8Split &split, hipStream_t s) {
     const Act8Kept k = act8_kept(a.B, a.K, a.L, gamma != nullptr);
     float *stat = (float *)(kept + k.stat);
     if (gamma) {
@@ -1059,8 +1068,9 @@ int act8_keep(const Act8 &a, const float *x, const float *gamma, const float *be
                            (double)momentum, (double)eps, frozen ? 1 : 0, stat, f.tab);
         P2N_CHECK_HIP(hipGetLastError());
     }
-    const Act8Keep keep{x, stat, gamma, beta, (signed char *)kept, (float *)(kept + k.scale), (unsigned *)(kept + k.bits), out, a.L, a.NB, a.K, (a.K + 3) / 4 * 4};
-    const dim3 grid((unsigned)((long)a.B * a.NB), (unsigned)((a.K + 31) / 32));
+    const Act8Keep keep{x, stat, gamma, beta, (signed char *)kept, (float *)(kept + k.scale), (unsigned *)(kept + k.bits), out, a.L, a.NB,
+                        ((long)split.CTP * split.KS + 3) / 4, a.K, (a.K + 3) / 4 * 4, split};
+    const dim3 grid((unsigned)(keep.split_wgs + (long)a.B * a.NB), (unsigned)((a.K + 31) / 32));
     if (out) hipLaunchKernelGGL((p2n_act8_keep_kernel<true, true>), grid, dim3(256), 0, s, keep);
     else if (gamma) hipLaunchKernelGGL((p2n_act8_keep_kernel<true, false>), grid, dim3(256), 0, s, keep);
     else hipLaunchKernelGGL((p2n_act8_keep_kernel<false, false>), grid, dim3(256), 0, s, keep);
@@ -1106,8 +1116,7 @@ extern "C" int p2n_act8_forward(const float *x, int B, int K, long L, const floa
     hipStream_t s = (hipStream_t)stream_;
     const int ps = p2n_prof_begin(P2N_K_ACT8_FWD, s);
     Act8Gemm g = {};
-    TRY(act8_keep(a, x, gamma, beta, running_mean, running_var, momentum, eps, (char *)kept, f, nullptr, s));
-    TRY(act8_split_weights(W, N, K, 0, a.CTf, a.KSf, f.img, s));
+    TRY(act8_keep(a, x, gamma, beta, running_mean, running_var, momentum, eps, (char *)kept, f, nullptr, Act8Split{W, f.img, N, K, 0, a.CTf, a.KSf}, s));
     g.x = x; g.img = f.img; g.tab = f.tab; g.bias = bias; g.out = h; g.L = L; g.NB = a.NB;
     g.K = K; g.Kpad = a.Kpad; g.KS = a.KSf; g.CTP = a.CTf; g.rows = N;
     const long groups = (long)B * a.NB;
@@ -1143,12 +1152,15 @@ extern "C" int p2n_act8_backward(const float *g, int B, int K, long L, const flo
         w.g = g; w.codes = codes; w.scale = scale; w.bits = bits; w.gamma = gamma; w.beta = beta; w.part = f.wpart;
         w.L = L; w.NB = a.NB; w.steps = (int)a.wsteps; w.N = N; w.K = K; w.K4 = K4; w.ntc = a.ntc; w.slices = a.slices;
         TRY(gamma ? act8_launch_wgrad<true>(a, w, s) : act8_launch_wgrad<false>(a, w, s));
-        const long n = (long)N * K + N;
-        hipLaunchKernelGGL(p2n_act8_join_kernel, dim3((unsigned)((n + 31) / 32)), dim3(1024), 0, s, f.wpart, n, (long)N * K, a.slices, dW, db);
+    }
+    if (dW || db || dx) {
+        const Act8Split split = dx ? Act8Split{W, f.img, K, N, 1, a.CTb, a.KSb} : Act8Split{};
+        const long n = dW || db ? (long)N * K + N : 0;
+        const int split_wgs = (split.CTP * split.KS + 15) / 16;
+        hipLaunchKernelGGL(p2n_act8_join_kernel, dim3((unsigned)(split_wgs + (n + 31) / 32)), dim3(1024), 0, s, f.wpart, n, (long)N * K, a.slices, dW, db, split, split_wgs);
         P2N_CHECK_HIP(hipGetLastError());
     }
     if (dx) {
-        TRY(act8_split_weights(W, K, N, 1, a.CTb, a.KSb, f.img, s));
         Act8Gemm q = {};
         q.x = g; q.img = f.img; q.out = dx; q.codes = codes; q.scale = scale; q.bits = bits; q.part = f.part; q.L = L; q.NB = a.NB;
         q.K = N; q.Kpad = (N + 63) / 64 * 64; q.KS = a.KSb; q.CTP = a.CTb; q.rows = K; q.rows4 = K4;
@@ -1179,7 +1191,7 @@ extern "C" int p2n_act8_norm_relu_forward(const float *x, int B, int C, long L, 
     const FwdSpace f = fwd_space(a, (char *)workspace);
     hipStream_t s = (hipStream_t)stream_;
     const int ps = p2n_prof_begin(P2N_K_ACT8_FWD, s);
-    TRY(act8_keep(a, x, gamma, beta, running_mean, running_var, momentum, eps, (char *)kept, f, out, s));
+    TRY(act8_keep(a, x, gamma, beta, running_mean, running_var, momentum, eps, (char *)kept, f, out, Act8Split{}, s));
     p2n_prof_end(ps, s);
     return P2N_OK;
 }
