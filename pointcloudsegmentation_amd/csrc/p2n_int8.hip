@@ -6,6 +6,7 @@
 // specification.  Two operators share the weight image and the rule (p2n_q8.h):
 //   p2n_int8_linear  rows of K values (tokens), float32 or bfloat16
 //   p2n_int8_mlp     the layers of a shared MLP over the columns of (B, C, L), register-resident
+#include <type_traits>
 #include "p2n_q8.h"
 
 #define MFMA_I8(a, b, c) __builtin_amdgcn_mfma_i32_32x32x32_i8((a), (b), (c), 0, 0, 0)
@@ -629,44 +630,48 @@ __device__ __forceinline__ void int8_mlp_load(const float *xb, long L, int C, in
     }
 }
 
-// A tile's values y (a ReLU behind them or not) to memory: channel tile ct of cloud b, columns of the wave's 32 points, or the maxima of its groups
-__device__ __forceinline__ void int8_mlp_out(const Int8MlpArgs &A, int N, bool relu, long b, long l, bool valid, unsigned off, int ct, int lane,
-                                             const float (&y)[16]) {
-    const int h = lane >> 5;
-    const long W = A.group ? A.L / A.group : A.L;   // columns of a result row
+// A tile's values y to memory: channel tile ct of cloud b, columns of the wave's 32 points
+__device__ __forceinline__ void int8_mlp_out(const Int8MlpArgs &A, int N, long b, bool valid, unsigned off, int ct, const float (&y)[16]) {
     // the resource starts at row 32ct and ends with the cloud's last row: channels past N are not written
-    const long left = (long)(N - 32 * ct) * W * 4;
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(A.out + (b * N + 32L * ct) * W, 0,
+    const long left = (long)(N - 32 * ct) * A.L * 4;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(A.out + (b * N + 32L * ct) * A.L, 0,
                                                                          (int)(left < 0xFFFFFFFFL ? left : 0xFFFFFFFFL), 0x00020000);
-    if (!A.group) {
-        if (valid && 32 * ct + 32 <= N) {
+    if (valid && 32 * ct + 32 <= N) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(y[e]), rs, off, (int)((8 * (e >> 2) + (e & 3)) * W * 4), 0);
-        } else if (valid) {
+        for (int e = 0; e < 16; ++e)
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(y[e]), rs, off, (int)((8 * (e >> 2) + (e & 3)) * A.L * 4), 0);
+    } else if (valid) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(y[e]), rs, off + (unsigned)((8 * (e >> 2) + (e & 3)) * W * 4), 0, 0);
-        }
-        return;
+        for (int e = 0; e < 16; ++e)
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(y[e]), rs, off + (unsigned)((8 * (e >> 2) + (e & 3)) * A.L * 4), 0, 0);
     }
-    // maximum over 32 (or 16) neighbouring points of every channel: the registers shrink 16 -> 1 while the lanes of a
-    // 16-lane row pair up; lane i of a row ends with register i's channel
-    int m[16];
+}
+
+__device__ __forceinline__ float int8_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }   // a NaN stays
+
+// The last layer before a maximum over groups, its operands the other way round: lane = channel, acc[e] = point 8(e>>2) + 4h + (e&3), so that
+// the maximum is formed in registers; ps: the scales of the 32 points.  Rounding keeps the order, so bias and ReLU follow the maximum, once.
+// l0: the tile's first column.
+__device__ __forceinline__ void int8_mlp_groups(const Int8MlpArgs &A, const MlpLayer &Y, int ct, const i32x16 &acc, const float *ps, long b, long l0, int lane) {
+    const int p = lane & 31, h = lane >> 5;
+    const float sc = Y.scale[32 * ct + p], bi = Y.bias[32 * ct + p];
+    float m[4];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) m[e] = relu ? __float_as_int(y[e]) : int8_key(y[e]);
-    p2n_halve_max<8, 0xB1>(m, lane & 1);
-    p2n_halve_max<4, 0x4E>(m, lane & 2);
-    p2n_halve_max<2, 0x124>(m, lane & 4);
-    p2n_halve_max<1, 0x128>(m, lane & 8);
-    if (A.group == 32) {
-        const int t = __builtin_amdgcn_ds_swizzle(m[0], 0x401F);   // lane ^ 16
-        m[0] = t > m[0] ? t : m[0];
+    for (int g = 0; g < 4; ++g) {
+        const f32x4 s = *reinterpret_cast<const f32x4 *>(ps + 8 * g + 4 * h);
+        float t[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = (float)acc[4 * g + j] * sc * s[j];
+        m[g] = int8_max(int8_max(int8_max(t[0], t[1]), t[2]), t[3]);
     }
-    const int i = lane & 15, c = 8 * (i >> 2) + 4 * h + (i & 3);
-    const int q = A.group == 32 ? (int)(l >> 5) : (int)(l >> 4);
-    if (valid && (A.group == 16 || !(lane & 16)))
-        __builtin_amdgcn_raw_buffer_store_b32(relu ? m[0] : int8_unkey(m[0]), rs, (int)((c * W + q) * 4), 0, 0);
+    // the halves of the wave hold every other four points: one exchange joins them, 16 points' maximum (32: both the same) to either half
+    float u = int8_max(m[0], m[1]), w = int8_max(m[2], m[3]);
+    if (A.group == 32) u = w = int8_max(u, w);
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_int(u), __float_as_int(w), false, false);
+    float y = int8_max(__int_as_float(x[0]), __int_as_float(x[1])) + bi;
+    if (A.last_relu) y = y <= 0.f ? 0.f : y;
+    const bool two = A.group == 16;
+    if (32 * ct + p < Y.N && (two ? l0 + 16 * h < A.L : h == 0)) A.out[(b * Y.N + 32 * ct + p) * (A.L / A.group) + (two ? l0 / 16 + h : l0 / 32)] = y;
 }
 
 // A tile's sums to its values: scales, bias, ReLU; into `am` the largest of them as bits.  The ReLU is a maximum of bit patterns: every NaN here has
@@ -708,72 +713,95 @@ __device__ __forceinline__ void int8_mlp_codes(const float (&e)[16], int real, c
     }
 }
 
+// the larger of the two halves of a wave
+__device__ __forceinline__ unsigned int8_halves(unsigned am) {
+    const auto x = __builtin_amdgcn_permlane32_swap(am, am, false, false);
+    return x[0] > x[1] ? x[0] : x[1];
+}
+
 // Up to 64 channels everywhere: one wave carries its 32 points through every layer in registers.
 __global__ __launch_bounds__(256, 4) void p2n_int8_mlp_narrow_kernel(Int8MlpArgs A) {
+    __shared__ __attribute__((aligned(16))) float scales[4][32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int p = lane & 31, h = lane >> 5;
     const i32x16 zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
     const long tile = (long)blockIdx.x * 4 + wave;
     if (tile >= A.total) return;
-    const long b = tile / A.tiles, l = (tile % A.tiles) * 32 + p;
-    const bool valid = l < A.L;
-    const float *xb = A.x + b * A.C * A.L;
-    const unsigned off = (unsigned)((4 * h * A.L + (valid ? l : A.L - 1)) * 4);   // bytes; L <= 2^24 keeps 32 rows below 2^31
     const int KT0 = A.layer[0].KT;
-    unsigned am = 0, o;
-    float v[2][16];
-    int cq[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    const long b = tile / A.tiles, l0 = tile % A.tiles * 32;
+    const bool valid = l0 + p < A.L;
+    const unsigned off = (unsigned)((4 * h * A.L + (valid ? l0 + p : A.L - 1)) * 4);   // bytes; L <= 2^24 keeps 32 rows below 2^31
+    unsigned am = 0;
+    float s, v[2][16];
+    int cq[2][4];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
-        if (kt < KT0) int8_mlp_load(xb, A.L, A.C, kt, off, v[kt]);
+        if (kt < KT0) int8_mlp_load(A.x + b * A.C * A.L, A.L, A.C, kt, off, v[kt]);
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
         if (kt < KT0) int8_mlp_top(v[kt], am);
-    o = (unsigned)__shfl_xor((int)am, 32);
-    float s = p2n_q8_scale(o > am ? o : am);
+    s = p2n_q8_scale(int8_halves(am));
     {
         const P2nQ8 Q = p2n_q8_make(s);
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) cq[kt][g] = 0;
             if (kt < KT0) int8_mlp_codes(v[kt], A.C - 32 * kt, Q, cq[kt]);
+        }
     }
 #pragma unroll 1
     for (int li = 0; li < A.nl; ++li) {
         const MlpLayer Y = A.layer[li];
         const bool last = li == A.nl - 1, relu = !last || A.last_relu;
         const i32x4 *wf = reinterpret_cast<const i32x4 *>(Y.img) + lane;
+        // the image has an even number of k-tiles: where the second holds no channels its codes are zero
+        if (last && A.group) {
+            scales[wave][p] = s;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");            // the wave's own row
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+            for (int ct = 0; ct < Y.CT; ++ct) {
+                const i32x4 w0 = wf[ct * Y.KTI * 64], w1 = wf[(ct * Y.KTI + 1) * 64];
+                i32x16 acc = MFMA_I8((i32x4{cq[0][0], cq[0][1], cq[0][2], cq[0][3]}), w0, zero);
+                acc = MFMA_I8((i32x4{cq[1][0], cq[1][1], cq[1][2], cq[1][3]}), w1, acc);
+                int8_mlp_groups(A, Y, ct, acc, scales[wave], b, l0, lane);
+            }
+            break;
+        }
+        float y[2][16];
         am = 0;
 #pragma unroll
         for (int ct = 0; ct < 2; ++ct)
             if (ct < Y.CT) {
-                i32x16 acc = MFMA_I8(wf[ct * Y.KTI * 64], (i32x4{cq[0][0], cq[0][1], cq[0][2], cq[0][3]}), zero);
-                // the image has an even number of k-tiles: where the second holds no channels its codes are zero
-                acc = MFMA_I8(wf[(ct * Y.KTI + 1) * 64], (i32x4{cq[1][0], cq[1][1], cq[1][2], cq[1][3]}), acc);
-                int8_mlp_values(acc, Y, ct, h, s, relu, v[ct], am);
+                const i32x4 w0 = wf[ct * Y.KTI * 64], w1 = wf[(ct * Y.KTI + 1) * 64];
+                i32x16 acc = MFMA_I8(w0, (i32x4{cq[0][0], cq[0][1], cq[0][2], cq[0][3]}), zero);
+                acc = MFMA_I8(w1, (i32x4{cq[1][0], cq[1][1], cq[1][2], cq[1][3]}), acc);
+                int8_mlp_values(acc, Y, ct, h, s, relu, y[ct], am);
             }
         if (last) {
 #pragma unroll
             for (int ct = 0; ct < 2; ++ct)
-                if (ct < Y.CT) int8_mlp_out(A, Y.N, relu, b, l, valid, off, ct, lane, v[ct]);
+                if (ct < Y.CT) int8_mlp_out(A, Y.N, b, valid, off, ct, y[ct]);
             break;
         }
-        o = (unsigned)__shfl_xor((int)am, 32);
-        s = p2n_q8_scale(o > am ? o : am);
+        s = p2n_q8_scale(int8_halves(am));
         const P2nQ8 Q = p2n_q8_make(s);
 #pragma unroll
         for (int ct = 0; ct < 2; ++ct)
-            if (ct < Y.CT) p2n_q8_pack(v[ct], Q, cq[ct]);
+            if (ct < Y.CT) p2n_q8_pack(y[ct], Q, cq[ct]);
     }
 }
 
 // Wider layers: NW waves carry 32 points together, a wave its share of the channel tiles.  Codes go round through LDS in operand order; a point's
 // maximum is joined over the waves there too.  Two barriers a layer; a layer's first weights are on their way before the last one ends.
-template <int NW>
+template <int NW, bool GROUPS>
 __global__ __launch_bounds__(64 * NW, 4) void p2n_int8_mlp_wide_kernel(Int8MlpArgs A) {
     constexpr int KTI = 4 * NW;      // k-tiles of the input: 1024 (512) channels in, a channel tile a wave: 256 (128) out
     constexpr int AHEAD = 4;                                // weight fragments on their way
     __shared__ __attribute__((aligned(16))) char codes[KTI * 1024];
     __shared__ unsigned top[NW][32];
+    __shared__ __attribute__((aligned(16))) float scales[32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int p = lane & 31, h = lane >> 5;
     const long tile = blockIdx.x, b = tile / A.tiles, l = (tile % A.tiles) * 32 + p;
@@ -798,8 +826,8 @@ __global__ __launch_bounds__(64 * NW, 4) void p2n_int8_mlp_wide_kernel(Int8MlpAr
         if (wave + NW * i < KT0) int8_mlp_top(v[i], am);
     // the largest of every point over the waves -> its scale
     auto join = [&]() __attribute__((always_inline)) {
-        const unsigned o = (unsigned)__shfl_xor((int)am, 32);
-        if (h == 0) top[wave][p] = o > am ? o : am;
+        const unsigned o = int8_halves(am);
+        if (h == 0) top[wave][p] = o;
         __syncthreads();
         unsigned m = 0;
 #pragma unroll
@@ -807,6 +835,7 @@ __global__ __launch_bounds__(64 * NW, 4) void p2n_int8_mlp_wide_kernel(Int8MlpAr
         return p2n_q8_scale(m);
     };
     float s = join();
+    if (GROUPS && threadIdx.x < 32) scales[p] = s;
     {
         const P2nQ8 Q = p2n_q8_make(s);
 #pragma unroll
@@ -823,27 +852,39 @@ __global__ __launch_bounds__(64 * NW, 4) void p2n_int8_mlp_wide_kernel(Int8MlpAr
         const MlpLayer Y = A.layer[li];
         const bool last = li == A.nl - 1, relu = !last || A.last_relu;
         am = 0;
-        const bool mine = wave < Y.CT;
+        const bool mine = wave < Y.CT, groups = GROUPS && last;
         if (mine) {
             const i32x4 *wf = reinterpret_cast<const i32x4 *>(Y.img) + (long)wave * Y.KTI * 64 + lane;
             i32x16 acc;
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[e] = 0;
-            for (int k0 = 0; k0 < Y.KT; k0 += AHEAD) {
+            auto product = [&](auto channels_in_registers) __attribute__((always_inline)) {
+                for (int k0 = 0; k0 < Y.KT; k0 += AHEAD) {
 #pragma unroll
-                for (int q = 0; q < AHEAD; ++q) {
-                    if (k0 + q < Y.KT) acc = MFMA_I8(w[q], *reinterpret_cast<const i32x4 *>(codes + ((k0 + q) * 64 + lane) * 16), acc);
-                    if (k0 + q + AHEAD < Y.KT) w[q] = wf[(k0 + q + AHEAD) * 64];
+                    for (int q = 0; q < AHEAD; ++q) {
+                        if (k0 + q < Y.KT) {
+                            const i32x4 x = *reinterpret_cast<const i32x4 *>(codes + ((k0 + q) * 64 + lane) * 16);
+                            acc = channels_in_registers ? MFMA_I8(w[q], x, acc) : MFMA_I8(x, w[q], acc);
+                        }
+                        if (k0 + q + AHEAD < Y.KT) w[q] = wf[(k0 + q + AHEAD) * 64];
+                    }
                 }
+            };
+            if (groups) {
+                product(std::false_type{});
+                int8_mlp_groups(A, Y, wave, acc, scales, b, l - p, lane);
+            } else {
+                product(std::true_type{});
+                int8_mlp_values(acc, Y, wave, h, s, relu, v[0], am);
             }
-            int8_mlp_values(acc, Y, wave, h, s, relu, v[0], am);
         }
         if (last) {
-            if (mine) int8_mlp_out(A, Y.N, relu, b, l, valid, off, wave, lane, v[0]);
+            if (mine && !groups) int8_mlp_out(A, Y.N, b, valid, off, wave, v[0]);
             break;
         }
         ahead(A.layer[li + 1], wave);
         s = join();                            // behind its barrier every wave has read this layer's codes
+        if (GROUPS && threadIdx.x < 32) scales[p] = s;   // read behind the next barrier, by the last layer alone
         if (mine) {
             const P2nQ8 Q = p2n_q8_make(s);
             int c[4];
@@ -886,8 +927,10 @@ extern "C" int p2n_int8_mlp(const float *x, int B, long L, int nl, const int *di
     const int ps = p2n_prof_begin(P2N_K_INT8_MLP, s);
     // one wave to 32 points up to 64 channels (fewer registers than four waves would share out), four up to 128, eight up to 256
     if (ctm <= 2 && ktm <= 2) hipLaunchKernelGGL(p2n_int8_mlp_narrow_kernel, dim3((unsigned)((a.total + 3) / 4)), dim3(256), 0, s, a);
-    else if (ctm <= 4 && ktm <= 16) hipLaunchKernelGGL(p2n_int8_mlp_wide_kernel<4>, dim3((unsigned)a.total), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(p2n_int8_mlp_wide_kernel<8>, dim3((unsigned)a.total), dim3(512), 0, s, a);
+    else if (ctm <= 4 && ktm <= 16 && group) hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<4, true>), dim3((unsigned)a.total), dim3(256), 0, s, a);
+    else if (ctm <= 4 && ktm <= 16) hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<4, false>), dim3((unsigned)a.total), dim3(256), 0, s, a);
+    else if (group) hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<8, true>), dim3((unsigned)a.total), dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<8, false>), dim3((unsigned)a.total), dim3(512), 0, s, a);
     p2n_prof_end(ps, s);
     P2N_CHECK_HIP(hipGetLastError());
     return P2N_OK;
