@@ -676,11 +676,14 @@ __device__ __forceinline__ void int8_mlp_groups(const Int8MlpArgs &A, const MlpL
 
 // A tile's sums to its values: scales, bias, ReLU; into `am` the largest of them as bits.  The ReLU is a maximum of bit patterns: every NaN here has
 // its sign bit clear (scales and biases are made so, and so is what the arithmetic makes) and stays.  Past it the bits order as they are.
-__device__ __forceinline__ void int8_mlp_values(const i32x16 &acc, const MlpLayer &Y, int ct, int h, float s, bool relu, float (&y)[16], unsigned &am) {
+// par: the tile's scales and biases in LDS, put there by one load of the wave (read from memory by every lane they would take eight).
+__device__ __forceinline__ float int8_mlp_par(const MlpLayer &Y, int ct, int lane) {     // scales in the lower half of the wave, biases in the upper
+    return Y.scale[32 * (ct + (lane >> 5) * Y.CT) + (lane & 31)];
+}
+__device__ __forceinline__ void int8_mlp_values(const i32x16 &acc, const float *par, int h, float s, bool relu, float (&y)[16], unsigned &am) {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-        const f32x4 sc = *reinterpret_cast<const f32x4 *>(Y.scale + 32 * ct + 8 * g + 4 * h);
-        const f32x4 bi = *reinterpret_cast<const f32x4 *>(Y.bias + 32 * ct + 8 * g + 4 * h);
+        const f32x4 sc = *reinterpret_cast<const f32x4 *>(par + 8 * g + 4 * h), bi = *reinterpret_cast<const f32x4 *>(par + 32 + 8 * g + 4 * h);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float v = (float)acc[4 * g + j] * sc[j] * s + bi[j];
@@ -721,14 +724,14 @@ __device__ __forceinline__ unsigned int8_halves(unsigned am) {
 
 // Up to 64 channels everywhere: one wave carries its 32 points through every layer in registers.
 __global__ __launch_bounds__(256, 4) void p2n_int8_mlp_narrow_kernel(Int8MlpArgs A) {
-    __shared__ __attribute__((aligned(16))) float scales[4][32];
+    __shared__ __attribute__((aligned(16))) float own[4][2][64];           // the wave's: parameters of its tiles, in the end scales of its points
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int p = lane & 31, h = lane >> 5;
     const i32x16 zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-    const long tile = (long)blockIdx.x * 4 + wave;
+    const unsigned tile = blockIdx.x * 4 + wave, tiles = (unsigned)A.tiles;          // both below 2^31
     if (tile >= A.total) return;
     const int KT0 = A.layer[0].KT;
-    const long b = tile / A.tiles, l0 = tile % A.tiles * 32;
+    const long b = tile / tiles, l0 = tile % tiles * 32;
     const bool valid = l0 + p < A.L;
     const unsigned off = (unsigned)((4 * h * A.L + (valid ? l0 + p : A.L - 1)) * 4);   // bytes; L <= 2^24 keeps 32 rows below 2^31
     unsigned am = 0;
@@ -757,15 +760,15 @@ __global__ __launch_bounds__(256, 4) void p2n_int8_mlp_narrow_kernel(Int8MlpArgs
         const i32x4 *wf = reinterpret_cast<const i32x4 *>(Y.img) + lane;
         // the image has an even number of k-tiles: where the second holds no channels its codes are zero
         if (last && A.group) {
-            scales[wave][p] = s;
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");            // the wave's own row
+            own[wave][0][p] = s;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
             for (int ct = 0; ct < Y.CT; ++ct) {
                 const i32x4 w0 = wf[ct * Y.KTI * 64], w1 = wf[(ct * Y.KTI + 1) * 64];
                 i32x16 acc = MFMA_I8((i32x4{cq[0][0], cq[0][1], cq[0][2], cq[0][3]}), w0, zero);
                 acc = MFMA_I8((i32x4{cq[1][0], cq[1][1], cq[1][2], cq[1][3]}), w1, acc);
-                int8_mlp_groups(A, Y, ct, acc, scales[wave], b, l0, lane);
+                int8_mlp_groups(A, Y, ct, acc, own[wave][0], b, l0, lane);
             }
             break;
         }
@@ -773,11 +776,16 @@ __global__ __launch_bounds__(256, 4) void p2n_int8_mlp_narrow_kernel(Int8MlpArgs
         am = 0;
 #pragma unroll
         for (int ct = 0; ct < 2; ++ct)
+            if (ct < Y.CT) own[wave][ct][lane] = int8_mlp_par(Y, ct, lane);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct)
             if (ct < Y.CT) {
                 const i32x4 w0 = wf[ct * Y.KTI * 64], w1 = wf[(ct * Y.KTI + 1) * 64];
                 i32x16 acc = MFMA_I8(w0, (i32x4{cq[0][0], cq[0][1], cq[0][2], cq[0][3]}), zero);
                 acc = MFMA_I8(w1, (i32x4{cq[1][0], cq[1][1], cq[1][2], cq[1][3]}), acc);
-                int8_mlp_values(acc, Y, ct, h, s, relu, y[ct], am);
+                int8_mlp_values(acc, own[wave][ct], h, s, relu, y[ct], am);
             }
         if (last) {
 #pragma unroll
@@ -801,10 +809,12 @@ __global__ __launch_bounds__(64 * NW, 4) void p2n_int8_mlp_wide_kernel(Int8MlpAr
     constexpr int AHEAD = 4;                                // weight fragments on their way
     __shared__ __attribute__((aligned(16))) char codes[KTI * 1024];
     __shared__ unsigned top[NW][32];
+    __shared__ __attribute__((aligned(16))) float par[NW][64];            // the wave's own row
     __shared__ __attribute__((aligned(16))) float scales[32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int p = lane & 31, h = lane >> 5;
-    const long tile = blockIdx.x, b = tile / A.tiles, l = (tile % A.tiles) * 32 + p;
+    const unsigned tiles = (unsigned)A.tiles;                    // below 2^31, as the grid
+    const long b = blockIdx.x / tiles, l = blockIdx.x % tiles * 32 + p;
     const bool valid = l < A.L;
     const float *xb = A.x + b * A.C * A.L;
     const unsigned off = (unsigned)((4 * h * A.L + (valid ? l : A.L - 1)) * 4);
@@ -815,10 +825,12 @@ __global__ __launch_bounds__(64 * NW, 4) void p2n_int8_mlp_wide_kernel(Int8MlpAr
     for (int i = 0; i < 4; ++i)
         if (wave + NW * i < KT0) int8_mlp_load(xb, A.L, A.C, wave + NW * i, off, v[i]);
     i32x4 w[AHEAD];
+    float pw;
     auto ahead = [&](const MlpLayer &Y, int ct) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
             w[i] = reinterpret_cast<const i32x4 *>(Y.img)[((ct < Y.CT ? ct : 0) * Y.KTI + (i < Y.KTI ? i : 0)) * 64 + lane];
+        pw = int8_mlp_par(Y, ct < Y.CT ? ct : 0, lane);
     };
     ahead(A.layer[0], wave);
 #pragma unroll
@@ -874,8 +886,11 @@ __global__ __launch_bounds__(64 * NW, 4) void p2n_int8_mlp_wide_kernel(Int8MlpAr
                 product(std::false_type{});
                 int8_mlp_groups(A, Y, wave, acc, scales, b, l - p, lane);
             } else {
+                par[wave][lane] = pw;
                 product(std::true_type{});
-                int8_mlp_values(acc, Y, wave, h, s, relu, v[0], am);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                int8_mlp_values(acc, par[wave], h, s, relu, v[0], am);
             }
         }
         if (last) {
