@@ -265,8 +265,10 @@ __device__ __forceinline__ float int8_value(int acc, float sx, float sw, float b
 
 // ---------------------------------------------------------------- product of fragments
 // D = X . W^T, registers = tokens, lane = channel.  WR x WC waves of 32 TM tokens x 32 TN channels each.  Both operands
-// pass through LDS by DMA, 64 values of k at a time, in a ring of four; a read of the next fragments is always on its
-// way while the matrix cores work on the present ones.
+// pass through LDS by DMA, 64 values of k at a time, in a ring of RING; a read of the next fragments is always on its
+// way while the matrix cores work on the present ones.  The largest tile is 128 x 256 by four waves, two workgroups on a compute unit: the
+// LDS then carries 288 cycles of traffic to 256 of products, and one workgroup's output goes on beside the other's products
+// (16384 x 2048 x 4096: 161 us, 1.7 POP/s; 256 x 256 by eight waves alone on a compute unit 166, by four waves 220).
 typedef __attribute__((address_space(3))) void int8_lds_t;
 
 // a tile's results to memory: lane = channel n, v[j] = token t + j
@@ -297,7 +299,7 @@ __device__ __forceinline__ void int8_store4(__bf16 *y, long t, long T, int N, in
     }
 }
 
-template <typename TY, int TM, int TN, int WR, int WC>
+template <typename TY, int TM, int TN, int WR, int WC, int RING>
 __global__ __launch_bounds__(64 * WR * WC, TM * TN >= 4 ? 2 : 4) void p2n_int8_gemm_kernel(const char *__restrict__ xi, const float *__restrict__ sx,
                                                                                           const char *__restrict__ wi, const float *__restrict__ sw,
                                                                                           const float *__restrict__ bias, long T, int N, long TT, int CT, int KT,
@@ -306,11 +308,11 @@ __global__ __launch_bounds__(64 * WR * WC, TM * TN >= 4 ? 2 : 4) void p2n_int8_g
     static_assert(TPW * WR * WC == TILES, "every wave fetches the same number of tiles");
     constexpr int STAGE = TILES * 2048;               // two k-tiles each
     constexpr int GROUP = 2 * TPW;                    // DMA instructions of a wave and stage
-    __shared__ __attribute__((aligned(16))) char ring[4 * STAGE];
+    __shared__ __attribute__((aligned(16))) char ring[RING * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int r = lane & 31, h = lane >> 5;
-    // neighbouring workgroups go to the eight dies in turn: each die takes a band of the tiles, in squares of 4 rows, so
-    // that what its L2 holds is used by several workgroups
+    // neighbouring workgroups go to the eight dies in turn: each die takes a part of the tiles, in bands of 4 rows, so that what its
+    // L2 holds is used by several workgroups (16384 x 2048 x 4096: bands of 1: 170 us, of 4: 161, of 8: 209)
     const long per = (tiles + 7) / 8, id = (long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if (id >= tiles) return;
     const long gy = tiles / gx, band = id / (4L * gx), rows = gy - 4 * band < 4 ? gy - 4 * band : 4, in = id - band * 4 * gx;
@@ -324,20 +326,20 @@ __global__ __launch_bounds__(64 * WR * WC, TM * TN >= 4 ? 2 : 4) void p2n_int8_g
         const long at = tile < WR * TM ? (t0 + tile < TT ? t0 + tile : TT - 1) : (c0 + ch < CT ? c0 + ch : CT - 1);
         src[i] = (tile < WR * TM ? xi : wi) + at * KT * 1024;
     }
-    auto stage = [&](int s) __attribute__((always_inline)) {
+    auto stage = [&](int s, int slot) __attribute__((always_inline)) {
         const int k = s < ns ? s : ns - 1;            // past the end the last stage again: the count of outstanding loads stays the same
 #pragma unroll
         for (int i = 0; i < TPW; ++i) {
             const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(src[i]), 0, KT * 1024, 0x00020000);
-            char *dst = ring + (s & 3) * STAGE + (wave * TPW + i) * 2048;
+            char *dst = ring + slot * STAGE + (wave * TPW + i) * 2048;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (int8_lds_t *)dst, 16, lane * 16, k * 2048, 0, 0);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (int8_lds_t *)(dst + 1024), 16, lane * 16, k * 2048 + 1024, 0, 0);
         }
     };
     const int wr = wave / WC, wc = wave % WC;
     i32x4 fa[2][TM], fb[2][TN];
-    auto read = [&](int s, int kt, i32x4 (&a)[TM], i32x4 (&b)[TN]) __attribute__((always_inline)) {
-        const char *base = ring + (s & 3) * STAGE + kt * 1024 + lane * 16;
+    auto read = [&](int slot, int kt, i32x4 (&a)[TM], i32x4 (&b)[TN]) __attribute__((always_inline)) {
+        const char *base = ring + slot * STAGE + kt * 1024 + lane * 16;
 #pragma unroll
         for (int i = 0; i < TM; ++i) a[i] = *reinterpret_cast<const i32x4 *>(base + (wr * TM + i) * 2048);
 #pragma unroll
@@ -351,31 +353,32 @@ __global__ __launch_bounds__(64 * WR * WC, TM * TN >= 4 ? 2 : 4) void p2n_int8_g
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][c][e] = 0;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        stage(s);
+    for (int s = 0; s < RING; ++s) {
+        stage(s, s);
         __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_s_waitcnt(((3 * GROUP) & 15) | (7 << 4) | (((3 * GROUP) >> 4) << 14));       // stage 0 has arrived
+    __builtin_amdgcn_s_waitcnt((((RING - 1) * GROUP) & 15) | (7 << 4) | ((((RING - 1) * GROUP) >> 4) << 14));       // stage 0 has arrived
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     read(0, 0, fa[0], fb[0]);
 #pragma unroll 1
-    for (int s = 0; s < ns; ++s) {
+    for (int s = 0, slot = 0; s < ns; ++s) {
         __builtin_amdgcn_sched_barrier(0);
-        read(s, 1, fa[1], fb[1]);
+        read(slot, 1, fa[1], fb[1]);
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int c = 0; c < TN; ++c) acc[i][c] = MFMA_I8(fa[0][i], fb[0][c], acc[i][c]);
         __builtin_amdgcn_sched_barrier(0);
-        // stage s+1 has arrived everywhere, and every wave has read the last of stage s, whose place stage s+4 takes
-        __builtin_amdgcn_s_waitcnt(((2 * GROUP) & 15) | (7 << 4) | (0 << 8) | (((2 * GROUP) >> 4) << 14));
+        // stage s+1 has arrived everywhere, and every wave has read the last of stage s, whose place stage s + RING takes
+        __builtin_amdgcn_s_waitcnt((((RING - 2) * GROUP) & 15) | (7 << 4) | (0 << 8) | ((((RING - 2) * GROUP) >> 4) << 14));
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        stage(s + 4);
-        read(s + 1, 0, fa[0], fb[0]);
+        stage(s + RING, slot);
+        slot = slot == RING - 1 ? 0 : slot + 1;
+        read(slot, 0, fa[0], fb[0]);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < TM; ++i)
@@ -517,12 +520,12 @@ static void int8_launch_few(const TX *x, int T, int K, long ld, const char *ws, 
     else hipLaunchKernelGGL((p2n_int8_few_kernel<TX, 4, false, VEC>), grid, blk, 0, s, x, T, K, ld, ws, sx, img, sw, b, N, I.KT, relu, y);
 }
 
-template <typename TX, int TM, int TN, int WR, int WC>
+template <typename TX, int TM, int TN, int WR, int WC, int RING>
 static void int8_launch_gemm(const char *ws, const float *sx, const char *img, const Int8Image &I, long T, int N, int relu, TX *y, hipStream_t s) {
     const long TT = (T + 31) / 32, gy = (TT + WR * TM - 1) / (WR * TM);
     const int gx = (I.CT + WC * TN - 1) / (WC * TN);
     const long tiles = gx * gy;
-    hipLaunchKernelGGL((p2n_int8_gemm_kernel<TX, TM, TN, WR, WC>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * WR * WC), 0, s, ws, sx, img,
+    hipLaunchKernelGGL((p2n_int8_gemm_kernel<TX, TM, TN, WR, WC, RING>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * WR * WC), 0, s, ws, sx, img,
                        (const float *)(img + I.scale), (const float *)(img + I.bias), T, N, TT, I.CT, I.KT, relu, gx, tiles, y);
 }
 
@@ -543,12 +546,12 @@ static int int8_linear_run(const TX *x, long T, int K, long ld, const char *img,
     if (int8_is_few(T)) {
         int8_launch_few<TX, VEC>(x, (int)T, K, ld, ws, sx, img, N, relu, y, s);
     } else {
-        // the largest tile that still gives the 256 compute units a workgroup each: larger tiles read less, fewer of them leave
-        // compute units idle
-        auto tiles = [&](int tm) { return ((TT + 2 * tm - 1) / (2 * tm)) * ((I.CT + 2 * tm - 1) / (2 * tm)); };
-        if (tiles(4) >= 256) int8_launch_gemm<TX, 4, 2, 2, 4>(ws, sx, img, I, T, N, relu, y, s);
-        else if (tiles(2) >= 256) int8_launch_gemm<TX, 2, 2, 2, 2>(ws, sx, img, I, T, N, relu, y, s);
-        else int8_launch_gemm<TX, 1, 1, 2, 2>(ws, sx, img, I, T, N, relu, y, s);
+        // the largest tile that still fills the 256 compute units, 128 x 256 with two workgroups each: larger tiles read less, fewer of
+        // them leave compute units idle (K = 2048, N = 4096: T = 2048 30 us against 26 with 128 x 128, T = 4096 45 against 46)
+        auto tiles = [&](int rows, int cols) { return ((TT + rows - 1) / rows) * ((I.CT + cols - 1) / cols); };
+        if (tiles(4, 8) >= 512) int8_launch_gemm<TX, 2, 4, 2, 2, 3>(ws, sx, img, I, T, N, relu, y, s);
+        else if (tiles(4, 4) >= 256) int8_launch_gemm<TX, 2, 2, 2, 2, 4>(ws, sx, img, I, T, N, relu, y, s);
+        else int8_launch_gemm<TX, 1, 1, 2, 2, 4>(ws, sx, img, I, T, N, relu, y, s);
     }
     P2N_CHECK_HIP(hipGetLastError());
     return P2N_OK;
