@@ -281,8 +281,10 @@ enum { ACT8_OUT = 0, ACT8_DY = 1 };         // epilogue
 
 typedef __attribute__((address_space(3))) void act8_lds_t;
 
+// bytes from base on that may be reached; none where base lies past the end (a step behind the last point of a cloud)
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t act8_rsrc(const void *base, long bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)(bytes < 0xFFFFFFFFL ? bytes : 0xFFFFFFFFL), 0x00020000);
+    const long n = bytes < 0 ? 0 : bytes < 0xFFFFFFFFL ? bytes : 0xFFFFFFFFL;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)n, 0x00020000);
 }
 
 // the six products of the three parts, the small ones first: l.h, h.l, m.m, m.h, h.m, h.h
@@ -372,7 +374,7 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : TABK <= 512 ? 2 : 1) void p2n_ac
         for (int s = 0; s < CKS; ++s) {
             const int k0 = 16 * (c * CKS + s);
             const long left = (long)(A.K - k0) * A.L * 4;
-            const __amdgpu_buffer_rsrc_t rs = act8_rsrc(xb + (long)k0 * A.L, left > 0 ? left : 0);   // rows past the last read as zero
+            const __amdgpu_buffer_rsrc_t rs = act8_rsrc(xb + (long)k0 * A.L, left);   // rows past the last read as zero
 #pragma unroll
             for (int i = 0; i < 8; ++i) raw[s][i] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, off + (unsigned)(i * A.L * 4), 0, 0));
         }

@@ -163,6 +163,23 @@ def test_layer_against_its_definition(B, K, L, N, mode):
             assert int(norm.num_batches_tracked) == 0
 
 
+@pytest.mark.parametrize("L", [4100, 4099, 4160])
+def test_wide_weight_gradient_with_part_of_a_block_at_the_end(L):
+    """long enough for 128 x 128 tiles of dW; the last block of a cloud ends in its first, its third piece of 32 points, rows start on 16
+    bytes or not, and the last tile holds 72 of 128 rows: what lies behind a cloud's last point is neither read nor added"""
+    from pointcloudsegmentation_amd import quant
+    B, K, N = 17, 130, 200
+    x, W, b, g, _ = make(B, K, L, N, False)
+    room = torch.full((B * N * L + 4096,), float("nan"), device="cuda")
+    room[:B * N * L] = g.reshape(-1)
+    g = room[:B * N * L].view(B, N, L)
+    ref = Definition(x, W, b, None).backward(g)
+    h = quant.act8_linear(x, W, b)
+    dW, db = torch.autograd.grad(h, [W, b], g)
+    close(dW, *ref["dW"], 6 * B * L + 16, "dW")
+    close(db, *ref["db"], B * L, "db")
+
+
 @pytest.mark.parametrize("mode", ["batch", "frozen", "untracked"])
 @pytest.mark.parametrize("B,C,L", [(1, 1, 2), (3, 5, 1), (2, 64, 130), (1, 100, 1025), (3, 33, 257), (2, 256, 64)])
 def test_norm_relu_against_its_definition(B, C, L, mode):
