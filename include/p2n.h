@@ -399,6 +399,7 @@ long p2n_int8_weight_bytes(int K, int N);        /* -1: K or N outside 1..65536 
 int p2n_int8_pack_weight(const float *W, const float *bias, int K, int N, void *image, void *stream);
 /* rows x[t*ld .. t*ld + K-1], t < T, ld >= K -> codes (T,K), scale (T) */
 int p2n_quantize_tokens(const void *x, int bf16, long T, int K, long ld, signed char *codes, float *scale, void *stream);
+/* T <= 2^30 */
 size_t p2n_int8_linear_workspace_bytes(long T, int K, int N);
 int p2n_int8_linear(const void *x, int bf16, long T, int K, long ld, const void *image, int N, int relu, void *y,
                     void *workspace, size_t workspace_bytes, void *stream);
@@ -421,7 +422,7 @@ int p2n_max_of_columns(const float *in, long rows, int ns, float *out, void *str
  *   dW = g . ah^T, db = sum g, dy = [y > 0] * (W^T . g), dbeta = sum dy, dgamma = sum dy*uh,
  *   dx = gamma*r*(dy - dbeta/P - uh*dgamma/P), P = B*L   (frozen: gamma*r*dy; without a norm: W^T . g)
  * dW and db may be NULL (not computed), and dx without a norm; with a norm dgamma and dbeta need dx.  Limits: 1..1024
- * channels, L <= 2^24.  kept and workspace 256-byte aligned; the workspace holds nothing between calls. */
+ * channels, L <= 2^24, B*ceil(L/128) < 2^24 - 1024.  kept and workspace 256-byte aligned; the workspace holds nothing between calls. */
 size_t p2n_act8_kept_bytes(int B, int C, long L, int norm);
 size_t p2n_act8_workspace_bytes(int B, int K, long L, int N);      /* N = 0: the norm + ReLU calls */
 int p2n_act8_forward(const float *x, int B, int K, long L, const float *W, const float *bias, int N,

@@ -937,7 +937,8 @@ int act8_init(Act8 &a, const char *fn, int B, int K, long L, int N) {
     P2N_REQUIRE(B >= 1 && L >= 1 && L <= (1L << 24), "%s: bad shape B=%d L=%ld (1 to 2^24 columns a cloud)", fn, B, L);
     P2N_REQUIRE(K >= 1 && K <= ACT8_MAX_C && N >= 0 && N <= ACT8_MAX_C, "%s: %d or %d channels, not in [1,%d]", fn, K, N, ACT8_MAX_C);
     a.B = B; a.K = K; a.N = N; a.L = L; a.NB = (L + ACT8_GROUP - 1) / ACT8_GROUP;
-    P2N_REQUIRE((long)B * a.NB * 4 < (1L << 30) && (long)B * a.NB * K < (1L << 31) && (long)B * ((L + 1023) / 1024) * K < (1L << 31), "%s: too many points", fn);
+    // a launch holds less than 2^32 threads: 2^24 workgroups of 256, of which the weight image takes up to 1024
+    P2N_REQUIRE((long)B * a.NB <= (1L << 24) - 1025, "%s: too many points (%ld blocks of 128)", fn, (long)B * a.NB);
     a.Kpad = (K + 63) / 64 * 64;
     const int cf = act8_tiles(N ? N : 1, (long)B * a.NB), cb = act8_tiles(K, (long)B * a.NB);
     a.KSf = act8_ksteps(K, cf); a.CTf = act8_padded(N ? N : 1, cf);

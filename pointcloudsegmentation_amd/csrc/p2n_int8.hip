@@ -490,12 +490,15 @@ extern "C" int p2n_quantize_tokens(const void *x, int bf16, long T, int K, long 
     if (T == 0) return P2N_OK;
     P2N_REQUIRE(x && codes && scale, "p2n_quantize_tokens: null pointer");
     hipStream_t s = (hipStream_t)stream_;
-    const dim3 grid((unsigned)((T + 3) / 4)), blk(256);
     const int ps = p2n_prof_begin(P2N_K_INT8_TOKENS, s);
-    if (bf16) hipLaunchKernelGGL(p2n_quantize_tokens_kernel<__bf16>, grid, blk, 0, s, (const __bf16 *)x, T, K, ld, codes, scale);
-    else hipLaunchKernelGGL(p2n_quantize_tokens_kernel<float>, grid, blk, 0, s, (const float *)x, T, K, ld, codes, scale);
+    for (long t = 0; t < T; t += 1L << 25) {              // a launch holds less than 2^32 threads
+        const long n = T - t < (1L << 25) ? T - t : 1L << 25;
+        const dim3 grid((unsigned)((n + 3) / 4)), blk(256);
+        if (bf16) hipLaunchKernelGGL(p2n_quantize_tokens_kernel<__bf16>, grid, blk, 0, s, (const __bf16 *)x + t * ld, n, K, ld, codes + t * K, scale + t);
+        else hipLaunchKernelGGL(p2n_quantize_tokens_kernel<float>, grid, blk, 0, s, (const float *)x + t * ld, n, K, ld, codes + t * K, scale + t);
+        P2N_CHECK_HIP(hipGetLastError());
+    }
     p2n_prof_end(ps, s);
-    P2N_CHECK_HIP(hipGetLastError());
     return P2N_OK;
 }
 
@@ -505,7 +508,7 @@ static bool int8_is_few(long T) { return T <= 64; }
 static bool int8_is_own(long T, int K) { return T <= 8 && K <= INT8_OWN_K; }
 
 extern "C" size_t p2n_int8_linear_workspace_bytes(long T, int K, int N) {
-    if (T < 1 || T >= (1L << 31) || K < 1 || K > INT8_MAX_K || N < 1 || N > INT8_MAX_N) return 0;
+    if (T < 1 || T > (1L << 30) || K < 1 || K > INT8_MAX_K || N < 1 || N > INT8_MAX_N) return 0;
     return int8_is_own(T, K) ? 0 : int8_tiles_bytes(T, K);
 }
 
@@ -559,7 +562,7 @@ static int int8_linear_run(const TX *x, long T, int K, long ld, const char *img,
 
 extern "C" int p2n_int8_linear(const void *x, int bf16, long T, int K, long ld, const void *image, int N, int relu, void *y, void *workspace,
                                size_t workspace_bytes, void *stream_) {
-    P2N_REQUIRE(T >= 0 && T < (1L << 31) && K >= 1 && K <= INT8_MAX_K && N >= 1 && N <= INT8_MAX_N && ld >= K,
+    P2N_REQUIRE(T >= 0 && T <= (1L << 30) && K >= 1 && K <= INT8_MAX_K && N >= 1 && N <= INT8_MAX_N && ld >= K,
                 "p2n_int8_linear: bad shape T=%ld K=%d N=%d ld=%ld", T, K, N, ld);
     if (T == 0) return P2N_OK;
     P2N_REQUIRE(x && image && y, "p2n_int8_linear: null pointer");
@@ -940,13 +943,14 @@ extern "C" int p2n_int8_mlp(const float *x, int B, long L, int nl, const int *di
         y.KT = (dims[l] + 31) / 32; y.KTI = I.KT; y.CT = I.CT; y.N = dims[l + 1];
         if (I.CT > ctm) ctm = I.CT;
     }
-    P2N_REQUIRE(a.total < (1L << 31), "p2n_int8_mlp: too many columns");
+    const int waves = ctm <= 2 && ktm <= 2 ? 1 : ctm <= 4 && ktm <= 16 ? 4 : 8;     // of 32 columns; a launch holds less than 2^32 threads
+    P2N_REQUIRE(a.total * waves * 64 <= (1L << 32) - 512, "p2n_int8_mlp: too many columns (%ld tiles of 32)", a.total);
     hipStream_t s = (hipStream_t)stream_;
     const int ps = p2n_prof_begin(P2N_K_INT8_MLP, s);
     // one wave to 32 points up to 64 channels (fewer registers than four waves would share out), four up to 128, eight up to 256
-    if (ctm <= 2 && ktm <= 2) hipLaunchKernelGGL(p2n_int8_mlp_narrow_kernel, dim3((unsigned)((a.total + 3) / 4)), dim3(256), 0, s, a);
-    else if (ctm <= 4 && ktm <= 16 && group) hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<4, true>), dim3((unsigned)a.total), dim3(256), 0, s, a);
-    else if (ctm <= 4 && ktm <= 16) hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<4, false>), dim3((unsigned)a.total), dim3(256), 0, s, a);
+    if (waves == 1) hipLaunchKernelGGL(p2n_int8_mlp_narrow_kernel, dim3((unsigned)((a.total + 3) / 4)), dim3(256), 0, s, a);
+    else if (waves == 4 && group) hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<4, true>), dim3((unsigned)a.total), dim3(256), 0, s, a);
+    else if (waves == 4) hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<4, false>), dim3((unsigned)a.total), dim3(256), 0, s, a);
     else if (group) hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<8, true>), dim3((unsigned)a.total), dim3(512), 0, s, a);
     else hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<8, false>), dim3((unsigned)a.total), dim3(512), 0, s, a);
     p2n_prof_end(ps, s);
@@ -967,7 +971,7 @@ __global__ __launch_bounds__(256) void p2n_int8_rowmax_kernel(const float *__res
 }
 
 extern "C" int p2n_max_of_columns(const float *in, long rows, int ns, float *out, void *stream_) {
-    P2N_REQUIRE(rows >= 0 && ns >= 1 && rows < (1L << 38), "p2n_max_of_columns: bad shape");
+    P2N_REQUIRE(rows >= 0 && ns >= 1 && rows <= (1L << 32) - 256, "p2n_max_of_columns: bad shape");
     if (rows == 0) return P2N_OK;
     P2N_REQUIRE(in && out, "p2n_max_of_columns: null pointer");
     hipLaunchKernelGGL(p2n_int8_rowmax_kernel, dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, (hipStream_t)stream_, in, rows, ns, out);

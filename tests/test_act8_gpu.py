@@ -386,6 +386,83 @@ def test_kept_bytes_and_peak_memory():
     assert held <= n + 8192, (held, n)
 
 
+@pytest.mark.parametrize("B,K,L,N,normed", [(1, 72, 2 ** 24, 72, False), (3, 40, 2 ** 23 - 57, 130, True)])
+def test_offsets_past_32_bits(B, K, L, N, normed):
+    """x and h are over 4 GiB: outputs and dx at columns from everywhere, and the sums over all columns, which are formed here from the
+    rule's codes in 64 bits, 2^20 columns (a multiple of 128) at a time"""
+    from pointcloudsegmentation_amd import quant
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(B, K, L, device="cuda", generator=gen)
+    W = torch.randn(N, K, device="cuda", generator=gen) / K ** 0.5
+    norm = None
+    if normed:
+        norm = nn.BatchNorm1d(K).cuda().eval()
+        with torch.no_grad():
+            norm.weight.uniform_(0.5, 1.5, generator=gen)
+            norm.bias.uniform_(-0.3, 0.3, generator=gen)
+    leaves = [x.requires_grad_(), W.requires_grad_()] + ([norm.weight, norm.bias] if normed else [])
+    h = quant.act8_linear(x, W, None, norm=norm)
+    g = torch.randn(B, N, L, device="cuda", generator=gen)
+    grads = [t.detach() for t in torch.autograd.grad(h, leaves, g)]
+    h, x, Wd = h.detach(), x.detach(), W.detach().double()
+    sums = [torch.zeros(2, N, K, device="cuda", dtype=torch.float64)] + [torch.zeros(2, K, device="cuda", dtype=torch.float64) for _ in range(2)]
+    for b in range(B):
+        for l in range(0, L, 2 ** 20):
+            n = min(2 ** 20, L - l)
+            v, gg = x[b, :, l:l + n], g[b, :, l:l + n].double()
+            mask = torch.ones((), device="cuda", dtype=torch.float64)
+            u = v
+            if normed:
+                r = (1 / (norm.running_var.double() + norm.eps).sqrt()).float()[:, None]
+                u = (v - norm.running_mean[:, None]) * r
+            s = (torch.nn.functional.pad(u.double(), (0, -n % GROUP)).view(K, -1, GROUP).abs().amax(2, keepdim=True) / 127).float().double()
+            uh = ((torch.nn.functional.pad(u.double(), (0, -n % GROUP)).view(K, -1, GROUP) / s.clamp_min(1e-300)).round().clamp(-127, 127) * s).reshape(K, -1)[:, :n]
+            a, ah, asize = u.double(), uh, uh.abs()
+            if normed:
+                ga, be = norm.weight.detach().double()[:, None], norm.bias.detach().double()[:, None]
+                y = ga * u.double() + be
+                mask = (y > 0).double()
+                a, ah, asize = y.clamp_min(0), mask * (ga * uh + be).clamp_min(0), (ga * uh).abs() + be.abs()
+            sums[0] += torch.stack([torch.matmul(gg, ah.t().contiguous()), torch.matmul(gg.abs(), asize.t().contiguous())])
+            da, dasize = torch.matmul(Wd.t().contiguous(), gg), torch.matmul(Wd.abs().t().contiguous(), gg.abs())
+            dy, dysize = mask * da, mask * dasize
+            sums[1] += torch.stack([(dy * uh).sum(1), (dysize * uh.abs()).sum(1)])
+            sums[2] += torch.stack([dy.sum(1), dysize.sum(1)])
+            if l in (0, L // 2 ** 21 * 2 ** 20) or l + n == L:
+                k = (ga * r.double()) if normed else torch.ones((), device="cuda", dtype=torch.float64)
+                for c in (slice(0, 2000), slice(n - 2000, n)):
+                    close(h[b, :, l:l + n][:, c], torch.matmul(Wd, a[:, c]), torch.matmul(Wd.abs(), a[:, c].abs() + (be.abs() if normed else 0)), 6 * K + 8, "h")
+                    close(grads[0][b, :, l:l + n][:, c], k * dy[:, c], k.abs() * dysize[:, c], 6 * N + 16, "dx")
+    # terms of either sign: a sum of k of them stays within 6 sqrt(k) of their deviation d, its rounding within 2^-24 of that; 6 P
+    # such roundings of either sign stay within 8 * 6 d sqrt(6 P P / 2) 2^-24 = 83 P d 2^-24, and the sum of magnitudes is 0.8 P d:
+    # 104 = 8 sqrt(169)
+    for name, got, want in zip(("dW", "dgamma", "dbeta"), grads[1:], sums):
+        close(got, want[0], want[1], 169, name)
+
+
+def test_two_streams_at_once():
+    """steps on two streams share nothing: each gives what it gives alone"""
+    from pointcloudsegmentation_amd import quant
+    def step(x, W, b, g, norm):
+        h = quant.act8_linear(x, W, b, norm=norm)
+        return (h.detach(),) + torch.autograd.grad(h, [x, W, b, norm.weight, norm.bias], g)
+    data = [make(2, 64, 3000, 128, True, seed=s, bias=True) for s in (0, 1)]
+    for d in data:
+        d[4].momentum = 0.0          # running statistics stay as they are
+    want = [step(*d) for d in data]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(6):
+        for d, s in zip(data, streams):
+            with torch.cuda.stream(s):
+                got.append(step(*d))
+    torch.cuda.synchronize()
+    for i, ts in enumerate(got):
+        for a, b in zip(ts, want[i % 2]):
+            assert torch.equal(a, b), i
+
+
 def test_captured_step_replays():
     from pointcloudsegmentation_amd import quant
     x, W, b, g, norm = make(2, 64, 700, 96, True)

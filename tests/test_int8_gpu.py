@@ -296,6 +296,85 @@ def test_mlp_leaves_memory_behind_its_result():
     assert bool((guard[2 * 33 * 45:] == 7.0).all())
 
 
+# ---------------------------------------------------------------- offsets past 32 bits, calls that overlap
+@pytest.mark.parametrize("T,K,N,dtype", [(2 ** 21 + 7, 1030, 40, torch.bfloat16), (2 ** 21 + 7, 32, 515, torch.float32)])
+def test_linear_offsets_past_32_bits(T, K, N, dtype):
+    """x, or y, is over 4 GiB: rows from everywhere equal the same rows on their own"""
+    from pointcloudsegmentation_amd import quant
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(T, K, device="cuda", dtype=dtype, generator=g)
+    w = quant.Int8Weight(torch.randn(N, K, device="cuda", generator=g), torch.randn(N, device="cuda", generator=g))
+    y = quant.int8_linear(x, w)
+    codes, scale = quant.quantize_tokens(x)
+    for t in (0, T // 2 - 30, T - 200):
+        assert torch.equal(y[t:t + 200], quant.int8_linear(x[t:t + 200].clone(), w)), t
+        c, s = quant.quantize_tokens(x[t:t + 200].clone())
+        assert torch.equal(codes[t:t + 200], c) and torch.equal(scale[t:t + 200], s), t
+
+
+def test_quantize_many_short_tokens():
+    """more tokens than one launch takes"""
+    from pointcloudsegmentation_amd import quant
+    T = 2 ** 25 + 5
+    x = torch.arange(T, device="cuda", dtype=torch.float32).remainder_(997).sub_(400).unsqueeze(1)
+    codes, scale = quant.quantize_tokens(x)
+    assert torch.equal(codes[:, 0], (x[:, 0].sign() * 127).to(torch.int8))
+    assert torch.equal(scale, (x[:, 0].abs().double() / 127).float())
+
+
+@pytest.mark.parametrize("dims,group", [([72, 72], 0), ([64, 64, 40], 0), ([66, 33], 32), ([64, 64], 16), ([6, 256], 0)])
+def test_mlp_offsets_past_32_bits(dims, group):
+    """the longest cloud: columns from everywhere equal the same columns on their own"""
+    from pointcloudsegmentation_amd import quant
+    L = 2 ** 24
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn(1, dims[0], L, device="cuda", generator=g)
+    ws = [quant.Int8Weight(torch.randn(n, k, device="cuda", generator=g), torch.randn(n, device="cuda", generator=g)) for k, n in zip(dims, dims[1:])]
+    y = quant.int8_mlp(x, ws, group=group)
+    for l in (0, L // 2 - 32, L - 320):
+        want = quant.int8_mlp(x[:, :, l:l + 320].contiguous(), ws, group=group)
+        d = group or 1
+        assert torch.equal(y[:, :, l // d:(l + 320) // d], want), l
+
+
+def test_two_streams_at_once():
+    """calls on two streams share nothing"""
+    from pointcloudsegmentation_amd import quant
+    x, W, b = make(3000, 512, 512)
+    w = quant.Int8Weight(W, b)
+    xm, layers = make_mlp(4, 4096, [6, 64, 64])
+    ws = [quant.Int8Weight(*l) for l in layers]
+    want, wantm = quant.int8_linear(x, w), quant.int8_mlp(xm, ws, group=32)
+    want5 = quant.int8_linear(x[:5], w)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append((quant.int8_linear(x, w), quant.int8_mlp(xm, ws, group=32), quant.int8_linear(x[:5], w)))
+    torch.cuda.synchronize()
+    for a, m, f in got:
+        assert torch.equal(a, want) and torch.equal(m, wantm) and torch.equal(f, want5)
+
+
+def test_mlp_captured_and_replayed():
+    from pointcloudsegmentation_amd import quant
+    for B, L, dims, group in ((2, 96, [6, 32, 64], 32), (2, 96, [131, 128, 64], 24)):
+        x, layers = make_mlp(B, L, dims)
+        ws = [quant.Int8Weight(*l) for l in layers]
+        quant.int8_mlp(x, ws, group=group)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = quant.int8_mlp(x, ws, group=group)
+        for i in range(4):
+            x.copy_(make_mlp(B, L, dims, seed=i)[0])
+            want = quant.int8_mlp(x, ws, group=group)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want), i
+
+
 # ---------------------------------------------------------------- refusals
 def test_refusals():
     from pointcloudsegmentation_amd import quant

@@ -30,6 +30,12 @@ def test_library_refuses_bad_shapes():
     assert lib.p2n_int8_mlp(16, 1, 8, 9, dims, images, 1, 0, 16, None) == 1
     assert lib.p2n_int8_mlp(None, 0, 8, 2, dims, images, 1, 0, None, None) == 0
     assert lib.p2n_max_of_columns(None, 4, 0, None, None) == 1
+    # more than a launch's 2^32 threads
+    assert lib.p2n_int8_linear(16, 0, (1 << 30) + 1, 1, 1, 16, 1, 0, 16, 16, 1 << 62, None) == 1
+    for B, wide in ((128, 32), (32, 100), (16, 200)):
+        assert lib.p2n_int8_mlp(16, B, 1 << 24, 1, (ctypes.c_int * 2)(6, wide), images, 1, 0, 16, None) == 1
+        assert b"too many columns" in lib.p2n_last_error()
+    assert lib.p2n_max_of_columns(16, 1 << 32, 1, 16, None) == 1
 
 
 def test_cpu_tensors_are_refused():
@@ -49,7 +55,7 @@ def test_checkpoint_layers_refuse_bad_shapes():
     # codes, scales, bits, mean and 1/deviation, each part rounded up to 256 bytes
     assert lib.p2n_act8_kept_bytes(2, 64, 300, 1) == 2 * 3 * 64 * 128 + 2 * 3 * 64 * 4 + 2 * 3 * 64 * 16 + 64 * 8
     assert lib.p2n_act8_kept_bytes(2, 6, 300, 0) == 2 * 3 * 6 * 128 + 256                # 6 scales as 8: 192 bytes
-    for bad in ((0, 64, 300, 1), (2, 0, 300, 1), (2, 1025, 300, 1), (2, 64, 0, 1), (2, 64, (1 << 24) + 1, 1), (1 << 20, 1024, 300, 1)):
+    for bad in ((0, 64, 300, 1), (2, 0, 300, 1), (2, 1025, 300, 1), (2, 64, 0, 1), (2, 64, (1 << 24) + 1, 1), (1 << 20, 1024, 3000, 1), (1 << 24, 1, 1, 0)):
         assert lib.p2n_act8_kept_bytes(*bad) == 0
         assert lib.p2n_act8_workspace_bytes(*bad[:3], 8) == 0
     a = 1 << 16     # an address that is never read: every call below is refused first
