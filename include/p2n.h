@@ -395,8 +395,10 @@ int p2n_forward_eval_raw(const double *points, const double *colors, int N, int 
  *     y[t][n] = fl(fl(fl(sum_k qx qw) * sw[n]) * sx[t]) + bias[n]      (the sum exact in int32), then ReLU if asked.
  * `bf16` non-zero: x and y are bfloat16, the arithmetic is the same and y is rounded once at the end. */
 long p2n_int8_weight_bytes(int K, int N);        /* -1: K or N outside 1..65536 */
-/* W (N,K) float32 and bias (N) (NULL: zeros) -> the image that the products read: codes in matrix-core fragment order, scales, bias */
-int p2n_int8_pack_weight(const float *W, const float *bias, int K, int N, void *image, void *stream);
+/* W (N,K) float32 and bias (N) (NULL: zeros) -> the image that the products read: codes in matrix-core fragment order, scales, bias.
+ * gamma not NULL: a BatchNorm behind the product folded in first, W s and (bias - mean) s + beta with s = gamma / sqrt(var + eps). */
+int p2n_int8_pack_weight(const float *W, const float *bias, int K, int N, const float *gamma, const float *beta, const float *mean,
+                         const float *var, double eps, void *image, void *stream);
 /* rows x[t*ld .. t*ld + K-1], t < T, ld >= K -> codes (T,K), scale (T) */
 int p2n_quantize_tokens(const void *x, int bf16, long T, int K, long ld, signed char *codes, float *scale, void *stream);
 /* T <= 2^30 */

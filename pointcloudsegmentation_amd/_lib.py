@@ -97,7 +97,7 @@ SIGNATURES = {
     "p2n_preprocess_points": (c_int, [c_vp, c_vp, ctypes.c_long, c_f, c_vp, c_vp, c_sz, c_vp]),
     "p2n_forward_eval_raw": (c_int, [c_vp, c_vp, c_int, c_int, c_f, c_vp, c_f, c_f, c_vp, c_sz, c_vp]),
     "p2n_int8_weight_bytes": (c_long, [c_int, c_int]),
-    "p2n_int8_pack_weight": (c_int, [c_f, c_f, c_int, c_int, c_vp, c_vp]),
+    "p2n_int8_pack_weight": (c_int, [c_f, c_f, c_int, c_int, c_f, c_f, c_f, c_f, ctypes.c_double, c_vp, c_vp]),
     "p2n_quantize_tokens": (c_int, [c_vp, c_int, c_long, c_int, c_long, c_vp, c_f, c_vp]),
     "p2n_int8_linear_workspace_bytes": (c_sz, [c_long, c_int, c_int]),
     "p2n_int8_linear": (c_int, [c_vp, c_int, c_long, c_int, c_long, c_vp, c_int, c_int, c_vp, c_vp, c_sz, c_vp]),

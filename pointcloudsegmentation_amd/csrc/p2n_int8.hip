@@ -34,18 +34,32 @@ static Int8Image int8_image(int K, int N) {
     return I;
 }
 
-// one wave per channel: maximum, scale, codes
+// one wave per channel: maximum, scale, codes.  A norm behind the product (gamma not NULL) is folded in: w s and (b - mean) s + beta
+// with s = gamma / sqrt(var + eps), in 64 bits until s and the bias are float32.
+struct Int8Norm {
+    const float *gamma, *beta, *mean, *var;
+    double eps;
+};
 __global__ __launch_bounds__(256) void p2n_int8_pack_kernel(const float *__restrict__ W, const float *__restrict__ bias, int K, int N,
                                                             int CT, int KT, char *__restrict__ img, float *__restrict__ scale,
-                                                            float *__restrict__ bimg) {
+                                                            float *__restrict__ bimg, Int8Norm B) {
     const int lane = threadIdx.x & 63;
     const int n = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (n >= 32 * CT) return;
     const float *w = W + (long)n * K;
+    float fold = 1.f, t = 0.f;
+    if (n < N) {
+        if (bias) t = bias[n];
+        if (B.gamma) {
+            const double f = (double)B.gamma[n] / sqrt((double)B.var[n] + B.eps);
+            fold = (float)f;
+            t = (float)(((double)t - (double)B.mean[n]) * f + (double)B.beta[n]);
+        }
+    }
     unsigned am = 0;
     if (n < N)
         for (int k = lane; k < K; k += 64) {
-            const unsigned b = p2n_absbits(w[k]);
+            const unsigned b = p2n_absbits(w[k] * fold);
             am = b > am ? b : am;
         }
 #pragma unroll
@@ -58,7 +72,7 @@ __global__ __launch_bounds__(256) void p2n_int8_pack_kernel(const float *__restr
     if (lane == 0) {
         scale[n] = n < N ? s : 0.f;
         // a NaN without a sign: the ReLU of p2n_int8_mlp is a maximum of bit patterns
-        bimg[n] = n < N && bias ? (bias[n] == bias[n] ? bias[n] : __uint_as_float(0x7FC00000u)) : 0.f;
+        bimg[n] = t == t ? t : __uint_as_float(0x7FC00000u);
     }
     const int ct = n >> 5, r = n & 31;
     const bool bad = !(s == s);
@@ -67,7 +81,7 @@ __global__ __launch_bounds__(256) void p2n_int8_pack_kernel(const float *__restr
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int k = 4 * k4 + j;
-            v[j] = (n < N && k < K) ? w[k] : 0.f;
+            v[j] = (n < N && k < K) ? w[k] * fold : 0.f;
         }
         int c[1];
         p2n_q8_pack(v, Q, c);
@@ -81,16 +95,18 @@ extern "C" long p2n_int8_weight_bytes(int K, int N) {
     return (long)int8_image(K, N).total;
 }
 
-extern "C" int p2n_int8_pack_weight(const float *W, const float *bias, int K, int N, void *image, void *stream_) {
+extern "C" int p2n_int8_pack_weight(const float *W, const float *bias, int K, int N, const float *gamma, const float *beta, const float *mean,
+                                    const float *var, double eps, void *image, void *stream_) {
     P2N_REQUIRE(K >= 1 && K <= INT8_MAX_K && N >= 1 && N <= INT8_MAX_N, "p2n_int8_pack_weight: K=%d or N=%d not in [1,%d]", K, N, INT8_MAX_K);
     P2N_REQUIRE(W && image, "p2n_int8_pack_weight: null pointer");
+    P2N_REQUIRE(!gamma || (beta && mean && var && eps >= 0), "p2n_int8_pack_weight: a norm needs gamma, beta, mean, variance and eps >= 0");
     P2N_REQUIRE(((uintptr_t)image & 15) == 0, "p2n_int8_pack_weight: the image must be 16-byte aligned");
     const Int8Image I = int8_image(K, N);
     char *img = (char *)image;
     hipStream_t s = (hipStream_t)stream_;
     const int ps = p2n_prof_begin(P2N_K_INT8_PACK, s);
     hipLaunchKernelGGL(p2n_int8_pack_kernel, dim3(8 * I.CT), dim3(256), 0, s, W, bias, K, N, I.CT, I.KT, img, (float *)(img + I.scale),
-                       (float *)(img + I.bias));
+                       (float *)(img + I.bias), Int8Norm{gamma, beta, mean, var, eps});
     p2n_prof_end(ps, s);
     P2N_CHECK_HIP(hipGetLastError());
     return P2N_OK;

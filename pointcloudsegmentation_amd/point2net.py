@@ -75,6 +75,8 @@ class _PackedCache:
 class PointNet2Encoder(nn.Module):
     """reference point2net.py:5-48."""
 
+    checkpoint = None                        # "int8": training keeps its activations in 8 bits (GPU tensors only)
+
     def __init__(self, in_channels=6):
         super().__init__()
         self.mlp1 = _mlp(in_channels, 64, 64)
@@ -82,7 +84,6 @@ class PointNet2Encoder(nn.Module):
         self.mlp3 = _mlp(128, 256, 256)
         self.in_channels = in_channels
         self.precision = DEFAULT_PRECISION   # "fp32" | "fp32x3" | "bf16" (GPU tensors only)
-        self.checkpoint = None               # "int8": training keeps its activations in 8 bits (GPU tensors only)
         self._cache = _PackedCache()
 
     def forward(self, x):

@@ -388,6 +388,10 @@ class SharedMLP(nn.Module):
     """[Conv1d(k=1) + BatchNorm1d + ReLU] x n over (B,C,L).  GPU tensors: eval = p2n_pointwise_layer (or the
     fused level kernels), train / autograd = p2n_mlp_train_forward + p2n_mlp_train_backward."""
 
+    # GPU tensors only, plain attributes (not part of the state_dict)
+    precision = "fp32"       # "int8": eval products in 8-bit integers (quant.int8_mlp)
+    checkpoint = None        # "int8": training keeps its activations in 8 bits (quant.act8_linear)
+
     def __init__(self, channels: List[int], last_plain: bool = False):
         super().__init__()
         layers = []
@@ -397,11 +401,6 @@ class SharedMLP(nn.Module):
             if not plain:
                 layers += [nn.BatchNorm1d(channels[i + 1]), nn.ReLU()]
         self.net = nn.Sequential(*layers)
-        # GPU tensors only, plain attributes (not part of the state_dict).  precision "int8": eval products in 8-bit integers
-        # (quant.int8_mlp).  checkpoint "int8": training keeps its activations in 8 bits (quant.act8_linear).
-        self.precision = "fp32"
-        self.checkpoint = None
-        self._int8 = (None, None)
 
     def _folded(self):
         out, mods, i = [], list(self.net), 0
@@ -425,13 +424,14 @@ class SharedMLP(nn.Module):
         return shared_mlp_train(self.net, x, group, eval_stats=not self.training, checkpoint=self.checkpoint)
 
     def int8_weights(self):
-        """[(Int8Weight of the layer, BatchNorm folded in)], last layer has a ReLU; rebuilt only when a parameter or buffer changed"""
-        tensors = [t for m in self.net for t in list(m.parameters()) + list(m.buffers())]
-        key = tuple((t.data_ptr(), t._version) for t in tensors)      # num_batches_tracked stands in for the running statistics
-        if key != self._int8[0]:
-            folded = self._folded()
-            self._int8 = (key, ([quant.Int8Weight(w * s[:, None], t) for w, s, t, _ in folded], bool(folded[-1][3])))
-        return self._int8[1]
+        """[Int8Weight of the layer, BatchNorm folded in], last layer has a ReLU.  Made from the parameters and buffers of the moment at
+        every call, one launch a layer: a captured graph follows them too."""
+        mods, out, i = list(self.net), [], 0
+        while i < len(mods):
+            norm = mods[i + 1] if i + 1 < len(mods) else None
+            out.append(quant.Int8Weight(mods[i].weight, mods[i].bias, norm=norm))
+            i += 3 if norm is not None else 1
+        return out, norm is not None
 
     def forward_int8(self, x, group: int = 0):
         """eval forward in 8-bit integers: (B,C,L) -> (B,Cout,L), or with group the maximum over groups of columns"""

@@ -81,10 +81,10 @@ def quantize_tokens(x: torch.Tensor):
 
 class Int8Weight:
     """A weight (N, K) -- or the (N, K, 1) of a Conv1d(kernel_size=1) -- and an optional bias (N), put into 8 bits with one scale
-    per output channel and laid out for the kernels.  Made once from the float32 values of that moment; make a new one after
-    the weights changed."""
+    per output channel and laid out for the kernels.  norm: a BatchNorm1d behind the product, folded in as eval mode applies it
+    (running statistics).  Made once from the float32 values of that moment; make a new one after they changed."""
 
-    def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None):
+    def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, norm: Optional[nn.BatchNorm1d] = None):
         weight = _gpu(weight, "weight", (torch.float32,)).detach()
         if weight.dim() == 3 and weight.size(2) == 1:
             weight = weight.squeeze(2)
@@ -97,6 +97,15 @@ class Int8Weight:
             if bias.shape != (self.out_features,) or bias.device != weight.device:
                 raise ValueError(f"bias must be ({self.out_features},) on {weight.device}, got {tuple(bias.shape)} on {bias.device}")
             bias = bias.contiguous()
+        fold = (None, None, None, None)
+        if norm is not None:
+            if not norm.affine or norm.running_mean is None:
+                raise NotImplementedError("only a BatchNorm1d with affine=True and track_running_stats=True folds into the weight")
+            if norm.num_features != self.out_features:
+                raise ValueError(f"norm has {norm.num_features} channels, the weight {self.out_features}")
+            fold = tuple(_gpu(t, "norm", (torch.float32,)).detach().contiguous() for t in (norm.weight, norm.bias, norm.running_mean, norm.running_var))
+            if any(t.device != weight.device for t in fold):
+                raise ValueError(f"norm must be on {weight.device}")
         L = _lib.lib()
         n = L.p2n_int8_weight_bytes(self.in_features, self.out_features)
         if n < 0:
@@ -104,7 +113,7 @@ class Int8Weight:
         weight = weight.contiguous()
         self.image = torch.empty(n, dtype=torch.uint8, device=weight.device)
         _call(L.p2n_int8_pack_weight, "p2n_int8_pack_weight", weight.device, weight.data_ptr(), _rt.ptr(bias), self.in_features,
-              self.out_features, self.image.data_ptr())
+              self.out_features, *(_rt.ptr(t) for t in fold), 0.0 if norm is None else norm.eps, self.image.data_ptr())
 
     @property
     def scale(self) -> torch.Tensor:

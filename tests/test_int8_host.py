@@ -10,8 +10,9 @@ def test_library_refuses_bad_shapes():
     assert lib.p2n_int8_weight_bytes(0, 4) == -1 and lib.p2n_int8_weight_bytes(4, 65537) == -1
     # 2 k-tiles of 32 (rounded up to even) x 1 channel tile of 1 KiB, 32 scales, 32 biases
     assert lib.p2n_int8_weight_bytes(6, 7) == 2 * 1024 + 8 * 32
-    assert lib.p2n_int8_pack_weight(None, None, 0, 4, None, None) == 1
-    assert lib.p2n_int8_pack_weight(None, None, 4, 4, None, None) == 1
+    assert lib.p2n_int8_pack_weight(None, None, 0, 4, None, None, None, None, 0.0, None, None) == 1
+    assert lib.p2n_int8_pack_weight(None, None, 4, 4, None, None, None, None, 0.0, None, None) == 1
+    assert lib.p2n_int8_pack_weight(16, None, 4, 4, 16, None, 16, 16, 1e-5, 16, None) == 1       # gamma without beta
     assert lib.p2n_quantize_tokens(None, 0, 4, 8, 7, None, None, None) == 1          # rows that overlap
     assert lib.p2n_quantize_tokens(None, 0, 0, 8, 8, None, None, None) == 0
     assert lib.p2n_int8_linear(None, 0, 4, 8, 8, None, 4, 0, None, None, 0, None) == 1

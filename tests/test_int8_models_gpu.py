@@ -56,6 +56,47 @@ def test_shared_mlp_eval_int8(cin, chans, last_plain, group):
             mlp(x)
 
 
+def test_int8_answers_follow_every_kind_of_change():
+    """writes through .data, a replaced parameter, a replayed graph that trains, another stream, a copy: never an old answer"""
+    import copy
+    from pointcloudsegmentation_amd import quant
+    from pointcloudsegmentation_amd.pointnet2 import SharedMLP
+    torch.manual_seed(3)
+    mlp = SharedMLP([6, 32, 64]).eval()
+    randomise(mlp, 8)
+    mlp = mlp.cuda()
+    mlp.precision = "int8"
+    x = torch.randn(2, 6, 96, device="cuda")
+
+    def fresh():
+        return quant.int8_mlp(x, [quant.Int8Weight(w * s[:, None], t) for w, s, t, _ in mlp._folded()])
+
+    with torch.no_grad():
+        first = mlp(x)
+        assert torch.equal(first, fresh())
+        mlp.net[0].weight.data.mul_(1.5)
+        assert torch.equal(mlp(x), fresh()) and not torch.equal(mlp(x), first)
+        mlp.net[3].weight = torch.nn.Parameter(torch.randn_like(mlp.net[3].weight))
+        assert torch.equal(mlp(x), fresh())
+        assert torch.equal(copy.deepcopy(mlp)(x), fresh())
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            other = mlp(x)
+        torch.cuda.current_stream().wait_stream(s)
+        assert torch.equal(other, fresh())
+        grown, answer = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(grown):
+            mlp.net[0].weight.mul_(1.1)          # what a captured optimiser step does: nothing on the host shows it
+        with torch.cuda.graph(answer):
+            y = mlp(x)
+        for _ in range(3):
+            grown.replay()
+            answer.replay()
+            want = fresh()
+            assert torch.equal(mlp(x), want) and torch.equal(y, want)
+
+
 def test_set_abstraction_eval_int8():
     from pointcloudsegmentation_amd import quant
     from pointcloudsegmentation_amd.pointnet2 import SetAbstraction, ball_query_torch, fps_torch
