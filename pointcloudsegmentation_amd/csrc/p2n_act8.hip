@@ -13,6 +13,7 @@
 // Products of float32 operands run on the bf16 matrix cores: each operand is the exact sum of three bf16 parts (24 bits),
 // and of the nine part products the six that reach 2^-16 of the largest are added in float32 -- float32 accuracy at
 // 1/6 of the bf16 rate, against 1/16 for the float32 instruction.
+#include <type_traits>
 #include "p2n_q8.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -603,8 +604,7 @@ __global__ __launch_bounds__(256) void p2n_act8_dx_kernel(float *__restrict__ dy
 // points inside a product is free as long as both operands agree.  A wave makes 32 RT x 32 CT of dW over its share of the
 // points, 32 at a time, a lane 16 of them: its codes are one 16-byte load, its g passes through a piece of
 // LDS that belongs to the wave alone (no barrier): it is read in whole cache lines, eight lanes a row (a lane reading its own row's
-// bytes keeps the address unit busy for 113 cycles an instruction), and handed over as rows.  The next step's g waits in
-// registers meanwhile, for a 128 x 128 tile, which has none left, in a second piece that LDS-DMA fills.  The four waves of a
+// bytes keeps the address unit busy for 113 cycles an instruction), and handed over as rows.  The four waves of a
 // workgroup are added in LDS, the workgroups by a second kernel, both in order.
 struct Act8Wgrad {
     const float *g;        // (B, N, L)
@@ -617,35 +617,120 @@ struct Act8Wgrad {
     int N, K, K4, ntc, slices, steps;        // steps of 32 points in all
 };
 
-// DMA (128 x 128 only): rows of g start 16-byte aligned (L a multiple of 4); without, its values are loaded as they are needed
-template <int RT, int CT, bool DMA, bool NORM>
-__global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : 2) void p2n_act8_wgrad_kernel(Act8Wgrad A) {
-    constexpr bool REG = RT * CT < 16;
-    constexpr int BUF = RT * 4096;                   // 32 RT rows of 128 bytes
-    constexpr int JOIN = (RT * CT * 1024 + 4 * 32 * RT) * 4;
-    constexpr int OWN = DMA ? 8 * BUF : REG ? 4 * BUF : 0;
-    __shared__ __attribute__((aligned(16))) char lds[OWN > JOIN ? OWN : JOIN];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int r = lane & 31, h = lane >> 5;
-    // neighbouring workgroups go to the eight dies in turn: the tiles of one slice stay on one die, whose L2 then holds its rows
-    const int nt = gridDim.x / A.slices, w8 = blockIdx.x >> 3, full = A.slices / 8 * 8;
+// neighbouring workgroups go to the eight dies in turn: the tiles of one slice stay on one die, whose L2 then holds its rows
+struct Act8Place {
     int tile, slice;
-    if ((int)blockIdx.x < full * nt) { tile = w8 % nt; slice = w8 / nt * 8 + (blockIdx.x & 7); }
-    else { const int i = blockIdx.x - full * nt; tile = i % nt; slice = full + i / nt; }
-    const int n0 = tile / A.ntc * 32 * RT, k0 = tile % A.ntc * 32 * CT;
-    // waves take turns: those that run at the same time read neighbouring lines of the same rows (shares of consecutive steps
-    // instead scatter the card's reads over as many pages of memory as there are rows in flight)
-    struct Step {
-        int b, q;                           // cloud, 32 points in it
-    };
-    const int turn = A.slices * 4, first = slice * 4 + wave, spc = (int)(4 * A.NB);
-    const int turn_b = turn / spc, turn_q = turn % spc;
-    auto after = [&](Step s) __attribute__((always_inline)) {
-        s.b += turn_b;
-        s.q += turn_q;
+};
+__device__ __forceinline__ Act8Place act8_place(const Act8Wgrad &A) {
+    const int nt = gridDim.x / A.slices, w8 = blockIdx.x >> 3, full = A.slices / 8 * 8, i = (int)blockIdx.x - full * nt;
+    return i < 0 ? Act8Place{w8 % nt, w8 / nt * 8 + (int)(blockIdx.x & 7)} : Act8Place{i % nt, full + i / nt};
+}
+
+// Waves take turns: those that run at the same time read neighbouring lines of the same rows (shares of consecutive steps
+// instead scatter the card's reads over as many pages of memory as there are rows in flight).
+struct Act8Step {
+    int b, q;                           // cloud, 32 points in it
+};
+struct Act8Turn {
+    int b, q, spc;                      // clouds, pieces between a wave's steps; steps of a cloud
+    __device__ __forceinline__ Act8Turn(const Act8Wgrad &A) : spc((int)(4 * A.NB)) {
+        b = A.slices * 4 / spc;
+        q = A.slices * 4 % spc;
+    }
+    __device__ __forceinline__ Act8Step after(Act8Step s) const {
+        s.b += b;
+        s.q += q;
         if (s.q >= spc) { s.q -= spc; s.b += 1; }
         return s;
-    };
+    }
+};
+
+// what was kept of a lane's channels: 16 codes each, scale, bits
+template <int CT>
+struct Act8Codes {
+    i32x4 q[CT];
+    float s[CT];
+    unsigned m[CT];
+};
+template <int CT, bool NORM>
+__device__ __forceinline__ void act8_codes(const Act8Wgrad &A, Act8Step s, int h, const int (&krow)[CT], Act8Codes<CT> &M) {
+    const long blk = s.b * A.NB + (s.q >> 2);
+    const int w = s.q & 3;
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+        M.q[t] = *reinterpret_cast<const i32x4 *>(A.codes + (blk * A.K + krow[t]) * ACT8_GROUP + 32 * w + 16 * h);
+        M.s[t] = A.scale[blk * A.K4 + krow[t]];
+        M.m[t] = NORM ? A.bits[(blk * 4 + w) * A.K4 + krow[t]] : 0u;
+    }
+}
+
+// eight points of a channel: their ah as an operand, its sign turned round in every other share (act8_flip; ah of a norm is not negative).
+// cs = gamma * scale, mb: the lane's bits from its first point's on
+template <bool NORM>
+__device__ __forceinline__ void act8_operand(const i32x4 &q, int j, float cs, float be, unsigned mb, unsigned flip, bf16x8 (&w)[3]) {
+    float v[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+        const float c = (float)(signed char)(q[2 * j + (x >> 2)] >> (8 * (x & 3)));
+        if (NORM) {
+            const float y = fmaxf(fmaf(cs, c, be), 0.f);
+            const unsigned on = (unsigned)((int)(mb << (31 - ((4 * j + (x >> 1)) + 16 * (x & 1)))) >> 31);
+            v[x] = __uint_as_float((__float_as_uint(y) & on) | flip);
+        } else {
+            v[x] = act8_flip(c * cs, flip);
+        }
+    }
+    act8_split(v, w[0], w[1], w[2]);
+}
+
+// the four waves' shares, added in order: a quarter of the tile's registers at a time, all waves at once
+template <int RT, int CT>
+__device__ __forceinline__ void act8_wgrad_end(const Act8Wgrad &A, float *join, const f32x16 (&acc)[RT][CT], float (&db)[RT], const float (&poison)[CT],
+                                               unsigned flip, int slice, int n0, int k0) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) db[t] += __shfl_xor(db[t], 32);
+    float *part = A.part + (long)slice * (A.N * A.K + A.N);
+    constexpr int Q = RT * CT * 4;          // registers of a quarter
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        __syncthreads();                    // the last rows (c = 0), the last quarter have been read
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+            const int v = c * Q + i, tk = v / 16, e = v % 16;
+            join[(wave * Q + i) * 64 + lane] = act8_flip(acc[tk / CT][tk % CT][e], flip) + poison[tk % CT];
+        }
+        if (c == 0 && h == 0)
+#pragma unroll
+            for (int t = 0; t < RT; ++t) join[RT * CT * 1024 + (wave * RT + t) * 32 + r] = db[t];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < Q / 4; ++i) {
+            const int o = i * 256 + threadIdx.x, v = c * Q + o / 64, tk = v / 16, e = v % 16, ln = o & 63;
+            const int row = n0 + 32 * (tk / CT) + 8 * (e >> 2) + 4 * (ln >> 5) + (e & 3), col = k0 + 32 * (tk % CT) + (ln & 31);
+            const float sum = ((join[o] + join[o + Q * 64]) + join[o + 2 * Q * 64]) + join[o + 3 * Q * 64];
+            if (row < A.N && col < A.K) part[(long)row * A.K + col] = sum;
+        }
+        if (c == 0 && k0 == 0 && threadIdx.x < 32 * RT && n0 + (int)threadIdx.x < A.N) {
+            const float *d = join + RT * CT * 1024 + threadIdx.x;
+            part[(long)A.N * A.K + n0 + threadIdx.x] = ((d[0] + d[32 * RT]) + d[64 * RT]) + d[96 * RT];
+        }
+    }
+}
+constexpr int act8_join_floats(int rt, int ct) { return rt * ct * 1024 + 4 * 32 * rt; }
+
+// up to 64 x 64 a wave, two waves or more on a SIMD; the next step's g and codes wait in registers
+template <int RT, int CT, bool NORM>
+__global__ __launch_bounds__(256, 2) void p2n_act8_wgrad_kernel(Act8Wgrad A) {
+    constexpr int BUF = RT * 4096, JOIN = act8_join_floats(RT, CT) * 4;      // bytes; 32 RT rows of 32 points
+    __shared__ __attribute__((aligned(16))) char lds[4 * BUF > JOIN ? 4 * BUF : JOIN];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int r = lane & 31, h = lane >> 5;
+    const Act8Place at = act8_place(A);
+    const int tile = at.tile, slice = at.slice;
+    const int n0 = tile / A.ntc * 32 * RT, k0 = tile % A.ntc * 32 * CT;
+    const Act8Turn take(A);
+    const int turn = A.slices * 4, first = slice * 4 + wave;
     const unsigned flip = (unsigned)((slice * 4 + wave) & 1) << 31;       // every other share with its sign turned round (act8_flip)
     const bool want_db = k0 == 0;
     int krow[CT];
@@ -668,26 +753,13 @@ __global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : 2) void p2n_act8_wgrad_kern
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][k][e] = 0.f;
     // LDS image of a step: row R's 16-byte piece q (points 4q .. 4q+3) lies in slot q ^ (R >> 1 & 7) of the row, so that the 16 rows of a
-    // read fall into different banks.  DMA instruction i fills rows 8i .. 8i+7: lane -> row lane >> 3, slot lane & 7.
-    char *const mine = lds + wave * (DMA ? 2 * BUF : BUF);
-    const int drow = lane >> 3, piece = (lane & 7) ^ (lane >> 4);
-    const int left = A.N - n0;              // rows past the last one read the last one
-    const unsigned off_full = (unsigned)(drow * A.L * 4), off_part = (unsigned)((drow < (left & 7) ? drow : (left & 7) - 1) * A.L * 4);
-    auto dma = [&](Step s, int buf) __attribute__((always_inline)) {
-        const long b = s.b, l0 = (long)s.q * 32;
-#pragma unroll
-        for (int i = 0; i < RT * 4; ++i) {
-            const bool part = 8 * i < left && left < 8 * i + 8, none = 8 * i >= left;        // wave-uniform
-            const long row = b * A.N + (none ? A.N - 1 : n0 + 8 * i);
-            const __amdgpu_buffer_rsrc_t rs = act8_rsrc(A.g + row * A.L + l0, ((b + 1) * A.N - row) * A.L * 4 - l0 * 4);
-            const unsigned off = (none ? 0u : part ? off_part : off_full) + 16u * (unsigned)(piece ^ (4 * (i & 1)));
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (act8_lds_t *)(mine + buf * BUF + i * 1024), 16, off, 0, 0, 0);
-        }
-    };
+    // read fall into different banks.  Load i fills rows 8i .. 8i+7: lane -> row lane >> 3, piece lane & 7.
+    char *const mine = lds + wave * BUF;
+    const int drow = lane >> 3, slot = (lane & 7) ^ (lane >> 4);
     int qn[CT][4];
     float sn[CT];
     unsigned mn[CT];
-    auto meta = [&](Step s) __attribute__((always_inline)) {
+    auto meta = [&](Act8Step s) __attribute__((always_inline)) {
         const long blk = s.b * A.NB + (s.q >> 2);
         const int w = s.q & 3;
 #pragma unroll
@@ -699,37 +771,29 @@ __global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : 2) void p2n_act8_wgrad_kern
             mn[t] = NORM ? A.bits[(blk * 4 + w) * A.K4 + krow[t]] : 0u;
         }
     };
-    f32x4 vn[REG ? RT * 4 : 1];
-    auto rows = [&](Step s) __attribute__((always_inline)) {
+    f32x4 vn[RT * 4];
+    auto rows = [&](Act8Step s) __attribute__((always_inline)) {
         const long b = s.b, l0 = (long)s.q * 32, l = l0 + 4 * (lane & 7);
         const bool tail = l0 + 32 > A.L;
 #pragma unroll
-        for (int i = 0; i < (REG ? RT * 4 : 0); ++i) {
+        for (int i = 0; i < RT * 4; ++i) {
             const int n = n0 + 8 * i + drow;
-            const float *p = A.g + (b * A.N + (n < A.N ? n : A.N - 1)) * A.L + l;
+            const float *p = A.g + (b * A.N + (n < A.N ? n : A.N - 1)) * A.L + l;      // rows past the last one read the last one
             if (!tail) vn[i] = *reinterpret_cast<const f32x4u *>(p);
             else
 #pragma unroll
                 for (int x = 0; x < 4; ++x) vn[i][x] = l + x < A.L ? p[x] : 0.f;
         }
     };
-    Step step = {first / spc, first % spc};
+    Act8Step step = {first / take.spc, first % take.spc};
     if (first < A.steps) {
-        if (DMA) dma(step, 0);
-        if (REG) rows(step);
+        rows(step);
         meta(step);
     }
-    int buf = 0;
 #pragma unroll 1
-    for (int s = first; s < A.steps; s += turn, buf ^= 1) {
-        if (DMA) {
-            __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));     // vmcnt(0): this step's rows and codes have arrived
-            asm volatile("" ::: "memory");
-        }
-        if (REG) {
+    for (int s = first; s < A.steps; s += turn) {
 #pragma unroll
-            for (int i = 0; i < (REG ? RT * 4 : 0); ++i) *reinterpret_cast<f32x4 *>(mine + i * 1024 + drow * 128 + (piece ^ (4 * (i & 1))) * 16) = vn[i];
-        }
+        for (int i = 0; i < RT * 4; ++i) *reinterpret_cast<f32x4 *>(mine + i * 1024 + drow * 128 + (slot ^ (4 * (i & 1))) * 16) = vn[i];
         int q[CT][4];
         float cs[CT];
         unsigned mb[CT];
@@ -741,45 +805,24 @@ __global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : 2) void p2n_act8_wgrad_kern
             poison[t] += cs[t] * 0.f;                       // NaN with a NaN scale
             mb[t] = mn[t] >> (8 * h);                       // points 16h .. 16h+15: bits 8h .. of either half-word
         }
-        const Step next = after(step);
+        const Act8Step next = take.after(step);
         if (s + turn < A.steps) {
-            if (DMA) dma(next, buf ^ 1);
-            if (REG) rows(next);
+            rows(next);
             meta(next);
         }
-        const long b = step.b, l0 = (long)step.q * 32;
         step = next;
-        const bool tail = l0 + 32 > A.L;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             bf16x8 a[RT][3], w[CT][3];
-            const long l = l0 + 16 * h + 8 * j;
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
                 float va[8];
-                if (REG || DMA) {
-                    const char *row = mine + (DMA ? buf * BUF : 0) + (32 * t + r) * 128;
-                    const int key = r >> 1 & 7;
-                    const f32x4 e0 = *reinterpret_cast<const f32x4 *>(row + ((4 * h + 2 * j) ^ key) * 16);
-                    const f32x4 e1 = *reinterpret_cast<const f32x4 *>(row + ((4 * h + 2 * j + 1) ^ key) * 16);
+                const char *row = mine + (32 * t + r) * 128;
+                const int key = r >> 1 & 7;
+                const f32x4 e0 = *reinterpret_cast<const f32x4 *>(row + ((4 * h + 2 * j) ^ key) * 16);
+                const f32x4 e1 = *reinterpret_cast<const f32x4 *>(row + ((4 * h + 2 * j + 1) ^ key) * 16);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) { va[x] = e0[x]; va[4 + x] = e1[x]; }
-                    if (DMA && tail) {
-#pragma unroll
-                        for (int x = 0; x < 8; ++x) va[x] = l + x < A.L ? va[x] : 0.f;
-                    }
-                } else {
-                    const int n = n0 + 32 * t + r;
-                    const float *p = A.g + (b * A.N + (n < A.N ? n : A.N - 1)) * A.L + l;
-                    if (!tail) {
-                        const f32x4u e0 = *reinterpret_cast<const f32x4u *>(p), e1 = *reinterpret_cast<const f32x4u *>(p + 4);
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) { va[x] = e0[x]; va[4 + x] = e1[x]; }
-                    } else {
-#pragma unroll
-                        for (int x = 0; x < 8; ++x) va[x] = l + x < A.L ? p[x] : 0.f;
-                    }
-                }
+                for (int x = 0; x < 4; ++x) { va[x] = e0[x]; va[4 + x] = e1[x]; }
                 if (want_db) db[t] += ((va[0] + va[1]) + (va[2] + va[3])) + ((va[4] + va[5]) + (va[6] + va[7]));
 #pragma unroll
                 for (int x = 0; x < 8; ++x) va[x] = act8_flip(va[x], flip);
@@ -809,36 +852,132 @@ __global__ __launch_bounds__(256, RT * CT >= 8 ? 1 : 2) void p2n_act8_wgrad_kern
                     for (int c = 0; c < 6; ++c) acc[t][k] = MFMAB(a[t][act8_first(c)], w[k][act8_second(c)], acc[t][k]);
         }
     }
-    // the four waves' shares, added in order: a quarter of the tile's registers at a time, all waves at once
+    act8_wgrad_end<RT, CT>(A, reinterpret_cast<float *>(lds), acc, db, poison, flip, slice, n0, k0);
+}
+
+// 128 x 128 a wave, the only one on its SIMD: splitting the operands (8 to 9 vector instructions a product) has to go on while the matrix
+// core works, so the operands of the next 24 products are formed between the products of the present 24, and a quarter of the other
+// side's next ones with them (256 x 256 over 131,072 points with the join: 127 us, 141 with each 16 points' operands formed first).
+// g comes by LDS-DMA, a step ahead, codes into registers, two ahead.  Rows of g start on 16 bytes, L a multiple of 4.
+template <bool NORM>
+__global__ __launch_bounds__(256, 1) void p2n_act8_wgrad_wide_kernel(Act8Wgrad A) {
+    constexpr int BUF = 4096;                                                // floats: 128 rows of 32 points
+    __shared__ __attribute__((aligned(16))) float lds[8 * BUF];
+    static_assert(8 * BUF >= act8_join_floats(4, 4), "the shares pass through the same memory");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int r = lane & 31, h = lane >> 5;
+    const Act8Place at = act8_place(A);
+    const int n0 = at.tile / A.ntc * 128, k0 = at.tile % A.ntc * 128;
+    const Act8Turn turn(A);
+    const int first = at.slice * 4 + wave, stride = A.slices * 4;
+    const unsigned flip = (unsigned)(first & 1) << 31;
+    int krow[4];
+    float ga[4], be[4], poison[4], db[4];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) db[t] += __shfl_xor(db[t], 32);
-    float *const join = reinterpret_cast<float *>(lds);
-    float *part = A.part + (long)slice * (A.N * A.K + A.N);
-    constexpr int Q = RT * CT * 4;          // registers of a quarter
+    for (int i = 0; i < 4; ++i) {
+        const int k = k0 + 32 * i + r;
+        krow[i] = k < A.K ? k : A.K - 1;
+        ga[i] = NORM ? A.gamma[krow[i]] : 1.f;
+        be[i] = NORM ? A.beta[krow[i]] : 0.f;
+        poison[i] = db[i] = 0.f;
+    }
+    f32x16 acc[4][4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        __syncthreads();                    // the last rows (c = 0), the last quarter have been read
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int i = 0; i < Q; ++i) {
-            const int v = c * Q + i, tk = v / 16, e = v % 16;
-            join[(wave * Q + i) * 64 + lane] = act8_flip(acc[tk / CT][tk % CT][e], flip) + poison[tk % CT];
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][k][e] = 0.f;
+    // a step's rows in LDS as above; instruction i fills rows 8i .. 8i+7, lane -> row lane >> 3, slot lane & 7.  The resource ends with the
+    // cloud: rows past the last one read as zero, and so do pieces behind a row's last point, which are given an offset past any end.
+    float *const mine = lds + wave * 2 * BUF;
+    const int piece = (lane & 7) ^ (lane >> 4);
+    const unsigned drow = (unsigned)((lane >> 3) * A.L * 4);
+    const long eight = 8 * A.L;
+    auto dma = [&](Act8Step s, int buf) __attribute__((always_inline)) {
+        const long l0 = (long)s.q * 32;
+        const float *src = A.g + ((long)s.b * A.N + n0) * A.L + l0;
+        long size = ((long)(A.N - n0) * A.L - l0) * 4;
+        unsigned off[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) off[i] = l0 + 4 * (piece ^ (4 * i)) < A.L ? drow + 16u * (piece ^ (4 * i)) : 0xFFFFFFF0u;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(act8_rsrc(src, size), (act8_lds_t *)(mine + buf * BUF + i * 256), 16, off[i & 1], 0, 0, 0);
+            src += eight;
+            size -= eight * 4;
         }
-        if (c == 0 && h == 0)
+    };
+    bf16x8 a[2][3], w[2][4][3];
+    Act8Codes<4> now, ahead;                                                 // a step's codes, the next one's
+    auto rows_of = [&](int t, int j, int buf, bf16x8 (&o)[3], bool counts = true) __attribute__((always_inline)) {
+        float va[8];
+        const float *row = mine + buf * BUF + (32 * t + r) * 32;
+        const int key = r >> 1 & 7;
+        const f32x4 e0 = *reinterpret_cast<const f32x4 *>(row + ((4 * h + 2 * j) ^ key) * 4);
+        const f32x4 e1 = *reinterpret_cast<const f32x4 *>(row + ((4 * h + 2 * j + 1) ^ key) * 4);
 #pragma unroll
-            for (int t = 0; t < RT; ++t) join[RT * CT * 1024 + (wave * RT + t) * 32 + r] = db[t];
-        __syncthreads();
+        for (int x = 0; x < 4; ++x) { va[x] = e0[x]; va[4 + x] = e1[x]; }
+        const float sum = ((va[0] + va[1]) + (va[2] + va[3])) + ((va[4] + va[5]) + (va[6] + va[7]));
+        db[t] += counts ? sum : 0.f;
+        act8_split(va, o[0], o[1], o[2]);
+    };
+    auto operand_of = [&](const Act8Codes<4> &M, int t, int j, bf16x8 (&o)[3]) __attribute__((always_inline)) {
+        const float cs = ga[t] * M.s[t];
+        if (j == 0) poison[t] += cs * 0.f;
+        act8_operand<NORM>(M.q[t], j, cs, be[t], M.m[t] >> (8 * h), flip, o);
+    };
+    if (first < A.steps) {
+        Act8Step next = {first / turn.spc, first % turn.spc};                // behind the last step: the last one again
+        act8_codes<4, NORM>(A, next, h, krow, now);
+        dma(next, 0);
+        if (first + stride < A.steps) next = turn.after(next);
+        act8_codes<4, NORM>(A, next, h, krow, ahead);
+        __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < Q / 4; ++i) {
-            const int o = i * 256 + threadIdx.x, v = c * Q + o / 64, tk = v / 16, e = v % 16, ln = o & 63;
-            const int row = n0 + 32 * (tk / CT) + 8 * (e >> 2) + 4 * (ln >> 5) + (e & 3), col = k0 + 32 * (tk % CT) + (ln & 31);
-            const float sum = ((join[o] + join[o + Q * 64]) + join[o + 2 * Q * 64]) + join[o + 3 * Q * 64];
-            if (row < A.N && col < A.K) part[(long)row * A.K + col] = sum;
-        }
-        if (c == 0 && want_db && threadIdx.x < 32 * RT && n0 + (int)threadIdx.x < A.N) {
-            const float *d = join + RT * CT * 1024 + threadIdx.x;
-            part[(long)A.N * A.K + n0 + threadIdx.x] = ((d[0] + d[32 * RT]) + d[64 * RT]) + d[96 * RT];
+        for (int t = 0; t < 4; ++t) operand_of(now, t, 0, w[0][t]);
+        rows_of(0, 0, 0, a[0]);
+        int buf = 0;
+#pragma unroll 1
+        for (int s = first; s < A.steps; s += stride) {
+            const bool more = s + stride < A.steps;
+            dma(next, buf ^ 1);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    if (j == 1 && t == 3) {
+                        __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));    // the next step's rows have arrived
+                        asm volatile("" ::: "memory");
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    operand_of(j ? ahead : now, t, j ^ 1, w[j ^ 1][t]);
+                    if (t < 3) rows_of(t + 1, j, buf, a[(t + 1) & 1]);
+                    else if (j == 0) rows_of(0, 1, buf, a[0]);
+                    else rows_of(0, 0, buf ^ 1, a[0], more);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int c = 0; c < 6; ++c) acc[t][k] = MFMAB(a[t & 1][act8_first(c)], w[j][k][act8_second(c)], acc[t][k]);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);       // LDS reads
+#pragma unroll
+                    for (int i = 0; i < 24; ++i) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // a product
+                        __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);   // vector instructions
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            now = ahead;
+            if (s + 2 * stride < A.steps) next = turn.after(next);
+            act8_codes<4, NORM>(A, next, h, krow, ahead);
+            buf ^= 1;
         }
     }
+    __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));                        // nothing may be on its way into LDS when the shares go there
+    asm volatile("" ::: "memory");
+    act8_wgrad_end<4, 4>(A, lds, acc, db, poison, flip, at.slice, n0, k0);
 }
 
 // out[i] = sum over slices, in a fixed order: 32 results a workgroup, the slices dealt to 32 rows of threads.  The first n0 results are
@@ -933,6 +1072,12 @@ int act8_ksteps(int k, int ct) {
 }
 int act8_padded(int rows, int ct) { return ((rows + 31) / 32 + ct - 1) / ct * ct; }
 
+void act8_wgrad_tiles(Act8 &a, int rt, int ct) {
+    a.RT = rt; a.CT = ct;
+    a.ntc = (a.K + 32 * ct - 1) / (32 * ct);
+    a.nt = ((a.N ? a.N : 1) + 32 * rt - 1) / (32 * rt) * a.ntc;
+}
+
 int act8_init(Act8 &a, const char *fn, int B, int K, long L, int N) {
     P2N_REQUIRE(B >= 1 && L >= 1 && L <= (1L << 24), "%s: bad shape B=%d L=%ld (1 to 2^24 columns a cloud)", fn, B, L);
     P2N_REQUIRE(K >= 1 && K <= ACT8_MAX_C && N >= 0 && N <= ACT8_MAX_C, "%s: %d or %d channels, not in [1,%d]", fn, K, N, ACT8_MAX_C);
@@ -950,13 +1095,11 @@ int act8_init(Act8 &a, const char *fn, int B, int K, long L, int N) {
     a.per = (blocks + s - 1) / s;
     a.S = (int)((blocks + a.per - 1) / a.per);
     // a wave makes up to 64 x 64, two of them on a SIMD; 128 x 128 (which fills the registers alone, and splits each operand half as
-    // often) where both sides are that long and there are points enough for such waves: 256 x 256 at 131,072 points 140 us against
+    // often) where both sides are that long and there are points enough for such waves: 256 x 256 at 131,072 points 127 us against
     // 155, 64 x 128 at 262,144 points 70 against 55 with 128 rows, 256 x 384 at 8,192 points 56 against 19
     a.wsteps = (long)B * a.NB * 4;
-    const bool big = N >= 128 && K >= 128 && a.wsteps >= 2048;
-    a.RT = big ? 4 : N <= 32 ? 1 : 2; a.CT = big ? 4 : K <= 32 ? 1 : 2;
-    a.ntc = (K + 32 * a.CT - 1) / (32 * a.CT);
-    a.nt = ((N ? N : 1) + 32 * a.RT - 1) / (32 * a.RT) * a.ntc;
+    const bool big = N >= 128 && K >= 128 && a.wsteps >= 2048 && L % 4 == 0;
+    act8_wgrad_tiles(a, big ? 4 : N <= 32 ? 1 : 2, big ? 4 : K <= 32 ? 1 : 2);
     const long wgs = a.RT * a.CT >= 8 ? 256 : a.RT * a.CT >= 4 ? 512 : a.RT * a.CT == 2 ? 768 : 1024;
     long sl = wgs / a.nt > 1 ? wgs / a.nt : 1;
     if (sl > (a.wsteps + 7) / 8) sl = (a.wsteps + 7) / 8;
@@ -1029,18 +1172,14 @@ int act8_launch_gemm(const Act8Gemm &g, long groups, hipStream_t s) {
     return act8_launch_gemm_tab<IN, EPI, 512>(g, groups, s);
 }
 
-template <int RT, int CT, bool DMA, bool NORM>
-void act8_launch_wgrad_as(const Act8 &a, const Act8Wgrad &w, hipStream_t s) {
-    hipLaunchKernelGGL((p2n_act8_wgrad_kernel<RT, CT, DMA, NORM>), dim3((unsigned)(a.nt * a.slices)), dim3(256), 0, s, w);
-}
 template <bool NORM>
 int act8_launch_wgrad(const Act8 &a, const Act8Wgrad &w, hipStream_t s) {
-    if (a.RT == 4 && a.L % 4 == 0 && ((uintptr_t)w.g & 15) == 0) act8_launch_wgrad_as<4, 4, true, NORM>(a, w, s);
-    else if (a.RT == 4) act8_launch_wgrad_as<4, 4, false, NORM>(a, w, s);
-    else if (a.RT == 2 && a.CT == 2) act8_launch_wgrad_as<2, 2, false, NORM>(a, w, s);
-    else if (a.RT == 2) act8_launch_wgrad_as<2, 1, false, NORM>(a, w, s);
-    else if (a.CT == 2) act8_launch_wgrad_as<1, 2, false, NORM>(a, w, s);
-    else act8_launch_wgrad_as<1, 1, false, NORM>(a, w, s);
+    const dim3 grid((unsigned)(a.nt * a.slices)), blk(256);
+    if (a.RT == 4) hipLaunchKernelGGL(p2n_act8_wgrad_wide_kernel<NORM>, grid, blk, 0, s, w);
+    else if (a.RT == 2 && a.CT == 2) hipLaunchKernelGGL((p2n_act8_wgrad_kernel<2, 2, NORM>), grid, blk, 0, s, w);
+    else if (a.RT == 2) hipLaunchKernelGGL((p2n_act8_wgrad_kernel<2, 1, NORM>), grid, blk, 0, s, w);
+    else if (a.CT == 2) hipLaunchKernelGGL((p2n_act8_wgrad_kernel<1, 2, NORM>), grid, blk, 0, s, w);
+    else hipLaunchKernelGGL((p2n_act8_wgrad_kernel<1, 1, NORM>), grid, blk, 0, s, w);
     P2N_CHECK_HIP(hipGetLastError());
     return P2N_OK;
 }
@@ -1138,6 +1277,7 @@ extern "C" int p2n_act8_backward(const float *g, int B, int K, long L, const flo
     TRY(act8_init(a, fn, B, K, L, N));
     P2N_REQUIRE(g && W && (!gamma || beta), "%s: null pointer", fn);
     P2N_REQUIRE(!gamma || dx || !(dgamma || dbeta), "%s: the norm's gradients need dx, through which they are formed", fn);
+    if (a.RT == 4 && ((uintptr_t)g & 15) != 0) act8_wgrad_tiles(a, 2, 2);      // the wide kernel takes 16 bytes at a time
     const Act8Kept k = act8_kept(B, K, L, gamma != nullptr);
     TRY(act8_space_check(fn, kept_, kept_bytes, k.total, "kept buffer"));
     TRY(act8_space_check(fn, workspace, workspace_bytes, bwd_space(a, nullptr).total, "workspace"));
