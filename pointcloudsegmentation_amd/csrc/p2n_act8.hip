@@ -145,22 +145,29 @@ struct Act8Split {
     __bf16 *img;
     int rows, cols, trans, CTP, KS;
 };
+__device__ __forceinline__ void act8_split_rounded(const float (&v)[8], bf16x8 &h, bf16x8 &m, bf16x8 &l) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        h[j] = (__bf16)v[j];
+        const float r = v[j] - (float)h[j];
+        m[j] = (__bf16)r;
+        l[j] = (__bf16)(r - (float)m[j]);
+    }
+}
 __device__ __forceinline__ void act8_split_weights(const Act8Split &A, long i) {      // i: (fragment without part, lane)
     const int lane = (int)(i & 63);
     const long f = i >> 6;
     if (f >= (long)A.CTP * A.KS) return;
     const int ct = (int)(f % A.CTP), ks = (int)(f / A.CTP);
     const int row = 32 * ct + (lane & 31), k0 = 16 * ks + 8 * (lane >> 5);
-    bf16x8 h, m, l;
+    float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const int k = k0 + j;
-        const float v = row < A.rows && k < A.cols ? (A.trans ? A.W[(long)k * A.rows + row] : A.W[(long)row * A.cols + k]) : 0.f;
-        h[j] = (__bf16)v;
-        const float r = v - (float)h[j];
-        m[j] = (__bf16)r;
-        l[j] = (__bf16)(r - (float)m[j]);
+        v[j] = row < A.rows && k < A.cols ? (A.trans ? A.W[(long)k * A.rows + row] : A.W[(long)row * A.cols + k]) : 0.f;
     }
+    bf16x8 h, m, l;
+    act8_split_rounded(v, h, m, l);
     bf16x8 *d = reinterpret_cast<bf16x8 *>(A.img) + f * 3 * 64 + lane;
     d[0] = h; d[64] = m; d[128] = l;
 }
@@ -633,9 +640,9 @@ struct Act8Step {
 };
 struct Act8Turn {
     int b, q, spc;                      // clouds, pieces between a wave's steps; steps of a cloud
-    __device__ __forceinline__ Act8Turn(const Act8Wgrad &A) : spc((int)(4 * A.NB)) {
-        b = A.slices * 4 / spc;
-        q = A.slices * 4 % spc;
+    __device__ __forceinline__ Act8Turn(const Act8Wgrad &A, int waves) : spc((int)(4 * A.NB)) {      // waves that share a tile
+        b = waves / spc;
+        q = waves % spc;
     }
     __device__ __forceinline__ Act8Step after(Act8Step s) const {
         s.b += b;
@@ -683,11 +690,11 @@ __device__ __forceinline__ void act8_operand(const i32x4 &q, int j, float cs, fl
     act8_split(v, w[0], w[1], w[2]);
 }
 
-// the four waves' shares, added in order: a quarter of the tile's registers at a time, all waves at once
+// the shares of four waves, added in order: a quarter of the tile's registers at a time, all waves at once
 template <int RT, int CT>
 __device__ __forceinline__ void act8_wgrad_end(const Act8Wgrad &A, float *join, const f32x16 (&acc)[RT][CT], float (&db)[RT], const float (&poison)[CT],
                                                unsigned flip, int slice, int n0, int k0) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 31, h = lane >> 5;
 #pragma unroll
     for (int t = 0; t < RT; ++t) db[t] += __shfl_xor(db[t], 32);
     float *part = A.part + (long)slice * (A.N * A.K + A.N);
@@ -706,20 +713,20 @@ __device__ __forceinline__ void act8_wgrad_end(const Act8Wgrad &A, float *join, 
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < Q / 4; ++i) {
-            const int o = i * 256 + threadIdx.x, v = c * Q + o / 64, tk = v / 16, e = v % 16, ln = o & 63;
+            const int o = i * 256 + tid, v = c * Q + o / 64, tk = v / 16, e = v % 16, ln = o & 63;
             const int row = n0 + 32 * (tk / CT) + 8 * (e >> 2) + 4 * (ln >> 5) + (e & 3), col = k0 + 32 * (tk % CT) + (ln & 31);
             const float sum = ((join[o] + join[o + Q * 64]) + join[o + 2 * Q * 64]) + join[o + 3 * Q * 64];
             if (row < A.N && col < A.K) part[(long)row * A.K + col] = sum;
         }
-        if (c == 0 && k0 == 0 && threadIdx.x < 32 * RT && n0 + (int)threadIdx.x < A.N) {
-            const float *d = join + RT * CT * 1024 + threadIdx.x;
-            part[(long)A.N * A.K + n0 + threadIdx.x] = ((d[0] + d[32 * RT]) + d[64 * RT]) + d[96 * RT];
+        if (c == 0 && k0 == 0 && tid < 32 * RT && n0 + tid < A.N) {
+            const float *d = join + RT * CT * 1024 + tid;
+            part[(long)A.N * A.K + n0 + tid] = ((d[0] + d[32 * RT]) + d[64 * RT]) + d[96 * RT];
         }
     }
 }
 constexpr int act8_join_floats(int rt, int ct) { return rt * ct * 1024 + 4 * 32 * rt; }
 
-// up to 64 x 64 a wave, two waves or more on a SIMD; the next step's g and codes wait in registers
+// up to 64 x 64 a wave, two waves or more on a SIMD; the next step's g and codes wait in registers (for more than 64 channels on a side)
 template <int RT, int CT, bool NORM>
 __global__ __launch_bounds__(256, 2) void p2n_act8_wgrad_kernel(Act8Wgrad A) {
     constexpr int BUF = RT * 4096, JOIN = act8_join_floats(RT, CT) * 4;      // bytes; 32 RT rows of 32 points
@@ -729,8 +736,9 @@ __global__ __launch_bounds__(256, 2) void p2n_act8_wgrad_kernel(Act8Wgrad A) {
     const Act8Place at = act8_place(A);
     const int tile = at.tile, slice = at.slice;
     const int n0 = tile / A.ntc * 32 * RT, k0 = tile % A.ntc * 32 * CT;
-    const Act8Turn take(A);
-    const int turn = A.slices * 4, first = slice * 4 + wave;
+    const int turn = A.slices * 4;
+    const Act8Turn take(A, turn);
+    const int first = slice * 4 + wave;
     const unsigned flip = (unsigned)((slice * 4 + wave) & 1) << 31;       // every other share with its sign turned round (act8_flip)
     const bool want_db = k0 == 0;
     int krow[CT];
@@ -868,8 +876,8 @@ __global__ __launch_bounds__(256, 1) void p2n_act8_wgrad_wide_kernel(Act8Wgrad A
     const int r = lane & 31, h = lane >> 5;
     const Act8Place at = act8_place(A);
     const int n0 = at.tile / A.ntc * 128, k0 = at.tile % A.ntc * 128;
-    const Act8Turn turn(A);
     const int first = at.slice * 4 + wave, stride = A.slices * 4;
+    const Act8Turn turn(A, stride);
     const unsigned flip = (unsigned)(first & 1) << 31;
     int krow[4];
     float ga[4], be[4], poison[4], db[4];
@@ -980,6 +988,192 @@ __global__ __launch_bounds__(256, 1) void p2n_act8_wgrad_wide_kernel(Act8Wgrad A
     act8_wgrad_end<4, 4>(A, lds, acc, db, poison, flip, at.slice, n0, k0);
 }
 
+// Few channels (N <= 64, K <= 64): both products of the backward pass are bound by reading g, so one kernel makes them.  A wave keeps
+// 32 RT x 32 of dW as above, and for the same 32 points W^T . g from the same piece of LDS (lane = point, its eight values of a
+// k-step from eight rows), the fragments of W^T in LDS too.  dy goes to dx's place, its two sums stay in registers to the end.
+// Either product alone comes from here too, so that it does not depend on what else is asked for.
+// 32 -> 64 over 1,048,576 points: 118 us against 93 + 104 for the two, 64 -> 64 over 524,288: 109 against 52 + 78.
+struct Act8Both {
+    Act8Wgrad w;
+    const float *W;
+    float *dx;             // (B, K, L): dy
+    float *part;           // NORM: {sum dy, sum dy*uh}[K][2][waves that share a tile]
+};
+template <int RT, bool NORM>
+__global__ __launch_bounds__(256, 2) void p2n_act8_both_kernel(Act8Both B) {
+    const Act8Wgrad &A = B.w;
+    constexpr int BUF = RT * 4096;                                           // bytes; 32 RT rows of 32 points
+    __shared__ __attribute__((aligned(16))) char lds[4 * BUF];
+    __shared__ __attribute__((aligned(16))) char wt[RT * 6144];              // k-step, part: 1 KiB
+    __shared__ __attribute__((aligned(16))) unsigned kept[NORM ? 4 : 1][320];       // the wave's: scales of its 32 channels, bits, codes (32 points a row)
+    static_assert(4 * BUF >= act8_join_floats(RT, 1) * 4, "the shares pass through the same memory");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int r = lane & 31, h = lane >> 5;
+    const Act8Place at = act8_place(A);
+    const int k0 = at.tile * 32, turn = A.slices * 4, first = at.slice * 4 + wave;
+    const Act8Turn take(A, turn);
+    const unsigned flip = (unsigned)(first & 1) << 31;                       // every other wave has g with its sign turned round (act8_flip)
+    for (int ks = wave; ks < 2 * RT; ks += 4) {
+        const int k = k0 + r, n = 16 * ks + 8 * h;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = n + i < A.N && k < A.K ? B.W[(long)(n + i) * A.K + k] : 0.f;
+        bf16x8 *d = reinterpret_cast<bf16x8 *>(wt + ks * 3072) + lane;
+        act8_split_rounded(v, d[0], d[64], d[128]);
+    }
+    __syncthreads();
+    const int krow = k0 + r < A.K ? k0 + r : A.K - 1;
+    const float ga = NORM ? A.gamma[krow] : 1.f, be = NORM ? A.beta[krow] : 0.f;
+    float poison[1] = {0.f}, db[RT], s1[16], s2[16];
+    f32x16 acc[RT][1];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        db[i] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][0][e] = 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s1[e] = s2[e] = 0.f;
+    char *const mine = lds + wave * BUF;
+    const int drow = lane >> 3, slot = (lane & 7) ^ (lane >> 4);
+    int qn[4];
+    float sn;
+    unsigned mn;
+    auto meta = [&](Act8Step s) __attribute__((always_inline)) {
+        const long blk = s.b * A.NB + (s.q >> 2);
+        const int w = s.q & 3;
+        const i32x4 q = *reinterpret_cast<const i32x4 *>(A.codes + (blk * A.K + krow) * ACT8_GROUP + 32 * w + 16 * h);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) qn[x] = q[x];
+        sn = A.scale[blk * A.K4 + krow];
+        mn = NORM ? A.bits[(blk * 4 + w) * A.K4 + krow] : 0u;
+    };
+    f32x4 vn[RT * 4];
+    const bool full = A.N == 32 * RT;
+    auto rows = [&](Act8Step s) __attribute__((always_inline)) {
+        const long b = s.b, l0 = (long)s.q * 32, l = l0 + 4 * (lane & 7);
+        const bool whole = full && l0 + 32 <= A.L;
+#pragma unroll
+        for (int i = 0; i < RT * 4; ++i) {
+            const int n = 8 * i + drow;
+            const float *p = A.g + (b * A.N + (n < A.N ? n : A.N - 1)) * A.L + l;
+            if (whole) vn[i] = *reinterpret_cast<const f32x4u *>(p);
+            else
+#pragma unroll
+                for (int x = 0; x < 4; ++x) vn[i][x] = n < A.N && l + x < A.L ? p[x] : 0.f;
+        }
+    };
+    Act8Step step = {first / take.spc, first % take.spc};
+    if (first < A.steps) {
+        rows(step);
+        meta(step);
+    }
+#pragma unroll 1
+    for (int s = first; s < A.steps; s += turn) {
+#pragma unroll
+        for (int i = 0; i < RT * 4; ++i) {
+            f32x4 v = vn[i];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[x] = act8_flip(v[x], flip);
+            *reinterpret_cast<f32x4 *>(mine + i * 1024 + drow * 128 + (slot ^ (4 * (i & 1))) * 16) = v;
+        }
+        int q[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) q[x] = qn[x];
+        const float cs = ga * sn;
+        poison[0] += cs * 0.f;                              // NaN with a NaN scale
+        const unsigned mb = mn >> (8 * h);                  // points 16h .. 16h+15: bits 8h .. of either half-word
+        if (NORM) {
+            *reinterpret_cast<i32x4 *>(&kept[wave][64 + 8 * r + 4 * h]) = i32x4{q[0], q[1], q[2], q[3]};
+            kept[wave][lane] = h ? mn : __float_as_uint(sn);
+        }
+        const Act8Step now = step;
+        step = take.after(step);
+        if (s + turn < A.steps) {
+            rows(step);
+            meta(step);
+        }
+        if (A.part) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                bf16x8 w[3];
+                act8_operand<NORM>(i32x4{q[0], q[1], q[2], q[3]}, j, cs, be, mb, 0u, w);
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    float va[8];
+                    const char *row = mine + (32 * t + r) * 128;
+                    const int key = r >> 1 & 7;
+                    const f32x4 e0 = *reinterpret_cast<const f32x4 *>(row + ((4 * h + 2 * j) ^ key) * 16);
+                    const f32x4 e1 = *reinterpret_cast<const f32x4 *>(row + ((4 * h + 2 * j + 1) ^ key) * 16);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) { va[x] = e0[x]; va[4 + x] = e1[x]; }
+                    if (k0 == 0) db[t] += ((va[0] + va[1]) + (va[2] + va[3])) + ((va[4] + va[5]) + (va[6] + va[7]));
+                    bf16x8 a[3];
+                    act8_split(va, a[0], a[1], a[2]);
+#pragma unroll
+                    for (int c = 0; c < 6; ++c) acc[t][0] = MFMAB(a[act8_first(c)], w[act8_second(c)], acc[t][0]);
+                    if (t & 1) __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (!B.dx) continue;
+        f32x16 da;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) da[e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < 2 * RT; ++ks) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                x[i] = *reinterpret_cast<const float *>(mine + (16 * ks + 8 * h + i) * 128 + ((r >> 2) ^ (4 * h + (i >> 1))) * 16 + (r & 3) * 4);
+            bf16x8 xp[3];
+            act8_split(x, xp[0], xp[1], xp[2]);
+            const bf16x8 *f = reinterpret_cast<const bf16x8 *>(wt + ks * 3072) + lane;
+#pragma unroll
+            for (int c = 0; c < 6; ++c) da = MFMAB(f[64 * act8_first(c)], xp[act8_second(c)], da);
+            if (ks & 1) __builtin_amdgcn_sched_barrier(0);
+        }
+        const long l = (long)now.q * 32 + r;
+        const __amdgpu_buffer_rsrc_t ro = act8_rsrc(B.dx + ((long)now.b * A.K + k0) * A.L, (long)(A.K - k0) * A.L * 4);    // channels past K are not stored
+        const unsigned oo = (unsigned)((4 * h * A.L + l) * 4);
+        const int bit = (r >> 1) + 16 * (r & 1);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            i32x4 sc = {0, 0, 0, 0}, on = {0, 0, 0, 0};
+            if (NORM) {
+                sc = *reinterpret_cast<const i32x4 *>(&kept[wave][8 * g + 4 * h]);
+                on = *reinterpret_cast<const i32x4 *>(&kept[wave][32 + 8 * g + 4 * h]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int e = 4 * g + j;
+                float dy = act8_flip(da[e], flip);
+                if (NORM) {
+                    const bool above = on[j] >> bit & 1;
+                    const int code = reinterpret_cast<const signed char *>(&kept[wave][64 + 8 * (8 * g + 4 * h + j)])[r];
+                    dy = above ? dy : 0.f;
+                    s1[e] += dy;
+                    s2[e] += above ? dy * ((float)code * __int_as_float(sc[j])) : 0.f;
+                }
+                if (l < A.L) __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(dy), ro, oo + (unsigned)((8 * g + j) * A.L * 4), 0, 0);
+            }
+        }
+    }
+    if (NORM && B.dx) {
+        const float t1 = act8_half_sum(s1, lane), t2 = act8_half_sum(s2, lane);
+        const int i = lane & 15, k = k0 + 8 * (i >> 2) + 4 * h + (i & 3);
+        if (!(lane & 16) && k < A.K) {
+            B.part[((long)k * 2) * turn + first] = t1;
+            B.part[((long)k * 2 + 1) * turn + first] = t2;
+        }
+    }
+    if (!A.part) return;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) db[t] = act8_flip(db[t], flip);
+    act8_wgrad_end<RT, 1>(A, reinterpret_cast<float *>(lds), acc, db, poison, flip, at.slice, 0, k0);
+}
+
 // out[i] = sum over slices, in a fixed order: 32 results a workgroup, the slices dealt to 32 rows of threads.  The first n0 results are
 // dW, the others db (either may be NULL).  The first split_wgs workgroups make the image of W^T.
 __global__ __launch_bounds__(1024) void p2n_act8_join_kernel(const float *__restrict__ part, long n, long n0, int slices, float *__restrict__ dW, float *__restrict__ db,
@@ -1057,6 +1251,7 @@ struct Act8 {
     long per;
     int RT, CT, ntc, nt, slices;     // weight gradient: 32-row tiles of a wave, tiles, slices of the points
     long wsteps;
+    int both, waves;                 // weight and data gradient in one kernel: 32-row tiles of a wave (0: no), waves that share a tile
 };
 
 // Channel tiles of a workgroup: all of them (the points are then read once), fewer where there are so few blocks of points that compute
@@ -1104,6 +1299,14 @@ int act8_init(Act8 &a, const char *fn, int B, int K, long L, int N) {
     long sl = wgs / a.nt > 1 ? wgs / a.nt : 1;
     if (sl > (a.wsteps + 7) / 8) sl = (a.wsteps + 7) / 8;
     a.slices = (int)sl;
+    // both gradients in one kernel, two workgroups of four waves a compute unit, up to 64 x 64: beyond, a wave's sums and rows leave no
+    // registers to overlap with (64 -> 128 over 262,144 points: 126 us against 46 + 49)
+    a.both = N < 1 || N > 64 || K > 64 ? 0 : N <= 32 ? 1 : 2;
+    a.waves = 0;
+    if (a.both) {
+        const long most = 2048 / ((K + 31) / 32);
+        a.waves = (int)((most < a.wsteps ? most : a.wsteps) + 3) / 4 * 4;
+    }
     return P2N_OK;
 }
 
@@ -1143,11 +1346,11 @@ struct BwdSpace {
 BwdSpace bwd_space(const Act8 &a, char *base) {
     Carve c{base, 0};
     BwdSpace f;
-    f.nparts = a.N ? (long)a.B * a.NB : a.S;
+    f.nparts = a.both ? a.waves : a.N ? (long)a.B * a.NB : a.S;
     f.part = c.take<float>((size_t)2 * a.K * f.nparts);
     f.tab = c.take<float>((size_t)3 * a.K);
-    f.img = c.take<__bf16>((size_t)a.CTb * a.KSb * 1536);
-    f.wpart = c.take<float>((size_t)a.slices * (a.N * (size_t)a.K + a.N));
+    f.img = c.take<__bf16>(a.both ? 0 : (size_t)a.CTb * a.KSb * 1536);
+    f.wpart = c.take<float>((size_t)(a.both ? a.waves / 4 : a.slices) * (a.N * (size_t)a.K + a.N));
     f.total = c.off;
     return f;
 }
@@ -1178,8 +1381,17 @@ int act8_launch_wgrad(const Act8 &a, const Act8Wgrad &w, hipStream_t s) {
     if (a.RT == 4) hipLaunchKernelGGL(p2n_act8_wgrad_wide_kernel<NORM>, grid, blk, 0, s, w);
     else if (a.RT == 2 && a.CT == 2) hipLaunchKernelGGL((p2n_act8_wgrad_kernel<2, 2, NORM>), grid, blk, 0, s, w);
     else if (a.RT == 2) hipLaunchKernelGGL((p2n_act8_wgrad_kernel<2, 1, NORM>), grid, blk, 0, s, w);
-    else if (a.CT == 2) hipLaunchKernelGGL((p2n_act8_wgrad_kernel<1, 2, NORM>), grid, blk, 0, s, w);
-    else hipLaunchKernelGGL((p2n_act8_wgrad_kernel<1, 1, NORM>), grid, blk, 0, s, w);
+    else hipLaunchKernelGGL((p2n_act8_wgrad_kernel<1, 2, NORM>), grid, blk, 0, s, w);      // N <= 32 means K > 64 here
+    P2N_CHECK_HIP(hipGetLastError());
+    return P2N_OK;
+}
+
+template <bool NORM>
+int act8_launch_both(const Act8 &a, Act8Both &b, hipStream_t s) {
+    b.w.slices = a.waves / 4;
+    const dim3 grid((unsigned)((a.K + 31) / 32 * b.w.slices)), blk(256);
+    if (a.both == 2) hipLaunchKernelGGL((p2n_act8_both_kernel<2, NORM>), grid, blk, 0, s, b);
+    else hipLaunchKernelGGL((p2n_act8_both_kernel<1, NORM>), grid, blk, 0, s, b);
     P2N_CHECK_HIP(hipGetLastError());
     return P2N_OK;
 }
@@ -1290,32 +1502,38 @@ extern "C" int p2n_act8_backward(const float *g, int B, int K, long L, const flo
     const int ps = p2n_prof_begin(P2N_K_ACT8_BWD, s);
     const long groups = (long)B * a.NB;
     const int K4 = (K + 3) / 4 * 4;
-    if (dW || db) {
-        Act8Wgrad w = {};
-        w.g = g; w.codes = codes; w.scale = scale; w.bits = bits; w.gamma = gamma; w.beta = beta; w.part = f.wpart;
-        w.L = L; w.NB = a.NB; w.steps = (int)a.wsteps; w.N = N; w.K = K; w.K4 = K4; w.ntc = a.ntc; w.slices = a.slices;
-        TRY(gamma ? act8_launch_wgrad<true>(a, w, s) : act8_launch_wgrad<false>(a, w, s));
+    const bool want = dW || db;
+    if (want || (dx && a.both)) {
+        Act8Both w = {};
+        w.w.g = g; w.w.codes = codes; w.w.scale = scale; w.w.bits = bits; w.w.gamma = gamma; w.w.beta = beta; w.w.part = want ? f.wpart : nullptr;
+        w.w.L = L; w.w.NB = a.NB; w.w.steps = (int)a.wsteps; w.w.N = N; w.w.K = K; w.w.K4 = K4; w.w.ntc = a.ntc; w.w.slices = a.slices;
+        w.W = W; w.dx = dx; w.part = f.part;
+        if (a.both) {
+            TRY(gamma ? act8_launch_both<true>(a, w, s) : act8_launch_both<false>(a, w, s));
+        } else {
+            TRY(gamma ? act8_launch_wgrad<true>(a, w.w, s) : act8_launch_wgrad<false>(a, w.w, s));
+        }
     }
-    if (dW || db || dx) {
-        const Act8Split split = dx ? Act8Split{W, f.img, K, N, 1, a.CTb, a.KSb} : Act8Split{};
-        const long n = dW || db ? (long)N * K + N : 0;
+    if (want || (dx && !a.both)) {
+        const Act8Split split = dx && !a.both ? Act8Split{W, f.img, K, N, 1, a.CTb, a.KSb} : Act8Split{};
+        const long n = want ? (long)N * K + N : 0;
         const int split_wgs = (split.CTP * split.KS + 15) / 16;
-        hipLaunchKernelGGL(p2n_act8_join_kernel, dim3((unsigned)(split_wgs + (n + 31) / 32)), dim3(1024), 0, s, f.wpart, n, (long)N * K, a.slices, dW, db, split, split_wgs);
+        hipLaunchKernelGGL(p2n_act8_join_kernel, dim3((unsigned)(split_wgs + (n + 31) / 32)), dim3(1024), 0, s, f.wpart, n, (long)N * K, a.both ? a.waves / 4 : a.slices,
+                           dW, db, split, split_wgs);
         P2N_CHECK_HIP(hipGetLastError());
     }
-    if (dx) {
+    if (dx && !a.both) {
         Act8Gemm q = {};
         q.x = g; q.img = f.img; q.out = dx; q.codes = codes; q.scale = scale; q.bits = bits; q.part = f.part; q.L = L; q.NB = a.NB;
         q.K = N; q.Kpad = (N + 63) / 64 * 64; q.KS = a.KSb; q.CTP = a.CTb; q.rows = K; q.rows4 = K4;
-        if (gamma) {
-            TRY((act8_launch_gemm<ACT8_PLAIN, ACT8_DY>(q, groups, s)));
-            hipLaunchKernelGGL(p2n_act8_sums_kernel, dim3(K), dim3(256), 0, s, f.part, f.nparts, K, (double)B * L, gamma, stat, frozen ? 1 : 0, dgamma, dbeta, f.tab);
-            P2N_CHECK_HIP(hipGetLastError());
-            hipLaunchKernelGGL(p2n_act8_dx_kernel, dim3((unsigned)groups, (unsigned)((K + 31) / 32)), dim3(256), 0, s, dx, K, K4, L, a.NB, f.tab, codes, scale);
-            P2N_CHECK_HIP(hipGetLastError());
-        } else {
-            TRY((act8_launch_gemm<ACT8_PLAIN, ACT8_OUT>(q, groups, s)));
-        }
+        if (gamma) TRY((act8_launch_gemm<ACT8_PLAIN, ACT8_DY>(q, groups, s)));
+        else TRY((act8_launch_gemm<ACT8_PLAIN, ACT8_OUT>(q, groups, s)));
+    }
+    if (dx && gamma) {
+        hipLaunchKernelGGL(p2n_act8_sums_kernel, dim3(K), dim3(256), 0, s, f.part, f.nparts, K, (double)B * L, gamma, stat, frozen ? 1 : 0, dgamma, dbeta, f.tab);
+        P2N_CHECK_HIP(hipGetLastError());
+        hipLaunchKernelGGL(p2n_act8_dx_kernel, dim3((unsigned)groups, (unsigned)((K + 31) / 32)), dim3(256), 0, s, dx, K, K4, L, a.NB, f.tab, codes, scale);
+        P2N_CHECK_HIP(hipGetLastError());
     }
     p2n_prof_end(ps, s);
     return P2N_OK;
