@@ -470,27 +470,24 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : TABK <= 512 ? 2 : 1) void p2n_ac
     if (c < nchunk) body(c, raw[0]);
     __builtin_amdgcn_s_waitcnt(7 << 4);               // nothing may be on its way into LDS when the workgroup ends
     asm volatile("" ::: "memory");
-    // what was kept of a channel tile: codes, bits, scales; one tile ahead of its use
+    // what was kept of a channel tile, one tile ahead of its use: a lane takes 16 codes of a channel and its scale or its bits, and they turn
+    // round in LDS (the weights' place, the wave's own 1280 bytes): scales, bits, codes by channel.  A lane reading its own point's bytes
+    // from memory keeps the return path busy for as long as the products take.
     struct Meta {
-        int q[16];
-        i32x4 w[4];
-        f32x4 s[4];
+        i32x4 q;
+        unsigned k;
     } meta[2];
     auto fetch_meta = [&](Meta &M, int ct) __attribute__((always_inline)) {
         const long blk = blockIdx.x;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int row = 32 * (ct0 + ct) + 8 * q + 4 * h, c4 = row < A.rows4 ? row : A.rows4 - 4;
-            M.w[q] = *reinterpret_cast<const i32x4 *>(A.bits + (blk * 4 + wave) * A.rows4 + c4);
-            M.s[q] = *reinterpret_cast<const f32x4 *>(A.scale + blk * A.rows4 + c4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int c = row + j < A.rows ? row + j : A.rows - 1;
-                M.q[4 * q + j] = A.codes[(blk * A.rows + c) * ACT8_GROUP + 32 * wave + p];
-            }
-        }
+        const int row = 32 * (ct0 + ct) + p, c = row < A.rows ? row : A.rows - 1;
+        M.q = *reinterpret_cast<const i32x4 *>(A.codes + (blk * A.rows + c) * ACT8_GROUP + 32 * wave + 16 * h);
+        M.k = h ? A.bits[(blk * 4 + wave) * A.rows4 + c] : reinterpret_cast<const unsigned *>(A.scale)[blk * A.rows4 + c];
     };
-    if (EPI == ACT8_DY) fetch_meta(meta[0], 0);
+    unsigned *const kept = reinterpret_cast<unsigned *>(wbuf[0]) + wave * 320;
+    if (EPI == ACT8_DY) {
+        fetch_meta(meta[0], 0);
+        __syncthreads();                              // every wave has read its last weights
+    }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         const int r0 = 32 * (ct0 + ct);
@@ -503,15 +500,22 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : TABK <= 512 ? 2 : 1) void p2n_ac
             float s1[16], s2[16];
             const int bit = (p >> 1) + 16 * (p & 1);
             const Meta &M = meta[ct & 1];
+            kept[lane] = M.k;
+            *reinterpret_cast<i32x4 *>(kept + 64 + 8 * p + 4 * h) = M.q;
             if (ct + 1 < CT) fetch_meta(meta[(ct + 1) & 1], ct + 1);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const bool on = M.w[e >> 2][e & 3] >> bit & 1;               // rows past the last one are not stored
-                const float uh = (float)M.q[e] * M.s[e >> 2][e & 3];
-                const float dy = on ? acc[ct][e] : 0.f;
-                acc[ct][e] = dy;
-                s1[e] = dy;
-                s2[e] = on ? dy * uh : 0.f;
+            for (int q = 0; q < 4; ++q) {
+                const i32x4 sc = *reinterpret_cast<const i32x4 *>(kept + 8 * q + 4 * h), w = *reinterpret_cast<const i32x4 *>(kept + 32 + 8 * q + 4 * h);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int e = 4 * q + j;
+                    const bool on = w[j] >> bit & 1;                             // rows past the last one are not stored
+                    const float uh = (float)reinterpret_cast<const signed char *>(kept + 64 + 8 * (8 * q + 4 * h + j))[p] * __int_as_float(sc[j]);
+                    const float dy = on ? acc[ct][e] : 0.f;
+                    acc[ct][e] = dy;
+                    s1[e] = dy;
+                    s2[e] = on ? dy * uh : 0.f;
+                }
             }
             const float t1 = act8_half_sum(s1, lane), t2 = act8_half_sum(s2, lane);
             const int i = lane & 15, c = 32 * ct + 8 * (i >> 2) + 4 * h + (i & 3);
