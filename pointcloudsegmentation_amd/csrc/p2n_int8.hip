@@ -5,7 +5,7 @@
 // each.  The reference has no 8-bit path (its layers are Conv1d, reference point2net.py:9-34): the formulas above are the
 // specification.  Two operators share the weight image and the rule (p2n_q8.h):
 //   p2n_int8_linear  rows of K values (tokens), float32 or bfloat16
-//   p2n_int8_mlp     the layers of a shared MLP over the columns of (B, C, L), register-resident
+//   p2n_int8_mlp     the layers of a shared MLP over the columns of (B, C, L), on chip from the input to the result
 #include <type_traits>
 #include "p2n_q8.h"
 
@@ -244,7 +244,8 @@ __device__ __forceinline__ float int8_token(const TX *row, int K, int KT, int i,
     return s;
 }
 
-// Tokens into fragments: tile tt of 32 tokens, fragment tt * KT + kt laid out as in the weight image; scales (32 TT).  The rows behind
+// Tokens into fragments: tile tt of 32 tokens, fragment tt * KT + kt laid out as in the weight image; scales (32 TT).  16384 x 2048
+// bfloat16: 38 us, 2.7 TB/s; memory alone would take 20, vector instructions fill half of the issue slots.  The rows behind
 // the last token of a tile are left as they are: what they give is not stored.
 template <typename TX, bool VEC>
 __global__ __launch_bounds__(256) void p2n_int8_tile_kernel(const TX *__restrict__ x, long T, int K, long ld, int KT, int shift, char *__restrict__ img,
@@ -426,7 +427,7 @@ __global__ __launch_bounds__(64 * WR * WC, TM * TN >= 4 ? 2 : 4) void p2n_int8_g
 // ---------------------------------------------------------------- few tokens
 // Up to 16 TT tokens: the weights' way from memory is the time, so a workgroup takes 16 channels and its eight waves share the length
 // K, each streaming its part of the weights straight from memory into 16 x 16 x 64 products; the eight sums meet in LDS
-// (whole numbers: any order).  OWN: up to 8 tokens of up to 4096 values are put into 8 bits here, a wave a token, into
+// (whole numbers: any order; 16 tokens x 4096 x 4096: 6.5 us, 2.6 TB/s of weights).  OWN: up to 8 tokens of up to 4096 values are put into 8 bits here, a wave a token, into
 // LDS; otherwise the tokens' fragments come from p2n_int8_tile_kernel.
 #define MFMA_I8_16(a, b, c) __builtin_amdgcn_mfma_i32_16x16x64_i8((a), (b), (c), 0, 0, 0)
 #define INT8_OWN_K 4096
@@ -744,7 +745,9 @@ __device__ __forceinline__ unsigned int8_halves(unsigned am) {
     return x[0] > x[1] ? x[0] : x[1];
 }
 
-// Up to 64 channels everywhere: one wave carries its 32 points through every layer in registers.
+// Up to 64 channels everywhere: one wave carries its 32 points through every layer in registers.  Bound by the vector instructions that
+// scale the sums and form the next codes, some 11 a value (78 % of the issue slots): 6-32-32-64 with groups of 32 over 16 x 65536 points
+// 53 us, of which the memory's share is 7; the maximum by exchanges between lanes instead of in registers: 62.
 __global__ __launch_bounds__(256, 4) void p2n_int8_mlp_narrow_kernel(Int8MlpArgs A) {
     __shared__ __attribute__((aligned(16))) float own[4][2][64];           // the wave's: parameters of its tiles, in the end scales of its points
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -825,6 +828,7 @@ __global__ __launch_bounds__(256, 4) void p2n_int8_mlp_narrow_kernel(Int8MlpArgs
 
 // Wider layers: NW waves carry 32 points together, a wave its share of the channel tiles.  Codes go round through LDS in operand order; a point's
 // maximum is joined over the waves there too.  Two barriers a layer; a layer's first weights are on their way before the last one ends.
+// 131-128-128-128-64 over 16 x 8192 points: 46 us (vector instructions 60 % of the issue slots, memory 20 us); one wave for all channels: 83.
 template <int NW, bool GROUPS>
 __global__ __launch_bounds__(64 * NW, 4) void p2n_int8_mlp_wide_kernel(Int8MlpArgs A) {
     constexpr int KTI = 4 * NW;      // k-tiles of the input: 1024 (512) channels in, a channel tile a wave: 256 (128) out
