@@ -293,9 +293,11 @@ enum { ACT8_OUT = 0, ACT8_DY = 1 };         // epilogue
 
 typedef __attribute__((address_space(3))) void act8_lds_t;
 
-// bytes from base on that may be reached; none where base lies past the end (a step behind the last point of a cloud)
+// bytes from base on that may be reached; none where base lies past the end (a step behind the last point of a cloud).  An offset of
+// ACT8_BEHIND is past every end.
+#define ACT8_BEHIND 0xFFFFFFF0L
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t act8_rsrc(const void *base, long bytes) {
-    const long n = bytes < 0 ? 0 : bytes < 0xFFFFFFFFL ? bytes : 0xFFFFFFFFL;
+    const long n = bytes < 0 ? 0 : bytes < ACT8_BEHIND ? bytes : ACT8_BEHIND;
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)n, 0x00020000);
 }
 
@@ -916,7 +918,7 @@ __global__ __launch_bounds__(256, 1) void p2n_act8_wgrad_wide_kernel(Act8Wgrad A
         long size = ((long)(A.N - n0) * A.L - l0) * 4;
         unsigned off[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) off[i] = l0 + 4 * (piece ^ (4 * i)) < A.L ? drow + 16u * (piece ^ (4 * i)) : 0xFFFFFFF0u;
+        for (int i = 0; i < 2; ++i) off[i] = l0 + 4 * (piece ^ (4 * i)) < A.L ? drow + 16u * (piece ^ (4 * i)) : (unsigned)ACT8_BEHIND;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(act8_rsrc(src, size), (act8_lds_t *)(mine + buf * BUF + i * 256), 16, off[i & 1], 0, 0, 0);
