@@ -20,6 +20,9 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 #define MFMAB(a, b, c) __builtin_amdgcn_mfma_f32_32x32x16_bf16((a), (b), (c), 0, 0, 0)
 #define ACT8_MAX_C 1024
 #define ACT8_GROUP 128
+// What a call only writes (h, the codes, dx) or reads for the last time goes past the caches, so
+// that x, g and dy stay there for the kernel that reads them next (32 -> 64 over 1,048,576 points: forward 79 -> 64 us, codes 44 -> 41, both gradients 119 -> 103).
+#define ACT8_ONCE 2        // the buffer instructions' bit for it
 
 #define TRY(expr)                  \
     do {                           \
@@ -177,7 +180,7 @@ __device__ __forceinline__ void act8_split_weights(const Act8Split &A, long i) {
 // What is kept of a block of 128 points, 32 channels a workgroup and 8 a wave, a lane two neighbouring points: u, the scales, codes,
 // the ReLU's bits.  The channels' maxima are formed by a halving exchange (8 registers shrink to one while lanes pair up), so lane i
 // holds the maximum of channel i & 7 and one division serves eight channels.  OUT (the end of a chain): relu(y) to `out` as well.
-// 16 x 256 x 8192 values: 45 us, 3.8 TB/s.  Formed by the product's workgroups instead, before their products, it costs 73: nothing
+// 16 x 256 x 8192 values: 43 us, 4.0 TB/s.  Formed by the product's workgroups instead, before their products, it costs 73: nothing
 // overlaps with it there.
 struct Act8Keep {
     const float *x;
@@ -266,7 +269,7 @@ __global__ __launch_bounds__(256) void p2n_act8_keep_kernel(Act8Keep A) {
         int code[1];
         p2n_q8_pack(e, R, code);
         if (!(R.s == R.s)) code[0] = 0;
-        *reinterpret_cast<unsigned short *>(A.codes + (blk * A.C + c0 + i) * ACT8_GROUP + 2 * lane) = (unsigned short)code[0];
+        __builtin_nontemporal_store((unsigned short)code[0], reinterpret_cast<unsigned short *>(A.codes + (blk * A.C + c0 + i) * ACT8_GROUP + 2 * lane));
     }
 }
 
@@ -274,7 +277,7 @@ __global__ __launch_bounds__(256) void p2n_act8_keep_kernel(Act8Keep A) {
 // D = M . X, lane = point, registers = channels.  A workgroup takes 128 points (one group of a cloud), a wave 32 of them and all of
 // CT*32 output channels; the weight fragments pass through LDS (a ring of three, LDS-DMA), X through registers.  Six part products a
 // multiply-add: the matrix cores are the bound with many channels (256 -> 256 over 131,072 points: 104 us forward, 990 TFLOP/s of part
-// products; 124 us with the backward's epilogue), memory with few (32 -> 64 over 1,048,576: 79 us, 5.1 TB/s).
+// products; 124 us with the backward's epilogue), memory with few (32 -> 64 over 1,048,576: 64 us, 6.3 TB/s).
 struct Act8Gemm {
     const float *x;        // (B, K, L)
     const __bf16 *img;
@@ -535,7 +538,7 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : TABK <= 512 ? 2 : 1) void p2n_ac
             for (int e = 0; e < 16; ++e) {
                 float v = acc[ct][e];
                 if (EPI == ACT8_OUT) v += bias[32 * ct + 8 * (e >> 2) + 4 * h + (e & 3)];
-                __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(v), ro, oo + (unsigned)((8 * (e >> 2) + (e & 3)) * A.L * 4), 0, 0);
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(v), ro, oo + (unsigned)((8 * (e >> 2) + (e & 3)) * A.L * 4), 0, EPI == ACT8_OUT ? ACT8_ONCE : 0);
             }
         }
     }
@@ -608,7 +611,7 @@ __global__ __launch_bounds__(256) void p2n_act8_dx_kernel(float *__restrict__ dy
         const float a = tab[c[i]], m1 = tab[C + c[i]], m2 = tab[2 * C + c[i]], s = scale[blk * C4 + c[i]];
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[i][j] = a * (v[i][j] - m1 - (float)(signed char)(q[i] >> (8 * j)) * s * m2);
-        if (whole) *reinterpret_cast<f32x4u *>(d[i]) = v[i];
+        if (whole) __builtin_nontemporal_store((f32x4u)v[i], reinterpret_cast<f32x4u *>(d[i]));
         else
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -1002,7 +1005,8 @@ __global__ __launch_bounds__(256, 1) void p2n_act8_wgrad_wide_kernel(Act8Wgrad A
 // 32 RT x 32 of dW as above, and for the same 32 points W^T . g from the same piece of LDS (lane = point, its eight values of a
 // k-step from eight rows), the fragments of W^T in LDS too.  dy goes to dx's place, its two sums stay in registers to the end.
 // Either product alone comes from here too, so that it does not depend on what else is asked for.
-// 32 -> 64 over 1,048,576 points: 118 us against 93 + 104 for the two, 64 -> 64 over 524,288: 109 against 52 + 78.
+// 32 -> 64 over 1,048,576 points: 103 us (118 before its g went past the caches) against 93 + 104 for the two, 64 -> 64 over 524,288:
+// 109 against 52 + 78.
 struct Act8Both {
     Act8Wgrad w;
     const float *W;
@@ -1067,7 +1071,7 @@ __global__ __launch_bounds__(256, 2) void p2n_act8_both_kernel(Act8Both B) {
         for (int i = 0; i < RT * 4; ++i) {
             const int n = 8 * i + drow;
             const float *p = A.g + (b * A.N + (n < A.N ? n : A.N - 1)) * A.L + l;
-            if (whole) vn[i] = *reinterpret_cast<const f32x4u *>(p);
+            if (whole) vn[i] = __builtin_nontemporal_load(reinterpret_cast<const f32x4u *>(p));
             else
 #pragma unroll
                 for (int x = 0; x < 4; ++x) vn[i][x] = n < A.N && l + x < A.L ? p[x] : 0.f;
