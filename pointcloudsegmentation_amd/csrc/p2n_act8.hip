@@ -20,9 +20,12 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 #define MFMAB(a, b, c) __builtin_amdgcn_mfma_f32_32x32x16_bf16((a), (b), (c), 0, 0, 0)
 #define ACT8_MAX_C 1024
 #define ACT8_GROUP 128
-// What a call only writes (h, the codes, dx) or reads for the last time goes past the caches, so
-// that x, g and dy stay there for the kernel that reads them next (32 -> 64 over 1,048,576 points: forward 79 -> 64 us, codes 44 -> 41, both gradients 119 -> 103).
+// What the next kernels do not read (codes; g at its last reading; h where it is larger than the last cache, so that none of it would be
+// there for the next layer) goes past the caches, and x, g and dy stay there for the kernel that reads them next: 32 -> 64
+// over 1,048,576 points: forward 79 -> 64 us, codes 44 -> 41, both gradients 119 -> 103.  A chain of layers whose h fits loses
+// 1 % if h goes past it (64-64-128-128 over 131,072 points).
 #define ACT8_ONCE 2        // the buffer instructions' bit for it
+#define ACT8_LAST_CACHE (256L << 20)
 
 #define TRY(expr)                  \
     do {                           \
@@ -292,7 +295,7 @@ struct Act8Gemm {
     int K, Kpad, KS, CTP, rows, rows4;
 };
 enum { ACT8_PLAIN = 0, ACT8_NORM = 1 };     // operand
-enum { ACT8_OUT = 0, ACT8_DY = 1 };         // epilogue
+enum { ACT8_OUT = 0, ACT8_DY = 1, ACT8_OUT_ONCE = 2 };      // epilogue
 
 typedef __attribute__((address_space(3))) void act8_lds_t;
 
@@ -360,7 +363,7 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : TABK <= 512 ? 2 : 1) void p2n_ac
     __shared__ __attribute__((aligned(16))) char wbuf[3][F * 1024];
     __shared__ __attribute__((aligned(16))) float tab[IN == ACT8_NORM ? 3 * TABK : 4];
     __shared__ float red[EPI == ACT8_DY ? 4 * 2 * 32 * CT : 1];
-    __shared__ float bias[EPI == ACT8_OUT ? 32 * CT : 1];
+    __shared__ float bias[EPI != ACT8_DY ? 32 * CT : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int p = lane & 31, h = lane >> 5;
     const long b = blockIdx.x / A.NB, nb = blockIdx.x % A.NB, l = nb * ACT8_GROUP + 32 * wave + p;
@@ -372,7 +375,7 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : TABK <= 512 ? 2 : 1) void p2n_ac
     const unsigned off = (unsigned)((8 * h * A.L + (valid ? l : A.L - 1)) * 4);
     if (IN == ACT8_NORM)
         for (int i = threadIdx.x; i < 3 * A.Kpad; i += 256) tab[i] = A.tab[i];
-    if (EPI == ACT8_OUT && (int)threadIdx.x < 32 * CT)
+    if (EPI != ACT8_DY && (int)threadIdx.x < 32 * CT)
         bias[threadIdx.x] = A.bias && 32 * ct0 + (int)threadIdx.x < A.rows ? A.bias[32 * ct0 + threadIdx.x] : 0.f;
 
     auto stage = [&](int c, int slot) __attribute__((always_inline)) {
@@ -537,8 +540,8 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : TABK <= 512 ? 2 : 1) void p2n_ac
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 float v = acc[ct][e];
-                if (EPI == ACT8_OUT) v += bias[32 * ct + 8 * (e >> 2) + 4 * h + (e & 3)];
-                __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(v), ro, oo + (unsigned)((8 * (e >> 2) + (e & 3)) * A.L * 4), 0, EPI == ACT8_OUT ? ACT8_ONCE : 0);
+                if (EPI != ACT8_DY) v += bias[32 * ct + 8 * (e >> 2) + 4 * h + (e & 3)];
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(v), ro, oo + (unsigned)((8 * (e >> 2) + (e & 3)) * A.L * 4), 0, EPI == ACT8_OUT_ONCE ? ACT8_ONCE : 0);
             }
         }
     }
@@ -611,7 +614,7 @@ __global__ __launch_bounds__(256) void p2n_act8_dx_kernel(float *__restrict__ dy
         const float a = tab[c[i]], m1 = tab[C + c[i]], m2 = tab[2 * C + c[i]], s = scale[blk * C4 + c[i]];
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[i][j] = a * (v[i][j] - m1 - (float)(signed char)(q[i] >> (8 * j)) * s * m2);
-        if (whole) __builtin_nontemporal_store((f32x4u)v[i], reinterpret_cast<f32x4u *>(d[i]));
+        if (whole) *reinterpret_cast<f32x4u *>(d[i]) = v[i];
         else
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -1488,8 +1491,9 @@ extern "C" int p2n_act8_forward(const float *x, int B, int K, long L, const floa
     g.x = x; g.img = f.img; g.tab = f.tab; g.bias = bias; g.out = h; g.L = L; g.NB = a.NB;
     g.K = K; g.Kpad = a.Kpad; g.KS = a.KSf; g.CTP = a.CTf; g.rows = N;
     const long groups = (long)B * a.NB;
-    if (gamma) TRY((act8_launch_gemm<ACT8_NORM, ACT8_OUT>(g, groups, s)));
-    else TRY((act8_launch_gemm<ACT8_PLAIN, ACT8_OUT>(g, groups, s)));
+    const bool once = (long)B * N * L * 4 >= ACT8_LAST_CACHE;
+    if (gamma) TRY((once ? act8_launch_gemm<ACT8_NORM, ACT8_OUT_ONCE>(g, groups, s) : act8_launch_gemm<ACT8_NORM, ACT8_OUT>(g, groups, s)));
+    else TRY((once ? act8_launch_gemm<ACT8_PLAIN, ACT8_OUT_ONCE>(g, groups, s) : act8_launch_gemm<ACT8_PLAIN, ACT8_OUT>(g, groups, s)));
     p2n_prof_end(ps, s);
     return P2N_OK;
 }

@@ -312,7 +312,7 @@ __device__ __forceinline__ void int8_store4(__bf16 *y, long t, long T, int N, in
         two[0] = (__bf16)(odd ? got : keep);
         two[1] = (__bf16)(odd ? keep : got);
         const long tt = t + 2 * p + (odd ? 1 : 0);
-        if (col && tt < T) __builtin_nontemporal_store(*reinterpret_cast<const unsigned *>(two), reinterpret_cast<unsigned *>(y + tt * N + (n & ~1)));
+        if (col && tt < T) *reinterpret_cast<unsigned *>(y + tt * N + (n & ~1)) = *reinterpret_cast<const unsigned *>(two);
     }
 }
 
@@ -662,7 +662,7 @@ __device__ __forceinline__ void int8_mlp_out(const Int8MlpArgs &A, int N, long b
     if (valid && 32 * ct + 32 <= N) {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-            __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(y[e]), rs, off, (int)((8 * (e >> 2) + (e & 3)) * A.L * 4), 2);
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(y[e]), rs, off, (int)((8 * (e >> 2) + (e & 3)) * A.L * 4), 0);
     } else if (valid) {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
