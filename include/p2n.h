@@ -420,7 +420,7 @@ int p2n_max_of_columns(const float *in, long rows, int ns, float *out, void *str
  * backward pass needs instead of x: the codes of u (of x) by the 8-bit rule above, one scale for 128 consecutive points of a
  * row, the bits [y > 0], mu and r -- 1.16 bytes a value.  running_mean / running_var (both or NULL) are updated in place with
  * `momentum` (unbiased variance); momentum < 0: the running statistics are used and left as they are (`frozen` in the
- * backward pass).  Backward, with uh and ah the values that the codes stand for:
+ * backward pass); batches (may be NULL) counts one more where the running statistics are updated.  Backward, with uh and ah the values that the codes stand for:
  *   dW = g . ah^T, db = sum g, dy = [y > 0] * (W^T . g), dbeta = sum dy, dgamma = sum dy*uh,
  *   dx = gamma*r*(dy - dbeta/P - uh*dgamma/P), P = B*L   (frozen: gamma*r*dy; without a norm: W^T . g)
  * dW and db may be NULL (not computed), and dx without a norm; with a norm dgamma and dbeta need dx.  Limits: 1..1024
@@ -428,14 +428,14 @@ int p2n_max_of_columns(const float *in, long rows, int ns, float *out, void *str
 size_t p2n_act8_kept_bytes(int B, int C, long L, int norm);
 size_t p2n_act8_workspace_bytes(int B, int K, long L, int N);      /* N = 0: the norm + ReLU calls */
 int p2n_act8_forward(const float *x, int B, int K, long L, const float *W, const float *bias, int N,
-                     const float *gamma, const float *beta, float *running_mean, float *running_var, float momentum, float eps,
-                     float *h, void *kept, size_t kept_bytes, void *workspace, size_t workspace_bytes, void *stream);
+                     const float *gamma, const float *beta, float *running_mean, float *running_var, long *batches,
+                     float momentum, float eps, float *h, void *kept, size_t kept_bytes, void *workspace, size_t workspace_bytes, void *stream);
 int p2n_act8_backward(const float *g, int B, int K, long L, const float *W, int N, const float *gamma, const float *beta,
                       int frozen, const void *kept, size_t kept_bytes, float *dx, float *dW, float *db, float *dgamma,
                       float *dbeta, void *workspace, size_t workspace_bytes, void *stream);
 /* the norm and ReLU alone: out = relu(norm(x)), the end of a chain */
 int p2n_act8_norm_relu_forward(const float *x, int B, int C, long L, const float *gamma, const float *beta,
-                               float *running_mean, float *running_var, float momentum, float eps, float *out,
+                               float *running_mean, float *running_var, long *batches, float momentum, float eps, float *out,
                                void *kept, size_t kept_bytes, void *workspace, size_t workspace_bytes, void *stream);
 int p2n_act8_norm_relu_backward(const float *g, int B, int C, long L, const float *gamma, int frozen, const void *kept,
                                 size_t kept_bytes, float *dx, float *dgamma, float *dbeta, void *workspace,

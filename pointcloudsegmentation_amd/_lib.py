@@ -105,11 +105,11 @@ SIGNATURES = {
     "p2n_max_of_columns": (c_int, [c_f, c_long, c_int, c_f, c_vp]),
     "p2n_act8_kept_bytes": (c_sz, [c_int, c_int, c_long, c_int]),
     "p2n_act8_workspace_bytes": (c_sz, [c_int, c_int, c_long, c_int]),
-    "p2n_act8_forward": (c_int, [c_f, c_int, c_int, c_long, c_f, c_f, c_int, c_f, c_f, c_f, c_f, c_float, c_float, c_f,
+    "p2n_act8_forward": (c_int, [c_f, c_int, c_int, c_long, c_f, c_f, c_int, c_f, c_f, c_f, c_f, c_vp, c_float, c_float, c_f,
                                  c_vp, c_sz, c_vp, c_sz, c_vp]),
     "p2n_act8_backward": (c_int, [c_f, c_int, c_int, c_long, c_f, c_int, c_f, c_f, c_int, c_vp, c_sz, c_f, c_f, c_f, c_f, c_f,
                                   c_vp, c_sz, c_vp]),
-    "p2n_act8_norm_relu_forward": (c_int, [c_f, c_int, c_int, c_long, c_f, c_f, c_f, c_f, c_float, c_float, c_f, c_vp, c_sz,
+    "p2n_act8_norm_relu_forward": (c_int, [c_f, c_int, c_int, c_long, c_f, c_f, c_f, c_f, c_vp, c_float, c_float, c_f, c_vp, c_sz,
                                            c_vp, c_sz, c_vp]),
     "p2n_act8_norm_relu_backward": (c_int, [c_f, c_int, c_int, c_long, c_f, c_int, c_vp, c_sz, c_f, c_f, c_f, c_vp, c_sz, c_vp]),
     "p2n_profile_enable": (c_int, [c_int]),

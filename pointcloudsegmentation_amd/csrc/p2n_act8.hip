@@ -63,12 +63,54 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float act8_relu(float y) { return y <= 0.f ? 0.f : y; }   // a NaN stays
 
 // ---------------------------------------------------------------- BatchNorm statistics
+// mu, r kept as float32; tab = {mu, gamma*r, beta} for the forward loader, zero behind the last channel; running statistics (unbiased
+// variance) and the count of batches brought up to date.  By one lane, of the channel's sums, or (frozen) from the running statistics.
+struct Act8Norm {
+    const float *x, *gamma, *beta;
+    float *rmean, *rvar;
+    long *batches;
+    double momentum, eps, P;
+    int frozen, C, Cpad;
+    long L;
+    float *stat, *tab;
+};
+__device__ __forceinline__ void act8_norm_finish(const Act8Norm &A, int c, double u, double v) {
+    double mean, var;
+    if (A.frozen) {
+        mean = A.rmean[c];
+        var = A.rvar[c];
+    } else {
+        const double d = u / A.P;
+        mean = (double)A.x[(long)c * A.L] + d;
+        var = v / A.P - d * d;
+        if (var < 0.0) var = 0.0;
+        if (A.batches && c == 0) *A.batches += 1;
+        if (A.rmean) {
+            A.rmean[c] = (float)((1.0 - A.momentum) * A.rmean[c] + A.momentum * mean);
+            A.rvar[c] = (float)((1.0 - A.momentum) * A.rvar[c] + A.momentum * var * (A.P / (A.P - 1.0)));
+        }
+    }
+    const float mu = (float)mean, r = (float)(1.0 / sqrt(var + A.eps));
+    A.stat[c] = mu;
+    A.stat[A.C + c] = r;
+    A.tab[c] = mu;
+    A.tab[A.Cpad + c] = A.gamma[c] * r;
+    A.tab[2 * A.Cpad + c] = A.beta[c];
+}
+
 // grid (C, S): sums of (x - pivot) and its square over a slice of the (cloud, block) list, in 64 bits, pivot = x[0][c][0].
-// One reading of x: 16 x 256 x 8192 values 28 us, 4.8 TB/s.
-__global__ __launch_bounds__(256) void p2n_act8_stats_kernel(const float *__restrict__ x, int B, int C, long L, long blocks, long per, double *__restrict__ part) {
+// One reading of x: 16 x 256 x 8192 values 28 us, 4.8 TB/s.  ALONE (S = 1): the workgroup has all of its channel and finishes it
+// (grid (Cpad, 1)).
+template <bool ALONE>
+__global__ __launch_bounds__(256) void p2n_act8_stats_kernel(const float *__restrict__ x, int B, int C, long L, long blocks, long per, double *__restrict__ part,
+                                                             Act8Norm A) {
     __shared__ double sh[8];
     const int c = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long NB = (L + 2047) / 2048;                      // a block: 2048 columns of a cloud
+    if (ALONE && c >= C) {
+        if (threadIdx.x < 3) A.tab[threadIdx.x * A.Cpad + c] = 0.f;
+        return;
+    }
     const float pivot = x[(long)c * L];
     double u = 0.0, v = 0.0;
     auto add = [&](float e) __attribute__((always_inline)) {
@@ -98,50 +140,35 @@ __global__ __launch_bounds__(256) void p2n_act8_stats_kernel(const float *__rest
     if (lane == 0) { sh[wave] = u; sh[4 + wave] = v; }
     __syncthreads();
     if (threadIdx.x == 0) {
-        part[((long)c * gridDim.y + blockIdx.y) * 2] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
-        part[((long)c * gridDim.y + blockIdx.y) * 2 + 1] = (sh[4] + sh[5]) + (sh[6] + sh[7]);
+        u = (sh[0] + sh[1]) + (sh[2] + sh[3]);
+        v = (sh[4] + sh[5]) + (sh[6] + sh[7]);
+        if (ALONE) {
+            act8_norm_finish(A, c, u, v);
+        } else {
+            part[((long)c * gridDim.y + blockIdx.y) * 2] = u;
+            part[((long)c * gridDim.y + blockIdx.y) * 2 + 1] = v;
+        }
     }
 }
 
-// mu, r kept as float32; tab = {mu, gamma*r, beta} for the forward loader, zero behind the last channel.  frozen: from the
-// running statistics.  One wave a channel.
-__global__ void p2n_act8_norm_kernel(const double *__restrict__ part, int S, const float *__restrict__ x, int C, int Cpad, long L, double P,
-                                     const float *__restrict__ gamma, const float *__restrict__ beta, float *__restrict__ rmean,
-                                     float *__restrict__ rvar, double momentum, double eps, int frozen, float *__restrict__ stat, float *__restrict__ tab) {
+// the slices' sums of a channel, by one wave
+__global__ void p2n_act8_norm_kernel(const double *__restrict__ part, int S, Act8Norm A) {
     const int c = blockIdx.x, lane = threadIdx.x;
-    if (c >= C) {
-        if (lane < 3) tab[lane * Cpad + c] = 0.f;
+    if (c >= A.C) {
+        if (lane < 3) A.tab[lane * A.Cpad + c] = 0.f;
         return;
     }
-    double mean, var;
-    if (frozen) {
-        mean = rmean[c];
-        var = rvar[c];
-    } else {
-        double u = 0.0, v = 0.0;
+    double u = 0.0, v = 0.0;
+    if (!A.frozen)
         for (int s = lane; s < S; s += 64) { u += part[((long)c * S + s) * 2]; v += part[((long)c * S + s) * 2 + 1]; }
 #pragma unroll
-        for (int m = 32; m > 0; m >>= 1) {
-            u += __shfl_xor(u, m);
-            v += __shfl_xor(v, m);
-        }
-        const double d = u / P;
-        mean = (double)x[(long)c * L] + d;
-        var = v / P - d * d;
-        if (var < 0.0) var = 0.0;
-        if (rmean && lane == 0) {
-            rmean[c] = (float)((1.0 - momentum) * rmean[c] + momentum * mean);
-            rvar[c] = (float)((1.0 - momentum) * rvar[c] + momentum * var * (P / (P - 1.0)));
-        }
+    for (int m = 32; m > 0; m >>= 1) {
+        u += __shfl_xor(u, m);
+        v += __shfl_xor(v, m);
     }
-    if (lane) return;
-    const float mu = (float)mean, r = (float)(1.0 / sqrt(var + eps));
-    stat[c] = mu;
-    stat[C + c] = r;
-    tab[c] = mu;
-    tab[Cpad + c] = gamma[c] * r;
-    tab[2 * Cpad + c] = beta[c];
+    if (lane == 0) act8_norm_finish(A, c, u, v);
 }
+
 
 // ---------------------------------------------------------------- weight image of a product
 // three-way split w = h + m + l: fragment (ks * CTP + ct) * 3 + part, 1 KiB: lane holds part(M[32ct + (lane&31)][16ks + 8(lane>>5) + i]),
@@ -559,16 +586,31 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : TABK <= 512 ? 2 : 1) void p2n_ac
 }
 
 // ---------------------------------------------------------------- the rest of the norm's backward
-// sums of a row's partials, in 64 bits and in order: dbeta, dgamma, and {gamma*r, m1, m2} for dx
-__global__ __launch_bounds__(256) void p2n_act8_sums_kernel(const float *__restrict__ part, long n, int C, double P, const float *__restrict__ gamma,
-                                                            const float *__restrict__ stat, int frozen, float *__restrict__ dgamma, float *__restrict__ dbeta,
-                                                            float *__restrict__ tab) {
+struct Act8Sums {
+    const float *part;             // [C][2][n]
+    long n;
+    int C, frozen;
+    double P;
+    const float *gamma, *stat;
+    float *dgamma, *dbeta;
+    float *tab;
+};
+// of a channel's two sums: dbeta, dgamma, and {gamma*r, m1, m2} for dx
+__device__ __forceinline__ void act8_sums_finish(const Act8Sums &A, int c, double u, double v, bool write, float (&t)[3]) {
+    if (write && A.dbeta) A.dbeta[c] = (float)u;
+    if (write && A.dgamma) A.dgamma[c] = (float)v;
+    t[0] = A.gamma[c] * A.stat[A.C + c];
+    t[1] = A.frozen ? 0.f : (float)(u / A.P);
+    t[2] = A.frozen ? 0.f : (float)(v / A.P);
+}
+// a row's partials in 64 bits and in order
+__global__ __launch_bounds__(256) void p2n_act8_sums_kernel(Act8Sums A) {
     __shared__ double sh[8];
     const int c = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     double u = 0.0, v = 0.0;
-    for (long i = threadIdx.x; i < n; i += 256) {
-        u += part[((long)c * 2) * n + i];
-        v += part[((long)c * 2 + 1) * n + i];
+    for (long i = threadIdx.x; i < A.n; i += 256) {
+        u += A.part[((long)c * 2) * A.n + i];
+        v += A.part[((long)c * 2 + 1) * A.n + i];
     }
 #pragma unroll
     for (int m = 32; m > 0; m >>= 1) {
@@ -578,19 +620,39 @@ __global__ __launch_bounds__(256) void p2n_act8_sums_kernel(const float *__restr
     if (lane == 0) { sh[wave] = u; sh[4 + wave] = v; }
     __syncthreads();
     if (threadIdx.x == 0) {
-        u = (sh[0] + sh[1]) + (sh[2] + sh[3]);
-        v = (sh[4] + sh[5]) + (sh[6] + sh[7]);
-        if (dbeta) dbeta[c] = (float)u;
-        if (dgamma) dgamma[c] = (float)v;
-        tab[c] = gamma[c] * stat[C + c];
-        tab[C + c] = frozen ? 0.f : (float)(u / P);
-        tab[2 * C + c] = frozen ? 0.f : (float)(v / P);
+        float t[3];
+        act8_sums_finish(A, c, (sh[0] + sh[1]) + (sh[2] + sh[3]), (sh[4] + sh[5]) + (sh[6] + sh[7]), true, t);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) A.tab[i * A.C + c] = t[i];
     }
 }
 
-// dx = gamma*r*(dy - m1 - uh*m2), in place: a workgroup takes 32 channels of a block of 128 points, a thread four points of four channels
-__global__ __launch_bounds__(256) void p2n_act8_dx_kernel(float *__restrict__ dy, int C, int C4, long L, long NB, const float *__restrict__ tab,
+// dx = gamma*r*(dy - m1 - uh*m2), in place: a workgroup takes 32 channels of a block of 128 points, a thread four points of four channels.
+// FEW: the sums are formed here too, by every workgroup for its channels (eight threads a channel), the first of a row writes them down.
+#define ACT8_FEW 64
+template <bool FEW>
+__global__ __launch_bounds__(256) void p2n_act8_dx_kernel(float *__restrict__ dy, int C, int C4, long L, long NB, Act8Sums A,
                                                           const signed char *__restrict__ codes, const float *__restrict__ scale) {
+    __shared__ float own[FEW ? 96 : 1];
+    if (FEW) {
+        const int c = blockIdx.y * 32 + (threadIdx.x >> 3), cc = c < C ? c : C - 1;
+        double u = 0.0, v = 0.0;
+        for (int i = threadIdx.x & 7; i < (int)A.n; i += 8) {
+            u += A.part[((long)cc * 2) * A.n + i];
+            v += A.part[((long)cc * 2 + 1) * A.n + i];
+        }
+#pragma unroll
+        for (int m = 4; m > 0; m >>= 1) {
+            u += __shfl_xor(u, m);
+            v += __shfl_xor(v, m);
+        }
+        float t[3];
+        act8_sums_finish(A, cc, u, v, blockIdx.x == 0 && c < C && (threadIdx.x & 7) == 0, t);
+        if ((threadIdx.x & 7) == 0)
+#pragma unroll
+            for (int i = 0; i < 3; ++i) own[32 * i + (threadIdx.x >> 3)] = t[i];
+        __syncthreads();
+    }
     const long blk = blockIdx.x, b = blk / NB, l0 = (blk % NB) * ACT8_GROUP;
     const int p = 4 * (threadIdx.x & 31);
     const bool whole = l0 + p + 4 <= L;
@@ -611,7 +673,8 @@ __global__ __launch_bounds__(256) void p2n_act8_dx_kernel(float *__restrict__ dy
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (c[i] >= C) continue;
-        const float a = tab[c[i]], m1 = tab[C + c[i]], m2 = tab[2 * C + c[i]], s = scale[blk * C4 + c[i]];
+        const float *t = FEW ? own + (c[i] & 31) : A.tab + c[i];
+        const float a = t[0], m1 = t[FEW ? 32 : C], m2 = t[FEW ? 64 : 2 * C], s = scale[blk * C4 + c[i]];
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[i][j] = a * (v[i][j] - m1 - (float)(signed char)(q[i] >> (8 * j)) * s * m2);
         if (whole) *reinterpret_cast<f32x4u *>(d[i]) = v[i];
@@ -1304,6 +1367,7 @@ int act8_init(Act8 &a, const char *fn, int B, int K, long L, int N) {
     long s = 2048 / K > 1 ? 2048 / K : 1;
     if (s > blocks) s = blocks;
     if (s > 1024) s = 1024;
+    if (blocks <= 4) s = 1;              // few enough for one workgroup a channel, which then needs no second kernel
     a.per = (blocks + s - 1) / s;
     a.S = (int)((blocks + a.per - 1) / a.per);
     // a wave makes up to 64 x 64, two of them on a SIMD; 128 x 128 (which fills the registers alone, and splits each operand half as
@@ -1423,20 +1487,23 @@ int act8_space_check(const char *fn, const void *p, size_t have, size_t need, co
 }
 
 // statistics and tables of x (norm), and what is kept of it; relu(y) to `out`, or the image of `split`
-int act8_keep(const Act8 &a, const float *x, const float *gamma, const float *beta, float *rmean, float *rvar, float momentum, float eps,
+int act8_keep(const Act8 &a, const float *x, const float *gamma, const float *beta, float *rmean, float *rvar, long *batches, float momentum, float eps,
               char *kept, const FwdSpace &f, float *out, const Act8Split &split, hipStream_t s) {
     const Act8Kept k = act8_kept(a.B, a.K, a.L, gamma != nullptr);
     float *stat = (float *)(kept + k.stat);
     if (gamma) {
         const bool frozen = momentum < 0.f;
-        const double P = (double)a.B * a.L;
-        if (!frozen) {
-            const long blocks = (long)a.B * ((a.L + 2047) / 2048);
-            hipLaunchKernelGGL(p2n_act8_stats_kernel, dim3(a.K, a.S), dim3(256), 0, s, x, a.B, a.K, a.L, blocks, a.per, f.part);
-            P2N_CHECK_HIP(hipGetLastError());
+        const Act8Norm n{x, gamma, beta, rmean, rvar, batches, (double)momentum, (double)eps, (double)a.B * a.L, frozen ? 1 : 0, a.K, a.Kpad, a.L, stat, f.tab};
+        const long blocks = (long)a.B * ((a.L + 2047) / 2048);
+        if (!frozen && a.S == 1) {
+            hipLaunchKernelGGL(p2n_act8_stats_kernel<true>, dim3(a.Kpad), dim3(256), 0, s, x, a.B, a.K, a.L, blocks, a.per, f.part, n);
+        } else {
+            if (!frozen) {
+                hipLaunchKernelGGL(p2n_act8_stats_kernel<false>, dim3(a.K, a.S), dim3(256), 0, s, x, a.B, a.K, a.L, blocks, a.per, f.part, n);
+                P2N_CHECK_HIP(hipGetLastError());
+            }
+            hipLaunchKernelGGL(p2n_act8_norm_kernel, dim3(a.Kpad), dim3(64), 0, s, f.part, a.S, n);
         }
-        hipLaunchKernelGGL(p2n_act8_norm_kernel, dim3(a.Kpad), dim3(64), 0, s, f.part, a.S, x, a.K, a.Kpad, a.L, P, gamma, beta, rmean, rvar,
-                           (double)momentum, (double)eps, frozen ? 1 : 0, stat, f.tab);
         P2N_CHECK_HIP(hipGetLastError());
     }
     const Act8Keep keep{x, stat, gamma, beta, (signed char *)kept, (float *)(kept + k.scale), (unsigned *)(kept + k.bits), out, a.L, a.NB,
@@ -1445,6 +1512,21 @@ int act8_keep(const Act8 &a, const float *x, const float *gamma, const float *be
     if (out) hipLaunchKernelGGL((p2n_act8_keep_kernel<true, true>), grid, dim3(256), 0, s, keep);
     else if (gamma) hipLaunchKernelGGL((p2n_act8_keep_kernel<true, false>), grid, dim3(256), 0, s, keep);
     else hipLaunchKernelGGL((p2n_act8_keep_kernel<false, false>), grid, dim3(256), 0, s, keep);
+    P2N_CHECK_HIP(hipGetLastError());
+    return P2N_OK;
+}
+
+// dy in dx's place -> dx, dgamma, dbeta
+int act8_through_norm(const Act8 &a, float *dx, const Act8Sums &n, const signed char *codes, const float *scale, hipStream_t s) {
+    const dim3 grid((unsigned)((long)a.B * a.NB), (unsigned)((a.K + 31) / 32));
+    const int C4 = (a.K + 3) / 4 * 4;
+    if (n.n <= ACT8_FEW) {
+        hipLaunchKernelGGL(p2n_act8_dx_kernel<true>, grid, dim3(256), 0, s, dx, a.K, C4, a.L, a.NB, n, codes, scale);
+    } else {
+        hipLaunchKernelGGL(p2n_act8_sums_kernel, dim3(a.K), dim3(256), 0, s, n);
+        P2N_CHECK_HIP(hipGetLastError());
+        hipLaunchKernelGGL(p2n_act8_dx_kernel<false>, grid, dim3(256), 0, s, dx, a.K, C4, a.L, a.NB, n, codes, scale);
+    }
     P2N_CHECK_HIP(hipGetLastError());
     return P2N_OK;
 }
@@ -1473,7 +1555,7 @@ extern "C" size_t p2n_act8_workspace_bytes(int B, int K, long L, int N) {
 }
 
 extern "C" int p2n_act8_forward(const float *x, int B, int K, long L, const float *W, const float *bias, int N, const float *gamma, const float *beta,
-                                float *running_mean, float *running_var, float momentum, float eps, float *h, void *kept, size_t kept_bytes,
+                                float *running_mean, float *running_var, long *batches, float momentum, float eps, float *h, void *kept, size_t kept_bytes,
                                 void *workspace, size_t workspace_bytes, void *stream_) {
     const char *fn = "p2n_act8_forward";
     Act8 a;
@@ -1487,7 +1569,7 @@ extern "C" int p2n_act8_forward(const float *x, int B, int K, long L, const floa
     hipStream_t s = (hipStream_t)stream_;
     const int ps = p2n_prof_begin(P2N_K_ACT8_FWD, s);
     Act8Gemm g = {};
-    TRY(act8_keep(a, x, gamma, beta, running_mean, running_var, momentum, eps, (char *)kept, f, nullptr, Act8Split{W, f.img, N, K, 0, a.CTf, a.KSf}, s));
+    TRY(act8_keep(a, x, gamma, beta, running_mean, running_var, batches, momentum, eps, (char *)kept, f, nullptr, Act8Split{W, f.img, N, K, 0, a.CTf, a.KSf}, s));
     g.x = x; g.img = f.img; g.tab = f.tab; g.bias = bias; g.out = h; g.L = L; g.NB = a.NB;
     g.K = K; g.Kpad = a.Kpad; g.KS = a.KSf; g.CTP = a.CTf; g.rows = N;
     const long groups = (long)B * a.NB;
@@ -1547,19 +1629,14 @@ extern "C" int p2n_act8_backward(const float *g, int B, int K, long L, const flo
         if (gamma) TRY((act8_launch_gemm<ACT8_PLAIN, ACT8_DY>(q, groups, s)));
         else TRY((act8_launch_gemm<ACT8_PLAIN, ACT8_OUT>(q, groups, s)));
     }
-    if (dx && gamma) {
-        hipLaunchKernelGGL(p2n_act8_sums_kernel, dim3(K), dim3(256), 0, s, f.part, f.nparts, K, (double)B * L, gamma, stat, frozen ? 1 : 0, dgamma, dbeta, f.tab);
-        P2N_CHECK_HIP(hipGetLastError());
-        hipLaunchKernelGGL(p2n_act8_dx_kernel, dim3((unsigned)groups, (unsigned)((K + 31) / 32)), dim3(256), 0, s, dx, K, K4, L, a.NB, f.tab, codes, scale);
-        P2N_CHECK_HIP(hipGetLastError());
-    }
+    if (dx && gamma) TRY(act8_through_norm(a, dx, Act8Sums{f.part, f.nparts, K, frozen ? 1 : 0, (double)B * L, gamma, stat, dgamma, dbeta, f.tab}, codes, scale, s));
     p2n_prof_end(ps, s);
     return P2N_OK;
 }
 
 extern "C" int p2n_act8_norm_relu_forward(const float *x, int B, int C, long L, const float *gamma, const float *beta, float *running_mean,
-                                          float *running_var, float momentum, float eps, float *out, void *kept, size_t kept_bytes, void *workspace,
-                                          size_t workspace_bytes, void *stream_) {
+                                          float *running_var, long *batches, float momentum, float eps, float *out, void *kept, size_t kept_bytes,
+                                          void *workspace, size_t workspace_bytes, void *stream_) {
     const char *fn = "p2n_act8_norm_relu_forward";
     Act8 a;
     TRY(act8_init(a, fn, B, C, L, 0));
@@ -1570,7 +1647,7 @@ extern "C" int p2n_act8_norm_relu_forward(const float *x, int B, int C, long L, 
     const FwdSpace f = fwd_space(a, (char *)workspace);
     hipStream_t s = (hipStream_t)stream_;
     const int ps = p2n_prof_begin(P2N_K_ACT8_FWD, s);
-    TRY(act8_keep(a, x, gamma, beta, running_mean, running_var, momentum, eps, (char *)kept, f, out, Act8Split{}, s));
+    TRY(act8_keep(a, x, gamma, beta, running_mean, running_var, batches, momentum, eps, (char *)kept, f, out, Act8Split{}, s));
     p2n_prof_end(ps, s);
     return P2N_OK;
 }
@@ -1594,10 +1671,7 @@ extern "C" int p2n_act8_norm_relu_backward(const float *g, int B, int C, long L,
     const int C4 = (C + 3) / 4 * 4;
     hipLaunchKernelGGL(p2n_act8_dy_kernel, dim3(C, a.S), dim3(256), 0, s, g, B, C, C4, L, a.NB, per, codes, scale, (const unsigned *)(kept + k.bits), dx, f.part);
     P2N_CHECK_HIP(hipGetLastError());
-    hipLaunchKernelGGL(p2n_act8_sums_kernel, dim3(C), dim3(256), 0, s, f.part, f.nparts, C, (double)B * L, gamma, stat, frozen ? 1 : 0, dgamma, dbeta, f.tab);
-    P2N_CHECK_HIP(hipGetLastError());
-    hipLaunchKernelGGL(p2n_act8_dx_kernel, dim3((unsigned)n, (unsigned)((C + 31) / 32)), dim3(256), 0, s, dx, C, C4, L, a.NB, f.tab, codes, scale);
-    P2N_CHECK_HIP(hipGetLastError());
+    TRY(act8_through_norm(a, dx, Act8Sums{f.part, f.nparts, C, frozen ? 1 : 0, (double)B * L, gamma, stat, dgamma, dbeta, f.tab}, codes, scale, s));
     p2n_prof_end(ps, s);
     return P2N_OK;
 }

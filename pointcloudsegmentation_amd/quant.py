@@ -192,38 +192,35 @@ def int8_mlp(x: torch.Tensor, weights: Sequence[Int8Weight], last_relu: bool = T
 
 # ------------------------------------------------------------------ activation checkpoints in 8 bits
 def _norm_args(norm: Optional[nn.BatchNorm1d], x: torch.Tensor):
-    """gamma, beta, running mean, running variance, momentum (< 0: running statistics used as they are), eps of a BatchNorm1d"""
+    """gamma, beta, running mean, running variance, batches tracked (where it counts), momentum (< 0: running statistics used as they
+    are), eps of a BatchNorm1d"""
     if norm is None:
-        return None, None, None, None, 0.0, 0.0
+        return None, None, None, None, None, 0.0, 0.0
     if not isinstance(norm, nn.BatchNorm1d):
         raise TypeError(f"norm must be a BatchNorm1d or None, got {type(norm).__name__}")
-    if not norm.affine:
+    # straight from the module's dictionaries: its attribute access costs as much as a launch
+    par, buf = norm._parameters, norm._buffers
+    gamma, beta, mean, var = par["weight"], par["bias"], buf["running_mean"], buf["running_var"]
+    if gamma is None:
         raise NotImplementedError("the 8-bit checkpoint layers need BatchNorm1d(affine=True)")
-    if norm.num_features != x.size(1):
-        raise ValueError(f"norm has {norm.num_features} channels, x has {x.size(1)}")
-    for t, name in ((norm.weight, "norm.weight"), (norm.bias, "norm.bias"), (norm.running_mean, "norm.running_mean"),
-                    (norm.running_var, "norm.running_var")):
-        if t is not None and not (t.device == x.device and t.dtype == torch.float32 and t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous float32 tensor on the input's GPU")
-    frozen = not norm.training and norm.running_mean is not None
-    if not frozen and x.size(0) * x.size(2) < 2:
-        raise ValueError(f"Expected more than 1 value per channel when training, got input size {tuple(x.shape)}")
-    if frozen:
-        momentum = -1.0
-    elif norm.training and norm.running_mean is not None:
+    if gamma.size(0) != x.size(1):
+        raise ValueError(f"norm has {gamma.size(0)} channels, x has {x.size(1)}")
+    for t, name in ((gamma, "weight"), (beta, "bias"), (mean, "running_mean"), (var, "running_var")):
+        if t is not None and not (t.dtype == torch.float32 and t.device == x.device and t.is_contiguous()):
+            raise ValueError(f"norm.{name} must be a contiguous float32 tensor on the input's GPU")
+    training, tracked = norm.training, mean is not None
+    if training or not tracked:
+        if x.size(0) * x.size(2) < 2:
+            raise ValueError(f"Expected more than 1 value per channel when training, got input size {tuple(x.shape)}")
+        if not training or not tracked:
+            return gamma, beta, None, None, None, 0.0, norm.eps
         if norm.momentum is None:
             raise NotImplementedError("BatchNorm1d(momentum=None) (cumulative average) is not implemented on the GPU path")
-        momentum = norm.momentum
-    else:
-        momentum = 0.0
-    tracked = frozen or (norm.training and norm.running_mean is not None)
-    return norm.weight, norm.bias, norm.running_mean if tracked else None, norm.running_var if tracked else None, momentum, norm.eps
-
-
-def _count_batch(norm: Optional[nn.BatchNorm1d]) -> None:
-    if norm is not None and norm.training and norm.num_batches_tracked is not None:
-        with torch.no_grad():
-            norm.num_batches_tracked += 1
+        batches = buf["num_batches_tracked"]
+        if batches is not None and not (batches.dtype == torch.int64 and batches.device == x.device):
+            raise ValueError("norm.num_batches_tracked must be an int64 tensor on the input's GPU")
+        return gamma, beta, mean, var, batches, norm.momentum, norm.eps
+    return gamma, beta, mean, var, None, -1.0, norm.eps
 
 
 def _bytes(n: int, device) -> torch.Tensor:
@@ -240,9 +237,21 @@ def _act8_bytes(what: str, B: int, C: int, L: int, norm: bool, N: int):
     return nkept, nws
 
 
+def _changed(mean, var, batches) -> None:
+    """the kernels wrote these buffers through their addresses: autograd, and what is kept by a buffer's version, has to know"""
+    if batches is not None:
+        torch.autograd.graph.increment_version((mean, var, batches))
+
+
+@torch.autograd.function.once_differentiable
+def _once(function, ctx, g):
+    """under create_graph: gradients that refuse to be differentiated (the decorator costs a launch's time, so it is taken only there)"""
+    return function.gradients(ctx, g)
+
+
 class _Act8Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, gamma, beta, running_mean, running_var, momentum, eps):
+    def forward(ctx, x, weight, bias, gamma, beta, running_mean, running_var, batches, momentum, eps):
         L_ = _lib.lib()
         B, K, L = x.shape
         N = weight.size(0)
@@ -252,15 +261,19 @@ class _Act8Linear(torch.autograd.Function):
         kept, ws = _bytes(nkept, dev), _bytes(nws, dev)
         h = torch.empty((B, N, L), dtype=torch.float32, device=dev)
         _call(L_.p2n_act8_forward, "p2n_act8_forward", dev, x.data_ptr(), B, K, L, weight.data_ptr(), _rt.ptr(bias), N, _rt.ptr(gamma),
-              _rt.ptr(beta), _rt.ptr(running_mean), _rt.ptr(running_var), momentum, eps, h.data_ptr(), kept.data_ptr(), nkept,
+              _rt.ptr(beta), _rt.ptr(running_mean), _rt.ptr(running_var), _rt.ptr(batches), momentum, eps, h.data_ptr(), kept.data_ptr(), nkept,
               ws.data_ptr(), nws)
+        _changed(running_mean, running_var, batches)
         ctx.save_for_backward(kept, weight, gamma, beta)
         ctx.meta = (B, K, L, N, normed and momentum < 0, bias is not None)
         return h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        return _once(_Act8Linear, ctx, g) if torch.is_grad_enabled() else _Act8Linear.gradients(ctx, g)
+
+    @staticmethod
+    def gradients(ctx, g):
         kept, weight, gamma, beta = ctx.saved_tensors
         B, K, L, N, frozen, has_bias = ctx.meta
         L_ = _lib.lib()
@@ -280,7 +293,7 @@ class _Act8Linear(torch.autograd.Function):
         _call(L_.p2n_act8_backward, "p2n_act8_backward", dev, g.data_ptr(), B, K, L, weight.data_ptr(), N, _rt.ptr(gamma), _rt.ptr(beta),
               int(frozen), kept.data_ptr(), nkept, _rt.ptr(dx), _rt.ptr(dW), _rt.ptr(db), _rt.ptr(dgamma), _rt.ptr(dbeta),
               ws.data_ptr(), nws)
-        return dx if need[0] else None, dW, db, dgamma, dbeta, None, None, None, None
+        return dx if need[0] else None, dW, db, dgamma, dbeta, None, None, None, None, None
 
 
 def act8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -301,14 +314,12 @@ def act8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     for t, name in ((w, "weight"), (bias, "bias")):
         if t is not None and not (t.device == x.device and t.dtype == torch.float32):
             raise ValueError(f"{name} must be a float32 tensor on the input's GPU")
-    h = _Act8Linear.apply(x.contiguous(), w.contiguous(), None if bias is None else bias.contiguous(), *_norm_args(norm, x))
-    _count_batch(norm)
-    return h
+    return _Act8Linear.apply(x.contiguous(), w.contiguous(), None if bias is None else bias.contiguous(), *_norm_args(norm, x))
 
 
 class _Act8NormRelu(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gamma, beta, running_mean, running_var, momentum, eps):
+    def forward(ctx, x, gamma, beta, running_mean, running_var, batches, momentum, eps):
         L_ = _lib.lib()
         B, C, L = x.shape
         dev = x.device
@@ -316,14 +327,19 @@ class _Act8NormRelu(torch.autograd.Function):
         kept, ws = _bytes(nkept, dev), _bytes(nws, dev)
         y = torch.empty((B, C, L), dtype=torch.float32, device=dev)
         _call(L_.p2n_act8_norm_relu_forward, "p2n_act8_norm_relu_forward", dev, x.data_ptr(), B, C, L, gamma.data_ptr(), beta.data_ptr(),
-              _rt.ptr(running_mean), _rt.ptr(running_var), momentum, eps, y.data_ptr(), kept.data_ptr(), nkept, ws.data_ptr(), nws)
+              _rt.ptr(running_mean), _rt.ptr(running_var), _rt.ptr(batches), momentum, eps, y.data_ptr(), kept.data_ptr(), nkept,
+              ws.data_ptr(), nws)
+        _changed(running_mean, running_var, batches)
         ctx.save_for_backward(kept, gamma)
         ctx.meta = (B, C, L, momentum < 0)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        return _once(_Act8NormRelu, ctx, g) if torch.is_grad_enabled() else _Act8NormRelu.gradients(ctx, g)
+
+    @staticmethod
+    def gradients(ctx, g):
         kept, gamma = ctx.saved_tensors
         B, C, L, frozen = ctx.meta
         L_ = _lib.lib()
@@ -335,7 +351,7 @@ class _Act8NormRelu(torch.autograd.Function):
         ws = _bytes(nws, dev)
         _call(L_.p2n_act8_norm_relu_backward, "p2n_act8_norm_relu_backward", dev, g.data_ptr(), B, C, L, gamma.data_ptr(), int(frozen),
               kept.data_ptr(), nkept, dx.data_ptr(), _rt.ptr(dgamma), _rt.ptr(dbeta), ws.data_ptr(), nws)
-        return dx, dgamma, dbeta, None, None, None, None
+        return dx, dgamma, dbeta, None, None, None, None, None
 
 
 def act8_norm_relu(x: torch.Tensor, norm: nn.BatchNorm1d) -> torch.Tensor:
@@ -346,6 +362,4 @@ def act8_norm_relu(x: torch.Tensor, norm: nn.BatchNorm1d) -> torch.Tensor:
         raise ValueError(f"x must be (B,C,L) with at least one value, got {tuple(x.shape)}")
     if norm is None:
         raise TypeError("norm must be a BatchNorm1d, got None")
-    y = _Act8NormRelu.apply(x.contiguous(), *_norm_args(norm, x))
-    _count_batch(norm)
-    return y
+    return _Act8NormRelu.apply(x.contiguous(), *_norm_args(norm, x))

@@ -220,7 +220,7 @@ def test_what_is_kept(B, K, L, norm):
     ws, h = torch.empty(nw, dtype=torch.uint8, device="cuda"), torch.empty(B, N, L, device="cuda")
     q = rt.ptr
     _lib.check(lib.p2n_act8_forward(x.data_ptr(), B, K, L, W.data_ptr(), b.data_ptr(), N, q(bn.weight) if norm else None, q(bn.bias) if norm else None,
-                                    None, None, 0.0, 1e-5, h.data_ptr(), kept.data_ptr(), nk, ws.data_ptr(), nw, rt.stream_handle(x.device)), "fwd")
+                                    None, None, None, 0.0, 1e-5, h.data_ptr(), kept.data_ptr(), nk, ws.data_ptr(), nw, rt.stream_handle(x.device)), "fwd")
     assert bool((kept[nk:] == 0x5A).all())
     NB, K4 = (L + 127) // 128, (K + 3) // 4 * 4
     up = lambda n: (n + 255) // 256 * 256                                             # noqa: E731

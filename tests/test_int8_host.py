@@ -62,7 +62,7 @@ def test_checkpoint_layers_refuse_bad_shapes():
     a = 1 << 16     # an address that is never read: every call below is refused first
 
     def fwd(x=a, K=8, N=8, gamma=None, beta=None, rm=None, rv=None, mom=0.1, h=a, kept=a, nk=1 << 20, ws=a, nw=1 << 24, B=1, L=50):
-        return lib.p2n_act8_forward(x, B, K, L, a, a, N, gamma, beta, rm, rv, mom, 1e-5, h, kept, nk, ws, nw, None)
+        return lib.p2n_act8_forward(x, B, K, L, a, a, N, gamma, beta, rm, rv, None, mom, 1e-5, h, kept, nk, ws, nw, None)
 
     assert fwd(x=None) == 1 and fwd(h=None) == 1 and fwd(N=0) == 1 and fwd(N=1025) == 1 and fwd(K=2000) == 1
     assert fwd(gamma=a) == 1                                  # gamma without beta
@@ -74,5 +74,5 @@ def test_checkpoint_layers_refuse_bad_shapes():
     assert fwd(nk=100) == 2 and fwd(nw=100) == 2 and fwd(kept=None) == 2
     assert lib.p2n_act8_backward(a, 1, 8, 50, a, 8, a, a, 0, a, 1 << 20, None, a, a, a, None, a, 1 << 24, None) == 1   # dgamma without dx
     assert lib.p2n_act8_backward(None, 1, 8, 50, a, 8, None, None, 0, a, 1 << 20, a, a, a, None, None, a, 1 << 24, None) == 1
-    assert lib.p2n_act8_norm_relu_forward(a, 1, 8, 50, None, None, None, None, 0.1, 1e-5, a, a, 1 << 20, a, 1 << 20, None) == 1
+    assert lib.p2n_act8_norm_relu_forward(a, 1, 8, 50, None, None, None, None, None, 0.1, 1e-5, a, a, 1 << 20, a, 1 << 20, None) == 1
     assert lib.p2n_act8_norm_relu_backward(a, 1, 8, 50, a, 0, a, 10, a, None, None, a, 1 << 20, None) == 2
