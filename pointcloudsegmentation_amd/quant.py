@@ -282,12 +282,11 @@ class _Act8Linear(torch.autograd.Function):
         need = ctx.needs_input_grad
         normed = gamma is not None
 
-        def out(*shape):
-            return torch.empty(shape, dtype=torch.float32, device=dev)
-
-        dgamma, dbeta = out(K) if normed and need[3] else None, out(K) if normed and need[4] else None
-        dx = out(B, K, L) if need[0] or dgamma is not None or dbeta is not None else None     # the norm's gradients are formed on its way
-        dW, db = out(N, K) if need[1] else None, out(N) if has_bias and need[2] else None
+        dgamma, dbeta = torch.empty_like(gamma) if normed and need[3] else None, torch.empty_like(beta) if normed and need[4] else None
+        # the norm's gradients are formed on dx's way
+        dx = torch.empty((B, K, L), dtype=torch.float32, device=dev) if need[0] or dgamma is not None or dbeta is not None else None
+        dW = torch.empty_like(weight) if need[1] else None
+        db = torch.empty(N, dtype=torch.float32, device=dev) if has_bias and need[2] else None
         nkept, nws = _act8_bytes("act8_linear", B, K, L, normed, N)
         ws = _bytes(nws, dev)
         _call(L_.p2n_act8_backward, "p2n_act8_backward", dev, g.data_ptr(), B, K, L, weight.data_ptr(), N, _rt.ptr(gamma), _rt.ptr(beta),
@@ -346,7 +345,7 @@ class _Act8NormRelu(torch.autograd.Function):
         g = g.contiguous()
         dev = g.device
         dx = torch.empty((B, C, L), dtype=torch.float32, device=dev)
-        dgamma, dbeta = (torch.empty(C, dtype=torch.float32, device=dev) if ctx.needs_input_grad[i] else None for i in (1, 2))
+        dgamma, dbeta = (torch.empty_like(gamma) if ctx.needs_input_grad[i] else None for i in (1, 2))
         nkept, nws = _act8_bytes("act8_norm_relu", B, C, L, True, 0)
         ws = _bytes(nws, dev)
         _call(L_.p2n_act8_norm_relu_backward, "p2n_act8_norm_relu_backward", dev, g.data_ptr(), B, C, L, gamma.data_ptr(), int(frozen),
