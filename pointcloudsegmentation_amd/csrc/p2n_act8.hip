@@ -406,7 +406,7 @@ __global__ __launch_bounds__(256, CT <= 4 ? 3 : TABK <= 512 ? 2 : 1) void p2n_ac
         bias[threadIdx.x] = A.bias && 32 * ct0 + (int)threadIdx.x < A.rows ? A.bias[32 * ct0 + threadIdx.x] : 0.f;
 
     auto stage = [&](int c, int slot) __attribute__((always_inline)) {
-        const __amdgpu_buffer_rsrc_t rs = act8_rsrc(A.img, (long)A.CTP * A.KS * 3072);
+        const __amdgpu_buffer_rsrc_t rs = act8_rsrc(A.img, (long)A.CTP * A.KS * 3 * 1024);
 #pragma unroll
         for (int i = 0; i < FW; ++i) {
             const int g = wave * FW + i, f = g < F ? g : F - 1;   // fragment of the chunk: k-step f / (3 CT), the rest in image order
@@ -1098,7 +1098,7 @@ __global__ __launch_bounds__(256, 2) void p2n_act8_both_kernel(Act8Both B) {
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = n + i < A.N && k < A.K ? B.W[(long)(n + i) * A.K + k] : 0.f;
-        bf16x8 *d = reinterpret_cast<bf16x8 *>(wt + ks * 3072) + lane;
+        bf16x8 *d = reinterpret_cast<bf16x8 *>(wt + ks * 3 * 1024) + lane;
         act8_split_rounded(v, d[0], d[64], d[128]);
     }
     __syncthreads();
@@ -1209,7 +1209,7 @@ __global__ __launch_bounds__(256, 2) void p2n_act8_both_kernel(Act8Both B) {
                 x[i] = *reinterpret_cast<const float *>(mine + (16 * ks + 8 * h + i) * 128 + ((r >> 2) ^ (4 * h + (i >> 1))) * 16 + (r & 3) * 4);
             bf16x8 xp[3];
             act8_split(x, xp[0], xp[1], xp[2]);
-            const bf16x8 *f = reinterpret_cast<const bf16x8 *>(wt + ks * 3072) + lane;
+            const bf16x8 *f = reinterpret_cast<const bf16x8 *>(wt + ks * 3 * 1024) + lane;
 #pragma unroll
             for (int c = 0; c < 6; ++c) da = MFMAB(f[64 * act8_first(c)], xp[act8_second(c)], da);
             if (ks & 1) __builtin_amdgcn_sched_barrier(0);

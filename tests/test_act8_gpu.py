@@ -332,6 +332,26 @@ def test_only_what_is_asked_for():
             t.requires_grad_(True)
 
 
+@pytest.mark.parametrize("B,K,L,N", [(2, 33, 131, 31), (1, 70, 45, 67), (3, 5, 129, 130), (17, 130, 4100, 200)])
+def test_memory_behind_the_results_is_left_as_it_was(B, K, L, N):
+    from pointcloudsegmentation_amd import _lib, runtime as rt
+    lib = _lib.lib()
+    x, W, b, g, bn = make(B, K, L, N, True)
+    nk, nw = lib.p2n_act8_kept_bytes(B, K, L, 1), lib.p2n_act8_workspace_bytes(B, K, L, N)
+    sizes = {"h": B * N * L, "dx": B * K * L, "dW": N * K, "db": N, "dgamma": K, "dbeta": K, "kept": nk // 4, "ws": (nw + 3) // 4}
+    room = {k: torch.full((n + 1024,), 7.0, device="cuda") for k, n in sizes.items()}
+    p = {k: t.data_ptr() for k, t in room.items()}
+    s = rt.stream_handle(x.device)
+    _lib.check(lib.p2n_act8_forward(x.data_ptr(), B, K, L, W.data_ptr(), rt.ptr(b), N, bn.weight.data_ptr(), bn.bias.data_ptr(), None, None, None, 0.0,
+                                    1e-5, p["h"], p["kept"], nk, p["ws"], nw, s), "forward")
+    _lib.check(lib.p2n_act8_backward(g.data_ptr(), B, K, L, W.data_ptr(), N, bn.weight.data_ptr(), bn.bias.data_ptr(), 0, p["kept"], nk, p["dx"], p["dW"],
+                                     p["db"], p["dgamma"], p["dbeta"], p["ws"], nw, s), "backward")
+    for k, n in sizes.items():
+        assert bool((room[k][n:] == 7.0).all()), k
+        if k not in ("kept", "ws"):
+            assert not bool((room[k][:n] == 7.0).any()), k
+
+
 def test_strides_expanded_gradients_and_second_backward():
     from pointcloudsegmentation_amd import quant
     x, W, b, g, norm = make(2, 40, 200, 24, True)
@@ -356,6 +376,44 @@ def test_strides_expanded_gradients_and_second_backward():
     with pytest.raises(RuntimeError):
         q = torch.autograd.grad(quant.act8_linear(x, W, b), [x], g, create_graph=True)[0]
         torch.autograd.grad(q.sum(), [W])
+
+
+def test_no_second_derivative():
+    """under create_graph the gradients are the same, and differentiating them is refused instead of answered with nothing"""
+    from pointcloudsegmentation_amd import quant
+    x, W, b, g, norm = make(2, 20, 150, 12, True)
+    plain = torch.autograd.grad(quant.act8_linear(x, W, b, norm=norm), [x, W], g)
+    g.requires_grad_()
+    again = torch.autograd.grad(quant.act8_linear(x, W, b, norm=norm), [x, W], g, create_graph=True)
+    for p, q in zip(plain, again):
+        assert torch.equal(p, q)
+        with pytest.raises(RuntimeError):
+            q.sum().backward(retain_graph=True)
+    go = torch.randn(2, 20, 150, device="cuda", requires_grad=True)
+    dx, = torch.autograd.grad(quant.act8_norm_relu(x, norm), [x], go, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+
+
+def test_buffers_show_that_they_changed():
+    """the running statistics and the count of batches are written by the kernels: their versions move, as BatchNorm1d moves them"""
+    from pointcloudsegmentation_amd import quant
+    x, W, b, g, norm = make(2, 20, 150, 12, True)
+    norm.train()
+    for call in (lambda: quant.act8_linear(x, W, b, norm=norm), lambda: quant.act8_norm_relu(x, norm)):
+        before = [t._version for t in norm.buffers()]
+        n = int(norm.num_batches_tracked)
+        call()
+        assert int(norm.num_batches_tracked) == n + 1
+        assert all(t._version > v for t, v in zip(norm.buffers(), before))
+    norm.eval()
+    before = [t._version for t in norm.buffers()]
+    quant.act8_linear(x, W, b, norm=norm)
+    assert [t._version for t in norm.buffers()] == before
+    norm.train()
+    norm.num_batches_tracked = norm.num_batches_tracked.cpu()
+    with pytest.raises(ValueError):
+        quant.act8_linear(x, W, b, norm=norm)
 
 
 def test_repeats_are_identical():

@@ -137,6 +137,23 @@ def test_linear_shapes_and_strides():
     assert torch.equal(quant.int8_linear(wideb[:, 3:43], w), quant.int8_linear(xb, w))
 
 
+@pytest.mark.parametrize("T,K,N", [(1, 5, 3), (7, 70, 33), (13, 5000, 17), (40, 66, 129), (130, 33, 65), (1000, 40, 300), (16500, 64, 1030)])
+def test_linear_leaves_memory_behind_its_result(T, K, N):
+    from pointcloudsegmentation_amd import _lib, quant, runtime as rt
+    lib = _lib.lib()
+    for dtype in (torch.float32, torch.bfloat16):
+        x, W, b = make(T, K, N, dtype)
+        w = quant.Int8Weight(W, b)
+        want = quant.int8_linear(x, w)
+        guard = torch.full((T * N + 4096,), 7.0, device="cuda", dtype=dtype)
+        nws = lib.p2n_int8_linear_workspace_bytes(T, K, N)
+        ws = torch.full((nws + 4096,), 0x5A, device="cuda", dtype=torch.uint8)
+        _lib.check(lib.p2n_int8_linear(x.data_ptr(), int(dtype == torch.bfloat16), T, K, K, w.image.data_ptr(), N, 0, guard.data_ptr(), ws.data_ptr(), nws,
+                                       rt.stream_handle(x.device)), "p2n_int8_linear")
+        assert torch.equal(guard[:T * N].view(T, N), want)
+        assert bool((guard[T * N:] == 7.0).all()) and bool((ws[nws:] == 0x5A).all())
+
+
 def test_linear_zero_and_nonfinite_tokens():
     """a token of zeros gives the bias; a NaN or an infinity spoils its own row and no other; so with the weight's rows"""
     from pointcloudsegmentation_amd import quant
