@@ -56,15 +56,23 @@ _TOKEN_TYPES = (torch.float32, torch.bfloat16)
 
 def _rows(x: torch.Tensor):
     """(..., K) -> T, K, row stride and a tensor whose memory holds those rows"""
-    if x.dim() < 1:
+    shape = x.shape
+    if not shape:
         raise ValueError("x must have at least one dimension")
-    K = x.size(-1)
+    K = shape[-1]
     if K < 1:
-        raise ValueError(f"x must have at least one value in a token, got {tuple(x.shape)}")
-    T = x.numel() // K
-    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= K:
-        return T, K, x.stride(0), x
-    return T, K, K, x.contiguous()
+        raise ValueError(f"x must have at least one value in a token, got {tuple(shape)}")
+    if len(shape) == 2:
+        ld, step = x.stride()
+        if step == 1 and ld >= K:
+            return shape[0], K, ld, x
+    return x.numel() // K, K, K, x.contiguous()
+
+
+@lru_cache(maxsize=256)
+def _linear_bytes(T: int, K: int, N: int) -> int:
+    """size of int8_linear's workspace (a number of the shape alone)"""
+    return _lib.lib().p2n_int8_linear_workspace_bytes(T, K, N)
 
 
 def quantize_tokens(x: torch.Tensor):
@@ -137,19 +145,25 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, relu: bool = False) -> torc
     T, K, ld, rows = _rows(x)
     if K != weight.in_features:
         raise ValueError(f"x has {K} values in a token, the weight takes {weight.in_features}")
-    if x.device != weight.device:
-        raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
-    L = _lib.lib()
+    dev = x.device
+    if dev != weight.device:
+        raise ValueError(f"x is on {dev}, the weight on {weight.device}")
     N = weight.out_features
-    y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    y = x.new_empty((*x.shape[:-1], N))
     if T == 0:
         return y
     # from torch's allocator and not from the stream's shared buffer: a captured graph keeps the memory it was captured with
-    nws = L.p2n_int8_linear_workspace_bytes(T, K, N)
-    ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
-    _call(L.p2n_int8_linear, "p2n_int8_linear", x.device, rows.data_ptr(), int(x.dtype == torch.bfloat16), T, K, ld,
+    nws = _linear_bytes(T, K, N)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
+    _call(_lib.lib().p2n_int8_linear, "p2n_int8_linear", dev, rows.data_ptr(), int(x.dtype == torch.bfloat16), T, K, ld,
           weight.image.data_ptr(), N, int(relu), y.data_ptr(), _rt.ptr(ws), nws)
     return y
+
+
+@lru_cache(maxsize=32)
+def _arrays(layers: int):
+    """C types of the widths and the images of so many layers"""
+    return ctypes.c_int * (layers + 1), ctypes.c_void_p * layers
 
 
 def int8_mlp(x: torch.Tensor, weights: Sequence[Int8Weight], last_relu: bool = True, group: int = 0) -> torch.Tensor:
@@ -165,12 +179,12 @@ def int8_mlp(x: torch.Tensor, weights: Sequence[Int8Weight], last_relu: bool = T
     if not weights:
         raise ValueError("int8_mlp needs at least one layer")
     B, C, L = x.shape
-    dims = [C]
+    dims, dev = [C], x.device
     for i, w in enumerate(weights):
         if w.in_features != dims[-1]:
             raise ValueError(f"layer {i} takes {w.in_features} channels, gets {dims[-1]}")
-        if w.device != x.device:
-            raise ValueError(f"x is on {x.device}, the weight of layer {i} on {w.device}")
+        if w.device != dev:
+            raise ValueError(f"x is on {dev}, the weight of layer {i} on {w.device}")
         dims.append(w.out_features)
     if group < 0 or (group and L % group):
         raise ValueError(f"columns per cloud ({L}) are not a multiple of the group size ({group})")
@@ -178,14 +192,14 @@ def int8_mlp(x: torch.Tensor, weights: Sequence[Int8Weight], last_relu: bool = T
     lib = _lib.lib()
     # in the kernel: groups of 16 or 32; larger multiples of 32 finish on the maxima of 32, other sizes on the columns
     inner = 0 if group <= 1 else group if group == 16 else 32 if group % 32 == 0 else 0
-    out = torch.empty((B, dims[-1], L // inner if inner else L), dtype=torch.float32, device=x.device)
-    arr = (ctypes.c_int * len(dims))(*dims)
-    images = (ctypes.c_void_p * len(weights))(*[w.image.data_ptr() for w in weights])
-    _call(lib.p2n_int8_mlp, "p2n_int8_mlp", x.device, x.data_ptr(), B, L, len(weights), arr, images, int(last_relu), inner, out.data_ptr())
+    out = x.new_empty((B, dims[-1], L // inner if inner else L))
+    ints, pointers = _arrays(len(weights))
+    _call(lib.p2n_int8_mlp, "p2n_int8_mlp", dev, x.data_ptr(), B, L, len(weights), ints(*dims), pointers(*[w.image.data_ptr() for w in weights]),
+          int(last_relu), inner, out.data_ptr())
     rest = group // inner if inner else group
     if rest > 1:
-        res = torch.empty((B, dims[-1], L // group), dtype=torch.float32, device=x.device)
-        _call(lib.p2n_max_of_columns, "p2n_max_of_columns", x.device, out.data_ptr(), res.numel(), rest, res.data_ptr())
+        res = x.new_empty((B, dims[-1], L // group))
+        _call(lib.p2n_max_of_columns, "p2n_max_of_columns", dev, out.data_ptr(), res.numel(), rest, res.data_ptr())
         out = res
     return out
 
