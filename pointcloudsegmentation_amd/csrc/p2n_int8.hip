@@ -427,8 +427,8 @@ __global__ __launch_bounds__(64 * WR * WC, TM * TN >= 4 ? 2 : 4) void p2n_int8_g
 // ---------------------------------------------------------------- few tokens
 // Up to 16 TT tokens: the weights' way from memory is the time, so a workgroup takes 16 channels and its eight waves share the length
 // K, each streaming its part of the weights straight from memory into 16 x 16 x 64 products; the eight sums meet in LDS
-// (whole numbers: any order; 16 tokens x 4096 x 4096: 6.5 us, 2.6 TB/s of weights).  OWN: up to 8 tokens of up to 4096 values are put into 8 bits here, a wave a token, into
-// LDS; otherwise the tokens' fragments come from p2n_int8_tile_kernel.
+// (whole numbers: any order; 16 tokens x 4096 x 4096: 6.5 us, 2.6 TB/s of weights).  OWN: up to 8 tokens of up to 4096 values are put
+// into 8 bits here, a wave a token, into LDS; otherwise the tokens' fragments come from p2n_int8_tile_kernel.
 #define MFMA_I8_16(a, b, c) __builtin_amdgcn_mfma_i32_16x16x64_i8((a), (b), (c), 0, 0, 0)
 #define INT8_OWN_K 4096
 template <typename TX, int TT, bool OWN, bool VEC>
@@ -519,8 +519,9 @@ extern "C" int p2n_quantize_tokens(const void *x, int bf16, long T, int K, long 
     return P2N_OK;
 }
 
-// Which kernel: up to 64 tokens the one that streams the weights once (16 tokens x 4096 x 4096: 7 us against 49 with 128 x 128
-// tiles), and of these up to 8 tokens of up to 4096 values put into 8 bits on the way (one launch instead of two).
+// Which kernel: up to 64 tokens the one that streams the weights once (16 tokens x 4096 x 4096: 7 us against 13 with 64 x 64 tiles), and
+// of these up to 8 tokens of up to 4096 values put into 8 bits on the way: one launch instead of two (one token of 512 values 4.5 us
+// against 4 + 3; 8 of 4096 12 against 4.5 + 6.8; 16 of 4096 19.5 against 4.7 + 6.5).
 static bool int8_is_few(long T) { return T <= 64; }
 static bool int8_is_own(long T, int K) { return T <= 8 && K <= INT8_OWN_K; }
 

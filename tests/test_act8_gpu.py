@@ -163,16 +163,17 @@ def test_layer_against_its_definition(B, K, L, N, mode):
             assert int(norm.num_batches_tracked) == 0
 
 
-@pytest.mark.parametrize("L", [4100, 4099, 4160])
-def test_wide_weight_gradient_with_part_of_a_block_at_the_end(L):
+@pytest.mark.parametrize("L,offset", [(4100, 0), (4099, 0), (4160, 0), (4100, 1), (4160, 3)])
+def test_wide_weight_gradient_with_part_of_a_block_at_the_end(L, offset):
     """long enough for 128 x 128 tiles of dW; the last block of a cloud ends in its first, its third piece of 32 points, rows start on 16
-    bytes or not, and the last tile holds 72 of 128 rows: what lies behind a cloud's last point is neither read nor added"""
+    bytes or not (by their length, by where g begins), and the last tile holds 72 of 128 rows: what lies behind a cloud's last point
+    is neither read nor added"""
     from pointcloudsegmentation_amd import quant
     B, K, N = 17, 130, 200
     x, W, b, g, _ = make(B, K, L, N, False)
     room = torch.full((B * N * L + 4096,), float("nan"), device="cuda")
-    room[:B * N * L] = g.reshape(-1)
-    g = room[:B * N * L].view(B, N, L)
+    room[offset:offset + B * N * L] = g.reshape(-1)
+    g = room[offset:offset + B * N * L].view(B, N, L)
     ref = Definition(x, W, b, None).backward(g)
     h = quant.act8_linear(x, W, b)
     dW, db = torch.autograd.grad(h, [W, b], g)
@@ -308,9 +309,10 @@ def test_gradients_against_differences():
         assert abs(float((grads[i] * d).sum()) - diff) <= 0.01 * size, i
 
 
-def test_only_what_is_asked_for():
+@pytest.mark.parametrize("B,K,L,N", [(2, 40, 200, 24), (2, 70, 200, 24), (2, 40, 200, 100), (17, 130, 4100, 200)])
+def test_only_what_is_asked_for(B, K, L, N):
     from pointcloudsegmentation_amd import quant
-    x, W, b, g, norm = make(2, 40, 200, 24, True)
+    x, W, b, g, norm = make(B, K, L, N, True)
     full = torch.autograd.grad(quant.act8_linear(x, W, b, norm=norm), [x, W, b, norm.weight, norm.bias], g)
     for wanted in ([0], [1], [2], [3], [4], [1, 2], [0, 3]):
         ts = [x, W, b, norm.weight, norm.bias]
