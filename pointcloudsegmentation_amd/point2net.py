@@ -124,7 +124,8 @@ class Point2Net(nn.Module):
         self._cache = _PackedCache()
 
     # Not in the reference: what training on GPU tensors keeps of the activations -- None (float32, as the reference) or
-    # "int8" (quant.act8_linear: 1.16 bytes a value, gradients from the kept values; the products stay float32-accurate)
+    # "int8" (quant.act8_linear: 1.16 bytes a value, gradients from the kept values; the products stay float32-accurate,
+    # whatever `precision` says, which then holds for eval alone)
     @property
     def checkpoint(self):
         return self.encoder.checkpoint
