@@ -705,25 +705,30 @@ __device__ __forceinline__ float int8_mlp_par(const MlpLayer &Y, int ct, int lan
     return Y.scale[32 * (ct + (lane >> 5) * Y.CT) + (lane & 31)];
 }
 __device__ __forceinline__ void int8_mlp_values(const i32x16 &acc, const float *par, int h, float s, bool relu, float (&y)[16], unsigned &am) {
+    const int floor = relu ? 0 : (int)0x80000000;        // nothing is below it as a whole number
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
         const f32x4 sc = *reinterpret_cast<const f32x4 *>(par + 8 * g + 4 * h), bi = *reinterpret_cast<const f32x4 *>(par + 32 + 8 * g + 4 * h);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float v = (float)acc[4 * g + j] * sc[j] * s + bi[j];
-            const int bv = __float_as_int(v), u = relu ? (bv > 0 ? bv : 0) : bv;
+            const int bv = __float_as_int(v), u = bv > floor ? bv : floor;
             y[4 * g + j] = __int_as_float(u);
             am = (unsigned)u > am ? (unsigned)u : am;
         }
     }
 }
 
-__device__ __forceinline__ void int8_mlp_top(const float (&e)[16], unsigned &am) {
+// real: channels from the tile's first on; groups of eight past them hold nothing
+__device__ __forceinline__ void int8_mlp_top(const float (&e)[16], int real, unsigned &am) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const unsigned u = p2n_absbits(e[i]);
-        am = u > am ? u : am;
-    }
+    for (int g = 0; g < 4; ++g)
+        if (8 * g < real)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const unsigned u = p2n_absbits(e[4 * g + j]);
+                am = u > am ? u : am;
+            }
 }
 
 // codes of an input tile; groups of eight channels past the last one are zero: nothing to form (a level's first layer has six)
@@ -747,10 +752,12 @@ __device__ __forceinline__ unsigned int8_halves(unsigned am) {
 }
 
 // Up to 64 channels everywhere: one wave carries its 32 points through every layer in registers.  Bound by the vector instructions that
-// scale the sums and form the next codes, some 11 a value (78 % of the issue slots): 6-32-32-64 with groups of 32 over 16 x 65536 points
-// 53 us, of which the memory's share is 7; the maximum by exchanges between lanes instead of in registers: 62.
-__global__ __launch_bounds__(256, 4) void p2n_int8_mlp_narrow_kernel(Int8MlpArgs A) {
-    __shared__ __attribute__((aligned(16))) float own[4][2][64];           // the wave's: parameters of its tiles, in the end scales of its points
+// scale the sums and form the next codes, some 11 a value: 6-32-32-64 with groups of 32 over 16 x 65536 points 48 us, of which
+// the memory's share is 7; the maximum by exchanges between lanes instead of in registers: 9 more.
+// HT: tiles of 32 channels that the input and the layers between have.  With one, five waves fit a SIMD instead of four (56 -> 48 us).
+template <int HT>
+__global__ __launch_bounds__(256, HT == 1 ? 5 : 4) void p2n_int8_mlp_narrow_kernel(Int8MlpArgs A) {
+    __shared__ __attribute__((aligned(16))) float own[4][HT][64];           // the wave's: parameters of its tiles, in the end scales of its points
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int p = lane & 31, h = lane >> 5;
     const i32x16 zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
@@ -761,19 +768,19 @@ __global__ __launch_bounds__(256, 4) void p2n_int8_mlp_narrow_kernel(Int8MlpArgs
     const bool valid = l0 + p < A.L;
     const unsigned off = (unsigned)((4 * h * A.L + (valid ? l0 + p : A.L - 1)) * 4);   // bytes; L <= 2^24 keeps 32 rows below 2^31
     unsigned am = 0;
-    float s, v[2][16];
-    int cq[2][4];
+    float s, v[HT][16];
+    int cq[HT][4];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int kt = 0; kt < HT; ++kt)
         if (kt < KT0) int8_mlp_load(A.x + b * A.C * A.L, A.L, A.C, kt, off, v[kt]);
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-        if (kt < KT0) int8_mlp_top(v[kt], am);
+    for (int kt = 0; kt < HT; ++kt)
+        if (kt < KT0) int8_mlp_top(v[kt], A.C - 32 * kt, am);
     s = p2n_q8_scale(int8_halves(am));
     {
         const P2nQ8 Q = p2n_q8_make(s);
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
+        for (int kt = 0; kt < HT; ++kt) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) cq[kt][g] = 0;
             if (kt < KT0) int8_mlp_codes(v[kt], A.C - 32 * kt, Q, cq[kt]);
@@ -782,47 +789,56 @@ __global__ __launch_bounds__(256, 4) void p2n_int8_mlp_narrow_kernel(Int8MlpArgs
 #pragma unroll 1
     for (int li = 0; li < A.nl; ++li) {
         const MlpLayer Y = A.layer[li];
-        const bool last = li == A.nl - 1, relu = !last || A.last_relu;
         const i32x4 *wf = reinterpret_cast<const i32x4 *>(Y.img) + lane;
+        i32x4 x[HT];
+#pragma unroll
+        for (int kt = 0; kt < HT; ++kt) x[kt] = i32x4{cq[kt][0], cq[kt][1], cq[kt][2], cq[kt][3]};
         // the image has an even number of k-tiles: where the second holds no channels its codes are zero
-        if (last && A.group) {
-            own[wave][0][p] = s;
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+        if (li == A.nl - 1) {
+            if (A.group) {
+                own[wave][0][p] = s;
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            }
 #pragma unroll 1
             for (int ct = 0; ct < Y.CT; ++ct) {
-                const i32x4 w0 = wf[ct * Y.KTI * 64], w1 = wf[(ct * Y.KTI + 1) * 64];
-                i32x16 acc = MFMA_I8((i32x4{cq[0][0], cq[0][1], cq[0][2], cq[0][3]}), w0, zero);
-                acc = MFMA_I8((i32x4{cq[1][0], cq[1][1], cq[1][2], cq[1][3]}), w1, acc);
-                int8_mlp_groups(A, Y, ct, acc, own[wave][0], b, l0, lane);
+                i32x16 acc = zero;
+                if (A.group) {
+#pragma unroll
+                    for (int kt = 0; kt < HT; ++kt) acc = MFMA_I8(x[kt], wf[(ct * Y.KTI + kt) * 64], acc);
+                    int8_mlp_groups(A, Y, ct, acc, own[wave][0], b, l0, lane);
+                } else {
+                    own[wave][0][lane] = int8_mlp_par(Y, ct, lane);
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                    for (int kt = 0; kt < HT; ++kt) acc = MFMA_I8(wf[(ct * Y.KTI + kt) * 64], x[kt], acc);
+                    float y[16];
+                    int8_mlp_values(acc, own[wave][0], h, s, A.last_relu, y, am);
+                    int8_mlp_out(A, Y.N, b, valid, off, ct, y);
+                }
             }
             break;
         }
-        float y[2][16];
+        float y[HT][16];
         am = 0;
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct)
+        for (int ct = 0; ct < HT; ++ct)
             if (ct < Y.CT) own[wave][ct][lane] = int8_mlp_par(Y, ct, lane);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct)
+        for (int ct = 0; ct < HT; ++ct)
             if (ct < Y.CT) {
-                const i32x4 w0 = wf[ct * Y.KTI * 64], w1 = wf[(ct * Y.KTI + 1) * 64];
-                i32x16 acc = MFMA_I8(w0, (i32x4{cq[0][0], cq[0][1], cq[0][2], cq[0][3]}), zero);
-                acc = MFMA_I8(w1, (i32x4{cq[1][0], cq[1][1], cq[1][2], cq[1][3]}), acc);
-                int8_mlp_values(acc, own[wave][ct], h, s, relu, y[ct], am);
-            }
-        if (last) {
+                i32x16 acc = zero;
 #pragma unroll
-            for (int ct = 0; ct < 2; ++ct)
-                if (ct < Y.CT) int8_mlp_out(A, Y.N, b, valid, off, ct, y[ct]);
-            break;
-        }
+                for (int kt = 0; kt < HT; ++kt) acc = MFMA_I8(wf[(ct * Y.KTI + kt) * 64], x[kt], acc);
+                int8_mlp_values(acc, own[wave][ct], h, s, true, y[ct], am);
+            }
         s = p2n_q8_scale(int8_halves(am));
         const P2nQ8 Q = p2n_q8_make(s);
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct)
+        for (int ct = 0; ct < HT; ++ct)
             if (ct < Y.CT) p2n_q8_pack(y[ct], Q, cq[ct]);
     }
 }
@@ -862,7 +878,7 @@ __global__ __launch_bounds__(64 * NW, 4) void p2n_int8_mlp_wide_kernel(Int8MlpAr
     ahead(A.layer[0], wave);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if (wave + NW * i < KT0) int8_mlp_top(v[i], am);
+        if (wave + NW * i < KT0) int8_mlp_top(v[i], A.C - 32 * (wave + NW * i), am);
     // the largest of every point over the waves -> its scale
     auto join = [&]() __attribute__((always_inline)) {
         const unsigned o = int8_halves(am);
@@ -954,7 +970,7 @@ extern "C" int p2n_int8_mlp(const float *x, int B, long L, int nl, const int *di
     Int8MlpArgs a = {};
     a.x = x; a.out = out; a.L = L; a.tiles = (L + 31) / 32; a.total = a.tiles * B;
     a.C = dims[0]; a.nl = nl; a.last_relu = last_relu ? 1 : 0; a.group = group;
-    int ctm = 0, ktm = (dims[0] + 31) / 32;
+    int ctm = 0, ktm = (dims[0] + 31) / 32, inside = ktm;      // tiles of the widest layer, of the input; of all that pass from layer to layer
     for (int l = 0; l < nl; ++l) {
         const char *img = (const char *)images_host[l];
         P2N_REQUIRE(img && ((uintptr_t)img & 15) == 0, "p2n_int8_mlp: the image of layer %d is null or not 16-byte aligned", l);
@@ -963,13 +979,15 @@ extern "C" int p2n_int8_mlp(const float *x, int B, long L, int nl, const int *di
         y.img = img; y.scale = (const float *)(img + I.scale); y.bias = (const float *)(img + I.bias);
         y.KT = (dims[l] + 31) / 32; y.KTI = I.KT; y.CT = I.CT; y.N = dims[l + 1];
         if (I.CT > ctm) ctm = I.CT;
+        if (l < nl - 1 && I.CT > inside) inside = I.CT;
     }
     const int waves = ctm <= 2 && ktm <= 2 ? 1 : ctm <= 4 && ktm <= 16 ? 4 : 8;     // of 32 columns; a launch holds less than 2^32 threads
     P2N_REQUIRE(a.total * waves * 64 <= (1L << 32) - 512, "p2n_int8_mlp: too many columns (%ld tiles of 32)", a.total);
     hipStream_t s = (hipStream_t)stream_;
     const int ps = p2n_prof_begin(P2N_K_INT8_MLP, s);
     // one wave to 32 points up to 64 channels (fewer registers than four waves would share out), four up to 128, eight up to 256
-    if (waves == 1) hipLaunchKernelGGL(p2n_int8_mlp_narrow_kernel, dim3((unsigned)((a.total + 3) / 4)), dim3(256), 0, s, a);
+    if (waves == 1 && inside == 1) hipLaunchKernelGGL(p2n_int8_mlp_narrow_kernel<1>, dim3((unsigned)((a.total + 3) / 4)), dim3(256), 0, s, a);
+    else if (waves == 1) hipLaunchKernelGGL(p2n_int8_mlp_narrow_kernel<2>, dim3((unsigned)((a.total + 3) / 4)), dim3(256), 0, s, a);
     else if (waves == 4 && group) hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<4, true>), dim3((unsigned)a.total), dim3(256), 0, s, a);
     else if (waves == 4) hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<4, false>), dim3((unsigned)a.total), dim3(256), 0, s, a);
     else if (group) hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<8, true>), dim3((unsigned)a.total), dim3(512), 0, s, a);
