@@ -845,10 +845,12 @@ __global__ __launch_bounds__(256, HT == 1 ? 5 : 4) void p2n_int8_mlp_narrow_kern
 
 // Wider layers: NW waves carry 32 points together, a wave its share of the channel tiles.  Codes go round through LDS in operand order; a point's
 // maximum is joined over the waves there too.  Two barriers a layer; a layer's first weights are on their way before the last one ends.
-// 131-128-128-128-64 over 16 x 8192 points: 46 us (vector instructions 60 % of the issue slots, memory 20 us); one wave for all channels: 83.
-template <int NW, bool GROUPS>
-__global__ __launch_bounds__(64 * NW, 4) void p2n_int8_mlp_wide_kernel(Int8MlpArgs A) {
-    constexpr int KTI = 4 * NW;      // k-tiles of the input: 1024 (512) channels in, a channel tile a wave: 256 (128) out
+// 131-128-128-128-64 over 16 x 8192 points: 43 us (vector instructions 65 % of the issue slots, memory 20 us); one wave for all channels: 83.
+// IR: k-tiles of the input a wave holds: 4, or 2 where that is enough and five waves a SIMD have work (43 us against 46).  With few
+// columns the registers are worth more than the fifth wave (384-256-256 over 515 columns: 9.2 us against 8.6).
+template <int NW, bool GROUPS, int IR>
+__global__ __launch_bounds__(64 * NW, IR == 2 ? 5 : 4) void p2n_int8_mlp_wide_kernel(Int8MlpArgs A) {
+    constexpr int KTI = IR * NW;     // k-tiles of the input, IR a wave; a channel tile a wave: 256 (128) out
     constexpr int AHEAD = 4;                                // weight fragments on their way
     __shared__ __attribute__((aligned(16))) char codes[KTI * 1024];
     __shared__ unsigned top[NW][32];
@@ -862,10 +864,10 @@ __global__ __launch_bounds__(64 * NW, 4) void p2n_int8_mlp_wide_kernel(Int8MlpAr
     const float *xb = A.x + b * A.C * A.L;
     const unsigned off = (unsigned)((4 * h * A.L + (valid ? l : A.L - 1)) * 4);
     const int KT0 = A.layer[0].KT;
-    float v[4][16];
+    float v[IR][16];
     unsigned am = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < IR; ++i)
         if (wave + NW * i < KT0) int8_mlp_load(xb, A.L, A.C, wave + NW * i, off, v[i]);
     i32x4 w[AHEAD];
     float pw;
@@ -877,7 +879,7 @@ __global__ __launch_bounds__(64 * NW, 4) void p2n_int8_mlp_wide_kernel(Int8MlpAr
     };
     ahead(A.layer[0], wave);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < IR; ++i)
         if (wave + NW * i < KT0) int8_mlp_top(v[i], A.C - 32 * (wave + NW * i), am);
     // the largest of every point over the waves -> its scale
     auto join = [&]() __attribute__((always_inline)) {
@@ -894,7 +896,7 @@ __global__ __launch_bounds__(64 * NW, 4) void p2n_int8_mlp_wide_kernel(Int8MlpAr
     {
         const P2nQ8 Q = p2n_q8_make(s);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < IR; ++i)
             if (wave + NW * i < KT0) {
                 int c[4];
                 int8_mlp_codes(v[i], A.C - 32 * (wave + NW * i), Q, c);
@@ -953,6 +955,16 @@ __global__ __launch_bounds__(64 * NW, 4) void p2n_int8_mlp_wide_kernel(Int8MlpAr
     }
 }
 
+template <int NW>
+static void int8_launch_wide(const Int8MlpArgs &a, int ktm, hipStream_t s) {
+    const dim3 grid((unsigned)a.total), blk(64 * NW);
+    const bool two = ktm <= 2 * NW && a.total * NW > 4096;          // more waves than four a SIMD hold
+    if (two && a.group) hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<NW, true, 2>), grid, blk, 0, s, a);
+    else if (two) hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<NW, false, 2>), grid, blk, 0, s, a);
+    else if (a.group) hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<NW, true, 4>), grid, blk, 0, s, a);
+    else hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<NW, false, 4>), grid, blk, 0, s, a);
+}
+
 // x (B, dims[0], L) -> out (B, dims[nl], L), or (B, dims[nl], L/group) with the maximum over groups of 16 or 32 consecutive
 // columns; images_host: HOST array of nl DEVICE pointers (p2n_int8_pack_weight).  ReLU behind every layer but the last,
 // behind that one if last_relu.
@@ -988,10 +1000,8 @@ extern "C" int p2n_int8_mlp(const float *x, int B, long L, int nl, const int *di
     // one wave to 32 points up to 64 channels (fewer registers than four waves would share out), four up to 128, eight up to 256
     if (waves == 1 && inside == 1) hipLaunchKernelGGL(p2n_int8_mlp_narrow_kernel<1>, dim3((unsigned)((a.total + 3) / 4)), dim3(256), 0, s, a);
     else if (waves == 1) hipLaunchKernelGGL(p2n_int8_mlp_narrow_kernel<2>, dim3((unsigned)((a.total + 3) / 4)), dim3(256), 0, s, a);
-    else if (waves == 4 && group) hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<4, true>), dim3((unsigned)a.total), dim3(256), 0, s, a);
-    else if (waves == 4) hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<4, false>), dim3((unsigned)a.total), dim3(256), 0, s, a);
-    else if (group) hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<8, true>), dim3((unsigned)a.total), dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((p2n_int8_mlp_wide_kernel<8, false>), dim3((unsigned)a.total), dim3(512), 0, s, a);
+    else if (waves == 4) int8_launch_wide<4>(a, ktm, s);
+    else int8_launch_wide<8>(a, ktm, s);
     p2n_prof_end(ps, s);
     P2N_CHECK_HIP(hipGetLastError());
     return P2N_OK;
