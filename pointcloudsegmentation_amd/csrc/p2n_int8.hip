@@ -752,9 +752,9 @@ __device__ __forceinline__ unsigned int8_halves(unsigned am) {
 }
 
 // Up to 64 channels everywhere: one wave carries its 32 points through every layer in registers.  Bound by the vector instructions that
-// scale the sums and form the next codes, some 11 a value: 6-32-32-64 with groups of 32 over 16 x 65536 points 48 us, of which
-// the memory's share is 7; the maximum by exchanges between lanes instead of in registers: 9 more.
-// HT: tiles of 32 channels that the input and the layers between have.  With one, five waves fit a SIMD instead of four (56 -> 48 us).
+// scale the sums and form the next codes, some 11 a value (88 % of the issue slots): 6-32-32-64 with groups of 32 over 16 x 65536 points 47 us,
+// of which the memory's share is 7; the maximum by exchanges between lanes instead of in registers: 9 more.
+// HT: tiles of 32 channels that the input and the layers between have.  With one, five waves fit a SIMD instead of four (53 -> 47 us).
 template <int HT>
 __global__ __launch_bounds__(256, HT == 1 ? 5 : 4) void p2n_int8_mlp_narrow_kernel(Int8MlpArgs A) {
     __shared__ __attribute__((aligned(16))) float own[4][HT][64];           // the wave's: parameters of its tiles, in the end scales of its points
