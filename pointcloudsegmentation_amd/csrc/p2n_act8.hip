@@ -1255,7 +1255,8 @@ __global__ __launch_bounds__(256, 2) void p2n_act8_both_kernel(Act8Both B) {
 }
 
 // out[i] = sum over slices, in a fixed order: the slices dealt to R rows of threads, 1024 / R results a workgroup; R = 4 where there are
-// few slices of so many results that the card is full (384 -> 256, 21 slices: 4.2 us against 8.7; 67 -> 100: 4.0 against 2.8).  The first n0 results are dW, the others db (either may be NULL).  The first split_wgs
+// few slices of so many results that the card is full (384 -> 256, 21 slices: 4.2 us against 8.7; 256 -> 256, 64: 8.8 against 9.5;
+// with 67 -> 100, 26 workgroups to 209, it gains nothing).  The first n0 results are dW, the others db (either may be NULL).  The first split_wgs
 // workgroups make the image of W^T.
 template <int R>
 __global__ __launch_bounds__(1024) void p2n_act8_join_kernel(const float *__restrict__ part, long n, long n0, int slices, float *__restrict__ dW, float *__restrict__ db,
