@@ -4,7 +4,7 @@ The 8-bit rule that all of them share: a set of values v has the scale s = float
 q = clamp(round_half_even(v / s), -127, 127), the quotient being exact; s = 0 gives q = 0.
 
   linear   int8_linear: rows of K values (tokens), one scale a row; weights (N, K), one scale a channel;
-           y = ((sum_k qx qw) * sw) * sx + b, ReLU if asked
+           y = ((sum_k qx qw) * sx) * sw + b, ReLU if asked
   mlp      int8_mlp: the same product over the columns of (B, C, L), layer after layer with ReLU between, the hidden
            float32 values put into 8 bits again for the next layer; optionally the maximum over groups of columns
   act8     act8_linear, forward and backward: h = W relu(norm(x)) + b (or W x + b) whose input is kept for the backward
@@ -150,7 +150,7 @@ def _plain_linear(state):
     x = state["x"]
     (qw, sw, b), = state["weights"]
     qx, sx = _rule(x, 1)
-    y = (qx @ qw.t()) * sw.t() * sx
+    y = (qx @ qw.t()) * sx * sw.t()
     y = y if b is None else y + b
     return (y.clamp_min(0) if state["case"]["relu"] else y).to(x.dtype)
 
@@ -159,7 +159,7 @@ def _plain_mlp(state):
     h, weights = state["x"], state["weights"]
     for i, (qw, sw, b) in enumerate(weights):
         qx, sx = _rule(h, 1)
-        h = torch.matmul(qw, qx) * sw * sx + b[:, None]        # K <= 1024: the sums are whole numbers below 2^24, exact
+        h = torch.matmul(qw, qx) * sx * sw + b[:, None]        # K <= 1024: the sums are whole numbers below 2^24, exact
         if i + 1 < len(weights) or state["case"]["last_relu"]:
             h = h.clamp_min(0)
     if state["case"]["group"]:
@@ -243,8 +243,8 @@ def exact(case, seed):
             acc = torch.einsum("nk,bkl->bnl", qw, q)
             if i + 1 < n:
                 # hidden values are float32 numbers by definition, each of the three steps rounded to one
-                t = (acc.float().double() * sw.reshape(1, -1, 1)).float().double()
-                t = (t * s).float().double()
+                t = (acc.float().double() * s).float().double()
+                t = (t * sw.reshape(1, -1, 1)).float().double()
                 h = torch.relu((t + b.reshape(1, -1, 1)).float().double())
             else:
                 h = acc * s * sw.reshape(1, -1, 1) + b.reshape(1, -1, 1)
