@@ -406,7 +406,8 @@ size_t p2n_int8_linear_workspace_bytes(long T, int K, int N);
 int p2n_int8_linear(const void *x, int bf16, long T, int K, long ld, const void *image, int N, int relu, void *y,
                     void *workspace, size_t workspace_bytes, void *stream);
 /* The layers of a shared MLP over the columns of x (B, dims[0], L): token = column, ReLU behind every layer but the last
- * (behind that one if last_relu), hidden values put into 8 bits again by the rule.  out (B, dims[nl], L), or with
+ * (behind that one if last_relu), hidden values put into 8 bits again by the rule: a hidden value is
+ * fl(fl(fl(sum) * sx[t]) * sw[n]) + bias[n] (the token's scale first: one step in it can move a code), a result as above.  out (B, dims[nl], L), or with
  * group = 16 or 32 (dividing L) the maximum over groups of consecutive columns, (B, dims[nl], L/group); a NaN in a group
  * is its maximum.  images_host: HOST array of nl device pointers.  1..8 layers, dims[0] <= 1024, others <= 256, L <= 2^24. */
 int p2n_int8_mlp(const float *x, int B, long L, int nl, const int *dims, const void *const *images_host, int last_relu,

@@ -2,7 +2,9 @@
 //     (sx_t, qx_t) = 8-bit rule over the K values of token t        (sw_n, qw_n) = 8-bit rule over row n of W (N, K)
 //     y[t][n] = fl(fl(fl(sum_k qx qw) * sw_n) * sx_t) + b_n, then ReLU if asked
 // The sum is exact in int32 (K <= 65536 keeps it below 2^31); its conversion to float32 and the two products round once
-// each.  The reference has no 8-bit path (its layers are Conv1d, reference point2net.py:9-34): the formulas above are the
+// each.  The values between the layers of p2n_int8_mlp take the token's scale first, fl(fl(fl(sum) * sx_t) * sw_n) + b_n: they are put
+// into 8 bits again, one step in them can move a code, and with it the results by a step of 8 bits, so there the order belongs to
+// the definition (a result's last step is all that it moves elsewhere).  The reference has no 8-bit path (its layers are Conv1d, reference point2net.py:9-34): the formulas above are the
 // specification.  Two operators share the weight image and the rule (p2n_q8.h):
 //   p2n_int8_linear  rows of K values (tokens), float32 or bfloat16
 //   p2n_int8_mlp     the layers of a shared MLP over the columns of (B, C, L), on chip from the input to the result
@@ -698,20 +700,26 @@ __device__ __forceinline__ void int8_mlp_groups(const Int8MlpArgs &A, const MlpL
     if (32 * ct + p < Y.N && (two ? l0 + 16 * h < A.L : h == 0)) A.out[(b * Y.N + 32 * ct + p) * (A.L / A.group) + (two ? l0 / 16 + h : l0 / 32)] = y;
 }
 
-// A tile's sums to its values: scales, bias, ReLU; into `am` the largest of them as bits.  The ReLU is a maximum of bit patterns: every NaN here has
+// A tile's sums to its values: scales, bias, ReLU; into `am` the largest of them as bits.  HIDDEN: a value for the next layer, the token's scale
+// first.  Sum times scale may pass the end of float32 where the value does not (a scale of more than 2^100): there the scale
+// goes in 2^24 times smaller, and the fma that adds the bias puts the 2^24 back; both are exact, and the fma costs what the addition does.  The ReLU is a maximum of bit patterns: every NaN here has
 // its sign bit clear (scales and biases are made so, and so is what the arithmetic makes) and stays.  Past it the bits order as they are.
 // par: the tile's scales and biases in LDS, put there by one load of the wave (read from memory by every lane they would take eight).
 __device__ __forceinline__ float int8_mlp_par(const MlpLayer &Y, int ct, int lane) {     // scales in the lower half of the wave, biases in the upper
     return Y.scale[32 * (ct + (lane >> 5) * Y.CT) + (lane & 31)];
 }
+template <bool HIDDEN>
 __device__ __forceinline__ void int8_mlp_values(const i32x16 &acc, const float *par, int h, float s, bool relu, float (&y)[16], unsigned &am) {
-    const int floor = relu ? 0 : (int)0x80000000;        // nothing is below it as a whole number
+    const int floor = HIDDEN || relu ? 0 : (int)0x80000000;        // nothing is below it as a whole number
+    const bool far = s > 0x1p100f;                                 // the sums are below 2^24 (at most 1024 channels)
+    const float st = far ? s * 0x1p-24f : s, up = far ? 0x1p24f : 1.f;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
         const f32x4 sc = *reinterpret_cast<const f32x4 *>(par + 8 * g + 4 * h), bi = *reinterpret_cast<const f32x4 *>(par + 32 + 8 * g + 4 * h);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float v = (float)acc[4 * g + j] * sc[j] * s + bi[j];
+            const float a = (float)acc[4 * g + j];
+            const float v = HIDDEN ? fmaf(a * st * sc[j], up, bi[j]) : a * sc[j] * s + bi[j];
             const int bv = __float_as_int(v), u = bv > floor ? bv : floor;
             y[4 * g + j] = __int_as_float(u);
             am = (unsigned)u > am ? (unsigned)u : am;
@@ -814,7 +822,7 @@ __global__ __launch_bounds__(256, HT == 1 ? 5 : 4) void p2n_int8_mlp_narrow_kern
 #pragma unroll
                     for (int kt = 0; kt < HT; ++kt) acc = MFMA_I8(wf[(ct * Y.KTI + kt) * 64], x[kt], acc);
                     float y[16];
-                    int8_mlp_values(acc, own[wave][0], h, s, A.last_relu, y, am);
+                    int8_mlp_values<false>(acc, own[wave][0], h, s, A.last_relu, y, am);
                     int8_mlp_out(A, Y.N, b, valid, off, ct, y);
                 }
             }
@@ -833,7 +841,7 @@ __global__ __launch_bounds__(256, HT == 1 ? 5 : 4) void p2n_int8_mlp_narrow_kern
                 i32x16 acc = zero;
 #pragma unroll
                 for (int kt = 0; kt < HT; ++kt) acc = MFMA_I8(wf[(ct * Y.KTI + kt) * 64], x[kt], acc);
-                int8_mlp_values(acc, own[wave][ct], h, s, true, y[ct], am);
+                int8_mlp_values<true>(acc, own[wave][ct], h, s, true, y[ct], am);
             }
         s = p2n_q8_scale(int8_halves(am));
         const P2nQ8 Q = p2n_q8_make(s);
@@ -907,7 +915,7 @@ __global__ __launch_bounds__(64 * NW, IR == 2 ? 5 : 4) void p2n_int8_mlp_wide_ke
 #pragma unroll 1
     for (int li = 0; li < A.nl; ++li) {
         const MlpLayer Y = A.layer[li];
-        const bool last = li == A.nl - 1, relu = !last || A.last_relu;
+        const bool last = li == A.nl - 1;
         am = 0;
         const bool mine = wave < Y.CT, groups = GROUPS && last;
         if (mine) {
@@ -935,13 +943,15 @@ __global__ __launch_bounds__(64 * NW, IR == 2 ? 5 : 4) void p2n_int8_mlp_wide_ke
                 product(std::true_type{});
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 __builtin_amdgcn_wave_barrier();
-                int8_mlp_values(acc, par[wave], h, s, relu, v[0], am);
+                if (last) {
+                    int8_mlp_values<false>(acc, par[wave], h, s, A.last_relu, v[0], am);
+                    int8_mlp_out(A, Y.N, b, valid, off, wave, v[0]);
+                } else {
+                    int8_mlp_values<true>(acc, par[wave], h, s, true, v[0], am);
+                }
             }
         }
-        if (last) {
-            if (mine && !groups) int8_mlp_out(A, Y.N, b, valid, off, wave, v[0]);
-            break;
-        }
+        if (last) break;
         ahead(A.layer[li + 1], wave);
         s = join();                            // behind its barrier every wave has read this layer's codes
         if (GROUPS && threadIdx.x < 32) scales[p] = s;   // read behind the next barrier, by the last layer alone

@@ -169,6 +169,8 @@ def _arrays(layers: int):
 def int8_mlp(x: torch.Tensor, weights: Sequence[Int8Weight], last_relu: bool = True, group: int = 0) -> torch.Tensor:
     """x (B, C, L) float32 -> (B, N, L): the products of `weights` one after another over the columns of x, ReLU between them
     (and behind the last if last_relu); what passes from a layer to the next is put into 8 bits again, one scale a column.
+    Such a hidden value is ((sum * token's scale) * channel's scale) + bias, each step rounded to float32, in that order: one step in it can
+    move a code.
     group > 0: followed by the maximum over groups of `group` consecutive columns -> (B, N, L // group).
     1..8 layers, C <= 1024, every layer's N <= 256."""
     x = _gpu(x, "x", (torch.float32,))

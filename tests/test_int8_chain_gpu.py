@@ -1,0 +1,65 @@
+"""GPU: the hidden values of quant.int8_mlp.  A hidden value is put into 8 bits again, so one float32 step in it can move a
+code, and with it the results by a whole step of 8 bits: the order of its three roundings -- the token's scale, the
+channel's, the bias -- belongs to the definition, and results are compared bit by bit.  Here every product is rounded to 24
+bits in 64-bit arithmetic, whose range does not end on the way, as the kernel's does not."""
+import pytest
+import torch
+
+from test_int8_gpu import make_mlp, rule64
+
+pytestmark = pytest.mark.gpu
+
+
+def f24(v):
+    """float64 rounded to 24 significant bits, ties to even, without an end of the range"""
+    m, e = torch.frexp(v)
+    return torch.ldexp((m * 2.0 ** 24).round(), e - 24)
+
+
+def chain(x, layers, last_relu, group):
+    h = x.detach().double().cpu()
+    for i, (W, b) in enumerate(layers):
+        q, s = rule64(h, 1)
+        qw, sw = rule64(W, 1)
+        acc = torch.matmul(qw, q)                                   # whole numbers below 2^24
+        hidden = i + 1 < len(layers)
+        t = f24(f24(acc * s) * sw) if hidden else f24(f24(acc * sw) * s)
+        h = t.float() + (0 if b is None else b.cpu()[:, None])      # one float32 rounding
+        if hidden or last_relu:
+            h = torch.where(h <= 0, torch.zeros_like(h), h)
+    if group:
+        h = h.view(h.shape[0], h.shape[1], -1, group).amax(3)
+    return h
+
+
+@pytest.mark.parametrize("B,L,dims,last_relu,group", [
+    (1, 1, [1, 1], True, 0), (1, 32, [32, 32, 32], True, 0), (3, 33, [6, 32, 32, 64], True, 0), (2, 300, [131, 128, 128, 256], True, 0),
+    (1, 515, [384, 256, 256], True, 0), (2, 100, [67, 64, 64, 128], False, 0), (1, 70, [1024, 256, 40], False, 0), (1, 130, [128, 128, 64], False, 0),
+    (2, 40, [3, 16, 16, 16, 16, 16, 16, 16, 9], True, 0), (4, 31, [200, 20, 250, 30], False, 0), (4, 8192, [131, 128, 128, 128, 64], False, 0),
+    (2, 96, [6, 32, 64], True, 32), (3, 48, [6, 32, 64], True, 16), (2, 128, [67, 64, 128], True, 64), (2, 72, [6, 32, 40], False, 24),
+    (1, 64, [131, 128, 256], False, 32), (2, 4096, [6, 32, 32, 64], True, 32), (1, 96, [40, 64, 64, 50], True, 16)])
+def test_hidden_values_take_the_tokens_scale_first(B, L, dims, last_relu, group):
+    from pointcloudsegmentation_amd import quant
+    x, layers = make_mlp(B, L, dims)
+    y = quant.int8_mlp(x, [quant.Int8Weight(W, b) for W, b in layers], last_relu=last_relu, group=group)
+    want = chain(x, layers, last_relu, group)
+    assert torch.equal(y.cpu(), want), float((y.cpu() - want).abs().max())
+
+
+@pytest.mark.parametrize("dims", [[40, 32, 32], [40, 64, 64], [96, 128, 64], [300, 200, 250]])
+def test_columns_of_every_size(dims):
+    """columns from the smallest float32 values to the largest: sum times scale passes the end of float32 on the way, the value
+    does not (the weights are small)"""
+    from pointcloudsegmentation_amd import quant
+    g = torch.Generator().manual_seed(sum(dims))
+    exps = torch.tensor([-140, -120, -100, -20, 0, 60, 99, 100, 101, 104, 110, 120, 126], dtype=torch.float64)
+    x = torch.randn(1, dims[0], len(exps), generator=g).double()
+    x = (x / x.abs().amax(1, keepdim=True) * torch.ldexp(torch.tensor(1.9, dtype=torch.float64), exps)).float().cuda()
+    layers = [((torch.randn(n, k, generator=g) / (8 * k)).cuda(), None) for k, n in zip(dims, dims[1:])]
+    y = quant.int8_mlp(x, [quant.Int8Weight(W) for W, _ in layers], last_relu=False).cpu()
+    assert bool(torch.isfinite(y).all())
+    want = chain(x, layers, False, 0)
+    normal = exps > -90                                             # below, the roundings of small numbers are coarser
+    assert torch.equal(y[:, :, normal], want[:, :, normal])
+    # there a product is off by half of the smallest step, 2^-150, before the next layer's weights make it smaller
+    assert bool(((y - want).abs()[:, :, ~normal] <= 2.0 ** -140 + 0.05 * want.abs()[:, :, ~normal].amax(1, keepdim=True)).all())
