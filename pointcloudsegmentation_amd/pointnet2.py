@@ -310,16 +310,16 @@ def _row_blocks(rows: int):
 CHECKPOINTS = (None, "int8")
 
 
-def _shared_mlp_act8(mods: List[nn.Module], x: torch.Tensor, group: int) -> torch.Tensor:
+def _shared_mlp_act8(mods: List[nn.Module], x: torch.Tensor, group: int, training: bool) -> torch.Tensor:
     """the layers of a shared MLP with their inputs kept in 8 bits: conv, (norm, ReLU, conv)*, and norm, ReLU at the end of a
-    chain whose last layer is not plain.  Every BatchNorm1d goes by its own training flag."""
+    chain whose last layer is not plain.  `training` stands for every BatchNorm1d's own flag, as it does without a checkpoint."""
     y = quant.act8_linear(x, mods[0].weight, mods[0].bias)
     i = 1
     while i < len(mods):                                    # mods[i], mods[i+1]: norm, ReLU
         if i + 2 < len(mods):
-            y = quant.act8_linear(y, mods[i + 2].weight, mods[i + 2].bias, norm=mods[i])
+            y = quant.act8_linear(y, mods[i + 2].weight, mods[i + 2].bias, norm=mods[i], training=training)
         else:
-            y = quant.act8_norm_relu(y, mods[i])
+            y = quant.act8_norm_relu(y, mods[i], training=training)
         i += 3
     if not group:
         return y
@@ -371,7 +371,7 @@ def shared_mlp_train(net: nn.Sequential, x: torch.Tensor, group: int = 0, eval_s
             buffers += [None, None]
             i += 1
     if checkpoint == "int8":
-        return _shared_mlp_act8(mods, _rt.require_cuda_f32(x, "x"), int(group))
+        return _shared_mlp_act8(mods, _rt.require_cuda_f32(x, "x"), int(group), not eval_stats)
     if eval_stats:
         return _SharedMLPTrainFn.apply(x, tuple(dims), last_plain, -1.0, tuple(buffers), int(group), *params)
     if len({bn.momentum for bn in bns}) > 1:

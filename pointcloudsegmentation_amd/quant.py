@@ -207,9 +207,9 @@ def int8_mlp(x: torch.Tensor, weights: Sequence[Int8Weight], last_relu: bool = T
 
 
 # ------------------------------------------------------------------ activation checkpoints in 8 bits
-def _norm_args(norm: Optional[nn.BatchNorm1d], x: torch.Tensor):
+def _norm_args(norm: Optional[nn.BatchNorm1d], x: torch.Tensor, training: Optional[bool] = None):
     """gamma, beta, running mean, running variance, batches tracked (where it counts), momentum (< 0: running statistics used as they
-    are), eps of a BatchNorm1d"""
+    are), eps of a BatchNorm1d; `training` in place of its own flag"""
     if norm is None:
         return None, None, None, None, None, 0.0, 0.0
     if not isinstance(norm, nn.BatchNorm1d):
@@ -224,7 +224,9 @@ def _norm_args(norm: Optional[nn.BatchNorm1d], x: torch.Tensor):
     for t, name in ((gamma, "weight"), (beta, "bias"), (mean, "running_mean"), (var, "running_var")):
         if t is not None and not (t.dtype == torch.float32 and t.device == x.device and t.is_contiguous()):
             raise ValueError(f"norm.{name} must be a contiguous float32 tensor on the input's GPU")
-    training, tracked = norm.training, mean is not None
+    tracked = mean is not None
+    if training is None:
+        training = norm.training
     if training or not tracked:
         if x.size(0) * x.size(2) < 2:
             raise ValueError(f"Expected more than 1 value per channel when training, got input size {tuple(x.shape)}")
@@ -312,12 +314,12 @@ class _Act8Linear(torch.autograd.Function):
 
 
 def act8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
-                norm: Optional[nn.BatchNorm1d] = None) -> torch.Tensor:
+                norm: Optional[nn.BatchNorm1d] = None, training: Optional[bool] = None) -> torch.Tensor:
     """x (B, K, L) float32 -> W relu(norm(x)) + b, or W x + b without a norm: (B, N, L), differentiable in x, weight (N, K) or
     (N, K, 1), bias and the norm's parameters.  The output is computed from the float32 values; for the backward pass the
     normalised input (the input itself without a norm) is kept in 8 bits, one scale for 128 consecutive points of a channel,
-    with one bit for each of the ReLU's decisions: 1.16 bytes a value instead of 4.  norm.training decides between the
-    batch's statistics (running statistics updated, as BatchNorm1d does) and the running ones.  1..1024 channels."""
+    with one bit for each of the ReLU's decisions: 1.16 bytes a value instead of 4.  norm.training (or `training`, if given) decides
+    between the batch's statistics (running statistics updated, as BatchNorm1d does) and the running ones.  1..1024 channels."""
     x = _gpu(x, "x", (torch.float32,))
     if x.dim() != 3 or 0 in x.shape:
         raise ValueError(f"x must be (B,K,L) with at least one value, got {tuple(x.shape)}")
@@ -329,7 +331,7 @@ def act8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     for t, name in ((w, "weight"), (bias, "bias")):
         if t is not None and not (t.device == x.device and t.dtype == torch.float32):
             raise ValueError(f"{name} must be a float32 tensor on the input's GPU")
-    return _Act8Linear.apply(x.contiguous(), w.contiguous(), None if bias is None else bias.contiguous(), *_norm_args(norm, x))
+    return _Act8Linear.apply(x.contiguous(), w.contiguous(), None if bias is None else bias.contiguous(), *_norm_args(norm, x, training))
 
 
 class _Act8NormRelu(torch.autograd.Function):
@@ -369,7 +371,7 @@ class _Act8NormRelu(torch.autograd.Function):
         return dx, dgamma, dbeta, None, None, None, None, None
 
 
-def act8_norm_relu(x: torch.Tensor, norm: nn.BatchNorm1d) -> torch.Tensor:
+def act8_norm_relu(x: torch.Tensor, norm: nn.BatchNorm1d, training: Optional[bool] = None) -> torch.Tensor:
     """x (B, C, L) float32 -> relu(norm(x)), differentiable in x and the norm's parameters; what the backward pass needs of x is
     kept in 8 bits and the ReLU's decisions as bits, as in act8_linear."""
     x = _gpu(x, "x", (torch.float32,))
@@ -377,4 +379,4 @@ def act8_norm_relu(x: torch.Tensor, norm: nn.BatchNorm1d) -> torch.Tensor:
         raise ValueError(f"x must be (B,C,L) with at least one value, got {tuple(x.shape)}")
     if norm is None:
         raise TypeError("norm must be a BatchNorm1d, got None")
-    return _Act8NormRelu.apply(x.contiguous(), *_norm_args(norm, x))
+    return _Act8NormRelu.apply(x.contiguous(), *_norm_args(norm, x, training))

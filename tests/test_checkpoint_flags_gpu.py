@@ -1,0 +1,57 @@
+"""GPU: shared MLPs that train on 8-bit checkpoints, where a norm's own training flag differs from what the call asks for."""
+import copy
+
+import pytest
+import torch
+import torch.nn as nn
+
+from test_int8_models_gpu import randomise, rel
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("last_plain", [False, True])
+@pytest.mark.parametrize("net_training,norm_training,eval_stats", [(True, True, True), (True, False, False), (False, False, False), (False, True, True),
+                                                                   (False, False, True), (True, True, False)])
+def test_the_call_decides_between_batch_and_running_statistics(net_training, norm_training, eval_stats, last_plain):
+    """with and without checkpoint the same output and the same buffers, whatever the norms' own flags say"""
+    from pointcloudsegmentation_amd.pointnet2 import SharedMLP, shared_mlp_train
+    torch.manual_seed(2)
+    ref = SharedMLP([6, 32, 64, 40], last_plain=last_plain)
+    randomise(ref, 5)
+    ref = ref.cuda().train(net_training)
+    for m in ref.modules():
+        if isinstance(m, nn.BatchNorm1d):
+            m.train(norm_training)
+    mlp = copy.deepcopy(ref)
+    x = torch.randn(2, 6, 300, device="cuda")
+    want = shared_mlp_train(ref.net, x, eval_stats=eval_stats)
+    got = shared_mlp_train(mlp.net, x, eval_stats=eval_stats, checkpoint="int8")
+    assert rel(got, want) <= 1e-5
+    for (k, a), (_, b) in zip(mlp.named_buffers(), ref.named_buffers()):
+        assert rel(a, b) <= 1e-5, k
+    if eval_stats:
+        for (k, a), (_, b) in zip(mlp.named_buffers(), SharedMLP([6, 32, 64, 40], last_plain=last_plain).named_buffers()):
+            if k.endswith("num_batches_tracked"):
+                assert int(a) == int(b) == 0
+    r = torch.randn_like(want)
+    (r1,), (r2,) = (torch.autograd.grad((y * r).sum(), [n.net[0].weight]) for y, n in ((got, mlp), (want, ref)))
+    assert rel(r1, r2) <= 0.009 * 3 * 3 ** 0.5 + 5e-4             # 8-bit noise of three layers, as test_int8_models_gpu derives it
+
+
+def test_a_model_with_one_level_of_frozen_norms():
+    """a norm put into eval() inside a model in train(): switching the checkpoint on changes neither the output nor the buffers"""
+    from pointcloudsegmentation_amd.point2net import Point2Net
+    torch.manual_seed(3)
+    ref = Point2Net().train()
+    randomise(ref, 7)
+    ref = ref.cuda()
+    for m in ref.encoder.mlp2.modules():
+        if isinstance(m, nn.BatchNorm1d):
+            m.eval()
+    m = copy.deepcopy(ref)
+    m.checkpoint = "int8"
+    x = torch.randn(2, 700, 6, device="cuda")
+    assert rel(m(x), ref(x)) <= 1e-5
+    for (k, a), (_, b) in zip(m.named_buffers(), ref.named_buffers()):
+        assert rel(a, b) <= 1e-5, k
