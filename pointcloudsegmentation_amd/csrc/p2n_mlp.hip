@@ -141,11 +141,12 @@ extern "C" int p2n_pointwise_layer(const float *in, int B, int Cin, long L, cons
 // in (C, ld): columns g*ns .. g*ns+ns-1 of a row are group g (g < G).  out (C, G) = the group's maximum, arg (C, G) =
 // the first position that attains it (what the backward routes the gradient to).  ns in {8, 16, 32, 64}: ns/4 lanes
 // read one group as consecutive 16-byte pieces (a wave reads 1 KiB contiguous per step) and reduce by xor-shuffles;
-// other ns: one thread per group.  Keys order as (value, lower position first); a NaN with its sign bit clear is the
-// largest value, as in torch.max.
+// other ns: one thread per group.  Keys order as (value, lower position first); a NaN of either sign is the largest
+// value, as in torch.max (a sum that met an infinity can leave either).
 __device__ __forceinline__ unsigned p2n_ordered_bits(float v) {
     unsigned b = __float_as_uint(v);
     b = b == 0x80000000u ? 0u : b;                    // -0 == +0: the first of them is the first maximum
+    if (v != v) return 0xFFFFFFFFu;
     return b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
 
