@@ -73,8 +73,7 @@ __global__ __launch_bounds__(256) void p2n_int8_pack_kernel(const float *__restr
     const P2nQ8 Q = p2n_q8_make(s);
     if (lane == 0) {
         scale[n] = n < N ? s : 0.f;
-        // a NaN without a sign: the ReLU of p2n_int8_mlp is a maximum of bit patterns
-        bimg[n] = t == t ? t : __uint_as_float(0x7FC00000u);
+        bimg[n] = t;
     }
     const int ct = n >> 5, r = n & 31;
     const bool bad = !(s == s);
@@ -700,17 +699,18 @@ __device__ __forceinline__ void int8_mlp_groups(const Int8MlpArgs &A, const MlpL
     if (32 * ct + p < Y.N && (two ? l0 + 16 * h < A.L : h == 0)) A.out[(b * Y.N + 32 * ct + p) * (A.L / A.group) + (two ? l0 / 16 + h : l0 / 32)] = y;
 }
 
-// A tile's sums to its values: scales, bias, ReLU; into `am` the largest of them as bits.  HIDDEN: a value for the next layer, the token's scale
+// A tile's sums to its values: scales, bias, ReLU; into `am` the largest of them as bits, where a NaN of either sign is on top.  HIDDEN: a value for the next layer, the token's scale
 // first.  Sum times scale may pass the end of float32 where the value does not (a scale of more than 2^100): there the scale
-// goes in 2^24 times smaller, and the fma that adds the bias puts the 2^24 back; both are exact, and the fma costs what the addition does.  The ReLU is a maximum of bit patterns: every NaN here has
-// its sign bit clear (scales and biases are made so, and so is what the arithmetic makes) and stays.  Past it the bits order as they are.
+// goes in 2^24 times smaller, and the fma that adds the bias puts the 2^24 back; both are exact, and the fma costs what the addition does.
+// The ReLU is the maximum that keeps a NaN of either sign (infinity and a bias of the other sign make one with the sign bit set here; a maximum
+// of bit patterns would take it for a negative value).  Past it the bits order as they are.
 // par: the tile's scales and biases in LDS, put there by one load of the wave (read from memory by every lane they would take eight).
 __device__ __forceinline__ float int8_mlp_par(const MlpLayer &Y, int ct, int lane) {     // scales in the lower half of the wave, biases in the upper
     return Y.scale[32 * (ct + (lane >> 5) * Y.CT) + (lane & 31)];
 }
 template <bool HIDDEN>
 __device__ __forceinline__ void int8_mlp_values(const i32x16 &acc, const float *par, int h, float s, bool relu, float (&y)[16], unsigned &am) {
-    const int floor = HIDDEN || relu ? 0 : (int)0x80000000;        // nothing is below it as a whole number
+    const float floor = HIDDEN || relu ? 0.f : -__builtin_inff();
     const bool far = s > 0x1p100f;                                 // the sums are below 2^24 (at most 1024 channels)
     const float st = far ? s * 0x1p-24f : s, up = far ? 0x1p24f : 1.f;
 #pragma unroll
@@ -720,9 +720,8 @@ __device__ __forceinline__ void int8_mlp_values(const i32x16 &acc, const float *
         for (int j = 0; j < 4; ++j) {
             const float a = (float)acc[4 * g + j];
             const float v = HIDDEN ? fmaf(a * st * sc[j], up, bi[j]) : a * sc[j] * s + bi[j];
-            const int bv = __float_as_int(v), u = bv > floor ? bv : floor;
-            y[4 * g + j] = __int_as_float(u);
-            am = (unsigned)u > am ? (unsigned)u : am;
+            y[4 * g + j] = int8_max(v, floor);
+            if (HIDDEN) am = __float_as_uint(y[4 * g + j]) > am ? __float_as_uint(y[4 * g + j]) : am;
         }
     }
 }

@@ -63,3 +63,24 @@ def test_columns_of_every_size(dims):
     assert torch.equal(y[:, :, normal], want[:, :, normal])
     # there a product is off by half of the smallest step, 2^-150, before the next layer's weights make it smaller
     assert bool(((y - want).abs()[:, :, ~normal] <= 2.0 ** -140 + 0.05 * want.abs()[:, :, ~normal].amax(1, keepdim=True)).all())
+
+
+@pytest.mark.parametrize("dims", [[40, 32, 32], [40, 64, 64], [96, 128, 64], [300, 200, 250]])
+def test_what_overflows_shows(dims):
+    """a hidden value past the end of float32 makes its column NaN, and so does an infinity met by a bias of the other sign (a NaN of
+    either sign passes the ReLU); the column beside it is as it would be alone"""
+    from pointcloudsegmentation_amd import quant
+    x, layers = make_mlp(1, 33, dims)
+    layers[0][0][5] = 1e30
+    layers[0][1][5] = 0.0
+    small = torch.zeros_like(x)
+    quiet = quant.int8_mlp(small, [quant.Int8Weight(W, b) for W, b in layers])
+    for bias in (0.0, -float("inf")):
+        layers[0][1][5] = bias
+        for v in (1e28, 1e36):                                      # row 5 alone is past the end
+            big = small.clone()
+            big[0, :, 7] = v
+            y = quant.int8_mlp(big, [quant.Int8Weight(W, b) for W, b in layers])
+            assert bool(torch.isnan(y[0, :, 7]).all()), (bias, v)
+            keep = torch.arange(33, device="cuda") != 7
+            assert torch.equal(y[:, :, keep], quiet[:, :, keep])
