@@ -675,11 +675,12 @@ __device__ __forceinline__ void int8_mlp_out(const Int8MlpArgs &A, int N, long b
 __device__ __forceinline__ float int8_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }   // a NaN stays
 
 // The last layer before a maximum over groups, its operands the other way round: lane = channel, acc[e] = point 8(e>>2) + 4h + (e&3), so that
-// the maximum is formed in registers; ps: the scales of the 32 points.  Rounding keeps the order, so bias and ReLU follow the maximum, once.
+// the maximum is formed in registers; ps: the scales of the 32 points.  Rounding keeps the order, so bias and ReLU follow the maximum, once
+// (under a bias of +inf it is the smallest value that shows: -inf makes a NaN, anything else +inf).
 // l0: the tile's first column.
 __device__ __forceinline__ void int8_mlp_groups(const Int8MlpArgs &A, const MlpLayer &Y, int ct, const i32x16 &acc, const float *ps, long b, long l0, int lane) {
     const int p = lane & 31, h = lane >> 5;
-    const float sc = Y.scale[32 * ct + p], bi = Y.bias[32 * ct + p];
+    const float bi = Y.bias[32 * ct + p], turn = bi == __builtin_inff() ? -1.f : 1.f, sc = Y.scale[32 * ct + p] * turn;
     float m[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -693,7 +694,7 @@ __device__ __forceinline__ void int8_mlp_groups(const Int8MlpArgs &A, const MlpL
     float u = int8_max(m[0], m[1]), w = int8_max(m[2], m[3]);
     if (A.group == 32) u = w = int8_max(u, w);
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_int(u), __float_as_int(w), false, false);
-    float y = int8_max(__int_as_float(x[0]), __int_as_float(x[1])) + bi;
+    float y = int8_max(__int_as_float(x[0]), __int_as_float(x[1])) * turn + bi;
     if (A.last_relu) y = y <= 0.f ? 0.f : y;
     const bool two = A.group == 16;
     if (32 * ct + p < Y.N && (two ? l0 + 16 * h < A.L : h == 0)) A.out[(b * Y.N + 32 * ct + p) * (A.L / A.group) + (two ? l0 / 16 + h : l0 / 32)] = y;

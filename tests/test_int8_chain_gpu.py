@@ -84,3 +84,26 @@ def test_what_overflows_shows(dims):
             assert bool(torch.isnan(y[0, :, 7]).all()), (bias, v)
             keep = torch.arange(33, device="cuda") != 7
             assert torch.equal(y[:, :, keep], quiet[:, :, keep])
+
+
+@pytest.mark.parametrize("dims", [[40, 32], [40, 64, 64], [96, 128], [300, 200, 250]])
+def test_groups_show_what_their_columns_show(dims):
+    """products past either end of float32 that meet a bias of either infinity, in the layer that the maximum over groups follows"""
+    from pointcloudsegmentation_amd import quant
+    x, layers = make_mlp(1, 96, dims)
+    W, b = layers[-1]
+    x[:, :, 5::16] *= 1e8
+    for row, bias in ((3, float("inf")), (4, -float("inf")), (5, 0.0)):
+        for sign, r in ((1, row), (-1, row + 10)):
+            W[r] = sign * 3e34
+            b[r] = bias
+    ws = [quant.Int8Weight(*layer) for layer in layers]
+    for relu in (True, False):
+        columns = quant.int8_mlp(x.abs(), ws, last_relu=relu)
+        for group in (16, 32, 96, 24):
+            got = quant.int8_mlp(x.abs(), ws, last_relu=relu, group=group)
+            parts = columns.view(1, dims[-1], -1, group)
+            bad = torch.isnan(parts).any(3)
+            assert torch.equal(torch.isnan(got), bad), (relu, group)
+            assert torch.equal(got[~bad], parts.amax(3)[~bad]), (relu, group)
+    assert bool(torch.isnan(columns).any()) and not bool(torch.isnan(columns).all())
