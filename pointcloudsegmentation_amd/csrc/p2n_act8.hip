@@ -769,6 +769,11 @@ __device__ __forceinline__ void act8_operand(const i32x4 &q, int j, float cs, fl
     act8_split(v, w[0], w[1], w[2]);
 }
 
+// What makes a column of dW NaN where the operand's ReLU does not let a NaN through (the maximum with zero takes it for one): a NaN of beta
+// from the start, and at every step a NaN of gamma * scale.
+template <bool NORM>
+__device__ __forceinline__ float act8_poison(float be) { return NORM && be != be ? be : 0.f; }
+
 // the shares of four waves, added in order: a quarter of the tile's registers at a time, all waves at once
 template <int RT, int CT>
 __device__ __forceinline__ void act8_wgrad_end(const Act8Wgrad &A, float *join, const f32x16 (&acc)[RT][CT], float (&db)[RT], const float (&poison)[CT],
@@ -830,7 +835,7 @@ __global__ __launch_bounds__(256, 2) void p2n_act8_wgrad_kernel(Act8Wgrad A) {
         krow[i] = k < A.K ? k : A.K - 1;
         ga[i] = NORM ? A.gamma[krow[i]] : 1.f;
         be[i] = NORM ? A.beta[krow[i]] : 0.f;
-        poison[i] = 0.f;
+        poison[i] = act8_poison<NORM>(be[i]);
     }
     f32x16 acc[RT][CT];
 #pragma unroll
@@ -966,7 +971,8 @@ __global__ __launch_bounds__(256, 1) void p2n_act8_wgrad_wide_kernel(Act8Wgrad A
         krow[i] = k < A.K ? k : A.K - 1;
         ga[i] = NORM ? A.gamma[krow[i]] : 1.f;
         be[i] = NORM ? A.beta[krow[i]] : 0.f;
-        poison[i] = db[i] = 0.f;
+        poison[i] = act8_poison<NORM>(be[i]);
+        db[i] = 0.f;
     }
     f32x16 acc[4][4];
 #pragma unroll
@@ -1104,7 +1110,7 @@ __global__ __launch_bounds__(256, 2) void p2n_act8_both_kernel(Act8Both B) {
     __syncthreads();
     const int krow = k0 + r < A.K ? k0 + r : A.K - 1;
     const float ga = NORM ? A.gamma[krow] : 1.f, be = NORM ? A.beta[krow] : 0.f;
-    float poison[1] = {0.f}, db[RT], s1[16], s2[16];
+    float poison[1] = {act8_poison<NORM>(be)}, db[RT], s1[16], s2[16];
     f32x16 acc[RT][1];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
