@@ -627,7 +627,7 @@ __global__ __launch_bounds__(256) void p2n_act8_sums_kernel(Act8Sums A) {
     }
 }
 
-// dx = gamma*r*(dy - m1 - uh*m2), in place: a workgroup takes 32 channels of a block of 128 points, a thread four points of four channels.
+// dx = gamma*r*(dy - m1 - uh*m2), in place (frozen: gamma*r*dy, where a NaN of the scale has no part): a workgroup takes 32 channels of a block of 128 points, a thread four points of four channels.
 // FEW: the sums are formed here too, by every workgroup for its channels (eight threads a channel), the first of a row writes them down.
 #define ACT8_FEW 64
 template <bool FEW>
@@ -674,7 +674,7 @@ __global__ __launch_bounds__(256) void p2n_act8_dx_kernel(float *__restrict__ dy
     for (int i = 0; i < 4; ++i) {
         if (c[i] >= C) continue;
         const float *t = FEW ? own + (c[i] & 31) : A.tab + c[i];
-        const float a = t[0], m1 = t[FEW ? 32 : C], m2 = t[FEW ? 64 : 2 * C], s = scale[blk * C4 + c[i]];
+        const float a = t[0], m1 = t[FEW ? 32 : C], m2 = t[FEW ? 64 : 2 * C], s = A.frozen ? 0.f : scale[blk * C4 + c[i]];
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[i][j] = a * (v[i][j] - m1 - (float)(signed char)(q[i] >> (8 * j)) * s * m2);
         if (whole) *reinterpret_cast<f32x4u *>(d[i]) = v[i];
