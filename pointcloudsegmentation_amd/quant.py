@@ -216,7 +216,10 @@ def _norm_args(norm: Optional[nn.BatchNorm1d], x: torch.Tensor, training: Option
         raise TypeError(f"norm must be a BatchNorm1d or None, got {type(norm).__name__}")
     # straight from the module's dictionaries: its attribute access costs as much as a launch
     par, buf = norm._parameters, norm._buffers
-    gamma, beta, mean, var = par["weight"], par["bias"], buf["running_mean"], buf["running_var"]
+    try:
+        gamma, beta, mean, var = par["weight"], par["bias"], buf["running_mean"], buf["running_var"]
+    except KeyError:                                     # parametrised: the values of the moment
+        gamma, beta, mean, var = norm.weight, norm.bias, norm.running_mean, norm.running_var
     if gamma is None:
         raise NotImplementedError("the 8-bit checkpoint layers need BatchNorm1d(affine=True)")
     if gamma.size(0) != x.size(1):

@@ -14,3 +14,17 @@ def test_the_call_may_decide_in_place_of_the_flag():
         assert args(norm)[5] == (0.25 if flag else -1.0)
         assert args(norm, True)[5] == 0.25 and args(norm, True)[4] is norm.num_batches_tracked
         assert args(norm, False)[5] == -1.0 and args(norm, False)[4] is None
+
+
+def test_a_parametrised_norm_is_taken_by_its_present_values():
+    from torch.nn.utils import parametrize
+
+    class Double(nn.Module):
+        def forward(self, w):
+            return 2 * w
+
+    norm = nn.BatchNorm1d(8)
+    parametrize.register_parametrization(norm, "weight", Double())
+    gamma, beta = args(norm)[:2]
+    assert torch.equal(gamma, torch.full((8,), 2.0)) and gamma.requires_grad
+    assert beta is norm.bias
