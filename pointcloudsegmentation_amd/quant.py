@@ -237,6 +237,8 @@ def _norm_args(norm: Optional[nn.BatchNorm1d], x: torch.Tensor, training: Option
             return gamma, beta, None, None, None, 0.0, norm.eps
         if norm.momentum is None:
             raise NotImplementedError("BatchNorm1d(momentum=None) (cumulative average) is not implemented on the GPU path")
+        if not 0.0 <= norm.momentum <= 1.0:              # the kernels take a negative one as "running statistics as they are"
+            raise ValueError(f"norm.momentum must be in [0,1], got {norm.momentum}")
         batches = buf["num_batches_tracked"]
         if batches is not None and not (batches.dtype == torch.int64 and batches.device == x.device):
             raise ValueError("norm.num_batches_tracked must be an int64 tensor on the input's GPU")

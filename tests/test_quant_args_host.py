@@ -1,4 +1,5 @@
 """CPU: what the 8-bit checkpoint layers take of a norm, and what the library refuses, before anything touches a device."""
+import pytest
 import torch
 import torch.nn as nn
 
@@ -28,3 +29,11 @@ def test_a_parametrised_norm_is_taken_by_its_present_values():
     gamma, beta = args(norm)[:2]
     assert torch.equal(gamma, torch.full((8,), 2.0)) and gamma.requires_grad
     assert beta is norm.bias
+
+
+@pytest.mark.parametrize("momentum", [-0.1, 1.5])
+def test_a_momentum_outside_its_range_is_refused(momentum):
+    """a negative one would mean "running statistics as they are" further down"""
+    with pytest.raises(ValueError):
+        args(nn.BatchNorm1d(8, momentum=momentum).train())
+    assert args(nn.BatchNorm1d(8, momentum=momentum).eval())[5] == -1.0       # not used there
