@@ -260,10 +260,10 @@ def _act8_bytes(what: str, B: int, C: int, L: int, norm: bool, N: int):
     return nkept, nws
 
 
-def _changed(mean, var, batches) -> None:
+def _changed(mean, var, batches, momentum: float) -> None:
     """the kernels wrote these buffers through their addresses: autograd, and what is kept by a buffer's version, has to know"""
-    if batches is not None:
-        torch.autograd.graph.increment_version((mean, var, batches))
+    if mean is not None and momentum >= 0:
+        torch.autograd.graph.increment_version((mean, var) if batches is None else (mean, var, batches))
 
 
 @torch.autograd.function.once_differentiable
@@ -286,7 +286,7 @@ class _Act8Linear(torch.autograd.Function):
         _call(L_.p2n_act8_forward, "p2n_act8_forward", dev, x.data_ptr(), B, K, L, weight.data_ptr(), _rt.ptr(bias), N, _rt.ptr(gamma),
               _rt.ptr(beta), _rt.ptr(running_mean), _rt.ptr(running_var), _rt.ptr(batches), momentum, eps, h.data_ptr(), kept.data_ptr(), nkept,
               ws.data_ptr(), nws)
-        _changed(running_mean, running_var, batches)
+        _changed(running_mean, running_var, batches, momentum)
         ctx.save_for_backward(kept, weight, gamma, beta)
         ctx.meta = (B, K, L, N, normed and momentum < 0, bias is not None)
         return h
@@ -351,7 +351,7 @@ class _Act8NormRelu(torch.autograd.Function):
         _call(L_.p2n_act8_norm_relu_forward, "p2n_act8_norm_relu_forward", dev, x.data_ptr(), B, C, L, gamma.data_ptr(), beta.data_ptr(),
               _rt.ptr(running_mean), _rt.ptr(running_var), _rt.ptr(batches), momentum, eps, y.data_ptr(), kept.data_ptr(), nkept,
               ws.data_ptr(), nws)
-        _changed(running_mean, running_var, batches)
+        _changed(running_mean, running_var, batches, momentum)
         ctx.save_for_backward(kept, gamma)
         ctx.meta = (B, C, L, momentum < 0)
         return y
