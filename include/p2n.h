@@ -401,7 +401,7 @@ int p2n_int8_pack_weight(const float *W, const float *bias, int K, int N, const 
                          const float *var, double eps, void *image, void *stream);
 /* rows x[t*ld .. t*ld + K-1], t < T, ld >= K -> codes (T,K), scale (T) */
 int p2n_quantize_tokens(const void *x, int bf16, long T, int K, long ld, signed char *codes, float *scale, void *stream);
-/* T <= 2^30 */
+/* T <= 2^30; y starts on 4 bytes (bfloat16 rows of an even length are stored as dwords) */
 size_t p2n_int8_linear_workspace_bytes(long T, int K, int N);
 int p2n_int8_linear(const void *x, int bf16, long T, int K, long ld, const void *image, int N, int relu, void *y,
                     void *workspace, size_t workspace_bytes, void *stream);

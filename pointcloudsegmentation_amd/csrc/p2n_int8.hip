@@ -591,6 +591,8 @@ extern "C" int p2n_int8_linear(const void *x, int bf16, long T, int K, long ld, 
         return P2N_EWORKSPACE;
     }
     P2N_REQUIRE((((uintptr_t)workspace | (uintptr_t)image) & 15) == 0, "p2n_int8_linear: workspace and image must be 16-byte aligned");
+    P2N_REQUIRE(((uintptr_t)x & (bf16 ? 1 : 3)) == 0, "p2n_int8_linear: x must be aligned to its type");
+    P2N_REQUIRE(((uintptr_t)y & (bf16 && (N & 1) ? 1 : 3)) == 0, "p2n_int8_linear: y must start on 4 bytes (bfloat16 rows of an odd length: on 2)");
     hipStream_t s = (hipStream_t)stream_;
     const int ps = p2n_prof_begin(P2N_K_INT8_GEMM, s);
     const bool vec = ld % 2 == 0 && ((uintptr_t)x & 3) == 0;        // bfloat16 rows that start on 4 bytes
