@@ -55,3 +55,30 @@ def test_a_model_with_one_level_of_frozen_norms():
     assert rel(m(x), ref(x)) <= 1e-5
     for (k, a), (_, b) in zip(m.named_buffers(), ref.named_buffers()):
         assert rel(a, b) <= 1e-5, k
+
+
+def test_a_parametrised_norm_trains():
+    """weight = twice what is kept: output as with the plain module of those values, the kept one's gradient twice gamma's"""
+    from pointcloudsegmentation_amd import quant
+    from torch.nn.utils import parametrize
+
+    class Double(nn.Module):
+        def forward(self, w):
+            return 2 * w
+
+    torch.manual_seed(5)
+    plain = nn.BatchNorm1d(40).cuda()
+    with torch.no_grad():
+        plain.weight.copy_(torch.rand(40) + 0.5)
+    norm = copy.deepcopy(plain)
+    with torch.no_grad():
+        plain.weight.mul_(2)
+    parametrize.register_parametrization(norm, "weight", Double())
+    x, W, g = torch.randn(2, 40, 200, device="cuda"), torch.randn(24, 40, device="cuda"), torch.randn(2, 24, 200, device="cuda")
+    a, b = quant.act8_linear(x, W, None, norm=norm), quant.act8_linear(x, W, None, norm=plain)
+    assert torch.equal(a, b)
+    d1, = torch.autograd.grad(a, [norm.parametrizations.weight.original], g)
+    d2, = torch.autograd.grad(b, [plain.weight], g)
+    assert torch.equal(d1, 2 * d2)
+    for (_, p), (_, q) in zip(norm.named_buffers(), plain.named_buffers()):
+        assert torch.equal(p, q)
