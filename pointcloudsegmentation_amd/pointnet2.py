@@ -529,7 +529,7 @@ class SetAbstraction(nn.Module):
             with torch.cuda.device(xyz.device):
                 _lib.check(L.p2n_sa_group(xyz.data_ptr(), new_xyz.data_ptr(), _rt.ptr(feat), gidx.data_ptr(), B, C, N, M,
                                           ns, grouped.data_ptr(), _rt.stream_handle(xyz.device)), "p2n_sa_group")
-            if self.mlp.precision == "int8" and not self.training:
+            if self.mlp.precision == "int8" and not self.mlp.training:
                 return new_xyz, self.mlp.forward_int8(grouped.view(B, C + 3, M * ns), group=ns)   # MLP + max over the group
             y = self.mlp(grouped.view(B, C + 3, M * ns))
             out = torch.empty((B, y.size(1), M), dtype=torch.float32, device=xyz.device)
