@@ -424,6 +424,7 @@ int p2n_max_of_columns(const float *in, long rows, int ns, float *out, void *str
  * backward pass); batches (may be NULL) counts one more where the running statistics are updated.  Backward, with uh and ah the values that the codes stand for:
  *   dW = g . ah^T, db = sum g, dy = [y > 0] * (W^T . g), dbeta = sum dy, dgamma = sum dy*uh,
  *   dx = gamma*r*(dy - dbeta/P - uh*dgamma/P), P = B*L   (frozen: gamma*r*dy; without a norm: W^T . g)
+ * Products are of three-way splits: an infinity among their operands (x, g, W) gives NaN.
  * dW and db may be NULL (not computed), and dx without a norm; with a norm dgamma and dbeta need dx.  Limits: 1..1024
  * channels, L <= 2^24, B*ceil(L/128) < 2^24 - 1024.  kept and workspace 256-byte aligned; the workspace holds nothing between calls. */
 size_t p2n_act8_kept_bytes(int B, int C, long L, int norm);

@@ -3,7 +3,8 @@
 // norm is BatchNorm over the B*L points of a channel (reference point2net.py:9-34 in train() mode): mean and biased variance
 // from sums in 64 bits, mu and r = 1/sqrt(var + eps) kept as float32, u = fl(fl(x - mu) * r), y = gamma*u + beta.
 // Kept instead of x: the codes of u (of x without a norm) by the 8-bit rule of p2n_q8.h, one scale for 128 consecutive points of a
-// (cloud, channel) row, and one bit [y > 0] for each value, so the ReLU's decisions stay exact: 1.16 bytes a value for 4.
+// (cloud, channel) row, and one bit [y > 0] for each value, so the ReLU's decisions stay exact: 1.16 bytes a value for 4.  (The
+// forward product forms y from x - mu and gamma*r in one fma: within a rounding of zero it may pass a value that size whose bit is clear.)
 // A NaN counts as above zero, so it goes on into everything that its value enters, on the way back too.
 // The backward pass works from uh = s*q and ah = [y > 0] * max(gamma*uh + beta, 0):
 //     dW = g . ah^T   db = sum g   da = W^T . g   dy = [y > 0] * da   dbeta = sum dy   dgamma = sum dy*uh
@@ -307,7 +308,7 @@ __global__ __launch_bounds__(256) void p2n_act8_keep_kernel(Act8Keep A) {
 // D = M . X, lane = point, registers = channels.  A workgroup takes 128 points (one group of a cloud), a wave 32 of them and all of
 // CT*32 output channels; the weight fragments pass through LDS (a ring of three, LDS-DMA), X through registers.  Six part products a
 // multiply-add: the matrix cores are the bound with many channels (256 -> 256 over 131,072 points: 104 us forward, 990 TFLOP/s of part
-// products; 124 us with the backward's epilogue), memory with few (32 -> 64 over 1,048,576: 64 us, 6.3 TB/s).
+// products; 122 us with the backward's epilogue), memory with few (32 -> 64 over 1,048,576: 64 to 67 us, 6 TB/s).
 struct Act8Gemm {
     const float *x;        // (B, K, L)
     const __bf16 *img;
@@ -949,7 +950,8 @@ __global__ __launch_bounds__(256, 2) void p2n_act8_wgrad_kernel(Act8Wgrad A) {
 
 // 128 x 128 a wave, the only one on its SIMD: splitting the operands (8 to 9 vector instructions a product) has to go on while the matrix
 // core works, so the operands of the next 24 products are formed between the products of the present 24, and a quarter of the other
-// side's next ones with them (256 x 256 over 131,072 points with the join: 127 us, 141 with each 16 points' operands formed first).
+// side's next ones with them (256 x 256 over 131,072 points with the join, in a stream of calls: 117 us; 127 on the card where forming
+// each 16 points' operands first took 141; alone in a kernel trace 142 + 9).
 // g comes by LDS-DMA, a step ahead, codes into registers, two ahead.  Rows of g start on 16 bytes, L a multiple of 4.
 template <bool NORM>
 __global__ __launch_bounds__(256, 1) void p2n_act8_wgrad_wide_kernel(Act8Wgrad A) {
@@ -1077,7 +1079,7 @@ __global__ __launch_bounds__(256, 1) void p2n_act8_wgrad_wide_kernel(Act8Wgrad A
 // 32 RT x 32 of dW as above, and for the same 32 points W^T . g from the same piece of LDS (lane = point, its eight values of a
 // k-step from eight rows), the fragments of W^T in LDS too.  dy goes to dx's place, its two sums stay in registers to the end.
 // Either product alone comes from here too, so that it does not depend on what else is asked for.
-// 32 -> 64 over 1,048,576 points: 103 us (118 before its g went past the caches) against 93 + 104 for the two, 64 -> 64 over 524,288:
+// 32 -> 64 over 1,048,576 points: 103 to 111 us (118 before its g went past the caches) against 93 + 104 for the two, 64 -> 64 over 524,288:
 // 109 against 52 + 78.
 struct Act8Both {
     Act8Wgrad w;

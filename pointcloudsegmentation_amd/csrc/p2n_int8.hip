@@ -762,7 +762,7 @@ __device__ __forceinline__ unsigned int8_halves(unsigned am) {
 }
 
 // Up to 64 channels everywhere: one wave carries its 32 points through every layer in registers.  Bound by the vector instructions that
-// scale the sums and form the next codes, some 11 a value (88 % of the issue slots): 6-32-32-64 with groups of 32 over 16 x 65536 points 47 us,
+// scale the sums and form the next codes, some 12 a value (89 % of the issue slots): 6-32-32-64 with groups of 32 over 16 x 65536 points 47 us,
 // of which the memory's share is 7; the maximum by exchanges between lanes instead of in registers: 9 more.
 // HT: tiles of 32 channels that the input and the layers between have.  With one, five waves fit a SIMD instead of four (53 -> 47 us).
 template <int HT>
@@ -855,7 +855,7 @@ __global__ __launch_bounds__(256, HT == 1 ? 5 : 4) void p2n_int8_mlp_narrow_kern
 
 // Wider layers: NW waves carry 32 points together, a wave its share of the channel tiles.  Codes go round through LDS in operand order; a point's
 // maximum is joined over the waves there too.  Two barriers a layer; a layer's first weights are on their way before the last one ends.
-// 131-128-128-128-64 over 16 x 8192 points: 43 us (vector instructions 65 % of the issue slots, memory 20 us); one wave for all channels: 83.
+// 131-128-128-128-64 over 16 x 8192 points: 41 us (14 vector instructions a value, 63 % of the issue slots, memory 20 us); one wave for all channels: 83.
 // IR: k-tiles of the input a wave holds: 4, or 2 where that is enough and five waves a SIMD have work (43 us against 46).  With few
 // columns the registers are worth more than the fifth wave (384-256-256 over 515 columns: 9.2 us against 8.6).
 template <int NW, bool GROUPS, int IR>

@@ -389,7 +389,7 @@ class SharedMLP(nn.Module):
     fused level kernels), train / autograd = p2n_mlp_train_forward + p2n_mlp_train_backward."""
 
     # GPU tensors only, plain attributes (not part of the state_dict)
-    precision = "fp32"       # "int8": eval products in 8-bit integers (quant.int8_mlp)
+    precision = "fp32"       # "int8": eval products in 8-bit integers (quant.int8_mlp); calls that gradients are wanted of stay float32
     checkpoint = None        # "int8": training keeps its activations in 8 bits (quant.act8_linear)
 
     def __init__(self, channels: List[int], last_plain: bool = False):
@@ -625,7 +625,7 @@ class Point2NetSA(nn.Module):
     @property
     def precision(self):
         """eval precision of the shared MLPs: "fp32" (the fused levels) or "int8" (products in 8-bit integers, level by
-        level; groups and channels as quant.int8_mlp takes them)"""
+        level; groups and channels as quant.int8_mlp takes them; without gradients, under torch.no_grad() -- otherwise float32)"""
         return self._uniform("precision")
 
     @precision.setter

@@ -321,7 +321,8 @@ class _Act8Linear(torch.autograd.Function):
 def act8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
                 norm: Optional[nn.BatchNorm1d] = None, training: Optional[bool] = None) -> torch.Tensor:
     """x (B, K, L) float32 -> W relu(norm(x)) + b, or W x + b without a norm: (B, N, L), differentiable in x, weight (N, K) or
-    (N, K, 1), bias and the norm's parameters.  The output is computed from the float32 values; for the backward pass the
+    (N, K, 1), bias and the norm's parameters.  The output is computed from the float32 values (finite ones: an infinity in a product's
+    operands gives NaN); for the backward pass the
     normalised input (the input itself without a norm) is kept in 8 bits, one scale for 128 consecutive points of a channel,
     with one bit for each of the ReLU's decisions: 1.16 bytes a value instead of 4.  norm.training (or `training`, if given) decides
     between the batch's statistics (running statistics updated, as BatchNorm1d does) and the running ones.  1..1024 channels."""
