@@ -379,7 +379,7 @@ class _Act8NormRelu(torch.autograd.Function):
 
 def act8_norm_relu(x: torch.Tensor, norm: nn.BatchNorm1d, training: Optional[bool] = None) -> torch.Tensor:
     """x (B, C, L) float32 -> relu(norm(x)), differentiable in x and the norm's parameters; what the backward pass needs of x is
-    kept in 8 bits and the ReLU's decisions as bits, as in act8_linear."""
+    kept in 8 bits and the ReLU's decisions as bits, as in act8_linear.  `training`, if given, in place of norm.training."""
     x = _gpu(x, "x", (torch.float32,))
     if x.dim() != 3 or 0 in x.shape:
         raise ValueError(f"x must be (B,C,L) with at least one value, got {tuple(x.shape)}")
